@@ -102,7 +102,8 @@ def draw(rng):
         batch = max(1, min(_log(rng, 1, 64), 10 ** 8 // (keys * kv_heads * head)))
         return _attention(None, 'attention', batch, min(keys, rng.choice([1, 1, 1, 2, 5])), keys, heads, kv_heads, head, dtype,
                           'feature', buckets, distance, True, 'cache')
-    keys = _log(rng, 1, 4096)
+    # (a single key has a probability of one and no gradient but rounding, so training starts at a few)
+    keys = _log(rng, 4 if kind == 'attention_training' else 1, 4096)
     queries = keys if rng.random() < 0.8 else _log(rng, 1, 4096)
     causal = queries == keys and rng.random() < 0.4
     batch = max(1, min(_log(rng, 1, 96), 2 ** 28 // (queries * keys * heads)))
