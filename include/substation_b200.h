@@ -315,6 +315,87 @@ int sb_mma_peak_probe(void* stream, int k_blocks, int bf16, double* flops);
 int sb_set_sm_budget(int n_sms);
 
 /* ------------------------------------------------------------------------- */
+/* Positions in attention                                                    */
+/* ------------------------------------------------------------------------- */
+
+/* Norms of queries and keys and their rotation by position, one pass over both.  For every head and token
+ *   n = x * rsqrt(mean_p x^2 + eps),   y = n * gain[p],
+ * then the first `rotary` features are turned in pairs: (a, b) -> (a cos - b sin, b cos + a sin) with the angle
+ * position * base^(-2 i / rotary) for pair i, which joins features i and i + rotary/2 (SB_PAIR_HALVES) or 2 i and 2 i + 1
+ * (SB_PAIR_ADJACENT).  Sums, angles and products are 32 bits or more (angles are reduced in 64, so that far positions keep
+ * their digits); one rounding at the end.  q, q_out: [P,H,B,J]; k, k_out: [P,G,B,J] with any number of heads, or k, k_gain
+ * and k_out all NULL; gains: [P], contiguous; positions: int32 [B,J], any strides (0 to share them), any sign.  P is at most
+ * 256, rotary even and at most P (0: no rotation).  An output may be its input (same pointer and strides).  No counterpart
+ * in the reference. */
+typedef enum sb_pairing { SB_PAIR_HALVES = 0, SB_PAIR_ADJACENT = 1 } sb_pairing;
+typedef struct sb_rotation {
+  double base;
+  int32_t rotary;
+  int32_t pairing; /* sb_pairing */
+  float eps;
+} sb_rotation;
+int sb_query_key_norm_rotation(void* stream, const sb_tensor* q, const sb_tensor* k, const sb_tensor* q_gain,
+                               const sb_tensor* k_gain, const sb_tensor* positions, const sb_tensor* q_out,
+                               const sb_tensor* k_out, const sb_rotation* rotation);
+/* Its gradients, from those of the outputs and the inputs of the forward call:
+ *   g = dout turned back,   dgain[p] = sum_{h,b,j} g n,   dx = rsqrt(..) * (g gain - n mean_p(g gain n)).
+ * scratch: sb_query_key_norm_scratch_bytes() of 16-byte aligned device memory, contents of no interest before or after, not
+ * shared by calls that may run at the same time.  Sums run in a fixed order.  dq may be dq_out or q, dk may be dk_out or k
+ * (same pointer and strides). */
+size_t sb_query_key_norm_scratch_bytes(void);
+int sb_backward_query_key_norm_rotation(void* stream, void* scratch, size_t scratch_bytes, const sb_tensor* dq_out,
+                                        const sb_tensor* dk_out, const sb_tensor* q, const sb_tensor* k,
+                                        const sb_tensor* q_gain, const sb_tensor* k_gain, const sb_tensor* positions,
+                                        const sb_tensor* dq, const sb_tensor* dk, const sb_tensor* dq_gain,
+                                        const sb_tensor* dk_gain, const sb_rotation* rotation);
+
+/* A learned bias for every head and bucket of relative positions.  The distance of a key from a query is the difference of
+ * their positions; starts[i] is the smallest distance in bucket i (host memory, starts[0] = 0, not decreasing; of several
+ * buckets that start together only the last is met).  With `bidirectional`, keys before the query and at its place use
+ * buckets 0 .. n-1 and keys behind it n .. 2n-1; without, keys behind it count as distance 0.  table: [2n or n, H].  At most
+ * 256 buckets a direction, and the last one starts at a distance of at most 832.  An entry of -inf, or one at or below
+ * -2^126 (which only bfloat16 has), hides the keys of its bucket. */
+typedef struct sb_relative_bias {
+  const sb_tensor* table;
+  int32_t n;
+  int32_t bidirectional;
+  const int32_t* starts;
+} sb_relative_bias;
+/* Which keys a query sees.  lengths, first: contiguous int32 [B] in device memory, or NULL.  Sample b has lengths[b] keys
+ * (NULL: all of them; values outside 0 .. K act as the nearer end); what the tensors hold behind them is not used, whatever it
+ * is.  first[b] is the position of the sample's first query on the keys' axis (NULL: 0), any sign; the others follow it.
+ * causal: a query sees no key behind its own position. */
+typedef struct sb_attention_span {
+  float scale;
+  int32_t causal;
+  const int32_t* lengths;
+  const int32_t* first;
+} sb_attention_span;
+/* Attention with that bias:  s = scale * sum_p q k + bias,  out = sum_k softmax_k(s) v,  lse = log sum_k exp(s).
+ * q, out: [P,H,B,J]; k, v: [P,G,B,K], H a multiple of G (head h reads h / (H/G)); P at most 128; lse: float32 [H,B,J] or
+ * NULL.  A query that sees no key gives out = 0 and lse = -inf.  Scores are not stored anywhere; exponentials are rounded to 16
+ * bits where they meet v, sums are fp32.  Few queries against many keys are split along the keys and joined by a second kernel.
+ * scratch: sb_relative_attention_scratch_bytes() for the same operands (may be 0), 16-byte aligned, as above. */
+int sb_relative_attention(void* stream, void* scratch, size_t scratch_bytes, const sb_tensor* q, const sb_tensor* k,
+                          const sb_tensor* v, const sb_relative_bias* bias, const sb_tensor* out, const sb_tensor* lse,
+                          const sb_attention_span* span);
+int sb_relative_attention_scratch_bytes(const sb_tensor* q, const sb_tensor* k, const sb_tensor* v,
+                                        const sb_relative_bias* bias, size_t* bytes);
+/* Its gradients, out and lse being the forward call's:
+ *   D = sum_p dout out,  ds = softmax * (sum_p dout v - D),  dv = sum_{j} softmax dout,  dk = scale sum_j ds q,
+ *   dq = scale sum_k ds k,  dtable[n,h] = sum of ds over the batch's pairs in bucket n.
+ * dk and dv of shared heads are sums over the query heads, and 0 behind a sample's length; every element of the five outputs
+ * is written.  Sums run in a fixed order: the same call gives the same bits.  No counterpart in the reference, which has
+ * neither positions nor padding. */
+int sb_backward_relative_attention(void* stream, void* scratch, size_t scratch_bytes, const sb_tensor* dout,
+                                   const sb_tensor* q, const sb_tensor* k, const sb_tensor* v,
+                                   const sb_relative_bias* bias, const sb_tensor* out, const sb_tensor* lse,
+                                   const sb_tensor* dq, const sb_tensor* dk, const sb_tensor* dv, const sb_tensor* dtable,
+                                   const sb_attention_span* span);
+int sb_backward_relative_attention_scratch_bytes(const sb_tensor* dout, const sb_tensor* q, const sb_tensor* k,
+                                                 const sb_tensor* v, const sb_relative_bias* bias, size_t* bytes);
+
+/* ------------------------------------------------------------------------- */
 /* Whole layer                                                               */
 /* ------------------------------------------------------------------------- */
 

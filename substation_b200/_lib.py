@@ -15,6 +15,7 @@ SB_OK = 0
 SB_MASK_EXPLICIT, SB_MASK_PHILOX = 0, 1
 SB_ACT_RELU, SB_ACT_GELU = 0, 1
 SB_GEMM_AUTO, SB_GEMM_TCGEN05, SB_GEMM_SIMT = 0, 1, 2
+SB_PAIR_HALVES, SB_PAIR_ADJACENT = 0, 1
 
 c_void_p, c_int, c_float, c_char_p = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_char_p
 
@@ -37,6 +38,19 @@ class SbEpilogue(ctypes.Structure):
                 ('logical_dims', c_char_p), ('discard_c', ctypes.c_int32)]
 
 
+class SbRotation(ctypes.Structure):
+    _fields_ = [('base', ctypes.c_double), ('rotary', ctypes.c_int32), ('pairing', ctypes.c_int32), ('eps', c_float)]
+
+
+class SbRelativeBias(ctypes.Structure):
+    _fields_ = [('table', ctypes.POINTER(SbTensor)), ('n', ctypes.c_int32), ('bidirectional', ctypes.c_int32),
+                ('starts', ctypes.POINTER(ctypes.c_int32))]
+
+
+class SbAttentionSpan(ctypes.Structure):
+    _fields_ = [('scale', c_float), ('causal', ctypes.c_int32), ('lengths', c_void_p), ('first', c_void_p)]
+
+
 class SbEncoderConfig(ctypes.Structure):
     _fields_ = [('batch', ctypes.c_int32), ('seq', ctypes.c_int32), ('heads', ctypes.c_int32),
                 ('embed', ctypes.c_int32), ('activation', ctypes.c_int32),
@@ -57,6 +71,8 @@ class SubstationError(RuntimeError):
 _T = ctypes.POINTER(SbTensor)
 _D = ctypes.POINTER(SbDropout)
 _PP = ctypes.POINTER(c_void_p)
+_SZ = ctypes.c_size_t
+_R, _RB, _AS = ctypes.POINTER(SbRotation), ctypes.POINTER(SbRelativeBias), ctypes.POINTER(SbAttentionSpan)
 
 #: every exported symbol with (restype, argtypes); the CPU test suite checks the
 #: library exports exactly these
@@ -87,6 +103,13 @@ SIGNATURES = {
                         ctypes.c_size_t]),
     'sb_einsum_fused': (c_int, [c_void_p, c_char_p, _T, c_char_p, _T, c_char_p, _T, c_float, ctypes.POINTER(SbEpilogue)]),
     'sb_einsum_last_impl': (c_int, []),
+    'sb_query_key_norm_rotation': (c_int, [c_void_p] + [_T] * 7 + [_R]),
+    'sb_query_key_norm_scratch_bytes': (_SZ, []),
+    'sb_backward_query_key_norm_rotation': (c_int, [c_void_p, c_void_p, _SZ] + [_T] * 11 + [_R]),
+    'sb_relative_attention': (c_int, [c_void_p, c_void_p, _SZ, _T, _T, _T, _RB, _T, _T, _AS]),
+    'sb_relative_attention_scratch_bytes': (c_int, [_T, _T, _T, _RB, ctypes.POINTER(_SZ)]),
+    'sb_backward_relative_attention': (c_int, [c_void_p, c_void_p, _SZ, _T, _T, _T, _T, _RB] + [_T] * 6 + [_AS]),
+    'sb_backward_relative_attention_scratch_bytes': (c_int, [_T, _T, _T, _T, _RB, ctypes.POINTER(_SZ)]),
     'sb_device_error': (c_int, [c_void_p, ctypes.POINTER(c_int)]),
     'sb_device_error_reset': (c_int, [c_void_p]),
     'sb_mma_peak_probe': (c_int, [c_void_p, c_int, c_int, ctypes.POINTER(ctypes.c_double)]),

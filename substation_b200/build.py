@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 #: one library per storage type (fp16 is the default one; the bf16 build is the same sources with -DSB_BF16)
 LIB_PATHS = {'fp16': LIB_PATH, 'bf16': os.path.join(PKG_DIR, 'libsubstation_b200_bf16.so')}
 DTYPE_FLAGS = {'fp16': [], 'bf16': ['-DSB_BF16']}
-SOURCES = ('api.cu', 'fused_ops.cu', 'fused_lnbwd.cu', 'gemm.cu')
+SOURCES = ('api.cu', 'fused_ops.cu', 'fused_lnbwd.cu', 'gemm.cu', 'qk_norm.cu', 'relative_attention.cu')
 NVCC_FLAGS = ['-gencode', 'arch=compute_100a,code=sm_100a', '-O3', '-lineinfo', '-std=c++17',
               '-Xcompiler', '-fPIC', '-shared', '--threads', '0']
 

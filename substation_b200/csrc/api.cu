@@ -194,6 +194,248 @@ extern "C" int sb_softmax_dropout(void* stream, const sb_tensor* beta, const sb_
   return launch_softmax_fwd((cudaStream_t)stream, dims4(beta), vb, va, vm, vd, scale, rng);
 }
 
+// ---------------------------------------------------------------------------
+// Positions in attention
+// ---------------------------------------------------------------------------
+namespace {
+
+int to_projection(const sb_tensor* t, const char* what, Proj* o) {
+  SB_TRY(check_tensor(t, 4, what));
+  SB_TRY(fits_int(t, what));
+  o->p = t->ptr; o->sP = t->stride[0]; o->sH = t->stride[1]; o->sB = t->stride[2]; o->sR = t->stride[3];
+  o->P = (int)t->size[0]; o->H = (int)t->size[1]; o->B = (int)t->size[2]; o->R = (int)t->size[3];
+  return SB_OK;
+}
+// An output has the extents of `like` and a place of its own for every element.
+int distinct(const sb_tensor* t, const char* what) {
+  for (int i = 0; i < t->ndim; ++i)
+    if (t->size[i] > 1 && t->stride[i] == 0) return fail(SB_ERR_ARG, std::string(what) + ": an output cannot repeat elements (zero stride)");
+  return SB_OK;
+}
+int to_projection_out(const sb_tensor* t, const sb_tensor* like, const char* what, Proj* o) {
+  SB_TRY(to_projection(t, what, o));
+  SB_TRY(same_shape(like, t, what));
+  return distinct(t, what);
+}
+int to_gain(const sb_tensor* t, const sb_tensor* x, const char* what, void** p) { return to_param(t, x->size[0], what, p); }
+
+// What forward and backward of the norms share.  Leaves k->H = 0 when there are no keys.
+int norm_operands(const sb_tensor* q, const sb_tensor* k, const sb_tensor* q_gain, const sb_tensor* k_gain, const sb_tensor* positions,
+                  const sb_rotation* rotation, Proj* pq, Proj* pk, void** gq, void** gk, View2* pos, Rotation* rot) {
+  memset(pk, 0, sizeof(*pk));
+  *gk = nullptr;
+  SB_TRY(to_projection(q, "norm.q", pq));
+  SB_TRY(to_gain(q_gain, q, "norm.q_gain", gq));
+  if (k) {
+    SB_TRY(to_projection(k, "norm.k", pk));
+    if (pk->P != pq->P || pk->B != pq->B || pk->R != pq->R) return fail(SB_ERR_ARG, "norm.k: extent mismatch between operands");
+    if (pk->H < 1) return fail(SB_ERR_ARG, "norm.k: no heads");
+    SB_TRY(to_gain(k_gain, k, "norm.k_gain", gk));
+  }
+  if (pq->P < 1 || pq->H < 1) return fail(SB_ERR_ARG, "norm.q: no features or no heads");
+  if (pq->P > kNormMaxHead)
+    return fail(SB_ERR_UNSUPPORTED, "norm: heads of " + std::to_string(pq->P) + " features, at most " + std::to_string(kNormMaxHead));
+  if ((long long)pq->B * pq->R > 0x7fffffffLL) return fail(SB_ERR_UNSUPPORTED, "norm: more than 2^31-1 tokens");
+  if ((long long)pq->H + pk->H > 65535) return fail(SB_ERR_UNSUPPORTED, "norm: more than 65535 heads");
+  SB_TRY(check_tensor(positions, 2, "norm.positions"));
+  if (positions->size[0] != pq->B || positions->size[1] != pq->R)
+    return fail(SB_ERR_ARG, "norm.positions: extent mismatch between operands");
+  pos->p = positions->ptr; pos->sB = positions->stride[0]; pos->sJ = positions->stride[1];
+  if (!rotation) return fail(SB_ERR_ARG, "norm: null rotation");
+  if (rotation->rotary < 0 || rotation->rotary > pq->P || rotation->rotary % 2)
+    return fail(SB_ERR_ARG, "norm: the rotated features are an even number, at most the head's");
+  if (rotation->pairing != SB_PAIR_HALVES && rotation->pairing != SB_PAIR_ADJACENT) return fail(SB_ERR_ARG, "norm: unknown pairing");
+  if (!(rotation->base > 0.0) || !std::isfinite(rotation->base)) return fail(SB_ERR_ARG, "norm: the rotation's base must be positive");
+  if (!(rotation->eps >= 0.f) || !std::isfinite(rotation->eps)) return fail(SB_ERR_ARG, "norm: eps must not be negative");
+  rot->base = rotation->base; rot->rotary = rotation->rotary; rot->pairing = rotation->pairing; rot->eps = rotation->eps;
+  return SB_OK;
+}
+
+// The norms may work in place, element on element; anything else that overlaps would be read after it is written.
+bool other_place(const Proj& a, const Proj& b) {
+  return a.p == b.p && (a.sP != b.sP || a.sH != b.sH || a.sB != b.sB || a.sR != b.sR);
+}
+
+}  // namespace
+
+extern "C" int sb_query_key_norm_rotation(void* stream, const sb_tensor* q, const sb_tensor* k, const sb_tensor* q_gain,
+                                          const sb_tensor* k_gain, const sb_tensor* positions, const sb_tensor* q_out,
+                                          const sb_tensor* k_out, const sb_rotation* rotation) {
+  Proj pq, pk, oq, ok;
+  void *gq, *gk;
+  View2 pos;
+  Rotation rot;
+  memset(&ok, 0, sizeof(ok));
+  if (!k != !k_gain || !k != !k_out) return fail(SB_ERR_ARG, "norm: k, k_gain and k_out are given together or not at all");
+  SB_TRY(norm_operands(q, k, q_gain, k_gain, positions, rotation, &pq, &pk, &gq, &gk, &pos, &rot));
+  SB_TRY(to_projection_out(q_out, q, "norm.q_out", &oq));
+  if (k) SB_TRY(to_projection_out(k_out, k, "norm.k_out", &ok));
+  if (other_place(pq, oq) || (k && other_place(pk, ok)))
+    return fail(SB_ERR_ARG, "norm: an output in its input's place needs its strides");
+  return launch_qk_norm_fwd((cudaStream_t)stream, pq, pk, gq, gk, pos, oq, ok, rot);
+}
+
+extern "C" size_t sb_query_key_norm_scratch_bytes(void) { return qk_norm_scratch_bytes(); }
+
+extern "C" int sb_backward_query_key_norm_rotation(void* stream, void* scratch, size_t scratch_bytes, const sb_tensor* dq_out,
+                                                   const sb_tensor* dk_out, const sb_tensor* q, const sb_tensor* k,
+                                                   const sb_tensor* q_gain, const sb_tensor* k_gain, const sb_tensor* positions,
+                                                   const sb_tensor* dq, const sb_tensor* dk, const sb_tensor* dq_gain,
+                                                   const sb_tensor* dk_gain, const sb_rotation* rotation) {
+  Proj pq, pk, gq_out, gk_out, oq, ok;
+  void *gq, *gk, *dgq, *dgk = nullptr;
+  View2 pos;
+  Rotation rot;
+  memset(&ok, 0, sizeof(ok));
+  memset(&gk_out, 0, sizeof(gk_out));
+  if (!k != !k_gain || !k != !dk_out || !k != !dk || !k != !dk_gain)
+    return fail(SB_ERR_ARG, "norm: k, k_gain, dk_out, dk and dk_gain are given together or not at all");
+  SB_TRY(norm_operands(q, k, q_gain, k_gain, positions, rotation, &pq, &pk, &gq, &gk, &pos, &rot));
+  SB_TRY(to_projection(dq_out, "norm.dq_out", &gq_out));
+  SB_TRY(same_shape(q, dq_out, "norm.dq_out"));
+  SB_TRY(to_projection_out(dq, q, "norm.dq", &oq));
+  SB_TRY(to_gain(dq_gain, q, "norm.dq_gain", &dgq));
+  if (k) {
+    SB_TRY(to_projection(dk_out, "norm.dk_out", &gk_out));
+    SB_TRY(same_shape(k, dk_out, "norm.dk_out"));
+    SB_TRY(to_projection_out(dk, k, "norm.dk", &ok));
+    SB_TRY(to_gain(dk_gain, k, "norm.dk_gain", &dgk));
+  }
+  if (other_place(gq_out, oq) || other_place(pq, oq) || (k && (other_place(gk_out, ok) || other_place(pk, ok))))
+    return fail(SB_ERR_ARG, "norm: an output in its input's place needs its strides");
+  if (!scratch || scratch_bytes < qk_norm_scratch_bytes()) return fail(SB_ERR_ARG, "norm: scratch is missing or too small");
+  if (!aligned(scratch, 16)) return fail(SB_ERR_ALIGNMENT, "norm: scratch is not 16-byte aligned");
+  return launch_qk_norm_bwd((cudaStream_t)stream, scratch, gq_out, gk_out, pq, pk, gq, gk, pos, oq, ok, dgq, dgk, rot);
+}
+
+namespace {
+
+int relative_operands(const sb_tensor* q, const sb_tensor* k, const sb_tensor* v, const sb_relative_bias* bias, Proj* pq, Proj* pk,
+                      Proj* pv, RelBias* rb) {
+  SB_TRY(to_projection(q, "relative attention.q", pq));
+  SB_TRY(to_projection(k, "relative attention.k", pk));
+  SB_TRY(to_projection(v, "relative attention.v", pv));
+  SB_TRY(same_shape(k, v, "relative attention.v"));
+  if (pk->P != pq->P || pk->B != pq->B) return fail(SB_ERR_ARG, "relative attention.k: extent mismatch between operands");
+  for (const Proj* x : {pq, pk})
+    if (x->P < 1 || x->H < 1 || x->B < 1 || x->R < 1) return fail(SB_ERR_ARG, "relative attention: every extent must be positive");
+  if (pq->H % pk->H) return fail(SB_ERR_ARG, "relative attention: the query heads are not a multiple of the key heads");
+  if (pq->P > kRelMaxHead)
+    return fail(SB_ERR_UNSUPPORTED, "relative attention: heads of " + std::to_string(pq->P) + " features, at most " + std::to_string(kRelMaxHead));
+  const long long units = (long long)pq->H * pq->B;
+  if (units * ((pq->R + 63) / 64) > 0x1fffffffLL || units * ((pk->R + 63) / 64) > 0x1fffffffLL || pq->R > 0x3fffffff || pk->R > 0x3fffffff)
+    return fail(SB_ERR_UNSUPPORTED, "relative attention: too many heads, samples and rows");
+  if (!bias || !bias->table || !bias->starts) return fail(SB_ERR_ARG, "relative attention: null bias, table or starts");
+  const int n = bias->n;
+  if (n < 1) return fail(SB_ERR_ARG, "relative attention: at least one bucket a direction");
+  if (n > kRelMaxBuckets)
+    return fail(SB_ERR_UNSUPPORTED, "relative attention: " + std::to_string(n) + " buckets a direction, at most " + std::to_string(kRelMaxBuckets));
+  SB_TRY(check_tensor(bias->table, 2, "relative attention.table"));
+  if (bias->table->size[0] != (bias->bidirectional ? 2 * n : n) || bias->table->size[1] != pq->H)
+    return fail(SB_ERR_ARG, "relative attention.table: extents are not [buckets, heads]");
+  if (bias->starts[0] != 0) return fail(SB_ERR_ARG, "relative attention: the first bucket starts at distance 0");
+  for (int i = 1; i < n; ++i)
+    if (bias->starts[i] < bias->starts[i - 1]) return fail(SB_ERR_ARG, "relative attention: bucket starts decrease");
+  if (bias->starts[n - 1] > kRelMaxReach)
+    return fail(SB_ERR_UNSUPPORTED, "relative attention: the last bucket starts at distance " + std::to_string(bias->starts[n - 1]) +
+                                        ", at most " + std::to_string(kRelMaxReach));
+  rb->table = bias->table->ptr; rb->sN = bias->table->stride[0]; rb->sH = bias->table->stride[1];
+  rb->n = n; rb->bidirectional = bias->bidirectional ? 1 : 0; rb->starts = bias->starts;
+  return SB_OK;
+}
+
+int to_span(const sb_attention_span* span, RelSpan* o) {
+  if (!span) return fail(SB_ERR_ARG, "relative attention: null span");
+  if (!std::isfinite(span->scale)) return fail(SB_ERR_ARG, "relative attention: the scale is not finite");
+  if (!aligned(span->lengths, 4) || !aligned(span->first, 4)) return fail(SB_ERR_ALIGNMENT, "relative attention: lengths and first are int32");
+  o->scale = span->scale; o->causal = span->causal ? 1 : 0; o->lengths = span->lengths; o->first = span->first;
+  return SB_OK;
+}
+
+int to_lse(const sb_tensor* t, const sb_tensor* q, RelRows* o) {
+  memset(o, 0, sizeof(*o));
+  if (!t) return SB_OK;
+  SB_TRY(check_tensor(t, 3, "relative attention.lse"));
+  for (int i = 0; i < 3; ++i)
+    if (t->size[i] != q->size[i + 1]) return fail(SB_ERR_ARG, "relative attention.lse: extent mismatch between operands");
+  o->p = reinterpret_cast<float*>(t->ptr); o->sH = t->stride[0]; o->sB = t->stride[1]; o->sJ = t->stride[2];
+  return SB_OK;
+}
+
+int check_scratch(const void* scratch, size_t have, size_t need) {
+  if (need == 0) return SB_OK;
+  if (!scratch || have < need) return fail(SB_ERR_ARG, "relative attention: scratch is missing or too small");
+  if (!aligned(scratch, 16)) return fail(SB_ERR_ALIGNMENT, "relative attention: scratch is not 16-byte aligned");
+  return SB_OK;
+}
+
+}  // namespace
+
+extern "C" int sb_relative_attention_scratch_bytes(const sb_tensor* q, const sb_tensor* k, const sb_tensor* v, const sb_relative_bias* bias,
+                                                   size_t* bytes) {
+  Proj pq, pk, pv;
+  RelBias rb;
+  if (!bytes) return fail(SB_ERR_ARG, "relative attention: null result");
+  SB_TRY(relative_operands(q, k, v, bias, &pq, &pk, &pv, &rb));
+  *bytes = rel_attn_scratch_bytes(pq, pk, pv, rb);
+  return SB_OK;
+}
+
+extern "C" int sb_relative_attention(void* stream, void* scratch, size_t scratch_bytes, const sb_tensor* q, const sb_tensor* k,
+                                     const sb_tensor* v, const sb_relative_bias* bias, const sb_tensor* out, const sb_tensor* lse,
+                                     const sb_attention_span* span) {
+  Proj pq, pk, pv, po;
+  RelBias rb;
+  RelSpan sp;
+  RelRows rows;
+  SB_TRY(relative_operands(q, k, v, bias, &pq, &pk, &pv, &rb));
+  SB_TRY(to_projection_out(out, q, "relative attention.out", &po));
+  SB_TRY(to_lse(lse, q, &rows));
+  if (lse) SB_TRY(distinct(lse, "relative attention.lse"));
+  SB_TRY(to_span(span, &sp));
+  SB_TRY(check_scratch(scratch, scratch_bytes, rel_attn_scratch_bytes(pq, pk, pv, rb)));
+  return launch_rel_attn_fwd((cudaStream_t)stream, scratch, pq, pk, pv, rb, po, rows, sp);
+}
+
+extern "C" int sb_backward_relative_attention_scratch_bytes(const sb_tensor* dout, const sb_tensor* q, const sb_tensor* k,
+                                                            const sb_tensor* v, const sb_relative_bias* bias, size_t* bytes) {
+  Proj pg, pq, pk, pv;
+  RelBias rb;
+  if (!bytes) return fail(SB_ERR_ARG, "relative attention: null result");
+  SB_TRY(relative_operands(q, k, v, bias, &pq, &pk, &pv, &rb));
+  SB_TRY(to_projection(dout, "relative attention.dout", &pg));
+  SB_TRY(same_shape(q, dout, "relative attention.dout"));
+  *bytes = rel_attn_bwd_scratch_bytes(pg, pq, pk, pv, rb);
+  return SB_OK;
+}
+
+extern "C" int sb_backward_relative_attention(void* stream, void* scratch, size_t scratch_bytes, const sb_tensor* dout, const sb_tensor* q,
+                                              const sb_tensor* k, const sb_tensor* v, const sb_relative_bias* bias, const sb_tensor* out,
+                                              const sb_tensor* lse, const sb_tensor* dq, const sb_tensor* dk, const sb_tensor* dv,
+                                              const sb_tensor* dtable, const sb_attention_span* span) {
+  Proj pg, pq, pk, pv, po, oq, ok, ov;
+  RelBias rb;
+  RelSpan sp;
+  RelRows rows;
+  SB_TRY(relative_operands(q, k, v, bias, &pq, &pk, &pv, &rb));
+  SB_TRY(to_projection(dout, "relative attention.dout", &pg));
+  SB_TRY(same_shape(q, dout, "relative attention.dout"));
+  SB_TRY(to_projection(out, "relative attention.out", &po));
+  SB_TRY(same_shape(q, out, "relative attention.out"));
+  if (!lse) return fail(SB_ERR_ARG, "relative attention: the backward pass needs the forward pass's lse");
+  SB_TRY(to_lse(lse, q, &rows));
+  SB_TRY(to_projection_out(dq, q, "relative attention.dq", &oq));
+  SB_TRY(to_projection_out(dk, k, "relative attention.dk", &ok));
+  SB_TRY(to_projection_out(dv, v, "relative attention.dv", &ov));
+  SB_TRY(check_tensor(dtable, 2, "relative attention.dtable"));
+  SB_TRY(same_shape(bias->table, dtable, "relative attention.dtable"));
+  SB_TRY(distinct(dtable, "relative attention.dtable"));
+  SB_TRY(to_span(span, &sp));
+  SB_TRY(check_scratch(scratch, scratch_bytes, rel_attn_bwd_scratch_bytes(pg, pq, pk, pv, rb)));
+  return launch_rel_attn_bwd((cudaStream_t)stream, scratch, pg, pq, pk, pv, rb, po, rows, oq, ok, ov, dtable->ptr, dtable->stride[0],
+                             dtable->stride[1], sp);
+}
+
 namespace {
 // [P,H,B,rows] projection as a View4 whose fields carry the (P,H,B,row) strides
 int to_proj(const sb_tensor* t, const sb_tensor* scores, const char* what, View4* v, int* P) {

@@ -91,6 +91,35 @@ int launch_flash_bwd(cudaStream_t s, int H, int B, int L, const void* kqv, long 
                      const void* dgamma, View4 dgv, void* dkqv, long long dslice, View4 dproj, float scale, const void* fwd_scratch,
                      void* bwd_scratch);
 
+// Positions in attention ---------------------------------------------------------
+// A projection [P, heads, B, rows] with any strides.
+struct Proj {
+  void* p;
+  long long sP, sH, sB, sR;
+  int P, H, B, R;
+};
+struct Rotation { double base; int rotary, pairing; float eps; };
+constexpr int kNormMaxHead = 256;
+size_t qk_norm_scratch_bytes();
+// k.H = 0: queries alone.  pos: int32 [B,J].
+int launch_qk_norm_fwd(cudaStream_t s, Proj q, Proj k, const void* q_gain, const void* k_gain, View2 pos, Proj q_out, Proj k_out,
+                       const Rotation& rot);
+int launch_qk_norm_bwd(cudaStream_t s, void* scratch, Proj dq_out, Proj dk_out, Proj q, Proj k, const void* q_gain, const void* k_gain,
+                       View2 pos, Proj dq, Proj dk, void* dq_gain, void* dk_gain, const Rotation& rot);
+
+// Bias per head and bucket: table[bucket * sN + head * sH]; starts[0 .. n-1] in host memory.
+struct RelBias { const void* table; long long sN, sH; int n, bidirectional; const int32_t* starts; };
+struct RelSpan { float scale; int causal; const int* lengths; const int* first; };
+struct RelRows { float* p; long long sH, sB, sJ; };   // float32 [H,B,J]
+constexpr int kRelMaxBuckets = 256;                   // of one direction
+constexpr int kRelMaxReach = 832;                     // first distance of the last bucket
+constexpr int kRelMaxHead = 128;
+size_t rel_attn_scratch_bytes(const Proj& q, const Proj& k, const Proj& v, const RelBias& bias);
+int launch_rel_attn_fwd(cudaStream_t s, void* scratch, Proj q, Proj k, Proj v, const RelBias& bias, Proj out, RelRows lse, const RelSpan& span);
+size_t rel_attn_bwd_scratch_bytes(const Proj& dout, const Proj& q, const Proj& k, const Proj& v, const RelBias& bias);
+int launch_rel_attn_bwd(cudaStream_t s, void* scratch, Proj dout, Proj q, Proj k, Proj v, const RelBias& bias, Proj out, RelRows lse,
+                        Proj dq, Proj dk, Proj dv, void* dtable, long long dt_sN, long long dt_sH, const RelSpan& span);
+
 // Contractions -----------------------------------------------------------------
 struct GemmProblem {
   long long batch, M, N, K;

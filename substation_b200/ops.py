@@ -6,7 +6,10 @@ reference's kernel harness drives one generated launcher at a time
 (pytorch_module/benchmark.py); it is also what the kernel-level parity tests call.
 """
 
+import bisect
+import contextlib
 import ctypes
+import functools
 import threading
 
 import torch
@@ -317,3 +320,162 @@ def set_sm_budget(n_sms):
     for key in ('fp16', 'bf16'):
         lib = _lib.load(key)
         _lib.check(lib.sb_set_sm_budget(int(n_sms)), lib)
+
+
+# ---- positions in attention ---------------------------------------------------------------------------------------
+_PAIRING = {'halves': _lib.SB_PAIR_HALVES, 'adjacent': _lib.SB_PAIR_ADJACENT}
+
+
+def _here(*tensors):
+    """All operands of a call are CUDA tensors of one device; returns it as the current one for the call."""
+    _check_cuda(*tensors)
+    dev = tensors[0].device
+    for t in tensors:
+        if t.device != dev:
+            raise ValueError(f'operands on {dev} and on {t.device}')
+    return torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _int32(t, what):
+    if t.dtype != torch.int32:
+        raise TypeError(f'{what} are int32, got {t.dtype}')
+
+
+def _scratch(nbytes, device):
+    """Device memory of one call, from torch's allocator: calls on several streams, and graphs that were captured with
+    them, have their own."""
+    if nbytes == 0:
+        return None, ctypes.c_void_p(None)
+    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return t, ctypes.c_void_p(t.data_ptr())
+
+
+def _rotation(q, base, rotary, pairing, eps):
+    r = _lib.SbRotation()
+    r.base, r.rotary, r.pairing, r.eps = float(base), q.shape[0] if rotary is None else int(rotary), _PAIRING[pairing], float(eps)
+    return ctypes.byref(r)
+
+
+def query_key_norm_rotation(q, k, q_gain, k_gain, positions, q_out, k_out, base=10000.0, rotary=None, pairing='halves', eps=1e-6):
+    """Root-mean-square norm of every head of q [P,H,B,J] and k [P,G,B,J] over its features, times the gains [P], then the
+    rotation of the first ``rotary`` features (None: all) by the tokens' int32 ``positions`` [B,J]; one pass over both.
+    ``pairing``: 'halves' turns features i and i + rotary/2 together, 'adjacent' 2i and 2i+1.  ``k``, ``k_gain`` and ``k_out``
+    may be None.  An output may be its input."""
+    some = _given(q, k, q_gain, k_gain, q_out, k_out)
+    with _here(*some, positions):
+        _half(*some); _int32(positions, 'positions')
+        check(_cur().sb_query_key_norm_rotation(_stream(), _d(q), _opt(k), _d(q_gain), _opt(k_gain), _d(positions), _d(q_out),
+                                                _opt(k_out), _rotation(q, base, rotary, pairing, eps)))
+
+
+def backward_query_key_norm_rotation(dq_out, dk_out, q, k, q_gain, k_gain, positions, dq, dk, dq_gain, dk_gain, base=10000.0,
+                                     rotary=None, pairing='halves', eps=1e-6):
+    """Gradients of ``query_key_norm_rotation`` with respect to q, k and the gains, from those of its outputs."""
+    some = _given(dq_out, dk_out, q, k, q_gain, k_gain, dq, dk, dq_gain, dk_gain)
+    with _here(*some, positions):
+        _half(*some); _int32(positions, 'positions')
+        lib = _cur()
+        nbytes = lib.sb_query_key_norm_scratch_bytes()
+        keep, ptr = _scratch(nbytes, q.device)
+        check(lib.sb_backward_query_key_norm_rotation(
+            _stream(), ptr, nbytes, _d(dq_out), _opt(dk_out), _d(q), _opt(k), _d(q_gain), _opt(k_gain), _d(positions), _d(dq),
+            _opt(dk), _d(dq_gain), _opt(dk_gain), _rotation(q, base, rotary, pairing, eps)))
+
+
+class RelativeBuckets:
+    """Which bucket a relative position falls into: ``starts[i]`` is the smallest distance in bucket i of one direction.
+    With ``bidirectional``, keys behind the query have buckets of their own, after the others; without, they count as
+    distance 0."""
+
+    def __init__(self, starts, bidirectional=True):
+        self.starts = tuple(int(s) for s in starts)
+        self.bidirectional = bool(bidirectional)
+        self._array = (ctypes.c_int32 * len(self.starts))(*self.starts)
+
+    def __len__(self):
+        """Entries of a table of biases."""
+        return len(self.starts) * (2 if self.bidirectional else 1)
+
+    def bucket(self, relative):
+        """Bucket of a key ``relative`` positions behind the query (negative: before it)."""
+        d = relative if relative > 0 and self.bidirectional else max(0, -relative)
+        b = bisect.bisect_right(self.starts, d) - 1
+        return b + (len(self.starts) if relative > 0 and self.bidirectional else 0)
+
+
+@functools.lru_cache(maxsize=64)
+def relative_buckets(num_buckets=32, max_distance=128, bidirectional=True):
+    """The usual buckets: half of a direction's buckets hold one distance each, the others grow by a constant ratio, so that
+    log(distance) falls into equal parts, and the last one takes everything from below ``max_distance`` on.  Borders are
+    found in whole numbers: some of them are distances themselves, and a rounded logarithm misses those."""
+    n = num_buckets // 2 if bidirectional else num_buckets
+    exact = n // 2
+    if n < 2 or (bidirectional and num_buckets % 2):
+        raise ValueError('at least two buckets a direction, and an even number of them for two directions')
+    if max_distance <= exact:
+        raise ValueError(f'max_distance {max_distance} has to exceed the {exact} distances with a bucket each')
+    steps, starts, d = n - exact, list(range(exact)), exact
+    for i in range(steps):
+        while d ** steps * exact ** i < max_distance ** i * exact ** steps:   # log(d/exact) / log(max/exact) < i / steps
+            d += 1
+        starts.append(d)
+    return RelativeBuckets(starts, bidirectional)
+
+
+def _relative_bias(table, buckets):
+    b = _lib.SbRelativeBias()
+    b.table = ctypes.pointer(tensor_desc(table))
+    b.n, b.bidirectional = len(buckets.starts), 1 if buckets.bidirectional else 0
+    b.starts = ctypes.cast(buckets._array, ctypes.POINTER(ctypes.c_int32))
+    return ctypes.byref(b)
+
+
+def _span(q, scale, causal, lengths, first):
+    s = _lib.SbAttentionSpan()
+    s.scale, s.causal = float(scale), 1 if causal else 0
+    for name, t in (('lengths', lengths), ('first', first)):
+        if t is None:
+            continue
+        _int32(t, name)
+        if tuple(t.shape) != (q.shape[2],) or not t.is_contiguous():
+            raise ValueError(f'{name} is one contiguous int32 per sample ({q.shape[2]}), got {tuple(t.shape)}')
+        setattr(s, name, t.data_ptr())
+    return ctypes.byref(s)
+
+
+def _rows(t):
+    if t is not None and t.dtype != torch.float32:
+        raise TypeError(f'lse is float32, got {t.dtype}')
+    return _opt(t)
+
+
+def relative_attention(q, k, v, table, out, lse=None, *, buckets, scale, causal=False, lengths=None, first=None):
+    """out = softmax(scale * q.k + table[bucket]) v without the scores in memory.  q, out: [P,H,B,J]; k, v: [P,G,B,K] with H
+    a multiple of G; ``table`` [len(buckets),H]; ``lse``: float32 [H,B,J], the rows' log-sum-exp, which the backward pass
+    needs.  ``lengths``: int32 [B], keys of each sample; ``first``: int32 [B], position of a sample's first query on the
+    keys' axis (None: 0); ``causal``: queries see no keys behind their position.  A query that sees nothing gives 0."""
+    half = [q, k, v, table, out]
+    with _here(*half, *_given(lse, lengths, first)):
+        _half(*half)
+        lib, bias, nbytes = _cur(), _relative_bias(table, buckets), ctypes.c_size_t(0)
+        span, rows = _span(q, scale, causal, lengths, first), _rows(lse)
+        dq, dk, dv = _d(q), _d(k), _d(v)
+        check(lib.sb_relative_attention_scratch_bytes(dq, dk, dv, bias, ctypes.byref(nbytes)))
+        keep, ptr = _scratch(nbytes.value, q.device)
+        check(lib.sb_relative_attention(_stream(), ptr, nbytes.value, dq, dk, dv, bias, _d(out), rows, span))
+
+
+def backward_relative_attention(dout, q, k, v, table, out, lse, dq, dk, dv, dtable, *, buckets, scale, causal=False, lengths=None,
+                                first=None):
+    """Gradients of ``relative_attention`` with respect to q, k, v and the table, from that of its output, its output and its
+    ``lse``.  The same call gives the same bits."""
+    half = [dout, q, k, v, table, out, dq, dk, dv, dtable]
+    with _here(*half, lse, *_given(lengths, first)):
+        _half(*half)
+        lib, bias, nbytes = _cur(), _relative_bias(table, buckets), ctypes.c_size_t(0)
+        span, rows = _span(q, scale, causal, lengths, first), _rows(lse)
+        dg, d1, d2, d3 = _d(dout), _d(q), _d(k), _d(v)
+        check(lib.sb_backward_relative_attention_scratch_bytes(dg, d1, d2, d3, bias, ctypes.byref(nbytes)))
+        keep, ptr = _scratch(nbytes.value, q.device)
+        check(lib.sb_backward_relative_attention(_stream(), ptr, nbytes.value, dg, d1, d2, d3, bias, _d(out), rows, _d(dq), _d(dk),
+                                                 _d(dv), _d(dtable), span))
