@@ -364,7 +364,7 @@ typedef struct sb_relative_bias {
 /* Which keys a query sees.  lengths, first: contiguous int32 [B] in device memory, or NULL.  Sample b has lengths[b] keys
  * (NULL: all of them; values outside 0 .. K act as the nearer end); what the tensors hold behind them is not used, whatever it
  * is.  first[b] is the position of the sample's first query on the keys' axis (NULL: 0), any sign; the others follow it.
- * causal: a query sees no key behind its own position. */
+ * causal: a query sees no key behind its own position.  scale is finite and not negative. */
 typedef struct sb_attention_span {
   float scale;
   int32_t causal;

@@ -346,7 +346,7 @@ int relative_operands(const sb_tensor* q, const sb_tensor* k, const sb_tensor* v
 
 int to_span(const sb_attention_span* span, RelSpan* o) {
   if (!span) return fail(SB_ERR_ARG, "relative attention: null span");
-  if (!std::isfinite(span->scale)) return fail(SB_ERR_ARG, "relative attention: the scale is not finite");
+  if (!std::isfinite(span->scale) || span->scale < 0.f) return fail(SB_ERR_ARG, "relative attention: the scale is not finite or negative");
   if (!aligned(span->lengths, 4) || !aligned(span->first, 4)) return fail(SB_ERR_ALIGNMENT, "relative attention: lengths and first are int32");
   o->scale = span->scale; o->causal = span->causal ? 1 : 0; o->lengths = span->lengths; o->first = span->first;
   return SB_OK;

@@ -690,6 +690,7 @@ splitk_reduce_kernel(const float* __restrict__ ws, int splits, long long batch, 
 #include "attn_fused.cuh"
 #include "score_contract.cuh"
 #include "flash_attn.cuh"
+#include "rel_attn.cuh"
 #include "peak_probe.cuh"
 
 // ---- host side ------------------------------------------------------------
@@ -1565,6 +1566,66 @@ int launch_flash_bwd(cudaStream_t s, int H, int B, int L, const void* kqv, long 
   const unsigned grid = (unsigned)std::min<long long>(p.items, sm_count());
   SB_LAUNCH_OK(launch_k(flash::flash_bwd_kernel, grid, flash::kBwdThreads, flash::kBwdSmem, s, mq, mk, mv, mg, p));
   return SB_OK;
+}
+
+bool rel_direct(const Proj& x) {
+  auto ok = [](long long n, long long stride) { return n == 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)); };
+  return (x.sP == 1 || x.P == 1) && (reinterpret_cast<uintptr_t>(x.p) & 15u) == 0 && ok(x.R, x.sR) && ok(x.H, x.sH) && ok(x.B, x.sB);
+}
+
+namespace {
+
+// Tensor map of [P, R, H, B] in boxes of 64 features x `rows` rows.
+bool rel_map(const Proj& x, int rows, CUtensorMap* map, std::string* why) {
+  const cuuint64_t dim[4] = {(cuuint64_t)x.P, (cuuint64_t)x.R, (cuuint64_t)x.H, (cuuint64_t)x.B};
+  const long long row = pad8(x.P);   // any legal stride where the extent is 1
+  const cuuint64_t str[3] = {(cuuint64_t)(x.R == 1 ? row : x.sR) * 2, (cuuint64_t)(x.H == 1 ? row : x.sH) * 2, (cuuint64_t)(x.B == 1 ? row : x.sB) * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  const CUresult r = g_encode(map, SB_TMAP_DTYPE, 4, x.p, dim, str, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { *why = "cuTensorMapEncodeTiled rejected it (code " + std::to_string((int)r) + ")"; return false; }
+  return true;
+}
+
+rel::Common rel_common(const Proj& q, const Proj& k, const RelTables& t, const RelSpan& span) {
+  rel::Common c;
+  c.J = q.R; c.K = k.R; c.H = q.H; c.G = k.H; c.B = q.B; c.P = q.P;
+  c.c2 = span.scale * 1.4426950408889634f;
+  c.causal = span.causal; c.lengths = span.lengths; c.first = span.first;
+  c.bias_rows = t.rows; c.pitch = t.pitch; c.reach = t.reach;
+  return c;
+}
+
+template <int P>
+int rel_fwd(cudaStream_t s, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, rel::FwdParams& p) {
+  using Cfg = rel::FwdCfg<P>;
+  constexpr int kMostPitch = (2 * kRelMaxReach + 1 + 2 * rel::kPad + 3) / 4 * 4;
+  static_assert(2 * (Cfg::kTiles + 2 * kMostPitch * 4 + 1024 + 256 + 1024) <= 233472, "two CTAs of the attention forward kernel per SM");
+  // Two CTAs per SM, but the machine may place one on each SM first: within a budget there is one for every SM of it.
+  const int ctas = sm_count() < device_sms() ? sm_count() : 2 * sm_count();
+  p.chunk = p.c.causal ? std::min(p.units, std::max(1, (4 * ctas + p.nq - 1) / p.nq)) : 1;
+  SB_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(rel::rel_fwd_kernel<P>), Cfg::smem(kMostPitch)));
+  SB_LAUNCH_OK(launch_k(rel::rel_fwd_kernel<P>, (unsigned)std::min(p.items, ctas), rel::kFwdThreads, Cfg::smem(p.c.pitch), s, mq, mk, mv, p));
+  return SB_OK;
+}
+
+}  // namespace
+
+int launch_rel_tiles_fwd(cudaStream_t s, Proj q, Proj k, Proj v, RelTables t, Proj out, RelRows lse, const RelSpan& span) {
+  std::call_once(g_encode_once, load_encode);
+  if (!g_encode) return fail(SB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  std::string why;
+  CUtensorMap mq, mk, mv;
+  if (!rel_map(q, 128, &mq, &why) || !rel_map(k, 128, &mk, &why) || !rel_map(v, 128, &mv, &why))
+    return fail(SB_ERR_UNSUPPORTED, "relative attention, operands: " + why);
+  rel::FwdParams p;
+  p.c = rel_common(q, k, t, span);
+  p.nq = (q.R + 127) / 128;
+  p.units = q.H * q.B;
+  p.items = p.units * p.nq;
+  p.out = out;
+  p.lse = lse;
+  return q.P <= 64 ? rel_fwd<64>(s, mq, mk, mv, p) : rel_fwd<128>(s, mq, mk, mv, p);
 }
 
 int gemm_device_error(cudaStream_t s, int* code) {

@@ -114,6 +114,12 @@ struct RelRows { float* p; long long sH, sB, sJ; };   // float32 [H,B,J]
 constexpr int kRelMaxBuckets = 256;                   // of one direction
 constexpr int kRelMaxReach = 832;                     // first distance of the last bucket
 constexpr int kRelMaxHead = 128;
+// Rows of biases over relative positions in units of log2, one per head (expand_bias_kernel); first distance of the last bucket.
+struct RelTables { const float* rows; int pitch, reach; };
+// What tensor maps can address: unit-stride features, 16-byte multiples everywhere else.
+bool rel_direct(const Proj& x);
+// The tcgen05 kernels; q, k, v are rel_direct.
+int launch_rel_tiles_fwd(cudaStream_t s, Proj q, Proj k, Proj v, RelTables t, Proj out, RelRows lse, const RelSpan& span);
 size_t rel_attn_scratch_bytes(const Proj& q, const Proj& k, const Proj& v, const RelBias& bias);
 int launch_rel_attn_fwd(cudaStream_t s, void* scratch, Proj q, Proj k, Proj v, const RelBias& bias, Proj out, RelRows lse, const RelSpan& span);
 size_t rel_attn_bwd_scratch_bytes(const Proj& dout, const Proj& q, const Proj& k, const Proj& v, const RelBias& bias);

@@ -2,6 +2,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 #include "ops.h"
 
@@ -10,6 +11,7 @@ namespace sb {
 namespace {
 
 constexpr int kMaxP = kRelMaxHead;
+constexpr int kRelPad = 160;                        // as the tile kernels' kPad
 constexpr float kHidden = -8.507059173023462e37f;   // -2^126: entries at or below hide their keys
 
 struct Starts { int s[kRelMaxBuckets]; };
@@ -44,52 +46,41 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
   return a.lengths ? max(0, min(a.K, a.lengths[b])) : a.K;
 }
 
-// One warp per query row, lanes along keys for scores and along features for the output.
+// rows[h][i] = log2(e) * bias of head h at relative position i - kRelPad - reach, which stays at its end values beyond the reach.
+// Finite biases stay finite, so that a row of nothing but the lowest ones still has a maximum.
 __global__ void __launch_bounds__(256)
-simple_fwd_kernel(const AttnArgs a, const Starts st) {
-  __shared__ float q[8][kMaxP];
+expand_bias_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, float* rows, int pitch, int reach) {
   grid_dependency_sync();
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long rows = (long long)a.H * a.B * a.J;
-  for (long long r = (long long)blockIdx.x * 8 + w; r < rows; r += (long long)gridDim.x * 8) {
-    const int j = (int)(r % a.J), b = (int)(r / a.J % a.B), h = (int)(r / a.J / a.B), hk = h / (a.H / a.G);
-    __syncwarp();
-    for (int p = lane; p < a.P; p += 32) q[w][p] = sb_h2f(row_of(a.q, h, b, j)[p * a.q.sP]);
-    __syncwarp();
-    const int pos = (a.first ? a.first[b] : 0) + j;
-    int n = keys_of(a, b);
-    if (a.causal) n = max(0, min(n, pos + 1));
-    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < n; k0 += 32) {
-      const int k = k0 + lane;
-      float s = -INFINITY;
-      if (k < n) {
-        const sb_half* kr = row_of(a.k, hk, b, k);
-        float dot = 0.f;
-        for (int p = 0; p < a.P; ++p) dot = fmaf(q[w][p], sb_h2f(kr[p * a.k.sP]), dot);
-        const float bias = sb_h2f(a.table[bucket_of(a, st, k - pos) * a.t_sN + h * a.t_sH]);
-        s = bias <= kHidden ? -INFINITY : fmaf(dot, a.scale, bias);
-      }
-      const float mx = fmaxf(m, group_max<32>(s));
-      if (mx == -INFINITY) continue;
-      const float f = expf(m - mx), e = expf(s - mx);
-      l = l * f + group_sum<32>(e);
-      m = mx;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[c] *= f;
-      for (int i = 0; i < min(32, n - k0); ++i) {
-        const float pe = __shfl_sync(0xffffffffu, e, i);
-        const sb_half* vr = row_of(a.v, hk, b, k0 + i);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (c * 32 + lane < a.P) acc[c] = fmaf(pe, sb_h2f(vr[(c * 32 + lane) * a.v.sP]), acc[c]);
-      }
+  const int i = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+  if (i >= pitch) return;
+  const int rel = max(-reach, min(reach, i - kRelPad - reach));
+  const float b = sb_h2f(a.table[bucket_of(a, st, rel) * a.t_sN + h * a.t_sH]);
+  rows[(long long)h * pitch + i] = b <= kHidden ? -INFINITY : b * 1.4426950408889634f;
+}
+
+// [P,H,B,R] of any strides -> [B][H][R][Pp], which tensor maps can address; 64 rows of one head and sample a block.
+__global__ void __launch_bounds__(256)
+pack_rows_kernel(const Proj x, sb_half* dst, int Pp, int along_rows) {
+  __shared__ sb_half tile[64][kMaxP + 2];
+  grid_dependency_sync();
+  const int blocks = (x.R + 63) / 64;
+  const long long all = (long long)x.H * x.B * blocks;
+  for (long long it = blockIdx.x; it < all; it += gridDim.x) {
+    const int r0 = (int)(it % blocks) * 64, h = (int)(it / blocks % x.H), b = (int)(it / blocks / x.H), n = min(64, x.R - r0);
+    const sb_half* src = row_of(x, h, b, r0);
+    __syncthreads();
+    if (along_rows) {
+      const int r = threadIdx.x & 63;
+      if (r < n)
+        for (int p = threadIdx.x >> 6; p < x.P; p += 4) tile[r][p] = src[p * x.sP + r * x.sR];
+    } else {
+      for (int r = threadIdx.x >> 5; r < n; r += 8)
+        for (int p = threadIdx.x & 31; p < x.P; p += 32) tile[r][p] = src[p * x.sP + r * x.sR];
     }
-    sb_half* out = const_cast<sb_half*>(row_of(a.o, h, b, j));
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (c * 32 + lane < a.P) out[(c * 32 + lane) * a.o.sP] = sb_f2h(l > 0.f ? acc[c] / l : 0.f);
-    if (a.lse.p && lane == 0) a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] = l > 0.f ? m + logf(l) : -INFINITY;
+    __syncthreads();
+    sb_half* d = dst + (((long long)b * x.H + h) * x.R + r0) * Pp;
+    for (int r = threadIdx.x >> 5; r < n; r += 8)
+      for (int p = threadIdx.x & 31; p < x.P; p += 32) d[(long long)r * Pp + p] = tile[r][p];
   }
 }
 
@@ -256,16 +247,55 @@ AttnArgs attn_args(const Proj& q, const Proj& k, const Proj& v, const RelBias& b
 }
 size_t dsum_bytes(const Proj& q) { return (sizeof(float) * (size_t)q.H * q.B * q.R + 255) / 256 * 256; }
 
+// Scratch: rows of biases, then a packed copy of each operand that tensor maps cannot address.
+struct Plan { int pitch, reach; size_t at[4], bytes; };
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+size_t packed_bytes(const Proj& x) { return align256(2 * (size_t)((x.P + 7) / 8 * 8) * x.H * x.B * x.R); }
+Plan plan_of(std::initializer_list<const Proj*> operands, int heads, const RelBias& bias) {
+  Plan p;
+  p.reach = std::max(1, bias.starts[bias.n - 1]);
+  p.pitch = (2 * p.reach + 1 + 2 * kRelPad + 3) / 4 * 4;
+  p.bytes = align256(sizeof(float) * (size_t)p.pitch * heads);
+  int i = 0;
+  for (const Proj* x : operands) {
+    p.at[i++] = p.bytes;
+    if (!rel_direct(*x)) p.bytes += packed_bytes(*x);
+  }
+  return p;
+}
+// x as tensor maps can address it: itself, or the copy at `at`.
+int direct_or_packed(cudaStream_t s, void* scratch, size_t at, Proj* x) {
+  if (rel_direct(*x)) return SB_OK;
+  const int Pp = (x->P + 7) / 8 * 8;
+  auto mag = [](long long v) { return v < 0 ? -v : v; };
+  sb_half* dst = reinterpret_cast<sb_half*>(reinterpret_cast<char*>(scratch) + at);
+  const long long blocks = (long long)x->H * x->B * ((x->R + 63) / 64);
+  SB_LAUNCH_OK(launch_k(pack_rows_kernel, (unsigned)std::min<long long>(blocks, 8 * usable_sms(device_facts().sms)), 256, 0, s, *x, dst, Pp,
+                        x->R > 1 && mag(x->sR) < mag(x->sP) ? 1 : 0));
+  x->p = dst;
+  x->sP = 1; x->sR = Pp; x->sH = (long long)Pp * x->R; x->sB = x->sH * x->H;
+  return SB_OK;
+}
+int expand_bias(cudaStream_t s, const AttnArgs& a, const Starts& st, void* scratch, const Plan& pl, RelTables* t) {
+  t->rows = reinterpret_cast<float*>(scratch); t->pitch = pl.pitch; t->reach = pl.reach;
+  SB_LAUNCH_OK(launch_k(expand_bias_kernel, dim3((pl.pitch + 255) / 256, a.H), 256, 0, s, a, st, reinterpret_cast<float*>(scratch), pl.pitch, pl.reach));
+  return SB_OK;
+}
+
 }  // namespace
 
-size_t rel_attn_scratch_bytes(const Proj&, const Proj&, const Proj&, const RelBias&) { return 0; }
+size_t rel_attn_scratch_bytes(const Proj& q, const Proj& k, const Proj& v, const RelBias& bias) { return plan_of({&q, &k, &v}, q.H, bias).bytes; }
 
-int launch_rel_attn_fwd(cudaStream_t s, void*, Proj q, Proj k, Proj v, const RelBias& bias, Proj out, RelRows lse, const RelSpan& span) {
+int launch_rel_attn_fwd(cudaStream_t s, void* scratch, Proj q, Proj k, Proj v, const RelBias& bias, Proj out, RelRows lse, const RelSpan& span) {
   Starts st;
   const AttnArgs a = attn_args(q, k, v, bias, out, lse, span, &st);
-  const long long rows = (long long)a.H * a.B * a.J;
-  SB_LAUNCH_OK(launch_k(simple_fwd_kernel, (unsigned)std::min<long long>((rows + 7) / 8, 1184), 256, 0, s, a, st));
-  return SB_OK;
+  const Plan pl = plan_of({&q, &k, &v}, q.H, bias);
+  RelTables t;
+  SB_TRY(expand_bias(s, a, st, scratch, pl, &t));
+  SB_TRY(direct_or_packed(s, scratch, pl.at[0], &q));
+  SB_TRY(direct_or_packed(s, scratch, pl.at[1], &k));
+  SB_TRY(direct_or_packed(s, scratch, pl.at[2], &v));
+  return launch_rel_tiles_fwd(s, q, k, v, t, out, lse, span);
 }
 
 size_t rel_attn_bwd_scratch_bytes(const Proj&, const Proj& q, const Proj&, const Proj&, const RelBias& bias) {

@@ -162,6 +162,7 @@ def _attention_call(backward=False, **kw):
     (dict(out=_t([64, 4, 2, 9])), 1, 'extent mismatch'),
     (dict(lse=_t([4, 2, 9])), 1, 'extent mismatch'),
     (dict(scale=math.nan), 1, 'finite'),
+    (dict(scale=-1.0), 1, 'negative'),
     (dict(lengths=0x1002), 5, 'int32'),
     (dict(first=0x1001), 5, 'int32'),
     (dict(span=False), 1, 'null span'),
