@@ -1628,6 +1628,50 @@ int launch_rel_tiles_fwd(cudaStream_t s, Proj q, Proj k, Proj v, RelTables t, Pr
   return q.P <= 64 ? rel_fwd<64>(s, mq, mk, mv, p) : rel_fwd<128>(s, mq, mk, mv, p);
 }
 
+namespace {
+
+template <int P>
+int rel_bwd(cudaStream_t s, const CUtensorMap (&m)[8], rel::BwdParams& p) {
+  using Cfg = rel::BwdCfg<P>;
+  constexpr int kMost = 232448;
+  // Two held pairs let an item's tiles arrive while the one before computes; they go first where the sums' rows leave no room,
+  // then streamed pairs beyond the two that the pipeline needs.
+  for (p.held = 2; p.held > 1 && Cfg::smem(2, p.held, p.c.pitch, p.c.reach) > kMost; --p.held) {}
+  for (p.stages = 6; p.stages > 2 && Cfg::smem(p.stages, p.held, p.c.pitch, p.c.reach) > kMost; --p.stages) {}
+  static_assert(Cfg::smem(2, 1, 2 * kRelMaxReach + 4 + 2 * rel::kPad, kRelMaxReach) <= kMost, "shared memory of the attention backward kernel");
+  const int ctas = sm_count();
+  p.chunk_k = p.c.causal ? std::min(p.c.G * p.c.B, std::max(1, (4 * ctas + p.nk - 1) / p.nk)) : 1;
+  p.chunk_q = p.c.causal ? std::min(p.c.H * p.c.B, std::max(1, (4 * ctas + p.nq - 1) / p.nq)) : 1;
+  SB_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(rel::rel_bwd_kernel<P>), kMost));
+  SB_LAUNCH_OK(launch_k(rel::rel_bwd_kernel<P>, (unsigned)std::min(p.items, ctas), rel::kBwdThreads,
+                        Cfg::smem(p.stages, p.held, p.c.pitch, p.c.reach), s, m[0], m[1], m[2], m[3], m[4], m[5], m[6], m[7], p));
+  return SB_OK;
+}
+
+}  // namespace
+
+int launch_rel_tiles_bwd(cudaStream_t s, Proj dout, Proj q, Proj k, Proj v, RelTables t, RelBackward w, Proj dq, Proj dk, Proj dv,
+                         const RelSpan& span) {
+  std::call_once(g_encode_once, load_encode);
+  if (!g_encode) return fail(SB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  std::string why;
+  CUtensorMap m[8];
+  const Proj* x[4] = {&q, &dout, &k, &v};
+  for (int i = 0; i < 8; ++i)
+    if (!rel_map(*x[i & 3], i < 4 ? 128 : 64, &m[i], &why)) return fail(SB_ERR_UNSUPPORTED, "relative attention, operands: " + why);
+  rel::BwdParams p;
+  memset(&p, 0, sizeof(p));
+  p.c = rel_common(q, k, t, span);
+  p.nq = (q.R + 127) / 128;
+  p.nk = (k.R + 127) / 128;
+  p.first_q = k.H * k.B * p.nk;
+  p.items = p.first_q + q.H * q.B * p.nq;
+  p.scale = span.scale;
+  p.records = w.records; p.partial = w.partial; p.next = w.next;
+  p.dq = dq; p.dk = dk; p.dv = dv;
+  return q.P <= 64 ? rel_bwd<64>(s, m, p) : rel_bwd<128>(s, m, p);
+}
+
 int gemm_device_error(cudaStream_t s, int* code) {
   int v = 0;
   SB_CUDA_OK(cudaMemcpyFromSymbolAsync(&v, g_tc_error, sizeof(int), 0, cudaMemcpyDeviceToHost, s));

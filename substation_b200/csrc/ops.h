@@ -120,6 +120,12 @@ struct RelTables { const float* rows; int pitch, reach; };
 bool rel_direct(const Proj& x);
 // The tcgen05 kernels; q, k, v are rel_direct.
 int launch_rel_tiles_fwd(cudaStream_t s, Proj q, Proj k, Proj v, RelTables t, Proj out, RelRows lse, const RelSpan& span);
+// Backward: `records` [B][H][ceil(J / 64)][192]: of 64 query rows the log-sum-exps in units of log2 (+inf: row without keys, or
+// none), D and the weight (0 or 1) of the row in the table's sums; `partial` [H][B * ceil(J / 128) * 2][2 * reach + 1] sums of
+// score gradients by relative position; `next`: a zero.
+struct RelBackward { const float* records; float* partial; int* next; };
+int launch_rel_tiles_bwd(cudaStream_t s, Proj dout, Proj q, Proj k, Proj v, RelTables t, RelBackward w, Proj dq, Proj dk, Proj dv,
+                         const RelSpan& span);
 size_t rel_attn_scratch_bytes(const Proj& q, const Proj& k, const Proj& v, const RelBias& bias);
 int launch_rel_attn_fwd(cudaStream_t s, void* scratch, Proj q, Proj k, Proj v, const RelBias& bias, Proj out, RelRows lse, const RelSpan& span);
 size_t rel_attn_bwd_scratch_bytes(const Proj& dout, const Proj& q, const Proj& k, const Proj& v, const RelBias& bias);

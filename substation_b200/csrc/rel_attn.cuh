@@ -453,4 +453,529 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   }
 }
 
+// ---- backward --------------------------------------------------------------------------------------------------
+constexpr int kBwdThreads = 320;                     // producer warp, MMA warp, two groups of four element warps
+constexpr int kRecord = 192;                         // floats of 64 query rows: log2-sum-exps, D, weights of the table's sums
+
+struct BwdParams {
+  Common c;
+  int nq, nk;                                        // tiles of 128 queries, of 128 keys
+  int first_q, items;                                // items below first_q: dK and dV of a key tile; the others: dQ of a query tile
+  int chunk_k, chunk_q;
+  int stages, held;                                  // ring of streamed pairs; held pairs (1 or 2)
+  float scale;
+  const float* records;                              // [B][H][ceil(J / 64)][kRecord]
+  float* partial;                                    // [H][B * nq * 2][2 * reach + 1]
+  int* next;                                         // work queue
+  Proj dq, dk, dv;
+};
+
+// An item holds one pair of 128-row tiles and streams pairs of 64-row tiles past it: (K, V) held and (Q, dOUT) of every query
+// head that shares them streamed, or (Q, dOUT) held and (K, V) streamed.  `b`, `h`, `t`: the held tile.
+struct BwdItem {
+  bool q;
+  int b, h, t, first, keys;
+  int tiles, each, t0;                               // streamed tiles: `each` from t0 on, for each head in turn
+};
+__device__ __forceinline__ BwdItem bwd_item(const BwdParams& p, int i) {
+  BwdItem it;
+  it.q = i >= p.first_q;
+  if (it.q) i -= p.first_q;
+  const int rows = it.q ? p.nq : p.nk, heads = it.q ? p.c.H : p.c.G, chunk = it.q ? p.chunk_q : p.chunk_k;
+  const int per = chunk * rows, c = i / per, r = i % per;
+  const int here = min(chunk, heads * p.c.B - c * chunk), unit = c * chunk + r % here;
+  it.t = it.q ? rows - 1 - r / here : r / here;      // long ones first where the span is causal
+  it.b = unit / heads;
+  it.h = unit % heads;
+  it.first = first_of(p.c, it.b);
+  it.keys = keys_of(p.c, it.b);
+  it.t0 = 0;
+  if (it.q) {
+    if (p.c.causal) it.keys = max(0, min(it.keys, it.first + min(p.c.J, it.t * 128 + 128)));
+    it.each = it.tiles = (it.keys + 63) >> 6;
+  } else {
+    const int all = (p.c.J + 63) >> 6;
+    if (p.c.causal) it.t0 = min(all, max(0, it.t * 128 - it.first) >> 6);
+    it.each = it.t * 128 < it.keys ? all - it.t0 : 0;
+    it.tiles = it.each * (p.c.H / p.c.G);
+  }
+  return it;
+}
+
+template <int P>
+struct BwdCfg {
+  static constexpr int kHeld = 2 * 128 * P * 2, kStream = 2 * 64 * P * 2, kStage = kStream + 1024;
+  static constexpr int kSets = P == 64 ? 2 : 1;      // accumulators: an item's results are stored while the next one computes
+  static constexpr uint32_t kAcc = 256;              // tensor memory: two buffers of scores and dP (64 columns each), accumulators
+  static constexpr int smem(int stages, int held, int pitch, int reach) {
+    return held * kHeld + stages * kStage + 2 * pitch * 4 + 8 * ((2 * reach + 4) & ~3) * 4 + 1024 + 512;
+  }
+};
+
+// Scores and dP of a thread's row of 64 columns -> exponentials and score gradients, 16-bit pairs over the columns they came
+// from.  Column c has the bias bp[DIR * c] (NEAR) or `flat`, row constants ls and ds.
+// What differs between the two kinds of items: in key tiles (KEYS) a thread is a key, log-sum-exps and D change along columns
+// (L, D in shared memory), visible columns are c >= lim; in query tiles a thread is a query and visible columns are c < lim.
+template <bool KEYS, bool NEAR, bool MASK, class Emit>
+__device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float flat, const float* L, const float* D, float lse, float dsum,
+                                          int lim, float c2, Emit&& emit) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t s[32], g[32];
+    tmem_ld32_nowait(ts + c * 32, s);
+    tmem_ld32_nowait(ts + 64 + c * 32, g);
+    attn::tmem_ld_wait32(s);
+    attn::tmem_ld_wait32(g);
+    uint32_t pm[16], dm[16];
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+      float4 l4, d4;
+      if (KEYS) {
+        l4 = *reinterpret_cast<const float4*>(L + c * 32 + e);
+        d4 = *reinterpret_cast<const float4*>(D + c * 32 + e);
+      }
+      float pv[4], dv[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int col = c * 32 + e + x;
+        const float l = KEYS ? (x == 0 ? l4.x : x == 1 ? l4.y : x == 2 ? l4.z : l4.w) : lse;
+        const float d = KEYS ? (x == 0 ? d4.x : x == 1 ? d4.y : x == 2 ? d4.z : d4.w) : dsum;
+        const float b = NEAR ? bp[KEYS ? -col : col] : flat;
+        float pr = attn::ex2_approx(fmaf(__uint_as_float(s[e + x]), c2, b - l));
+        float ds = pr * (__uint_as_float(g[e + x]) - d);
+        if (MASK) {
+          const bool seen = KEYS ? col >= lim : col < lim;
+          pr = seen ? pr : 0.f;
+          ds = seen ? ds : 0.f;
+        }
+        pv[x] = pr;
+        dv[x] = ds;
+        emit(c, e + x, ds);
+      }
+      if (KEYS) {
+        pm[e / 2] = flash::pack2(pv[0], pv[1]);
+        pm[e / 2 + 1] = flash::pack2(pv[2], pv[3]);
+      }
+      dm[e / 2] = flash::pack2(dv[0], dv[1]);
+      dm[e / 2 + 1] = flash::pack2(dv[2], dv[3]);
+    }
+    if (KEYS) tmem_st16(ts + c * 16, pm);
+    tmem_st16(ts + 64 + c * 16, dm);
+  }
+}
+
+// One CTA per SM, work items from a queue (which item runs where changes nothing in its results).  The two groups of element
+// warps take the streamed tiles in turn: while one turns scores and dP into exponentials and score gradients, the tensor cores
+// multiply for the other.  Both results go back into tensor memory, where the second products take them from.  Everything is
+// computed twice, once per kind of item; the alternative, dQ summed over key tiles in memory, needs atomics whose order
+// changes the result, or a partial dQ for every key tile.
+// The table's gradient: a score gradient belongs to its relative position, a diagonal of the tile.  A warp moves each column of
+// its 32 x 32 blocks so that lane l holds diagonals l and l - 32 (one shuffle a column), adds the sums of a block to its own row
+// of sums over relative positions, and a group of warps adds up its four rows per item.  Tiles outside the varying part of the
+// bias have one sum.  Everything in a fixed order.
+template <int P>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__ CUtensorMap tmGh, const __grid_constant__ CUtensorMap tmKh,
+               const __grid_constant__ CUtensorMap tmVh, const __grid_constant__ CUtensorMap tmQs, const __grid_constant__ CUtensorMap tmGs,
+               const __grid_constant__ CUtensorMap tmKs, const __grid_constant__ CUtensorMap tmVs, const __grid_constant__ BwdParams p) {
+  using Cfg = BwdCfg<P>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t sheld = (raw + 1023u) & ~1023u, ring = sheld + p.held * Cfg::kHeld;
+  const uint32_t sbias = ring + p.stages * Cfg::kStage;
+  const int width = (2 * p.c.reach + 4) & ~3;        // floats of a warp's row of sums
+  const uint32_t ssums = sbias + 2u * p.c.pitch * 4u, bars = ssums + 8u * width * 4u;
+  const uint32_t item_full = bars, item_empty = bars + 32, h_full = bars + 64, h_empty = bars + 80, b_full = bars + 96, b_empty = bars + 112;
+  const uint32_t s_full = bars + 128, pd_full = bars + 144, acc_full = bars + 160, acc_empty = bars + 176, full = bars + 192, empty = bars + 256;
+  uint8_t* gen = smem_raw + (sheld - raw);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (bars + 320 - sheld));
+  volatile int* queue = reinterpret_cast<volatile int*>(gen + (bars + 336 - sheld));
+  const uint32_t g_sync = bars + 352;
+  const float* bias_s = reinterpret_cast<const float*>(gen + (sbias - sheld));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(item_full + 8 * i, 1);
+      mbar_init(item_empty + 8 * i, 9);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(h_full + 8 * i, 1);
+      mbar_init(h_empty + 8 * i, 1);
+      mbar_init(b_full + 8 * i, 1);
+      mbar_init(b_empty + 8 * i, 8);
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(pd_full + 8 * i, 4);
+      mbar_init(acc_full + 8 * i, 1);
+      mbar_init(acc_empty + 8 * i, 8);
+      mbar_init(g_sync + 8 * i, 4);
+    }
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  {
+    float* sums = reinterpret_cast<float*>(gen + (ssums - sheld));
+    for (int i = threadIdx.x; i < 8 * width; i += kBwdThreads) sums[i] = 0.f;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  grid_dependency_sync();
+
+  // Consumers read every item of the queue in turn.
+  uint32_t taken = 0;
+  auto take = [&](BwdItem* it, bool* ok) {
+    const uint32_t s = taken & 3u;
+    *ok = __all_sync(0xffffffffu, mbar_wait(item_full + 8 * s, (taken >> 2) & 1u, 51));
+    if (!*ok) return false;
+    const int id = queue[s];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(item_empty + 8 * s);
+    ++taken;
+    if (id >= p.items) return false;
+    *it = bwd_item(p, id);
+    return true;
+  };
+
+  if (warp == 0) {
+    // ---------------- producer ----------------
+    // live: items with tiles; run: tiles of one head in an item, which share a row of biases
+    uint32_t seq = 0, live = 0, run = 0, st = 0, st_phase = 1;
+    const int rep = p.c.H / p.c.G, blocks = (p.c.J + 63) >> 6;
+    bool ok = true;
+    int id = blockIdx.x;
+    while (ok) {
+      int after = 0;
+      if (lane == 0 && id < p.items) after = atomicAdd(p.next, 1) + (int)gridDim.x;
+      const uint32_t s = seq & 3u;
+      ok = __all_sync(0xffffffffu, mbar_wait(item_empty + 8 * s, ((seq >> 2) & 1u) ^ 1u, 52));
+      if (!ok) break;
+      if (lane == 0) {
+        queue[s] = id;
+        mbar_arrive(item_full + 8 * s);
+      }
+      __syncwarp();
+      ++seq;
+      if (id >= p.items) break;
+      const BwdItem w = bwd_item(p, id);
+      if (w.tiles > 0) {
+        const uint32_t hb = p.held == 2 ? live & 1u : 0u, hp = p.held == 2 ? live >> 1 : live;
+        ok = __all_sync(0xffffffffu, mbar_wait(h_empty + 8 * hb, (hp & 1u) ^ 1u, 53));
+        if (!ok) break;
+        if (lane == 0) {
+          const uint32_t d = sheld + hb * Cfg::kHeld;
+          mbar_expect_tx(h_full + 8 * hb, Cfg::kHeld);
+          load_rows<P, 128>(d, w.q ? &tmQh : &tmKh, h_full + 8 * hb, w.t * 128, w.h, w.b);
+          load_rows<P, 128>(d + Cfg::kHeld / 2, w.q ? &tmGh : &tmVh, h_full + 8 * hb, w.t * 128, w.h, w.b);
+        }
+        __syncwarp();
+        ++live;
+      }
+      int head = w.q ? w.h : w.h * rep, t = w.t0, left = w.each;
+      for (int i = 0; i < w.tiles && ok; ++i) {
+        if (left == w.each) {
+          const uint32_t bb = run & 1u;
+          ok = __all_sync(0xffffffffu, mbar_wait(b_empty + 8 * bb, ((run >> 1) & 1u) ^ 1u, 54));
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_expect_tx(b_full + 8 * bb, p.c.pitch * 4);
+            bulk_load(sbias + bb * p.c.pitch * 4, p.c.bias_rows + (long long)head * p.c.pitch, p.c.pitch * 4, b_full + 8 * bb);
+          }
+          __syncwarp();
+          ++run;
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * st, st_phase, 55));
+        if (!ok) break;
+        if (lane == 0) {
+          const uint32_t d = ring + st * Cfg::kStage, bar = full + 8 * st;
+          mbar_expect_tx(bar, Cfg::kStream + (w.q ? 0 : 512));
+          if (w.q) {
+            load_rows<P, 64>(d, &tmKs, bar, t * 64, w.h / rep, w.b);
+            load_rows<P, 64>(d + Cfg::kStream / 2, &tmVs, bar, t * 64, w.h / rep, w.b);
+          } else {
+            load_rows<P, 64>(d, &tmQs, bar, t * 64, head, w.b);
+            load_rows<P, 64>(d + Cfg::kStream / 2, &tmGs, bar, t * 64, head, w.b);
+            bulk_load(d + Cfg::kStream, p.records + (((long long)w.b * p.c.H + head) * blocks + t) * kRecord, 512, bar);
+          }
+        }
+        __syncwarp();
+        if (++st == (uint32_t)p.stages) { st = 0; st_phase ^= 1u; }
+        ++t;
+        if (--left == 0) { ++head; t = w.t0; left = w.each; }
+      }
+      id = __shfl_sync(0xffffffffu, after, 0);
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer: scores at most two tiles ahead of the products that read what became of them ----------------
+    struct Work { int q, tiles, keys; };
+    Work even{0, 0, 0}, odd{0, 0, 0};                  // the live item of an even or odd number
+    uint32_t sa = 0, sb = 0, na = 0, nb = 0;           // live items and tiles: scores (a) and products (b)
+    int ta = 0, tb = 0;
+    uint32_t ra = 0, ra_phase = 0, rb = 0;             // ring slots
+    bool ok = true, in_a = false, end = false;
+    while (ok) {
+      const bool pending = na != nb;
+      bool step_a = !end && na - nb < 2u && sa - sb < (uint32_t)p.held;   // (a third live item would overwrite the first's place)
+      if (step_a && !in_a) {
+        // the next live item, without waiting while products are due
+        if (pending && !__all_sync(0xffffffffu, mbar_try(item_full + 8 * (taken & 3u), (taken >> 2) & 1u))) step_a = false;
+        else {
+          BwdItem w;
+          if (!take(&w, &ok)) {
+            end = true;
+          } else if (w.tiles > 0) {
+            (sa & 1u ? odd : even) = Work{w.q ? 1 : 0, w.tiles, w.keys};
+            in_a = true;
+            ta = 0;
+          }
+          continue;
+        }
+      }
+      if (!step_a && !pending) {
+        if (end) break;
+        continue;                                       // (not reached: with nothing pending the next item may start)
+      }
+      if (step_a) {
+        const Work w = sa & 1u ? odd : even;
+        const uint32_t hb = p.held == 2 ? sa & 1u : 0u, hp = p.held == 2 ? sa >> 1 : sa;
+        if (ta == 0) ok = __all_sync(0xffffffffu, mbar_wait(h_full + 8 * hb, hp & 1u, 56));
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(full + 8 * ra, ra_phase, 56));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t x = ring + ra * Cfg::kStage, hd = sheld + hb * Cfg::kHeld, ts = tmem + (na & 1u) * 128u;
+        if (w.q && w.keys - ta * 64 < 64) zero_rows<P, 64>(gen + (x - sheld), w.keys - ta * 64, lane);
+        if (flash::elect_one()) {
+          mma_rows<P, 64>(ts, hd, x);
+          mma_rows<P, 64>(ts + 64u, hd + Cfg::kHeld / 2, x + Cfg::kStream / 2);
+          umma_commit(s_full + 8 * (na & 1u));
+        }
+        __syncwarp();
+        if (++ra == (uint32_t)p.stages) { ra = 0; ra_phase ^= 1u; }
+        ++na;
+        if (++ta == w.tiles) { in_a = false; ++sa; }
+      } else {
+        const Work w = sb & 1u ? odd : even;
+        const uint32_t set = Cfg::kSets == 2 ? sb & 1u : 0u, sp = Cfg::kSets == 2 ? sb >> 1 : sb;
+        ok = __all_sync(0xffffffffu, mbar_wait(pd_full + 8 * (nb & 1u), (nb >> 1) & 1u, 57));
+        if (ok && tb == 0) ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * set, (sp & 1u) ^ 1u, 58));
+        if (!ok) break;
+        tc_fence_after();
+        const bool last = tb == w.tiles - 1;
+        if (flash::elect_one()) {
+          const uint32_t x = ring + rb * Cfg::kStage, ts = tmem + (nb & 1u) * 128u, acc = tmem + Cfg::kAcc + set * 2u * P;
+          mma_weighted<P, 64>(acc, ts + 64u, x, tb > 0);                                               // dK += ds Q, dQ += ds K
+          if (!w.q) mma_weighted<P, 64>(acc + (uint32_t)P, ts, x + Cfg::kStream / 2, tb > 0);          // dV += softmax dOUT
+          umma_commit(empty + 8 * rb);
+          if (last) {
+            umma_commit(h_empty + 8 * (p.held == 2 ? sb & 1u : 0u));
+            umma_commit(acc_full + 8 * set);
+          }
+        }
+        __syncwarp();
+        if (++rb == (uint32_t)p.stages) rb = 0;
+        ++nb;
+        if (++tb == w.tiles) { tb = 0; ++sb; }
+      }
+    }
+  } else {
+    // ---------------- element warps ----------------
+    const int q = warp & 3, g = (warp - 2) >> 2, rt = q * 32 + lane;
+    const uint32_t lanes = (uint32_t)(q * 32) << 16, ts = tmem + lanes + g * 128u;
+    const int blocks = (p.c.J + 63) >> 6, reach = p.c.reach, entries = 2 * reach + 1;
+    float* group_sums = reinterpret_cast<float*>(gen + (ssums - sheld)) + g * 4 * width;
+    float* sums = group_sums + ((warp - 2) & 3) * width;
+    const int in_group = ((warp - 2) & 3) * 32 + lane;
+    uint32_t n = 0, live = 0, run = 0, st = 0, st_phase = 0;
+    bool ok = true, have = false;
+    BwdItem prev;
+    float below = 0.f, above = 0.f;                    // sums outside the varying part of the bias
+    // An item's results: dK (group 0) and dV (group 1) of a key, or dQ of a query, 32 features in turn.
+    auto store = [&](const BwdItem& it, uint32_t acc, bool zero) {
+      const int r = it.t * 128 + rt;
+      const Proj& o = it.q ? p.dq : g ? p.dv : p.dk;
+      sb_half* out = reinterpret_cast<sb_half*>(o.p) + (long long)it.h * o.sH + (long long)it.b * o.sB + (long long)r * o.sR;
+      const float f = it.q || !g ? p.scale : 1.f;
+#pragma unroll 1
+      for (int c = it.q ? g : 0; c < P / 32; c += it.q ? 2 : 1) {
+        uint32_t v[32];
+        if (!zero) {
+          tmem_ld32_nowait(acc + lanes + (it.q || !g ? 0u : (uint32_t)P) + c * 32, v);
+          attn::tmem_ld_wait32(v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0u;
+        }
+        if (r < (it.q ? p.c.J : p.c.K) && c * 32 < p.c.P) store_features(out + c * 32 * o.sP, o.sP, v, f, min(32, p.c.P - c * 32));
+      }
+    };
+    auto finish = [&](const BwdItem& it, uint32_t s) {
+      const uint32_t set = Cfg::kSets == 2 ? s & 1u : 0u, sp = Cfg::kSets == 2 ? s >> 1 : s;
+      ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * set, sp & 1u, 59));
+      if (!ok) return;
+      tc_fence_after();
+      store(it, tmem + Cfg::kAcc + set * 2u * P, false);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty + 8 * set);
+    };
+    auto add = [&](int rel, float v) {
+      if (rel <= -reach) below += v;
+      else if (rel >= reach) above += v;
+      else sums[rel + reach] += v;
+      __syncwarp();
+    };
+    // a barrier of the group's four warps whose wait is bounded like all others
+    uint32_t syncs = 0;
+    auto group_sync = [&] {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(g_sync + 8 * g);
+      ok = __all_sync(0xffffffffu, mbar_wait(g_sync + 8 * g, syncs & 1u, 61));
+      ++syncs;
+      return ok;
+    };
+    // the group's sums of a query tile to memory
+    auto flush = [&](const BwdItem& it) {
+      const float lo = warp_sum(below), hi = warp_sum(above);
+      below = above = 0.f;
+      if (lane == 0) {
+        sums[0] = lo;
+        sums[2 * reach] = hi;
+      }
+      if (!group_sync()) return;
+      float* out = p.partial + (((long long)it.h * p.c.B * p.nq + (long long)it.b * p.nq + it.t) * 2 + g) * entries;
+      for (int i = in_group; i < entries; i += 128) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          v += group_sums[w * width + i];
+          group_sums[w * width + i] = 0.f;
+        }
+        out[i] = v;
+      }
+      group_sync();
+    };
+    BwdItem w;
+    while (ok && take(&w, &ok)) {
+      if (w.tiles == 0) {
+        store(w, 0u, true);
+        if (w.q) flush(w);
+        continue;
+      }
+      const int r = w.t * 128 + rt;                    // query or key of this thread
+      float lse = INFINITY, dsum = 0.f, weight = 0.f;
+      if (w.q && r < p.c.J) {
+        const float* rec = p.records + (((long long)w.b * p.c.H + w.h) * blocks + (r >> 6)) * kRecord + (r & 63);
+        lse = rec[0];
+        dsum = rec[64];
+        weight = rec[128];
+      }
+      int mine = w.keys;
+      if (w.q && p.c.causal) mine = min(mine, w.first + r + 1);
+      bool due = have;                                 // the previous item's results are still to be stored
+      int t = w.t0, left = w.each;
+      for (int i = 0; i < w.tiles; ++i, ++n) {
+        const uint32_t bb = run & 1u;
+        if ((int)(n & 1u) == g) {
+          ok = __all_sync(0xffffffffu, mbar_wait(b_full + 8 * bb, (run >> 1) & 1u, 60)) &&
+               __all_sync(0xffffffffu, mbar_wait(full + 8 * st, st_phase, 60)) &&
+               __all_sync(0xffffffffu, mbar_wait(s_full + 8 * g, (n >> 1) & 1u, 60));
+          if (!ok) break;
+          tc_fence_after();
+          const float* bias = bias_s + bb * p.c.pitch;
+          if (w.q) {
+            const int k0 = t * 64, pos0 = w.first + w.t * 128 + q * 32, lo = k0 - pos0 - 31, hi = k0 + 63 - pos0;
+            const bool near = hi > -reach && lo < reach;
+            const int lim = mine - k0;
+            const bool mask = __any_sync(0xffffffffu, lim < 64);
+            if (near) {
+              float up[2] = {0.f, 0.f}, down[2] = {0.f, 0.f};   // diagonals `lane` and `lane - 32` of the two blocks
+              auto emit = [&](int c, int e, float ds) {
+                const float v = __shfl_sync(0xffffffffu, ds * weight, (e - lane) & 31);
+                if (lane <= e) up[c] += v;
+                else down[c] += v;
+              };
+              const float* bp = bias + (k0 - (w.first + r) + reach + kPad);
+              if (mask) turn_tile<false, true, true>(ts, bp, 0.f, nullptr, nullptr, lse, dsum, lim, p.c.c2, emit);
+              else turn_tile<false, true, false>(ts, bp, 0.f, nullptr, nullptr, lse, dsum, lim, p.c.c2, emit);
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                add(k0 + 32 * c - pos0 + lane, up[c]);
+                add(k0 + 32 * c - pos0 + lane - 32, down[c]);
+              }
+            } else {
+              float sum = 0.f;
+              auto emit = [&](int, int, float ds) { sum += ds; };
+              const float flat = bias[kPad + (lo >= reach ? 2 * reach : 0)];
+              if (mask) turn_tile<false, false, true>(ts, nullptr, flat, nullptr, nullptr, lse, dsum, lim, p.c.c2, emit);
+              else turn_tile<false, false, false>(ts, nullptr, flat, nullptr, nullptr, lse, dsum, lim, p.c.c2, emit);
+              if (lo >= reach) above += sum * weight;
+              else below += sum * weight;
+            }
+          } else {
+            const int pos0 = w.first + t * 64, lo = w.t * 128 + q * 32 - pos0 - 63, hi = w.t * 128 + q * 32 + 31 - pos0;
+            const bool near = hi > -reach && lo < reach;
+            const int lim = r < w.keys ? (p.c.causal ? r - pos0 : 0) : 64;
+            const bool mask = __any_sync(0xffffffffu, lim > 0);
+            const float* L = reinterpret_cast<const float*>(gen + (ring - sheld) + st * Cfg::kStage + Cfg::kStream);
+            auto emit = [&](int, int, float) {};
+            if (near) {
+              const float* bp = bias + (r - pos0 + reach + kPad);
+              if (mask) turn_tile<true, true, true>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, emit);
+              else turn_tile<true, true, false>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, emit);
+            } else {
+              const float flat = bias[kPad + (lo >= reach ? 2 * reach : 0)];
+              if (mask) turn_tile<true, false, true>(ts, nullptr, flat, L, L + 64, 0.f, 0.f, lim, p.c.c2, emit);
+              else turn_tile<true, false, false>(ts, nullptr, flat, L, L + 64, 0.f, 0.f, lim, p.c.c2, emit);
+            }
+          }
+          attn::tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(pd_full + 8 * g);
+          if (due) {
+            finish(prev, live - 1u);
+            if (!ok) break;
+            due = false;
+          }
+        }
+        if (++st == (uint32_t)p.stages) { st = 0; st_phase ^= 1u; }
+        ++t;
+        if (--left == 0) {
+          t = w.t0;
+          left = w.each;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(b_empty + 8 * bb);
+          ++run;
+        }
+      }
+      if (!ok) break;
+      if (due) {
+        finish(prev, live - 1u);
+        if (!ok) break;
+      }
+      if (w.q) flush(w);
+      prev = w;
+      have = true;
+      ++live;
+    }
+    if (ok && have) finish(prev, live - 1u);
+  }
+  flash::drain_after_error();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
 }  // namespace rel

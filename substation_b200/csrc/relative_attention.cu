@@ -16,10 +16,8 @@ constexpr float kHidden = -8.507059173023462e37f;   // -2^126: entries at or bel
 
 struct Starts { int s[kRelMaxBuckets]; };
 struct AttnArgs {
-  Proj q, k, v, o, g, dq, dk, dv;
+  Proj q, k, v, o, g;
   RelRows lse;
-  float* dsum;              // [H][B][J]
-  float* partial;           // [H][B][row blocks][buckets]
   const sb_half* table;
   long long t_sN, t_sH;
   int n, bidirectional, buckets;
@@ -41,6 +39,9 @@ __device__ __forceinline__ int bucket_of(const AttnArgs& a, const Starts& st, in
 }
 __device__ __forceinline__ const sb_half* row_of(const Proj& v, int h, int b, int r) {
   return reinterpret_cast<const sb_half*>(v.p) + (long long)h * v.sH + (long long)b * v.sB + (long long)r * v.sR;
+}
+__device__ __forceinline__ int first_of(const AttnArgs& a, int b) {
+  return a.first ? max(-(1 << 29), min(1 << 29, a.first[b])) : 0;
 }
 __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
   return a.lengths ? max(0, min(a.K, a.lengths[b])) : a.K;
@@ -84,151 +85,83 @@ pack_rows_kernel(const Proj x, sb_half* dst, int Pp, int along_rows) {
   }
 }
 
-// dq, D and the table's sums: eight query rows of one head and sample per block, one warp each.
+// What the backward pass knows of 64 query rows (RelBackward in ops.h); four threads a row.  `vec`: both tensors have unit-stride
+// features in 16-byte pieces; else lanes run along rows.
 __global__ void __launch_bounds__(256)
-simple_dq_kernel(const AttnArgs a, const Starts st) {
-  extern __shared__ float smem[];
-  float* bins = smem;                                  // [8][buckets]
-  float* qs = bins + 8 * a.buckets;                    // [8][P]
-  float* gs = qs + 8 * kMaxP;                          // [8][P]
+row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, float* records, int* next, int vec) {
+  __shared__ float part[4][64];
   grid_dependency_sync();
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int blocks = (a.J + 7) / 8;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *next = 0;
+  const int blocks = (a.J + 63) / 64;
   const long long all = (long long)a.H * a.B * blocks;
   for (long long it = blockIdx.x; it < all; it += gridDim.x) {
-    const int j = (int)(it % blocks) * 8 + w, b = (int)(it / blocks % a.B), h = (int)(it / blocks / a.B), hk = h / (a.H / a.G);
-    __syncthreads();
-    for (int i = threadIdx.x; i < 8 * a.buckets; i += 256) bins[i] = 0.f;
-    float dsum = 0.f;
-    if (j < a.J)
-      for (int p = lane; p < a.P; p += 32) {
-        qs[w * kMaxP + p] = sb_h2f(row_of(a.q, h, b, j)[p * a.q.sP]);
-        const float g = sb_h2f(row_of(a.g, h, b, j)[p * a.g.sP]);
-        gs[w * kMaxP + p] = g;
-        dsum = fmaf(g, sb_h2f(row_of(a.o, h, b, j)[p * a.o.sP]), dsum);
-      }
-    __syncthreads();
-    dsum = group_sum<32>(dsum);
-    if (j < a.J) {
-      if (lane == 0) a.dsum[((long long)h * a.B + b) * a.J + j] = dsum;
-      const float lse = a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ];
-      const int pos = (a.first ? a.first[b] : 0) + j;
-      int n = keys_of(a, b);
-      if (a.causal) n = max(0, min(n, pos + 1));
-      if (lse == -INFINITY) n = 0;
-      // a row's ds sum to zero, so a row whose keys all share a bucket adds nothing to the table; its sum would be D's rounding
-      const bool mixed = n > 0 && bucket_of(a, st, -pos) != bucket_of(a, st, n - 1 - pos);
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int k0 = 0; k0 < n; k0 += 32) {
-        const int k = k0 + lane;
-        float ds = 0.f;
-        int bucket = 0;
-        if (k < n) {
-          const sb_half* kr = row_of(a.k, hk, b, k);
-          const sb_half* vr = row_of(a.v, hk, b, k);
-          float dot = 0.f, dp = 0.f;
-          for (int p = 0; p < a.P; ++p) {
-            dot = fmaf(qs[w * kMaxP + p], sb_h2f(kr[p * a.k.sP]), dot);
-            dp = fmaf(gs[w * kMaxP + p], sb_h2f(vr[p * a.v.sP]), dp);
-          }
-          bucket = bucket_of(a, st, k - pos);
-          const float bias = sb_h2f(a.table[bucket * a.t_sN + h * a.t_sH]);
-          ds = bias <= kHidden ? 0.f : expf(fmaf(dot, a.scale, bias) - lse) * (dp - dsum);
-        }
-        for (int i = 0; i < min(32, n - k0); ++i) {
-          const float d = __shfl_sync(0xffffffffu, ds, i);
-          const int bk = __shfl_sync(0xffffffffu, bucket, i);
-          const sb_half* kr = row_of(a.k, hk, b, k0 + i);
-          if (lane == 0 && mixed) bins[w * a.buckets + bk] += d;
+    const int j0 = (int)(it % blocks) * 64, h = (int)(it / blocks % a.H), b = (int)(it / blocks / a.H);
+    const int row = vec ? threadIdx.x >> 2 : threadIdx.x & 63, i = vec ? threadIdx.x & 3 : threadIdx.x >> 6;
+    float sum = 0.f;
+    if (j0 + row < a.J) {
+      const sb_half* g = row_of(a.g, h, b, j0 + row);
+      const sb_half* o = row_of(a.o, h, b, j0 + row);
+      if (vec) {
+        for (int p = i * 8; p < a.P; p += 32) {
+          float x[8], y[8];
+          unpack8(*reinterpret_cast<const uint4*>(g + p), x);
+          unpack8(*reinterpret_cast<const uint4*>(o + p), y);
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (c * 32 + lane < a.P) acc[c] = fmaf(d, sb_h2f(kr[(c * 32 + lane) * a.k.sP]), acc[c]);
+          for (int e = 0; e < 8; ++e) sum = fmaf(x[e], y[e], sum);
         }
+      } else {
+        for (int p = i; p < a.P; p += 4) sum = fmaf(sb_h2f(g[p * a.g.sP]), sb_h2f(o[p * a.o.sP]), sum);
       }
-      sb_half* out = const_cast<sb_half*>(row_of(a.dq, h, b, j));
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (c * 32 + lane < a.P) out[(c * 32 + lane) * a.dq.sP] = sb_f2h(acc[c] * a.scale);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < a.buckets; i += 256) {
-      float s = 0.f;
-      for (int x = 0; x < 8; ++x) s += bins[x * a.buckets + i];
-      a.partial[it * a.buckets + i] = s;
+    part[i][row] = sum;
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      const int j = j0 + threadIdx.x;
+      float lse = INFINITY, weight = 0.f;
+      if (j < a.J) {
+        lse = a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] * 1.4426950408889634f;
+        if (lse == -INFINITY) lse = INFINITY;
+        const int pos = first_of(a, b) + j;
+        int n = keys_of(a, b);
+        if (a.causal) n = max(0, min(n, pos + 1));
+        // a row's score gradients sum to zero, so a row whose keys all share a bucket adds nothing to the table: its sum would
+        // only be what D, from the rounded output, is off by
+        if (n > 0 && bucket_of(a, st, -pos) != bucket_of(a, st, n - 1 - pos)) weight = 1.f;
+      }
+      float* r = records + it * 192 + threadIdx.x;
+      r[0] = lse;
+      r[64] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+      r[128] = weight;
     }
   }
 }
 
-// One warp per key row: lanes along queries, then along features.
-__global__ void __launch_bounds__(256)
-simple_dkv_kernel(const AttnArgs a, const Starts st) {
-  __shared__ float ks[8][kMaxP], vs[8][kMaxP];
+// dtable[n,h] = the head's sums over the relative positions of bucket n; one block each, in a fixed order.
+__global__ void __launch_bounds__(128)
+table_finish_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const float* partial, int rows, int reach,
+                    sb_half* out, long long sN, long long sH) {
+  __shared__ float part[4];
   grid_dependency_sync();
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.H / a.G;
-  const long long rows = (long long)a.G * a.B * a.K;
-  for (long long r = (long long)blockIdx.x * 8 + w; r < rows; r += (long long)gridDim.x * 8) {
-    const int k = (int)(r % a.K), b = (int)(r / a.K % a.B), hk = (int)(r / a.K / a.B);
-    float dk[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
-    if (k < keys_of(a, b)) {
-      __syncwarp();
-      for (int p = lane; p < a.P; p += 32) {
-        ks[w][p] = sb_h2f(row_of(a.k, hk, b, k)[p * a.k.sP]);
-        vs[w][p] = sb_h2f(row_of(a.v, hk, b, k)[p * a.v.sP]);
-      }
-      __syncwarp();
-      const int first = a.first ? a.first[b] : 0;
-      for (int h = hk * group; h < (hk + 1) * group; ++h)
-        for (int j0 = 0; j0 < a.J; j0 += 32) {
-          const int j = j0 + lane;
-          float pr = 0.f, ds = 0.f;
-          if (j < a.J && !(a.causal && k > first + j)) {
-            const sb_half* qr = row_of(a.q, h, b, j);
-            const sb_half* gr = row_of(a.g, h, b, j);
-            float dot = 0.f, dp = 0.f;
-            for (int p = 0; p < a.P; ++p) {
-              dot = fmaf(ks[w][p], sb_h2f(qr[p * a.q.sP]), dot);
-              dp = fmaf(vs[w][p], sb_h2f(gr[p * a.g.sP]), dp);
-            }
-            const float bias = sb_h2f(a.table[bucket_of(a, st, k - first - j) * a.t_sN + h * a.t_sH]);
-            const float lse = a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ];
-            pr = bias <= kHidden || lse == -INFINITY ? 0.f : expf(fmaf(dot, a.scale, bias) - lse);
-            ds = pr * (dp - a.dsum[((long long)h * a.B + b) * a.J + j]);
-          }
-          for (int i = 0; i < min(32, a.J - j0); ++i) {
-            const float x = __shfl_sync(0xffffffffu, pr, i), d = __shfl_sync(0xffffffffu, ds, i);
-            const sb_half* qr = row_of(a.q, h, b, j0 + i);
-            const sb_half* gr = row_of(a.g, h, b, j0 + i);
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (c * 32 + lane < a.P) {
-                dv[c] = fmaf(x, sb_h2f(gr[(c * 32 + lane) * a.g.sP]), dv[c]);
-                dk[c] = fmaf(d, sb_h2f(qr[(c * 32 + lane) * a.q.sP]), dk[c]);
-              }
-          }
-        }
-    }
-    sb_half* ok = const_cast<sb_half*>(row_of(a.dk, hk, b, k));
-    sb_half* ov = const_cast<sb_half*>(row_of(a.dv, hk, b, k));
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (c * 32 + lane < a.P) {
-        ok[(c * 32 + lane) * a.dk.sP] = sb_f2h(dk[c] * a.scale);
-        ov[(c * 32 + lane) * a.dv.sP] = sb_f2h(dv[c]);
-      }
-  }
-}
-
-// dtable[n,h] = sum of the head's partial rows, one warp each in a fixed order.
-__global__ void __launch_bounds__(256)
-table_finish_kernel(const float* partial, int rows, int buckets, int H, sb_half* out, long long sN, long long sH) {
-  grid_dependency_sync();
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (i >= buckets * H) return;
-  const int h = i / buckets, n = i % buckets;
+  const int n = blockIdx.x, h = blockIdx.y, entries = 2 * reach + 1;
+  const bool behind = n >= a.n;
+  const int i = behind ? n - a.n : n;
+  // distances [lo, hi]; without `bidirectional` every key behind the query has distance 0
+  int lo = st.s[i], hi = i + 1 < a.n ? st.s[i + 1] - 1 : reach;
+  if (behind) lo = max(lo, 1);
+  hi = min(hi, reach);
+  int from = behind ? reach + lo : reach - hi, to = behind ? reach + hi : reach - lo;
+  if (!a.bidirectional && lo == 0 && hi >= 0) to = 2 * reach;
+  const int run = max(0, to - from + 1);
+  const float* base = partial + (long long)h * rows * entries + from;
+  const long long all = (long long)rows * run;
   float s = 0.f;
-  for (int r = lane; r < rows; r += 32) s += partial[((long long)h * rows + r) * buckets + n];
+#pragma unroll 4
+  for (long long e = threadIdx.x; e < all; e += 128) s += base[e / run * entries + e % run];
   s = group_sum<32>(s);
-  if (lane == 0) out[n * sN + h * sH] = sb_f2h(s);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) out[n * sN + h * sH] = sb_f2h((part[0] + part[1]) + (part[2] + part[3]));
 }
 
 AttnArgs attn_args(const Proj& q, const Proj& k, const Proj& v, const RelBias& bias, const Proj& out, const RelRows& lse, const RelSpan& span,
@@ -245,8 +178,6 @@ AttnArgs attn_args(const Proj& q, const Proj& k, const Proj& v, const RelBias& b
   for (int i = 0; i < bias.n; ++i) st->s[i] = bias.starts[i];
   return a;
 }
-size_t dsum_bytes(const Proj& q) { return (sizeof(float) * (size_t)q.H * q.B * q.R + 255) / 256 * 256; }
-
 // Scratch: rows of biases, then a packed copy of each operand that tensor maps cannot address.
 struct Plan { int pitch, reach; size_t at[4], bytes; };
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
@@ -298,22 +229,49 @@ int launch_rel_attn_fwd(cudaStream_t s, void* scratch, Proj q, Proj k, Proj v, c
   return launch_rel_tiles_fwd(s, q, k, v, t, out, lse, span);
 }
 
-size_t rel_attn_bwd_scratch_bytes(const Proj&, const Proj& q, const Proj&, const Proj&, const RelBias& bias) {
-  return dsum_bytes(q) + sizeof(float) * (size_t)q.H * q.B * ((q.R + 7) / 8) * (bias.bidirectional ? 2 : 1) * bias.n;
+namespace {
+// and for the backward pass records, sums and the queue's counter
+struct BwdPlan { Plan p; size_t records, partial, next, bytes; int rows; };
+BwdPlan bwd_plan(const Proj& dout, const Proj& q, const Proj& k, const Proj& v, const RelBias& bias) {
+  BwdPlan b;
+  b.p = plan_of({&dout, &q, &k, &v}, q.H, bias);
+  b.rows = q.B * ((q.R + 127) / 128) * 2;
+  b.records = b.p.bytes;
+  b.partial = b.records + align256(sizeof(float) * 192 * (size_t)q.H * q.B * ((q.R + 63) / 64));
+  b.next = b.partial + align256(sizeof(float) * (size_t)q.H * b.rows * (2 * b.p.reach + 1));
+  b.bytes = b.next + 256;
+  return b;
+}
+}  // namespace
+
+size_t rel_attn_bwd_scratch_bytes(const Proj& dout, const Proj& q, const Proj& k, const Proj& v, const RelBias& bias) {
+  return bwd_plan(dout, q, k, v, bias).bytes;
 }
 
 int launch_rel_attn_bwd(cudaStream_t s, void* scratch, Proj dout, Proj q, Proj k, Proj v, const RelBias& bias, Proj out, RelRows lse,
                         Proj dq, Proj dk, Proj dv, void* dtable, long long dt_sN, long long dt_sH, const RelSpan& span) {
   Starts st;
   AttnArgs a = attn_args(q, k, v, bias, out, lse, span, &st);
-  a.g = dout; a.dq = dq; a.dk = dk; a.dv = dv;
-  a.dsum = reinterpret_cast<float*>(scratch);
-  a.partial = reinterpret_cast<float*>(reinterpret_cast<char*>(scratch) + dsum_bytes(q));
-  const int blocks = (a.J + 7) / 8;
-  const size_t smem = sizeof(float) * (8 * a.buckets + 16 * kMaxP);
-  SB_LAUNCH_OK(launch_k(simple_dq_kernel, (unsigned)std::min<long long>((long long)a.H * a.B * blocks, 1184), 256, smem, s, a, st));
-  SB_LAUNCH_OK(launch_k(simple_dkv_kernel, (unsigned)std::min<long long>(((long long)a.G * a.B * a.K + 7) / 8, 1184), 256, 0, s, a, st));
-  SB_LAUNCH_OK(launch_k(table_finish_kernel, (unsigned)((a.buckets * a.H + 7) / 8), 256, 0, s, a.partial, a.B * blocks, a.buckets, a.H,
+  a.g = dout;
+  const BwdPlan pl = bwd_plan(dout, q, k, v, bias);
+  char* base = reinterpret_cast<char*>(scratch);
+  RelTables t;
+  SB_TRY(expand_bias(s, a, st, scratch, pl.p, &t));
+  auto pieces = [](const Proj& x) {
+    return x.sP == 1 && x.P % 8 == 0 && !((x.sH | x.sB | x.sR) & 7) && !(reinterpret_cast<uintptr_t>(x.p) & 15u);
+  };
+  float* records = reinterpret_cast<float*>(base + pl.records);
+  int* next = reinterpret_cast<int*>(base + pl.next);
+  const long long blocks = (long long)a.H * a.B * ((a.J + 63) / 64);
+  SB_LAUNCH_OK(launch_k(row_records_kernel, (unsigned)std::min<long long>(blocks, 8 * usable_sms(device_facts().sms)), 256, 0, s, a, st, records,
+                        next, pieces(dout) && pieces(out) ? 1 : 0));
+  SB_TRY(direct_or_packed(s, scratch, pl.p.at[0], &dout));
+  SB_TRY(direct_or_packed(s, scratch, pl.p.at[1], &q));
+  SB_TRY(direct_or_packed(s, scratch, pl.p.at[2], &k));
+  SB_TRY(direct_or_packed(s, scratch, pl.p.at[3], &v));
+  float* partial = reinterpret_cast<float*>(base + pl.partial);
+  SB_TRY(launch_rel_tiles_bwd(s, dout, q, k, v, t, RelBackward{records, partial, next}, dq, dk, dv, span));
+  SB_LAUNCH_OK(launch_k(table_finish_kernel, dim3(a.buckets, a.H), 128, 0, s, a, st, partial, pl.rows, pl.p.reach,
                         reinterpret_cast<sb_half*>(dtable), dt_sN, dt_sH));
   return SB_OK;
 }
