@@ -85,6 +85,305 @@ pack_rows_kernel(const Proj x, sb_half* dst, int Pp, int along_rows) {
   }
 }
 
+// ---- few queries ------------------------------------------------------------------------------------------------
+// The rows of a key head are the queries of all heads that share it, J for each.  A CTA takes 16 of them (one mma.sync tile) and a
+// share of the keys; its four warps walk pieces of those keys in turn, each with a ring of its own filled by cp.async (which
+// also puts zeros behind a sequence's end), softmax state and accumulator, joined at the end.  With more than one share, a
+// second kernel joins those.  Bound by reading keys and values once: tcgen05's smallest tile would be 64 or 128 rows for the
+// one to 16 there are, and the matrix work here is a few percent of the time.
+constexpr int kFewThreads = 128;
+template <int P>
+struct FewCfg {
+  static constexpr int kKeys = P == 64 ? 32 : 16;    // of a piece
+  static constexpr int kStages = 3;
+  static constexpr int kHalf = kKeys * P * 2;        // bytes of a piece's keys
+  static constexpr int kWarp = kStages * 2 * kHalf;
+  static constexpr int kSmem = 4 * kWarp;
+  static_assert(4 * (16 * P + 32) * 4 <= kSmem, "results of the warps in the rings' place");
+};
+struct FewParams {
+  AttnArgs a;
+  int rows, blocks, splits, reach;                   // rows of a key head, blocks of 16 of them
+  float* partial;                                    // [B][G][rows][splits][P + 2]: output, reference, sum; null with one share
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+#ifdef SB_BF16
+#define SB_MMA_TYPES "f32.bf16.bf16.f32"
+#else
+#define SB_MMA_TYPES "f32.f16.f16.f32"
+#endif
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col." SB_MMA_TYPES " {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_pair(float x, float y) {
+  const sb_half2 h = sb_f2h2(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int P>
+__global__ void __launch_bounds__(kFewThreads)
+few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ Starts st) {
+  using Cfg = FewCfg<P>;
+  constexpr int kKeys = Cfg::kKeys, kStages = Cfg::kStages, kSteps = P / 16, kTiles = kKeys / 8;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int starts[kRelMaxBuckets];
+  const AttnArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_dependency_sync();
+  const int split = blockIdx.x % p.splits, block = blockIdx.x / p.splits % p.blocks, unit = blockIdx.x / p.splits / p.blocks;
+  const int hk = unit % a.G, b = unit / a.G, rep = a.H / a.G;
+  const int first = first_of(a, b);
+  // keys that some row of the sample sees, and this CTA's share of them
+  int keys = keys_of(a, b);
+  if (a.causal) keys = max(0, min(keys, first + a.J));
+  const int share = ((keys + p.splits - 1) / p.splits + 31) & ~31;
+  const int k_from = min(keys, split * share), k_to = min(keys, k_from + share);
+  const int pieces = (k_to - k_from + kKeys - 1) / kKeys, mine = pieces > warp ? (pieces - warp + 3) >> 2 : 0;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * Cfg::kWarp;
+  const sb_half* kp = row_of(a.k, hk, b, 0);
+  const sb_half* vp = row_of(a.v, hk, b, 0);
+
+  // piece i of this warp into its slot: 16-byte chunk c of row r at c ^ (r & 7)
+  auto fetch = [&](int i) {
+    if (i < mine) {
+      const int k0 = k_from + (warp + 4 * i) * kKeys;
+      const uint32_t slot = ring + (i % kStages) * 2 * Cfg::kHalf;
+#pragma unroll
+      for (int x = lane; x < kKeys * (P / 8); x += 32) {
+        const int r = x / (P / 8), c = x % (P / 8), k = min(k0 + r, a.K - 1);
+        const int bytes = k0 + r < k_to ? max(0, min(16, (a.P - c * 8) * 2)) : 0;
+        const int from = bytes > 0 ? c * 8 : 0;
+        const uint32_t d = slot + r * (P * 2) + ((c ^ (r & 7)) << 4);
+        cp_async16(d, kp + (long long)k * a.k.sR + from, bytes);
+        cp_async16(d + Cfg::kHalf, vp + (long long)k * a.v.sR + from, bytes);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(i);
+  for (int i = threadIdx.x; i < a.n; i += kFewThreads) starts[i] = st.s[i];
+
+  // this lane's two rows: queries as operands, positions, biases outside the varying part
+  const int r0 = block * 16 + (lane >> 2);
+  uint32_t qf[kSteps][4];
+  int pos[2], head[2];
+  float lo[2], hi[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int r = r0 + 8 * x, rc = min(r, p.rows - 1), j = rc % a.J;
+    head[x] = hk * rep + rc / a.J;
+    pos[x] = first + j;
+    const sb_half* q = row_of(a.q, head[x], b, j);
+    const int f = (lane & 3) * 2;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int e = s * 16 + y * 8 + f;
+        float u = 0.f, v = 0.f;
+        if (r < p.rows && e < a.P) u = sb_h2f(q[e * a.q.sP]);
+        if (r < p.rows && e + 1 < a.P) v = sb_h2f(q[(e + 1) * a.q.sP]);
+        qf[s][y * 2 + x] = pack_pair(u, v);
+      }
+  }
+  __syncthreads();
+  auto bias_at = [&](int rel, int h) {
+    const int d = rel > 0 ? (a.bidirectional ? rel : 0) : -rel;
+    int l = 0, u = a.n - 1;
+    while (l < u) {
+      const int mid = (l + u + 1) >> 1;
+      if (starts[mid] <= d) l = mid; else u = mid - 1;
+    }
+    const float v = sb_h2f(a.table[(l + (a.bidirectional && rel > 0 ? a.n : 0)) * a.t_sN + h * a.t_sH]);
+    return v <= kHidden ? -INFINITY : v * 1.4426950408889634f;
+  };
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    lo[x] = bias_at(-p.reach, head[x]);
+    hi[x] = bias_at(p.reach, head[x]);
+  }
+  const float c2 = a.scale * 1.4426950408889634f;
+  float o[P / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < P / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+  const int pos_lo = first, pos_hi = first + a.J - 1;
+
+  for (int i = 0; i < mine; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    __syncwarp();
+    fetch(i + kStages - 1);
+    const int k0 = k_from + (warp + 4 * i) * kKeys;
+    const uint32_t ks = ring + (i % kStages) * 2 * Cfg::kHalf, vs = ks + Cfg::kHalf;
+    float s[kTiles][4];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
+#pragma unroll
+    for (int t = 0; t < kTiles; t += 2)
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        uint32_t f[4];
+        const int r = t * 8 + (lane & 7) + ((lane >> 4) << 3), ch = c * 2 + ((lane >> 3) & 1);
+        ldsm4(ks + r * (P * 2) + ((ch ^ (r & 7)) << 4), f);
+        mma16816(s[t], qf[c], f[0], f[1]);
+        mma16816(s[t + 1], qf[c], f[2], f[3]);
+      }
+    // biases, what is hidden, maxima
+    const bool near = k0 + kKeys - 1 - pos_lo > -p.reach && k0 - pos_hi < p.reach;
+    const bool after = k0 - pos_hi >= p.reach;
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int x = e >> 1, k = k0 + t * 8 + (lane & 3) * 2 + (e & 1);
+        const float bias = near ? bias_at(k - pos[x], head[x]) : after ? hi[x] : lo[x];
+        const bool seen = k < k_to && !(a.causal && k > pos[x]);
+        s[t][e] = seen ? fmaf(s[t][e], c2, bias) : -INFINITY;
+        mx[x] = fmaxf(mx[x], s[t][e]);
+      }
+    bool raise = false;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
+      mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
+      raise |= mx[x] > m[x];
+    }
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float now = fmaxf(m[x], mx[x]), f = now == -INFINITY ? 1.f : ex2_unit(m[x] - now);
+        m[x] = now;
+        l[x] *= f;
+#pragma unroll
+        for (int t = 0; t < P / 8; ++t) {
+          o[t][2 * x] *= f;
+          o[t][2 * x + 1] *= f;
+        }
+      }
+    }
+    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[t][e] = ex2_unit(s[t][e] - ref[e >> 1]);
+        l[e >> 1] += s[t][e];
+      }
+#pragma unroll
+    for (int c = 0; c < kKeys / 16; ++c) {
+      const uint32_t pf[4] = {pack_pair(s[2 * c][0], s[2 * c][1]), pack_pair(s[2 * c][2], s[2 * c][3]),
+                              pack_pair(s[2 * c + 1][0], s[2 * c + 1][1]), pack_pair(s[2 * c + 1][2], s[2 * c + 1][3])};
+#pragma unroll
+      for (int t = 0; t < P / 8; t += 2) {
+        uint32_t f[4];
+        const int r = c * 16 + (lane & 15), ch = t + (lane >> 4);
+        ldsm4_t(vs + r * (P * 2) + ((ch ^ (r & 7)) << 4), f);
+        mma16816(o[t], pf, f[0], f[1]);
+        mma16816(o[t + 1], pf, f[2], f[3]);
+      }
+    }
+    __syncwarp();
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  // the warps' results side by side: output [4][16][P], then references and sums [4][16]
+  float* so = reinterpret_cast<float*>(smem);
+  float* sm = so + 4 * 16 * P;
+  float* sl = sm + 64;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+    const int r = (lane >> 2) + 8 * x;
+    if ((lane & 3) == 0) {
+      sm[warp * 16 + r] = m[x];
+      sl[warp * 16 + r] = l[x];
+    }
+#pragma unroll
+    for (int t = 0; t < P / 8; ++t)
+      *reinterpret_cast<float2*>(so + (warp * 16 + r) * P + t * 8 + (lane & 3) * 2) = make_float2(o[t][2 * x], o[t][2 * x + 1]);
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < 16 * P; x += kFewThreads) {
+    const int r = x / P, f = x % P, row = block * 16 + r;
+    if (row >= p.rows) break;
+    float mm = sm[r];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) mm = fmaxf(mm, sm[w * 16 + r]);
+    float sum = 0.f, v = 0.f;
+    if (mm > -INFINITY) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float e = ex2_unit(sm[w * 16 + r] - mm);
+        sum = fmaf(sl[w * 16 + r], e, sum);
+        v = fmaf(so[(w * 16 + r) * P + f], e, v);
+      }
+    }
+    const int h = hk * rep + row / a.J, j = row % a.J;
+    if (p.partial) {
+      float* d = p.partial + (((long long)unit * p.rows + row) * p.splits + split) * (P + 2);
+      d[f] = v;
+      if (f == 0) {
+        d[P] = mm;
+        d[P + 1] = sum;
+      }
+    } else {
+      if (f < a.P) const_cast<sb_half*>(row_of(a.o, h, b, j))[f * a.o.sP] = sb_f2h(sum > 0.f ? v / sum : 0.f);
+      if (f == 0 && a.lse.p) a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] = sum > 0.f ? (mm + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    }
+  }
+}
+
+// One warp per row joins its shares.
+template <int P>
+__global__ void __launch_bounds__(128)
+join_splits_kernel(const __grid_constant__ FewParams p) {
+  grid_dependency_sync();
+  const AttnArgs& a = p.a;
+  const long long it = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (it >= (long long)a.B * a.G * p.rows) return;
+  const int row = (int)(it % p.rows), unit = (int)(it / p.rows), hk = unit % a.G, b = unit / a.G;
+  const int h = hk * (a.H / a.G) + row / a.J, j = row % a.J;
+  const float* src = p.partial + it * p.splits * (P + 2);
+  float mm = -INFINITY;
+  for (int s = lane; s < p.splits; s += 32) mm = fmaxf(mm, src[s * (P + 2) + P]);
+  mm = group_max<32>(mm);
+  float sum = 0.f, v[P / 32];
+#pragma unroll
+  for (int c = 0; c < P / 32; ++c) v[c] = 0.f;
+  if (mm > -INFINITY)
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+      const float* d = src + s * (P + 2);
+      const float e = ex2_unit(d[P] - mm);
+      sum = fmaf(d[P + 1], e, sum);
+#pragma unroll
+      for (int c = 0; c < P / 32; ++c) v[c] = fmaf(d[c * 32 + lane], e, v[c]);
+    }
+  sb_half* out = const_cast<sb_half*>(row_of(a.o, h, b, j));
+#pragma unroll
+  for (int c = 0; c < P / 32; ++c)
+    if (c * 32 + lane < a.P) out[(c * 32 + lane) * a.o.sP] = sb_f2h(sum > 0.f ? v[c] / sum : 0.f);
+  if (lane == 0 && a.lse.p) a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] = sum > 0.f ? (mm + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+}
+
 // What the backward pass knows of 64 query rows (RelBackward in ops.h); four threads a row.  `vec`: both tensors have unit-stride
 // features in 16-byte pieces; else lanes run along rows.
 __global__ void __launch_bounds__(256)
@@ -194,9 +493,8 @@ Plan plan_of(std::initializer_list<const Proj*> operands, int heads, const RelBi
   }
   return p;
 }
-// x as tensor maps can address it: itself, or the copy at `at`.
-int direct_or_packed(cudaStream_t s, void* scratch, size_t at, Proj* x) {
-  if (rel_direct(*x)) return SB_OK;
+// x becomes the copy at `at`.
+int pack(cudaStream_t s, void* scratch, size_t at, Proj* x) {
   const int Pp = (x->P + 7) / 8 * 8;
   auto mag = [](long long v) { return v < 0 ? -v : v; };
   sb_half* dst = reinterpret_cast<sb_half*>(reinterpret_cast<char*>(scratch) + at);
@@ -207,6 +505,7 @@ int direct_or_packed(cudaStream_t s, void* scratch, size_t at, Proj* x) {
   x->sP = 1; x->sR = Pp; x->sH = (long long)Pp * x->R; x->sB = x->sH * x->H;
   return SB_OK;
 }
+int direct_or_packed(cudaStream_t s, void* scratch, size_t at, Proj* x) { return rel_direct(*x) ? SB_OK : pack(s, scratch, at, x); }
 int expand_bias(cudaStream_t s, const AttnArgs& a, const Starts& st, void* scratch, const Plan& pl, RelTables* t) {
   t->rows = reinterpret_cast<float*>(scratch); t->pitch = pl.pitch; t->reach = pl.reach;
   SB_LAUNCH_OK(launch_k(expand_bias_kernel, dim3((pl.pitch + 255) / 256, a.H), 256, 0, s, a, st, reinterpret_cast<float*>(scratch), pl.pitch, pl.reach));
@@ -215,11 +514,67 @@ int expand_bias(cudaStream_t s, const AttnArgs& a, const Starts& st, void* scrat
 
 }  // namespace
 
-size_t rel_attn_scratch_bytes(const Proj& q, const Proj& k, const Proj& v, const RelBias& bias) { return plan_of({&q, &k, &v}, q.H, bias).bytes; }
+namespace {
+
+// Rows in 16-byte pieces, any strides between them.
+bool piecewise(const Proj& x) {
+  auto ok = [](long long n, long long stride) { return n == 1 || stride % 8 == 0; };
+  return (x.sP == 1 || x.P == 1) && !(reinterpret_cast<uintptr_t>(x.p) & 15u) && ok(x.H, x.sH) && ok(x.B, x.sB) && ok(x.R, x.sR);
+}
+
+// The forward pass with few queries: how many shares the keys are cut into, 0 when the tile kernel is to run.
+int few_splits(const Proj& q, const Proj& k) {
+  const long long rows = (long long)(q.H / k.H) * q.R;
+  if (rows > 64) return 0;
+  const long long ctas = (long long)k.B * k.H * ((rows + 15) / 16);
+  // about four CTAs for each of 148 SMs, at least 256 keys a share
+  return (int)std::max<long long>(1, std::min<long long>({(592 + ctas - 1) / ctas, (k.R + 255) / 256, 64}));
+}
+struct FewPlan { int splits; size_t k, v, bytes; };
+FewPlan few_plan(const Proj& q, const Proj& k, const Proj& v) {
+  FewPlan f;
+  f.splits = few_splits(q, k);
+  f.bytes = f.splits > 1 ? align256(sizeof(float) * (size_t)q.H * q.B * q.R * f.splits * ((q.P <= 64 ? 64 : 128) + 2)) : 0;
+  f.k = f.bytes;
+  if (!piecewise(k)) f.bytes += packed_bytes(k);
+  f.v = f.bytes;
+  if (!piecewise(v)) f.bytes += packed_bytes(v);
+  return f;
+}
+
+template <int P>
+int launch_few(cudaStream_t s, const FewParams& p, const Starts& st) {
+  SB_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(few_queries_kernel<P>), FewCfg<P>::kSmem));
+  const long long units = (long long)p.a.B * p.a.G;
+  SB_LAUNCH_OK(launch_k(few_queries_kernel<P>, (unsigned)(units * p.blocks * p.splits), kFewThreads, FewCfg<P>::kSmem, s, p, st));
+  if (p.splits > 1)
+    SB_LAUNCH_OK(launch_k(join_splits_kernel<P>, (unsigned)((units * p.rows + 3) / 4), 128, 0, s, p));
+  return SB_OK;
+}
+
+}  // namespace
+
+size_t rel_attn_scratch_bytes(const Proj& q, const Proj& k, const Proj& v, const RelBias& bias) {
+  return few_splits(q, k) ? few_plan(q, k, v).bytes : plan_of({&q, &k, &v}, q.H, bias).bytes;
+}
 
 int launch_rel_attn_fwd(cudaStream_t s, void* scratch, Proj q, Proj k, Proj v, const RelBias& bias, Proj out, RelRows lse, const RelSpan& span) {
   Starts st;
-  const AttnArgs a = attn_args(q, k, v, bias, out, lse, span, &st);
+  AttnArgs a = attn_args(q, k, v, bias, out, lse, span, &st);
+  if (few_splits(q, k)) {
+    const FewPlan f = few_plan(q, k, v);
+    if (!piecewise(k)) SB_TRY(pack(s, scratch, f.k, &k));
+    if (!piecewise(v)) SB_TRY(pack(s, scratch, f.v, &v));
+    FewParams p;
+    a.k = k; a.v = v;
+    p.a = a;
+    p.rows = (q.H / k.H) * q.R;
+    p.blocks = (p.rows + 15) / 16;
+    p.splits = f.splits;
+    p.reach = std::max(1, bias.starts[bias.n - 1]);
+    p.partial = f.splits > 1 ? reinterpret_cast<float*>(scratch) : nullptr;
+    return q.P <= 64 ? launch_few<64>(s, p, st) : launch_few<128>(s, p, st);
+  }
   const Plan pl = plan_of({&q, &k, &v}, q.H, bias);
   RelTables t;
   SB_TRY(expand_bias(s, a, st, scratch, pl, &t));
