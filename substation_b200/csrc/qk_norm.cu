@@ -10,9 +10,8 @@ namespace sb {
 
 namespace {
 
-constexpr int kTokens = 32;            // tokens of a block of the tile kernels
 constexpr int kMaxPairs = kNormMaxHead / 2;
-constexpr int kMaxPartials = 1184;     // rows of partial sums of the gains' gradients: eight blocks of 148 SMs
+constexpr int kMaxPartials = 1184;     // rows of partial sums of a gain's gradient: eight blocks of 148 SMs
 
 // Turns per position of pair i: base^(-2i/rotary) / (2 pi).  Angles are counted in turns and reduced to a fraction of one in
 // 64 bits: a position of 2^31 then still has 22 bits behind the binary point.
@@ -23,9 +22,10 @@ struct NormArgs {
   const sb_half* gain[2];
   const int* pos;
   long long pos_sB, pos_sJ;
-  float* partial;                      // backward: [blocks of tokens][2][P]
+  float* partial[2];                   // backward: a row of P sums per block for the gain's gradient
   int J, tokens, P, rotary, pairing;
-  int vary_tokens[2][3];               // the tile kernels' lanes run along tokens (x, g, y)
+  int tile, tiles;                     // tokens of a tile, tiles
+  int blocks[2], chunk;                // blocks of queries and of keys; lanes-along-tokens kernel: heads of a block
   float eps;
 };
 
@@ -35,159 +35,286 @@ __device__ __forceinline__ float2 cos_sin(int pos, double turns_per_position) {
   sincospif(2.f * (float)(t - rint(t)), &s, &c);
   return make_float2(c, s);
 }
-
-__device__ __forceinline__ long long row_offset(const Proj& v, int token, int J, int h) {
-  return (long long)(token / J) * v.sB + (long long)(token % J) * v.sR + (long long)h * v.sH;
+__device__ __forceinline__ int position(const NormArgs& a, int token) {
+  return a.pos[(long long)(token / a.J) * a.pos_sB + (long long)(token % a.J) * a.pos_sJ];
+}
+__device__ __forceinline__ long long token_offset(const Proj& v, int token, int J) {
+  return (long long)(token / J) * v.sB + (long long)(token % J) * v.sR;
 }
 
-// tile[t][p] = v[p, h, tokens t0 ...], lanes along tokens or along features, whichever is nearer in memory
-__device__ __forceinline__ void load_rows(float* tile, int pitch, const Proj& v, const NormArgs& a, int t0, int h, bool along_tokens) {
-  const sb_half* base = reinterpret_cast<const sb_half*>(v.p);
-  const int n = min(kTokens, a.tokens - t0);
-  if (along_tokens) {
-    const int t = threadIdx.x & 31;
-    if (t < n) {
-      const long long o = row_offset(v, t0 + t, a.J, h);
-      for (int p = threadIdx.x >> 5; p < a.P; p += 8) tile[t * pitch + p] = sb_h2f(base[o + (long long)p * v.sP]);
-    }
-  } else {
-    for (int t = threadIdx.x >> 5; t < n; t += 8) {
-      const long long o = row_offset(v, t0 + t, a.J, h);
-      for (int p = threadIdx.x & 31; p < a.P; p += 32) tile[t * pitch + p] = sb_h2f(base[o + (long long)p * v.sP]);
-    }
-  }
-}
-__device__ __forceinline__ void store_rows(const float* tile, int pitch, const Proj& v, const NormArgs& a, int t0, int h, bool along_tokens) {
-  sb_half* base = reinterpret_cast<sb_half*>(v.p);
-  const int n = min(kTokens, a.tokens - t0);
-  if (along_tokens) {
-    const int t = threadIdx.x & 31;
-    if (t < n) {
-      const long long o = row_offset(v, t0 + t, a.J, h);
-      for (int p = threadIdx.x >> 5; p < a.P; p += 8) base[o + (long long)p * v.sP] = sb_f2h(tile[t * pitch + p]);
-    }
-  } else {
-    for (int t = threadIdx.x >> 5; t < n; t += 8) {
-      const long long o = row_offset(v, t0 + t, a.J, h);
-      for (int p = threadIdx.x & 31; p < a.P; p += 32) base[o + (long long)p * v.sP] = sb_f2h(tile[t * pitch + p]);
-    }
-  }
-}
-
-// Any strides, any head size: a block takes 32 tokens, keeps their angles in shared memory and walks the heads; eight threads
-// a row.  Forward and backward (BWD), queries and keys one after the other.
-template <bool BWD>
-__global__ void __launch_bounds__(256)
-norm_tile_kernel(const NormArgs a, const Turns turns) {
-  extern __shared__ float smem[];
-  const int pairs = a.rotary / 2, pitch = a.P | 1;
-  float* tx = smem;                                 // [kTokens][pitch]
-  float* tg = tx + kTokens * pitch;                 // the same, backward only
-  float2* cs = reinterpret_cast<float2*>(smem + (((BWD ? 2 : 1) * kTokens * pitch + 1) & ~1));
+// Unit-stride features in 16-byte pieces.  A row belongs to LANES threads with two pieces each, so chosen that both members of
+// every pair are in one thread: a row's norm is a few shuffles and its rotation none.  A block takes a tile of tokens, puts
+// their angles into shared memory once, and its groups of threads walk the query (or key) heads of a token each.  In the backward pass
+// sum x^2 and sum g gain x are all that a row needs from its other threads; the gains' gradients stay in registers until the
+// block's last tile.
+template <int LANES, bool BWD, bool HALVES>
+__global__ void __launch_bounds__(256, 2)
+norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Turns turns) {
+  constexpr int kGroups = 256 / LANES, kRows = BWD ? 2 : 4;   // rows in flight
+  extern __shared__ float2 cs[];                              // [tile][rotary / 2]; at the end the warps' sums
   grid_dependency_sync();
-  const int part = threadIdx.x & 7, t = threadIdx.x >> 3;
+  const int pairs = a.rotary / 2, turned = a.rotary / 16, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const uint32_t members = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
+  const bool on = lane < a.P / 16, rotates = lane < turned;
+  const int f0 = rotates ? 8 * lane : a.rotary + 16 * (lane - turned), f1 = rotates ? f0 + pairs : f0 + 8;
+  const int across = kGroups / a.tile, tok = group / across, first_head = group % across;
   const float inv = 1.f / (float)a.P;
-  for (int which = 0; which < 2; ++which)
-    if (BWD && a.x[which].H > 0)
-      for (int p = threadIdx.x; p < a.P; p += 256) a.partial[((long long)blockIdx.x * 2 + which) * a.P + p] = 0.f;
-  for (int t0 = blockIdx.x * kTokens; t0 < a.tokens; t0 += gridDim.x * kTokens) {
+  const int w = (int)blockIdx.x < a.blocks[0] ? 0 : 1, mine = (int)blockIdx.x - (w ? a.blocks[0] : 0);
+  const Proj &vx = a.x[w], &vg = a.g[w], &vy = a.y[w];
+  uint4 gain[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    sb_half* h = reinterpret_cast<sb_half*>(&gain[x]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = on ? a.gain[w][(x ? f1 : f0) + e] : sb_f2h(0.f);
+  }
+  float sum[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sum[e] = 0.f;
+  for (int t = mine; t < a.tiles; t += a.blocks[w]) {
+    const int t0 = t * a.tile, token = t0 + tok;
     __syncthreads();
-    for (int i = threadIdx.x; i < kTokens * pairs; i += 256) {
-      const int tt = t0 + i / pairs;
-      cs[i] = tt < a.tokens ? cos_sin(a.pos[(long long)(tt / a.J) * a.pos_sB + (long long)(tt % a.J) * a.pos_sJ], turns.t[i % pairs])
-                            : make_float2(1.f, 0.f);
-    }
-    for (int which = 0; which < 2; ++which) {
-      const Proj& vx = a.x[which];
-      for (int h = 0; h < vx.H; ++h) {
-        __syncthreads();
-        load_rows(tx, pitch, vx, a, t0, h, a.vary_tokens[which][0]);
-        if (BWD) load_rows(tg, pitch, a.g[which], a, t0, h, a.vary_tokens[which][1]);
-        __syncthreads();
-        const bool row = t0 + t < a.tokens;
-        float* x = tx + t * pitch;
-        float* g = tg + t * pitch;
-        float sum = 0.f;
-        if (row)
-          for (int p = part; p < a.P; p += 8) sum = fmaf(x[p], x[p], sum);
-        const float r = rsqrtf(group_sum<8>(sum) * inv + a.eps);
-        auto pair = [&](int i, int* p, int* q) {
-          if (a.pairing == SB_PAIR_HALVES) { *p = i; *q = i + pairs; }
-          else { *p = 2 * i; *q = 2 * i + 1; }
-        };
-        const sb_half* gain = a.gain[which];
-        if (!BWD) {
-          if (row) {
-            for (int i = part; i < pairs; i += 8) {
-              int p, q;
-              pair(i, &p, &q);
-              const float2 w = cs[t * pairs + i];
-              const float u = x[p] * r * sb_h2f(gain[p]), v = x[q] * r * sb_h2f(gain[q]);
-              x[p] = u * w.x - v * w.y;
-              x[q] = v * w.x + u * w.y;
-            }
-            for (int p = a.rotary + part; p < a.P; p += 8) x[p] = x[p] * r * sb_h2f(gain[p]);
+    for (int i = threadIdx.x; i < a.tile * pairs; i += 256)
+      if (t0 + i / pairs < a.tokens) cs[i] = cos_sin(position(a, t0 + i / pairs), turns.t[i % pairs]);
+    __syncthreads();
+    if (token >= a.tokens) continue;
+    // halves: the angles of pairs (f0 + e, f1 + e); adjacent: four of the first piece, four of the second
+    float2 ang[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      ang[e] = rotates ? cs[tok * pairs + (HALVES ? f0 + e : (e < 4 ? f0 / 2 + e : f1 / 2 + e - 4))] : make_float2(1.f, 0.f);
+    auto turn = [&](float (&u)[8], float (&v)[8], float sign) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float& p = HALVES ? u[e] : (e < 4 ? u[2 * (e & 3)] : v[2 * (e & 3)]);
+        float& q = HALVES ? v[e] : (e < 4 ? u[2 * (e & 3) + 1] : v[2 * (e & 3) + 1]);
+        const float s = sign * ang[e].y, x = p, y = q;
+        p = x * ang[e].x - y * s;
+        q = y * ang[e].x + x * s;
+      }
+    };
+const sb_half* px = reinterpret_cast<const sb_half*>(vx.p) + token_offset(vx, token, a.J);
+    const sb_half* pg = BWD ? reinterpret_cast<const sb_half*>(vg.p) + token_offset(vg, token, a.J) : nullptr;
+    sb_half* py = reinterpret_cast<sb_half*>(vy.p) + token_offset(vy, token, a.J);
+    float gf[2][8];
+    unpack8(gain[0], gf[0]);
+    unpack8(gain[1], gf[1]);
+    for (int h0 = first_head; h0 < vx.H; h0 += across * kRows) {
+      uint4 x[kRows][2], g[kRows][2];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const int h = h0 + r * across;
+        x[r][0] = x[r][1] = g[r][0] = g[r][1] = make_uint4(0u, 0u, 0u, 0u);
+        if (on && h < vx.H) {
+          const sb_half* s = px + h * vx.sH;
+          x[r][0] = *reinterpret_cast<const uint4*>(s + f0);
+          x[r][1] = *reinterpret_cast<const uint4*>(s + f1);
+          if (BWD) {
+            const sb_half* d = pg + h * vg.sH;
+            g[r][0] = *reinterpret_cast<const uint4*>(d + f0);
+            g[r][1] = *reinterpret_cast<const uint4*>(d + f1);
           }
-        } else {
-          // g turned back; x becomes n
-          float dot = 0.f;
-          if (row) {
-            for (int i = part; i < pairs; i += 8) {
-              int p, q;
-              pair(i, &p, &q);
-              const float2 w = cs[t * pairs + i];
-              const float u = g[p], v = g[q];
-              g[p] = u * w.x + v * w.y;
-              g[q] = v * w.x - u * w.y;
-              x[p] *= r;
-              x[q] *= r;
-              dot += g[p] * sb_h2f(gain[p]) * x[p] + g[q] * sb_h2f(gain[q]) * x[q];
-            }
-            for (int p = a.rotary + part; p < a.P; p += 8) {
-              x[p] *= r;
-              dot += g[p] * sb_h2f(gain[p]) * x[p];
-            }
-          }
-          const float mean = group_sum<8>(dot) * inv;
-          __syncthreads();
-          const int n = min(kTokens, a.tokens - t0);
-          for (int p = threadIdx.x; p < a.P; p += 256) {
-            float s = 0.f;
-            for (int k = 0; k < n; ++k) s = fmaf(tg[k * pitch + p], tx[k * pitch + p], s);
-            a.partial[((long long)blockIdx.x * 2 + which) * a.P + p] += s;
-          }
-          __syncthreads();
-          if (row)
-            for (int p = part; p < a.P; p += 8) x[p] = r * (g[p] * sb_h2f(gain[p]) - x[p] * mean);
         }
-        __syncthreads();
-        store_rows(tx, pitch, a.y[which], a, t0, h, a.vary_tokens[which][2]);
+      }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const int h = h0 + r * across;
+        float u[8], v[8], p[8], q[8], sq = 0.f, dot = 0.f;
+        unpack8(x[r][0], u);
+        unpack8(x[r][1], v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sq = fmaf(u[e], u[e], fmaf(v[e], v[e], sq));
+        if (BWD) {
+          unpack8(g[r][0], p);
+          unpack8(g[r][1], q);
+          turn(p, q, -1.f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dot = fmaf(p[e] * gf[0][e], u[e], fmaf(q[e] * gf[1][e], v[e], dot));
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+          sq += __shfl_xor_sync(members, sq, o);
+          if (BWD) dot += __shfl_xor_sync(members, dot, o);
+        }
+        const float rs = rsqrtf(fmaf(sq, inv, a.eps));
+        if (!BWD) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            u[e] *= rs * gf[0][e];
+            v[e] *= rs * gf[1][e];
+          }
+          turn(u, v, 1.f);
+        } else {
+          const float mean = dot * rs * inv;                  // of g gain n
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float nu = u[e] * rs, nv = v[e] * rs;
+            sum[e] = fmaf(p[e], nu, sum[e]);
+            sum[8 + e] = fmaf(q[e], nv, sum[8 + e]);
+            u[e] = rs * (p[e] * gf[0][e] - nu * mean);
+            v[e] = rs * (q[e] * gf[1][e] - nv * mean);
+          }
+        }
+        if (on && h < vx.H) {
+          sb_half* d = py + h * vy.sH;
+          *reinterpret_cast<uint4*>(d + f0) = pack8(u);
+          *reinterpret_cast<uint4*>(d + f1) = pack8(v);
+        }
       }
     }
   }
+  if (BWD) {
+    // the block's sums: over a warp's groups by shuffles, over the warps in shared memory
+    float* part = reinterpret_cast<float*>(cs);               // [8][P]
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      float v = sum[e];
+#pragma unroll
+      for (int o = 16; o >= LANES; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if ((threadIdx.x & 31) < LANES && on) part[(threadIdx.x >> 5) * a.P + (e < 8 ? f0 : f1 - 8) + e] = v;
+    }
+    __syncthreads();
+    for (int p = threadIdx.x; p < a.P; p += 256) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += part[i * a.P + p];
+      a.partial[w][(long long)mine * a.P + p] = v;
+    }
+  }
 }
 
-// out[which][p] = sum of the blocks' partial sums in a fixed order: 16 threads a column take every 16th row, then a tree.
-__global__ void __launch_bounds__(512)
-gain_finish_kernel(const float* __restrict__ partial, int blocks, int P, sb_half* q, sb_half* k) {
-  __shared__ float part[16][33];
+// Any strides, any head size, lanes along tokens (what head-first projections have side by side).  Warp w of a block has the
+// pairs w, w + 8, .. of features (rotary pairs, then neighbours), SLOTS at most, of TOKENS tokens per lane, and keeps their
+// angles in registers while the block walks its heads; a row's sums go through shared memory.
+template <int SLOTS, int TOKENS, bool BWD>
+__global__ void __launch_bounds__(256)
+norm_strided_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Turns turns) {
+  __shared__ float2 part[2][8][32 * TOKENS];
   grid_dependency_sync();
-  const int which = blockIdx.y, p = blockIdx.x * 32 + (threadIdx.x & 31), i = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pairs = a.rotary / 2, slots = (a.P + 1) / 2;
+  const int w = (int)blockIdx.x < a.blocks[0] ? 0 : 1, mine = (int)blockIdx.x - (w ? a.blocks[0] : 0);
+  const int chunks = (a.x[w].H + a.chunk - 1) / a.chunk, stride = a.blocks[w] / chunks;
+  const int h_from = mine % chunks * a.chunk, h_to = min(a.x[w].H, h_from + a.chunk);
+  const float inv = 1.f / (float)a.P;
+  const sb_half* X = reinterpret_cast<const sb_half*>(a.x[w].p);
+  const sb_half* G = reinterpret_cast<const sb_half*>(a.g[w].p);
+  sb_half* Y = reinterpret_cast<sb_half*>(a.y[w].p);
+  // features of slot i: f (always there where the slot is) and f2
+  auto first = [&](int i) { const int u = warp + 8 * i; return u < pairs ? (a.pairing == SB_PAIR_HALVES ? u : 2 * u) : 2 * u; };
+  auto second = [&](int i) { const int u = warp + 8 * i; return u < pairs && a.pairing == SB_PAIR_HALVES ? u + pairs : 2 * u + 1; };
+  float gain[SLOTS][2], sum[SLOTS][2];
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) {
+    const bool there = warp + 8 * i < slots;
+    gain[i][0] = there ? sb_h2f(a.gain[w][first(i)]) : 0.f;
+    gain[i][1] = there && second(i) < a.P ? sb_h2f(a.gain[w][second(i)]) : 0.f;
+    sum[i][0] = sum[i][1] = 0.f;
+  }
+  int turnstile = 0;
+  for (int t = mine / chunks; t < a.tiles; t += stride) {
+    int token[TOKENS];
+    bool live[TOKENS];
+    float2 ang[SLOTS][TOKENS];
+    long long ox[TOKENS], og[TOKENS], oy[TOKENS];
+#pragma unroll
+    for (int k = 0; k < TOKENS; ++k) {
+      token[k] = t * 32 * TOKENS + k * 32 + lane;
+      live[k] = token[k] < a.tokens;
+      const int tc = live[k] ? token[k] : 0, pos = position(a, tc);
+#pragma unroll
+      for (int i = 0; i < SLOTS; ++i) ang[i][k] = warp + 8 * i < pairs ? cos_sin(pos, turns.t[warp + 8 * i]) : make_float2(1.f, 0.f);
+      ox[k] = token_offset(a.x[w], tc, a.J);
+      og[k] = BWD ? token_offset(a.g[w], tc, a.J) : 0;
+      oy[k] = token_offset(a.y[w], tc, a.J);
+    }
+    for (int h = h_from; h < h_to; ++h, turnstile ^= 1) {
+      sb_half xr[SLOTS][TOKENS][2], gr[SLOTS][TOKENS][2];
+#pragma unroll
+      for (int i = 0; i < SLOTS; ++i)
+#pragma unroll
+        for (int k = 0; k < TOKENS; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int f = e ? second(i) : first(i);
+            const bool there = live[k] && warp + 8 * i < slots && f < a.P;
+            xr[i][k][e] = there ? X[ox[k] + h * a.x[w].sH + f * a.x[w].sP] : sb_f2h(0.f);
+            if (BWD) gr[i][k][e] = there ? G[og[k] + h * a.g[w].sH + f * a.g[w].sP] : sb_f2h(0.f);
+          }
+      float sq[TOKENS], dot[TOKENS];
+#pragma unroll
+      for (int k = 0; k < TOKENS; ++k) {
+        sq[k] = dot[k] = 0.f;
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) {
+          const float u = sb_h2f(xr[i][k][0]), v = sb_h2f(xr[i][k][1]);
+          sq[k] = fmaf(u, u, fmaf(v, v, sq[k]));
+          if (BWD) {
+            const float c = ang[i][k].x, s = ang[i][k].y, p = sb_h2f(gr[i][k][0]), q = sb_h2f(gr[i][k][1]);
+            dot[k] = fmaf((p * c + q * s) * gain[i][0], u, fmaf((q * c - p * s) * gain[i][1], v, dot[k]));
+          }
+        }
+        part[turnstile][warp][k * 32 + lane] = make_float2(sq[k], dot[k]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < TOKENS; ++k) {
+        sq[k] = dot[k] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 s = part[turnstile][i][k * 32 + lane];
+          sq[k] += s.x;
+          dot[k] += s.y;
+        }
+        const float rs = rsqrtf(fmaf(sq[k], inv, a.eps)), mean = dot[k] * rs * inv;
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) {
+          const float c = ang[i][k].x, s = ang[i][k].y;
+          float u = sb_h2f(xr[i][k][0]) * rs, v = sb_h2f(xr[i][k][1]) * rs;
+          if (!BWD) {
+            const float p = u * gain[i][0], q = v * gain[i][1];
+            u = p * c - q * s;
+            v = q * c + p * s;
+          } else {
+            const float y = sb_h2f(gr[i][k][0]), z = sb_h2f(gr[i][k][1]), p = y * c + z * s, q = z * c - y * s;
+            sum[i][0] = fmaf(p, u, sum[i][0]);
+            sum[i][1] = fmaf(q, v, sum[i][1]);
+            u = rs * (p * gain[i][0] - u * mean);
+            v = rs * (q * gain[i][1] - v * mean);
+          }
+          if (live[k] && warp + 8 * i < slots) {
+            Y[oy[k] + h * a.y[w].sH + first(i) * a.y[w].sP] = sb_f2h(u);
+            if (second(i) < a.P) Y[oy[k] + h * a.y[w].sH + second(i) * a.y[w].sP] = sb_f2h(v);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; BWD && i < SLOTS; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float v = warp_sum(sum[i][e]);
+      const int f = e ? second(i) : first(i);
+      if (lane == 0 && warp + 8 * i < slots && f < a.P) a.partial[w][(long long)mine * a.P + f] = v;
+    }
+}
+
+// out[p] = sum of the blocks' rows in a fixed order: 32 threads a column take every 32nd row, then a tree.
+__global__ void __launch_bounds__(1024)
+gain_finish_kernel(const float* q_partial, const float* k_partial, int q_rows, int k_rows, int P, sb_half* q, sb_half* k) {
+  __shared__ float part[32][33];
+  grid_dependency_sync();
+  const float* partial = blockIdx.y ? k_partial : q_partial;
+  const int rows = blockIdx.y ? k_rows : q_rows, p = blockIdx.x * 32 + (threadIdx.x & 31), i = threadIdx.x >> 5;
   float s = 0.f;
   if (p < P)
-    for (int b = i; b < blocks; b += 16) s += partial[((long long)b * 2 + which) * P + p];
+#pragma unroll 8
+    for (int b = i; b < rows; b += 32) s += partial[(long long)b * P + p];
   part[i][threadIdx.x & 31] = s;
   __syncthreads();
-  if (i == 0 && p < P) {
-    float v[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = part[j][threadIdx.x & 31];
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1)
-#pragma unroll
-      for (int j = 0; j < o; ++j) v[j] += v[j + o];
-    (which ? k : q)[p] = sb_f2h(v[0]);
-  }
+  s = warp_sum(part[threadIdx.x & 31][i]);                    // warp i: column i
+  if ((threadIdx.x & 31) == 0 && blockIdx.x * 32 + i < P) (blockIdx.y ? k : q)[blockIdx.x * 32 + i] = sb_f2h(s);
 }
 
 // The frequencies of one rotation, remembered per thread: a program uses one or two.
@@ -204,11 +331,6 @@ const Turns& turns_of(const Rotation& r) {
   return t;
 }
 
-bool along_tokens(const Proj& v) {
-  auto mag = [](long long s) { return s < 0 ? -s : s; };
-  return v.R > 1 && mag(v.sR) < mag(v.sP);
-}
-
 NormArgs norm_args(const Proj& q, const Proj& k, const void* q_gain, const void* k_gain, const View2& pos, const Rotation& rot) {
   NormArgs a;
   memset(&a, 0, sizeof(a));
@@ -221,19 +343,59 @@ NormArgs norm_args(const Proj& q, const Proj& k, const void* q_gain, const void*
   return a;
 }
 
-template <bool BWD>
-int launch_tiles(cudaStream_t s, NormArgs& a, const Rotation& rot, int* blocks) {
+// Unit-stride features in 16-byte pieces that both members of a pair are two of.
+bool in_pieces(const Proj& v, int rotary) {
+  auto ok = [](long long n, long long stride) { return n == 1 || stride % 8 == 0; };
+  return v.H == 0 || (v.sP == 1 && v.P % 16 == 0 && rotary % 16 == 0 && ok(v.H, v.sH) && ok(v.B, v.sB) && ok(v.R, v.sR) &&
+                      !(reinterpret_cast<uintptr_t>(v.p) & 15u));
+}
+
+template <int LANES, bool BWD>
+int launch_pieces(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
+  // Four groups of threads a token, so that one has several heads to fetch at a time; fewer tokens a block where that leaves SMs
+  // without one (single tokens).
+  const int sms = usable_sms(device_facts().sms), groups = 256 / LANES;
+  for (a.tile = groups / 4; a.tile > 1 && (a.tokens + a.tile - 1) / a.tile < sms; a.tile /= 2) {}
+  a.tiles = (a.tokens + a.tile - 1) / a.tile;
   for (int w = 0; w < 2; ++w) {
-    a.vary_tokens[w][0] = along_tokens(a.x[w]);
-    a.vary_tokens[w][1] = along_tokens(a.g[w]);
-    a.vary_tokens[w][2] = along_tokens(a.y[w]);
+    // (the backward pass bounds their number by its rows of sums, of which each kind has its share)
+    const int most = BWD ? (int)std::max<long long>(1, std::min(4 * sms, kMaxPartials) * (long long)a.x[w].H / (a.x[0].H + a.x[1].H)) : a.tiles;
+    a.blocks[w] = rows[w] = a.x[w].H > 0 ? std::min(a.tiles, most) : 0;
   }
-  const int pitch = a.P | 1;
-  const size_t smem = sizeof(float) * ((((BWD ? 2 : 1) * kTokens * pitch + 1) & ~1) + kTokens * a.rotary);
-  SB_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(norm_tile_kernel<BWD>), 100 * 1024));
-  *blocks = std::min((a.tokens + kTokens - 1) / kTokens, kMaxPartials);
-  SB_LAUNCH_OK(launch_k(norm_tile_kernel<BWD>, *blocks, 256, smem, s, a, turns_of(rot)));
+  const size_t smem = std::max(sizeof(float2) * a.tile * (a.rotary / 2), BWD ? sizeof(float) * 8 * a.P : (size_t)0);
+  SB_LAUNCH_OK(launch_k(a.pairing == SB_PAIR_HALVES ? norm_pieces_kernel<LANES, BWD, true> : norm_pieces_kernel<LANES, BWD, false>, a.blocks[0] + a.blocks[1], 256,
+                        smem, s, a, turns_of(rot)));
   return SB_OK;
+}
+template <int SLOTS, int TOKENS, bool BWD>
+int launch_strided(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
+  const int sms = usable_sms(device_facts().sms), heads = a.x[0].H + a.x[1].H;
+  a.tiles = (a.tokens + 32 * TOKENS - 1) / (32 * TOKENS);
+  // up to eight heads a block, which share the angles; fewer where SMs would be without a block
+  for (a.chunk = 8; a.chunk > 1 && (long long)a.tiles * ((heads + a.chunk - 1) / a.chunk) < 2 * sms; a.chunk /= 2) {}
+  for (int w = 0; w < 2; ++w) {
+    const int chunks = (a.x[w].H + a.chunk - 1) / a.chunk;
+    // (every chunk has the same number of blocks; the backward pass bounds their number by its rows of sums)
+    const int each = BWD && chunks > 0 ? std::max(1, std::min(a.tiles, kMaxPartials / chunks)) : a.tiles;
+    a.blocks[w] = rows[w] = chunks * each;
+  }
+  SB_LAUNCH_OK(launch_k(norm_strided_kernel<SLOTS, TOKENS, BWD>, a.blocks[0] + a.blocks[1], 256, 0, s, a, turns_of(rot)));
+  return SB_OK;
+}
+template <bool BWD>
+int launch_norm(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
+  bool pieces = true;
+  for (int w = 0; w < 2; ++w)
+    for (const Proj* v : {&a.x[w], &a.y[w], &a.g[w]}) pieces = pieces && (v->p == nullptr || in_pieces(*v, a.rotary));
+  if (pieces) {
+    if (a.P <= 16) return launch_pieces<1, BWD>(s, a, rot, rows);
+    if (a.P <= 32) return launch_pieces<2, BWD>(s, a, rot, rows);
+    if (a.P <= 64) return launch_pieces<4, BWD>(s, a, rot, rows);
+    if (a.P <= 128) return launch_pieces<8, BWD>(s, a, rot, rows);
+    return launch_pieces<16, BWD>(s, a, rot, rows);
+  }
+  return a.P <= 64 ? launch_strided<4, 2, BWD>(s, a, rot, rows) : a.P <= 128 ? launch_strided<8, 1, BWD>(s, a, rot, rows)
+                                                                             : launch_strided<16, 1, BWD>(s, a, rot, rows);
 }
 
 }  // namespace
@@ -245,8 +407,8 @@ int launch_qk_norm_fwd(cudaStream_t s, Proj q, Proj k, const void* q_gain, const
   NormArgs a = norm_args(q, k, q_gain, k_gain, pos, rot);
   if (a.tokens == 0) return SB_OK;
   a.y[0] = q_out; a.y[1] = k_out;
-  int blocks;
-  return launch_tiles<false>(s, a, rot, &blocks);
+  int rows[2];
+  return launch_norm<false>(s, a, rot, rows);
 }
 
 int launch_qk_norm_bwd(cudaStream_t s, void* scratch, Proj dq_out, Proj dk_out, Proj q, Proj k, const void* q_gain, const void* k_gain,
@@ -254,10 +416,11 @@ int launch_qk_norm_bwd(cudaStream_t s, void* scratch, Proj dq_out, Proj dk_out, 
   NormArgs a = norm_args(q, k, q_gain, k_gain, pos, rot);
   a.g[0] = dq_out; a.g[1] = dk_out;
   a.y[0] = dq; a.y[1] = dk;
-  a.partial = reinterpret_cast<float*>(scratch);
-  int blocks = 0;                        // without tokens the gains' gradients are 0
-  if (a.tokens > 0) SB_TRY(launch_tiles<true>(s, a, rot, &blocks));
-  SB_LAUNCH_OK(launch_k(gain_finish_kernel, dim3((a.P + 31) / 32, k.H > 0 ? 2 : 1), 512, 0, s, a.partial, blocks, a.P,
+  a.partial[0] = reinterpret_cast<float*>(scratch);
+  a.partial[1] = a.partial[0] + kMaxPartials * kNormMaxHead;
+  int rows[2] = {0, 0};                  // without tokens the gains' gradients are 0
+  if (a.tokens > 0) SB_TRY(launch_norm<true>(s, a, rot, rows));
+  SB_LAUNCH_OK(launch_k(gain_finish_kernel, dim3((a.P + 31) / 32, k.H > 0 ? 2 : 1), 1024, 0, s, a.partial[0], a.partial[1], rows[0], rows[1], a.P,
                         reinterpret_cast<sb_half*>(dq_gain), reinterpret_cast<sb_half*>(dk_gain)));
   return SB_OK;
 }
