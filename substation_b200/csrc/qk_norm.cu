@@ -10,6 +10,7 @@ namespace sb {
 
 namespace {
 
+constexpr int kDepth = 4;              // rows that a thread of the pieces kernel has on their way
 constexpr int kMaxPairs = kNormMaxHead / 2;
 constexpr int kMaxPartials = 1184;     // rows of partial sums of a gain's gradient: eight blocks of 148 SMs
 
@@ -42,16 +43,23 @@ __device__ __forceinline__ long long token_offset(const Proj& v, int token, int 
   return (long long)(token / J) * v.sB + (long long)(token % J) * v.sR;
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // Unit-stride features in 16-byte pieces.  A row belongs to LANES threads with two pieces each, so chosen that both members of
-// every pair are in one thread: a row's norm is a few shuffles and its rotation none.  A block takes a tile of tokens, puts
-// their angles into shared memory once, and its groups of threads walk the query (or key) heads of a token each.  In the backward pass
-// sum x^2 and sum g gain x are all that a row needs from its other threads; the gains' gradients stay in registers until the
-// block's last tile.
+// every pair are in one thread: a row's norm is a few shuffles and its rotation none.  A block takes tiles of tokens, puts
+// their angles into shared memory, and its groups of threads walk the query (or key) heads of a token each.  Rows are fetched
+// kDepth ahead into a ring that belongs to the thread alone, so that nothing has to be waited for but the copy itself; as
+// registers they held half as many bytes in flight.  In the backward pass sum x^2 and sum g gain x are all that a row needs
+// from its other threads; the gains' gradients stay in registers until the block's last tile.
 template <int LANES, bool BWD, bool HALVES>
 __global__ void __launch_bounds__(256, 2)
 norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Turns turns) {
-  constexpr int kGroups = 256 / LANES, kRows = BWD ? 2 : 4;   // rows in flight
-  extern __shared__ float2 cs[];                              // [tile][rotary / 2]; at the end the warps' sums
+  constexpr int kGroups = 256 / LANES, kPieces = BWD ? 4 : 2;
+  extern __shared__ uint4 smem[];                             // ring [kDepth][kPieces][256], frequencies, angles [2][tile][pairs]
+  double* freq = reinterpret_cast<double*>(smem + kDepth * kPieces * 256);
+  float2* cs = reinterpret_cast<float2*>(freq + a.rotary / 2);
   grid_dependency_sync();
   const int pairs = a.rotary / 2, turned = a.rotary / 16, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const uint32_t members = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
@@ -61,28 +69,70 @@ norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ T
   const float inv = 1.f / (float)a.P;
   const int w = (int)blockIdx.x < a.blocks[0] ? 0 : 1, mine = (int)blockIdx.x - (w ? a.blocks[0] : 0);
   const Proj &vx = a.x[w], &vg = a.g[w], &vy = a.y[w];
-  uint4 gain[2];
+  const int heads = vx.H;
+  uint4* slots = smem + threadIdx.x;
+  const uint32_t slots_at = (uint32_t)__cvta_generic_to_shared(slots);
+
+  // the row that is fetched next
+  int ft = mine, fh = first_head, fslot = 0;
+  const sb_half *fx = nullptr, *fg = nullptr;
+  bool flive = false;
+  auto at_token = [&] {
+    const int token = ft * a.tile + tok;
+    flive = on && ft < a.tiles && token < a.tokens && first_head < heads;
+    if (flive) {
+      fx = reinterpret_cast<const sb_half*>(vx.p) + token_offset(vx, token, a.J);
+      if (BWD) fg = reinterpret_cast<const sb_half*>(vg.p) + token_offset(vg, token, a.J);
+    }
+  };
+  auto fetch = [&] {
+    if (flive) {
+      const uint32_t d = slots_at + fslot * kPieces * 4096;
+      const sb_half* s = fx + fh * vx.sH;
+      cp_async16(d, s + f0);
+      cp_async16(d + 4096, s + f1);
+      if (BWD) {
+        s = fg + fh * vg.sH;
+        cp_async16(d + 2 * 4096, s + f0);
+        cp_async16(d + 3 * 4096, s + f1);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (++fslot == kDepth) fslot = 0;
+    fh += across;
+    if (fh >= heads) {
+      fh = first_head;
+      ft += a.blocks[w];
+      at_token();
+    }
+  };
+  at_token();
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    sb_half* h = reinterpret_cast<sb_half*>(&gain[x]);
+  for (int i = 0; i < kDepth - 1; ++i) fetch();
+
+  float gf[2][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = on ? a.gain[w][(x ? f1 : f0) + e] : sb_f2h(0.f);
-  }
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) gf[x][e] = on ? sb_h2f(a.gain[w][(x ? f1 : f0) + e]) : 0.f;
+  for (int i = threadIdx.x; i < pairs; i += 256) freq[i] = turns.t[i];
+  __syncthreads();
   float sum[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) sum[e] = 0.f;
-  for (int t = mine; t < a.tiles; t += a.blocks[w]) {
+  int slot = 0, buffer = 0;
+  for (int t = mine; t < a.tiles; t += a.blocks[w], buffer ^= 1) {
     const int t0 = t * a.tile, token = t0 + tok;
-    __syncthreads();
+    float2* table = cs + buffer * a.tile * pairs;             // (two in turn: one barrier a tile)
     for (int i = threadIdx.x; i < a.tile * pairs; i += 256)
-      if (t0 + i / pairs < a.tokens) cs[i] = cos_sin(position(a, t0 + i / pairs), turns.t[i % pairs]);
+      if (t0 + i / pairs < a.tokens) table[i] = cos_sin(position(a, t0 + i / pairs), freq[i % pairs]);
     __syncthreads();
-    if (token >= a.tokens) continue;
+    const bool live = token < a.tokens;
     // halves: the angles of pairs (f0 + e, f1 + e); adjacent: four of the first piece, four of the second
     float2 ang[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      ang[e] = rotates ? cs[tok * pairs + (HALVES ? f0 + e : (e < 4 ? f0 / 2 + e : f1 / 2 + e - 4))] : make_float2(1.f, 0.f);
+      ang[e] = rotates && live ? table[tok * pairs + (HALVES ? f0 + e : (e < 4 ? f0 / 2 + e : f1 / 2 + e - 4))] : make_float2(1.f, 0.f);
     auto turn = [&](float (&u)[8], float (&v)[8], float sign) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -93,79 +143,60 @@ norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ T
         q = y * ang[e].x + x * s;
       }
     };
-const sb_half* px = reinterpret_cast<const sb_half*>(vx.p) + token_offset(vx, token, a.J);
-    const sb_half* pg = BWD ? reinterpret_cast<const sb_half*>(vg.p) + token_offset(vg, token, a.J) : nullptr;
-    sb_half* py = reinterpret_cast<sb_half*>(vy.p) + token_offset(vy, token, a.J);
-    float gf[2][8];
-    unpack8(gain[0], gf[0]);
-    unpack8(gain[1], gf[1]);
-    for (int h0 = first_head; h0 < vx.H; h0 += across * kRows) {
-      uint4 x[kRows][2], g[kRows][2];
+    sb_half* py = reinterpret_cast<sb_half*>(vy.p) + (live ? token_offset(vy, token, a.J) : 0);
+    for (int h = first_head; h < heads; h += across) {
+      fetch();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+      const uint4* in = slots + slot * kPieces * 256;
+      if (++slot == kDepth) slot = 0;
+      if (!live) continue;
+      float u[8], v[8], p[8], q[8], sq = 0.f, dot = 0.f;
+      unpack8(on ? in[0] : make_uint4(0u, 0u, 0u, 0u), u);
+      unpack8(on ? in[256] : make_uint4(0u, 0u, 0u, 0u), v);
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const int h = h0 + r * across;
-        x[r][0] = x[r][1] = g[r][0] = g[r][1] = make_uint4(0u, 0u, 0u, 0u);
-        if (on && h < vx.H) {
-          const sb_half* s = px + h * vx.sH;
-          x[r][0] = *reinterpret_cast<const uint4*>(s + f0);
-          x[r][1] = *reinterpret_cast<const uint4*>(s + f1);
-          if (BWD) {
-            const sb_half* d = pg + h * vg.sH;
-            g[r][0] = *reinterpret_cast<const uint4*>(d + f0);
-            g[r][1] = *reinterpret_cast<const uint4*>(d + f1);
-          }
-        }
+      for (int e = 0; e < 8; ++e) sq = fmaf(u[e], u[e], fmaf(v[e], v[e], sq));
+      if (BWD) {
+        unpack8(on ? in[512] : make_uint4(0u, 0u, 0u, 0u), p);
+        unpack8(on ? in[768] : make_uint4(0u, 0u, 0u, 0u), q);
+        turn(p, q, -1.f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot = fmaf(p[e] * gf[0][e], u[e], fmaf(q[e] * gf[1][e], v[e], dot));
       }
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const int h = h0 + r * across;
-        float u[8], v[8], p[8], q[8], sq = 0.f, dot = 0.f;
-        unpack8(x[r][0], u);
-        unpack8(x[r][1], v);
+      for (int o = LANES / 2; o > 0; o >>= 1) {
+        sq += __shfl_xor_sync(members, sq, o);
+        if (BWD) dot += __shfl_xor_sync(members, dot, o);
+      }
+      const float rs = rsqrtf(fmaf(sq, inv, a.eps));
+      if (!BWD) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sq = fmaf(u[e], u[e], fmaf(v[e], v[e], sq));
-        if (BWD) {
-          unpack8(g[r][0], p);
-          unpack8(g[r][1], q);
-          turn(p, q, -1.f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) dot = fmaf(p[e] * gf[0][e], u[e], fmaf(q[e] * gf[1][e], v[e], dot));
+        for (int e = 0; e < 8; ++e) {
+          u[e] *= rs * gf[0][e];
+          v[e] *= rs * gf[1][e];
         }
+        turn(u, v, 1.f);
+      } else {
+        const float mean = dot * rs * inv;                    // of g gain n
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) {
-          sq += __shfl_xor_sync(members, sq, o);
-          if (BWD) dot += __shfl_xor_sync(members, dot, o);
+        for (int e = 0; e < 8; ++e) {
+          const float nu = u[e] * rs, nv = v[e] * rs;
+          sum[e] = fmaf(p[e], nu, sum[e]);
+          sum[8 + e] = fmaf(q[e], nv, sum[8 + e]);
+          u[e] = rs * (p[e] * gf[0][e] - nu * mean);
+          v[e] = rs * (q[e] * gf[1][e] - nv * mean);
         }
-        const float rs = rsqrtf(fmaf(sq, inv, a.eps));
-        if (!BWD) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            u[e] *= rs * gf[0][e];
-            v[e] *= rs * gf[1][e];
-          }
-          turn(u, v, 1.f);
-        } else {
-          const float mean = dot * rs * inv;                  // of g gain n
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float nu = u[e] * rs, nv = v[e] * rs;
-            sum[e] = fmaf(p[e], nu, sum[e]);
-            sum[8 + e] = fmaf(q[e], nv, sum[8 + e]);
-            u[e] = rs * (p[e] * gf[0][e] - nu * mean);
-            v[e] = rs * (q[e] * gf[1][e] - nv * mean);
-          }
-        }
-        if (on && h < vx.H) {
-          sb_half* d = py + h * vy.sH;
-          *reinterpret_cast<uint4*>(d + f0) = pack8(u);
-          *reinterpret_cast<uint4*>(d + f1) = pack8(v);
-        }
+      }
+      if (on) {
+        sb_half* d = py + h * vy.sH;
+        *reinterpret_cast<uint4*>(d + f0) = pack8(u);
+        *reinterpret_cast<uint4*>(d + f1) = pack8(v);
       }
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (BWD) {
     // the block's sums: over a warp's groups by shuffles, over the warps in shared memory
-    float* part = reinterpret_cast<float*>(cs);               // [8][P]
+    float* part = reinterpret_cast<float*>(smem);             // [8][P]
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -357,14 +388,15 @@ int launch_pieces(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
   const int sms = usable_sms(device_facts().sms), groups = 256 / LANES;
   for (a.tile = groups / 4; a.tile > 1 && (a.tokens + a.tile - 1) / a.tile < sms; a.tile /= 2) {}
   a.tiles = (a.tokens + a.tile - 1) / a.tile;
-  for (int w = 0; w < 2; ++w) {
-    // (the backward pass bounds their number by its rows of sums, of which each kind has its share)
-    const int most = BWD ? (int)std::max<long long>(1, std::min(4 * sms, kMaxPartials) * (long long)a.x[w].H / (a.x[0].H + a.x[1].H)) : a.tiles;
-    a.blocks[w] = rows[w] = a.x[w].H > 0 ? std::min(a.tiles, most) : 0;
-  }
-  const size_t smem = std::max(sizeof(float2) * a.tile * (a.rotary / 2), BWD ? sizeof(float) * 8 * a.P : (size_t)0);
-  SB_LAUNCH_OK(launch_k(a.pairing == SB_PAIR_HALVES ? norm_pieces_kernel<LANES, BWD, true> : norm_pieces_kernel<LANES, BWD, false>, a.blocks[0] + a.blocks[1], 256,
-                        smem, s, a, turns_of(rot)));
+  // Two blocks an SM at a time, the queries' and the keys' share of them by their heads; the backward pass has room for the sums
+  // of so many.
+  const int most = std::min(2 * sms, kMaxPartials), heads = a.x[0].H + a.x[1].H;
+  for (int w = 0; w < 2; ++w)
+    a.blocks[w] = rows[w] = a.x[w].H > 0 ? std::min(a.tiles, std::max(1, (int)(most * (long long)a.x[w].H / heads))) : 0;
+  const size_t smem = kDepth * (BWD ? 4 : 2) * 4096 + sizeof(double) * (a.rotary / 2) + 2 * sizeof(float2) * a.tile * (a.rotary / 2);
+  auto kernel = a.pairing == SB_PAIR_HALVES ? norm_pieces_kernel<LANES, BWD, true> : norm_pieces_kernel<LANES, BWD, false>;
+  SB_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), 100 * 1024));
+  SB_LAUNCH_OK(launch_k(kernel, a.blocks[0] + a.blocks[1], 256, smem, s, a, turns_of(rot)));
   return SB_OK;
 }
 template <int SLOTS, int TOKENS, bool BWD>
