@@ -49,6 +49,46 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t db,
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
       ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {   // (no wait)
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
+// Wait for the tensor-memory loads under way; no use of the registers can be scheduled above it.
+__device__ __forceinline__ void tmem_wait16(uint32_t* a, uint32_t* b) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]), "+r"(a[8]), "+r"(a[9]),
+                 "+r"(a[10]), "+r"(a[11]), "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15]),
+                 "+r"(b[0]), "+r"(b[1]), "+r"(b[2]), "+r"(b[3]), "+r"(b[4]), "+r"(b[5]), "+r"(b[6]), "+r"(b[7]), "+r"(b[8]), "+r"(b[9]),
+                 "+r"(b[10]), "+r"(b[11]), "+r"(b[12]), "+r"(b[13]), "+r"(b[14]), "+r"(b[15])
+               :: "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 x, x, y, z;\n"
+      " mov.b64 {%0, %1}, x;\n}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 pair(const uint32_t* r, int i) { return make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])); }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
@@ -149,64 +189,106 @@ struct FwdCfg {
   static int smem(int pitch) { return kTiles + 2 * pitch * 4 + 1024 + 256; }
 };
 
-// One tile of scores of a thread's row against its 128 keys.  NEAR: the bias varies, bp[c] is column c's; else it is `flat`.
-// MASK: columns from lim on are hidden.
-template <bool NEAR, bool MASK>
-__device__ __forceinline__ float row_max(uint32_t s, const float* bp, float flat, int lim, float c2) {
-  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+// A row's state: reference of its exponentials, their sum so far.
+struct Row { float m, l; };
+
+// The reference rises: what stands in tensor memory, the output (where `started`) and the tile's first `chunks` chunks of
+// exponentials, is brought to it.  Rare.
+template <int P>
+__device__ __noinline__ void rescale(uint32_t to, uint32_t tp, bool started, int chunks, float f) {
+  if (started) {
+#pragma unroll 1
+    for (int c = 0; c < P / 32; ++c) {
+      uint32_t r[32];
+      tmem_ld32_nowait(to + c * 32, r);
+      attn::tmem_ld_wait32(r);
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t r[32];
-    tmem_ld32_nowait(s + c * 32, r);
-    float b[32];
-    if (NEAR) {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) b[e] = bp[c * 32 + e];
-    }
-    attn::tmem_ld_wait32(r);
-#pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      float t = __uint_as_float(r[e]);
-      if (NEAR) t = fmaf(t, c2, b[e]);
-      if (MASK && c * 32 + e >= lim) t = -INFINITY;
-      mx[e & 3] = fmaxf(mx[e & 3], t);
+      for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+      attn::tmem_st32(to + c * 32, r);
     }
   }
-  const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-  return NEAR || m == -INFINITY ? m : fmaf(m, c2, flat);
-}
-// Exponentials against 2^ref as 16-bit pairs into tensor memory; returns their sum.
-template <bool NEAR, bool MASK>
-__device__ __forceinline__ float row_exp(uint32_t s, uint32_t dst, const float* bp, float flat, float ref, int lim, float c2) {
-  float l0 = 0.f, l1 = 0.f;
-  const float off = flat - ref;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t r[32], w[16];
-    tmem_ld32_nowait(s + c * 32, r);
-    float b[32];
-    if (NEAR) {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) b[e] = bp[c * 32 + e] - ref;
-    }
-    attn::tmem_ld_wait32(r);
+  attn::tmem_st_wait();
+#pragma unroll 1
+  for (int c = 0; c < chunks; ++c) {
+    uint32_t r[16];
+    tmem_ld16(tp + c * 16, r);
+    tmem_ld_wait();
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      float x = fmaf(__uint_as_float(r[2 * e]), c2, NEAR ? b[2 * e] : off);
-      float y = fmaf(__uint_as_float(r[2 * e + 1]), c2, NEAR ? b[2 * e + 1] : off);
-      if (MASK) {
-        if (c * 32 + 2 * e >= lim) x = -INFINITY;
-        if (c * 32 + 2 * e + 1 >= lim) y = -INFINITY;
-      }
-      x = attn::ex2_approx(x);
-      y = attn::ex2_approx(y);
-      l0 += x;
-      l1 += y;
-      w[e] = flash::pack2(x, y);
+      const float2 v = sb_h22f2(*reinterpret_cast<const sb_half2*>(&r[e]));
+      r[e] = flash::pack2(v.x * f, v.y * f);
     }
-    tmem_st16(dst + c * 16, w);
+    tmem_st16(tp + c * 16, r);
   }
-  return l0 + l1;
+  attn::tmem_st_wait();
+}
+
+// A thread's row of 128 scores, 32 columns at a time while the next 32 are on their way: exponentials against the row's
+// reference as 16-bit pairs into tensor memory (where they may overwrite scores already read).  The reference lags behind the
+// maximum by at most 2^kLazy; a chunk that exceeds it makes it rise before its own exponentials are taken.
+// NEAR: the bias varies, bp[c] is column c's; else it is `flat`.  MASK: columns from lim on are hidden.
+template <int P, bool NEAR, bool MASK>
+__device__ __forceinline__ void row_tile(uint32_t s, uint32_t tp, uint32_t to, bool started, const float* bp, float flat, int lim, float c2,
+                                         Row& row) {
+  float2 sum = make_float2(0.f, 0.f);
+  const float2 c22 = make_float2(c2, c2);
+  auto chunk = [&](int c, uint32_t* r, uint32_t* coming) {
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      float2 t = pair(r, e);
+      if (NEAR) t = fma2(t, c22, make_float2(bp[c * 32 + e], bp[c * 32 + e + 1]));
+      if (MASK) {
+        if (c * 32 + e >= lim) t.x = -INFINITY;
+        if (c * 32 + e + 1 >= lim) t.y = -INFINITY;
+      }
+      if (NEAR || MASK) {
+        r[e] = __float_as_uint(t.x);
+        r[e + 1] = __float_as_uint(t.y);
+      }
+      mx[(e >> 1) & 3] = fmaxf(fmaxf(mx[(e >> 1) & 3], t.x), t.y);
+    }
+    float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    if (!NEAR && m > -INFINITY) m = fmaf(m, c2, flat);
+    if (!started && c == 0) {
+      row.m = m;
+    } else {
+      const bool raise = m - row.m > kLazy;              // no finite score so far: true as soon as one comes
+      if (__any_sync(0xffffffffu, raise)) {
+        const float f = raise ? attn::ex2_approx(row.m - m) : 1.f;
+        if (raise) row.m = m;
+        row.l *= f;
+        sum.x *= f;
+        sum.y *= f;
+        attn::tmem_ld_wait32(coming);                    // (a call moves registers)
+        rescale<P>(to, tp, started, c, f);
+      }
+    }
+    const float ref = row.m == -INFINITY ? 0.f : row.m;
+    const float2 off = make_float2((NEAR ? 0.f : flat) - ref, (NEAR ? 0.f : flat) - ref);
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      float2 x = NEAR ? add2(pair(r, e), off) : fma2(pair(r, e), c22, off);
+      x.x = attn::ex2_approx(x.x);
+      x.y = attn::ex2_approx(x.y);
+      sum = add2(sum, x);
+      w[e >> 1] = flash::pack2(x.x, x.y);
+    }
+    tmem_st16(tp + c * 16, w);
+  };
+  uint32_t ra[32], rb[32];
+  tmem_ld32_nowait(s, ra);
+#pragma unroll 1
+  for (int c = 0; c < 4; c += 2) {
+    attn::tmem_ld_wait32(ra);
+    tmem_ld32_nowait(s + c * 32 + 32, rb);
+    chunk(c, ra, rb);
+    attn::tmem_ld_wait32(rb);
+    if (c == 0) tmem_ld32_nowait(s + 64, ra);
+    chunk(c + 1, rb, ra);
+  }
+  row.l += sum.x + sum.y;
 }
 
 // One CTA: 128 queries of one unit against its keys in tiles of 128; two CTAs per SM, so that one's tensor and copy work runs
@@ -359,7 +441,7 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       const bool row = j < p.c.J;
       int mine = w.keys;                                 // keys that this row sees
       if (p.c.causal) mine = min(mine, pos + 1);
-      float m = -INFINITY, l = 0.f;
+      Row state = {-INFINITY, 0.f};
       const uint32_t bb = it & 1u;
       const float* bias = bias_s + bb * p.c.pitch;
       if (w.tiles > 0) {
@@ -371,42 +453,21 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         const int rel0 = kb * 128 - pos;                 // relative position of the first column
         const int lo = kb * 128 - (w.first + w.t * 128 + q * 32 + 31), hi = kb * 128 + 127 - (w.first + w.t * 128 + q * 32);
         const bool near = hi > -p.c.reach && lo < p.c.reach;
-        const float flat = near ? 0.f : bias[kPad + (lo >= p.c.reach ? 2 * p.c.reach : 0)];
-        const float* bp = bias + (near ? rel0 + p.c.reach + kPad : 0);
         const bool mask = __any_sync(0xffffffffu, lim < 128);
+        // outside the varying part, a place in the row where 128 entries have the end's value
+        const float* bp = bias + (near ? rel0 + p.c.reach + kPad : lo >= p.c.reach ? kPad + 2 * p.c.reach : 0);
+        const float flat = bp[0];
         ok = __all_sync(0xffffffffu, mbar_wait(s_full, n & 1u, 46));
         if (!ok) break;
         tc_fence_after();
-        float mx;
-        if (near) mx = mask ? row_max<true, true>(ts, bp, 0.f, lim, p.c.c2) : row_max<true, false>(ts, bp, 0.f, lim, p.c.c2);
-        else mx = mask ? row_max<false, true>(ts, bp, flat, lim, p.c.c2) : row_max<false, false>(ts, bp, flat, lim, p.c.c2);
         if (n > 0) {                                     // the previous output product has read its exponentials
           ok = __all_sync(0xffffffffu, mbar_wait(p_free, (n - 1u) & 1u, 47));
           if (!ok) break;
           tc_fence_after();
         }
-        if (kb == 0) {
-          m = mx;
-        } else {
-          const bool raise = mx - m > kLazy;             // -inf so far: true as soon as a finite score comes
-          if (__any_sync(0xffffffffu, raise)) {
-            const float f = raise ? attn::ex2_approx(m - mx) : 1.f;
-            if (raise) m = mx;
-            l *= f;
-#pragma unroll 1
-            for (int c = 0; c < P / 32; ++c) {
-              uint32_t r[32];
-              tmem_ld32_nowait(to + c * 32, r);
-              attn::tmem_ld_wait32(r);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
-              attn::tmem_st32(to + c * 32, r);
-            }
-          }
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-        if (near) l += mask ? row_exp<true, true>(ts, tp, bp, 0.f, ref, lim, p.c.c2) : row_exp<true, false>(ts, tp, bp, 0.f, ref, lim, p.c.c2);
-        else l += mask ? row_exp<false, true>(ts, tp, bp, flat, ref, lim, p.c.c2) : row_exp<false, false>(ts, tp, bp, flat, ref, lim, p.c.c2);
+        if (mask) row_tile<P, true, true>(ts, tp, to, kb > 0, bp, 0.f, lim, p.c.c2, state);
+        else if (near) row_tile<P, true, false>(ts, tp, to, kb > 0, bp, 0.f, lim, p.c.c2, state);
+        else row_tile<P, false, false>(ts, tp, to, kb > 0, bp, flat, lim, p.c.c2, state);
         attn::tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -414,7 +475,7 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       }
       if (!ok) break;
       sb_half* out = reinterpret_cast<sb_half*>(p.out.p) + (long long)w.h * p.out.sH + (long long)w.b * p.out.sB + (long long)j * p.out.sR;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = state.l > 0.f ? 1.f / state.l : 0.f;
       if (w.tiles > 0) {
         if (lane == 0) mbar_arrive(b_empty + 8 * bb);
         ok = __all_sync(0xffffffffu, mbar_wait(p_free, (n - 1u) & 1u, 47));
@@ -435,7 +496,7 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       }
       if (row && p.lse.p)
         p.lse.p[(long long)w.h * p.lse.sH + (long long)w.b * p.lse.sB + (long long)j * p.lse.sJ] =
-            l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+            state.l > 0.f ? (state.m + log2f(state.l)) * 0.6931471805599453f : -INFINITY;
       if (w.tiles > 0) {
         tc_fence_before();
         __syncwarp();
@@ -513,54 +574,62 @@ struct BwdCfg {
 };
 
 // Scores and dP of a thread's row of 64 columns -> exponentials and score gradients, 16-bit pairs over the columns they came
-// from.  Column c has the bias bp[DIR * c] (NEAR) or `flat`, row constants ls and ds.
+// from, 16 columns at a time while the next 16 are on their way.  Column c has the bias bp[c] (key tiles: bp[-c]; NEAR) or `flat`.
 // What differs between the two kinds of items: in key tiles (KEYS) a thread is a key, log-sum-exps and D change along columns
 // (L, D in shared memory), visible columns are c >= lim; in query tiles a thread is a query and visible columns are c < lim.
-template <bool KEYS, bool NEAR, bool MASK, class Emit>
+// `emit` gets every score gradient, `block` is told after each 32 columns.
+template <bool KEYS, bool NEAR, bool MASK, class Emit, class Block>
 __device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float flat, const float* L, const float* D, float lse, float dsum,
-                                          int lim, float c2, Emit&& emit) {
+                                          int lim, float c2, Emit&& emit, Block&& block) {
+  const float2 c22 = make_float2(c2, c2), minus = make_float2(-1.f, -1.f);
+  auto chunk = [&](int c, uint32_t* s, uint32_t* g) {
+    uint32_t pm[8], dm[8];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t s[32], g[32];
-    tmem_ld32_nowait(ts + c * 32, s);
-    tmem_ld32_nowait(ts + 64 + c * 32, g);
-    attn::tmem_ld_wait32(s);
-    attn::tmem_ld_wait32(g);
-    uint32_t pm[16], dm[16];
-#pragma unroll
-    for (int e = 0; e < 32; e += 4) {
-      float4 l4, d4;
+    for (int e = 0; e < 16; e += 4) {
+      float4 l4 = make_float4(lse, lse, lse, lse), d4 = make_float4(dsum, dsum, dsum, dsum);
       if (KEYS) {
-        l4 = *reinterpret_cast<const float4*>(L + c * 32 + e);
-        d4 = *reinterpret_cast<const float4*>(D + c * 32 + e);
+        l4 = *reinterpret_cast<const float4*>(L + c * 16 + e);
+        d4 = *reinterpret_cast<const float4*>(D + c * 16 + e);
       }
-      float pv[4], dv[4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int col = c * 32 + e + x;
-        const float l = KEYS ? (x == 0 ? l4.x : x == 1 ? l4.y : x == 2 ? l4.z : l4.w) : lse;
-        const float d = KEYS ? (x == 0 ? d4.x : x == 1 ? d4.y : x == 2 ? d4.z : d4.w) : dsum;
-        const float b = NEAR ? bp[KEYS ? -col : col] : flat;
-        float pr = attn::ex2_approx(fmaf(__uint_as_float(s[e + x]), c2, b - l));
-        float ds = pr * (__uint_as_float(g[e + x]) - d);
+      for (int x = 0; x < 4; x += 2) {
+        const int i = e + x, col = c * 16 + i;
+        const float2 l = x ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y), d = x ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
+        const float2 b = NEAR ? (KEYS ? make_float2(bp[-col], bp[-col - 1]) : make_float2(bp[col], bp[col + 1])) : make_float2(flat, flat);
+        float2 pr = fma2(pair(s, i), c22, fma2(l, minus, b));
+        pr.x = attn::ex2_approx(pr.x);
+        pr.y = attn::ex2_approx(pr.y);
+        float2 ds = mul2(pr, fma2(d, minus, pair(g, i)));
         if (MASK) {
-          const bool seen = KEYS ? col >= lim : col < lim;
-          pr = seen ? pr : 0.f;
-          ds = seen ? ds : 0.f;
+          const bool seen0 = KEYS ? col >= lim : col < lim, seen1 = KEYS ? col + 1 >= lim : col + 1 < lim;
+          pr = make_float2(seen0 ? pr.x : 0.f, seen1 ? pr.y : 0.f);
+          ds = make_float2(seen0 ? ds.x : 0.f, seen1 ? ds.y : 0.f);
         }
-        pv[x] = pr;
-        dv[x] = ds;
-        emit(c, e + x, ds);
+        emit((c & 1) * 16 + i, ds.x);
+        emit((c & 1) * 16 + i + 1, ds.y);
+        if (KEYS) pm[i >> 1] = flash::pack2(pr.x, pr.y);
+        dm[i >> 1] = flash::pack2(ds.x, ds.y);
       }
-      if (KEYS) {
-        pm[e / 2] = flash::pack2(pv[0], pv[1]);
-        pm[e / 2 + 1] = flash::pack2(pv[2], pv[3]);
-      }
-      dm[e / 2] = flash::pack2(dv[0], dv[1]);
-      dm[e / 2 + 1] = flash::pack2(dv[2], dv[3]);
     }
-    if (KEYS) tmem_st16(ts + c * 16, pm);
-    tmem_st16(ts + 64 + c * 16, dm);
+    if (KEYS) tmem_st8(ts + c * 8, pm);
+    tmem_st8(ts + 64 + c * 8, dm);
+  };
+  uint32_t sa[16], ga[16], sb[16], gb[16];
+  tmem_ld16(ts, sa);
+  tmem_ld16(ts + 64, ga);
+#pragma unroll 1
+  for (int c = 0; c < 4; c += 2) {
+    tmem_wait16(sa, ga);
+    tmem_ld16(ts + c * 16 + 16, sb);
+    tmem_ld16(ts + 64 + c * 16 + 16, gb);
+    chunk(c, sa, ga);
+    tmem_wait16(sb, gb);
+    if (c == 0) {
+      tmem_ld16(ts + 32, sa);
+      tmem_ld16(ts + 96, ga);
+    }
+    chunk(c + 1, sb, gb);
+    block(c >> 1);
   }
 }
 
@@ -871,13 +940,14 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         continue;
       }
       const int r = w.t * 128 + rt;                    // query or key of this thread
-      float lse = INFINITY, dsum = 0.f, weight = 0.f;
+      float lse = INFINITY, dsum = 0.f, weight = 1.f;
       if (w.q && r < p.c.J) {
         const float* rec = p.records + (((long long)w.b * p.c.H + w.h) * blocks + (r >> 6)) * kRecord + (r & 63);
         lse = rec[0];
         dsum = rec[64];
         weight = rec[128];
       }
+      const bool weighted = __any_sync(0xffffffffu, weight != 1.f);
       int mine = w.keys;
       if (w.q && p.c.causal) mine = min(mine, w.first + r + 1);
       bool due = have;                                 // the previous item's results are still to be stored
@@ -896,29 +966,28 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
             const bool near = hi > -reach && lo < reach;
             const int lim = mine - k0;
             const bool mask = __any_sync(0xffffffffu, lim < 64);
-            if (near) {
-              float up[2] = {0.f, 0.f}, down[2] = {0.f, 0.f};   // diagonals `lane` and `lane - 32` of the two blocks
-              auto emit = [&](int c, int e, float ds) {
-                const float v = __shfl_sync(0xffffffffu, ds * weight, (e - lane) & 31);
-                if (lane <= e) up[c] += v;
-                else down[c] += v;
+            // outside the varying part, a place in the row where 64 entries have the end's value
+            const float* bp = bias + (near ? k0 - (w.first + r) + reach + kPad : lo >= reach ? kPad + 2 * reach : 0);
+            if (near || mask || weighted) {
+              float up = 0.f, down = 0.f;              // diagonals `lane` and `lane - 32` of a block
+              auto block = [&](int c) {
+                add(k0 + 32 * c - pos0 + lane, up);
+                add(k0 + 32 * c - pos0 + lane - 32, down);
+                up = down = 0.f;
               };
-              const float* bp = bias + (k0 - (w.first + r) + reach + kPad);
-              if (mask) turn_tile<false, true, true>(ts, bp, 0.f, nullptr, nullptr, lse, dsum, lim, p.c.c2, emit);
-              else turn_tile<false, true, false>(ts, bp, 0.f, nullptr, nullptr, lse, dsum, lim, p.c.c2, emit);
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                add(k0 + 32 * c - pos0 + lane, up[c]);
-                add(k0 + 32 * c - pos0 + lane - 32, down[c]);
-              }
+              auto sum = [&](int e, float ds) {
+                const float v = __shfl_sync(0xffffffffu, ds, e - lane);
+                if (lane <= e) up += v;
+                else down += v;
+              };
+              auto weigh = [&](int e, float ds) { sum(e, ds * weight); };
+              if (mask || weighted) turn_tile<false, true, true>(ts, bp, 0.f, nullptr, nullptr, lse, dsum, lim, p.c.c2, weigh, block);
+              else turn_tile<false, true, false>(ts, bp, 0.f, nullptr, nullptr, lse, dsum, lim, p.c.c2, sum, block);
             } else {
-              float sum = 0.f;
-              auto emit = [&](int, int, float ds) { sum += ds; };
-              const float flat = bias[kPad + (lo >= reach ? 2 * reach : 0)];
-              if (mask) turn_tile<false, false, true>(ts, nullptr, flat, nullptr, nullptr, lse, dsum, lim, p.c.c2, emit);
-              else turn_tile<false, false, false>(ts, nullptr, flat, nullptr, nullptr, lse, dsum, lim, p.c.c2, emit);
-              if (lo >= reach) above += sum * weight;
-              else below += sum * weight;
+              float2 sum = make_float2(0.f, 0.f);
+              auto emit = [&](int e, float ds) { (e & 1 ? sum.y : sum.x) += ds; };
+              turn_tile<false, false, false>(ts, bp, bp[0], nullptr, nullptr, lse, dsum, lim, p.c.c2, emit, [](int) {});
+              (lo >= reach ? above : below) += sum.x + sum.y;
             }
           } else {
             const int pos0 = w.first + t * 64, lo = w.t * 128 + q * 32 - pos0 - 63, hi = w.t * 128 + q * 32 + 31 - pos0;
@@ -926,16 +995,12 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
             const int lim = r < w.keys ? (p.c.causal ? r - pos0 : 0) : 64;
             const bool mask = __any_sync(0xffffffffu, lim > 0);
             const float* L = reinterpret_cast<const float*>(gen + (ring - sheld) + st * Cfg::kStage + Cfg::kStream);
-            auto emit = [&](int, int, float) {};
-            if (near) {
-              const float* bp = bias + (r - pos0 + reach + kPad);
-              if (mask) turn_tile<true, true, true>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, emit);
-              else turn_tile<true, true, false>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, emit);
-            } else {
-              const float flat = bias[kPad + (lo >= reach ? 2 * reach : 0)];
-              if (mask) turn_tile<true, false, true>(ts, nullptr, flat, L, L + 64, 0.f, 0.f, lim, p.c.c2, emit);
-              else turn_tile<true, false, false>(ts, nullptr, flat, L, L + 64, 0.f, 0.f, lim, p.c.c2, emit);
-            }
+            const float* bp = bias + (near ? r - pos0 + reach + kPad : lo >= reach ? kPad + 2 * reach + 64 : 64);
+            auto none = [](int, float) {};
+            auto after = [](int) {};
+            if (mask) turn_tile<true, true, true>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
+            else if (near) turn_tile<true, true, false>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
+            else turn_tile<true, false, false>(ts, bp, bp[0], L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
           }
           attn::tmem_st_wait();
           tc_fence_before();
