@@ -1635,10 +1635,10 @@ int rel_bwd(cudaStream_t s, const CUtensorMap (&m)[8], rel::BwdParams& p) {
   using Cfg = rel::BwdCfg<P>;
   constexpr int kMost = 232448;
   // Two held pairs let an item's tiles arrive while the one before computes; they go first where the sums' rows leave no room,
-  // then streamed pairs beyond the two that the pipeline needs.
-  for (p.held = 2; p.held > 1 && Cfg::smem(2, p.held, p.c.pitch, p.c.reach) > kMost; --p.held) {}
-  for (p.stages = 6; p.stages > 2 && Cfg::smem(p.stages, p.held, p.c.pitch, p.c.reach) > kMost; --p.stages) {}
-  static_assert(Cfg::smem(2, 1, 2 * kRelMaxReach + 4 + 2 * rel::kPad, kRelMaxReach) <= kMost, "shared memory of the attention backward kernel");
+  // then streamed pairs beyond those that scores run ahead.
+  for (p.held = 2; p.held > 1 && Cfg::smem(Cfg::kBuf, p.held, p.c.pitch, p.c.reach) > kMost; --p.held) {}
+  for (p.stages = 6; p.stages > Cfg::kBuf && Cfg::smem(p.stages, p.held, p.c.pitch, p.c.reach) > kMost; --p.stages) {}
+  static_assert(Cfg::smem(Cfg::kBuf, 1, 2 * kRelMaxReach + 4 + 2 * rel::kPad, kRelMaxReach) <= kMost, "shared memory of the attention backward kernel");
   const int ctas = sm_count();
   p.chunk_k = p.c.causal ? std::min(p.c.G * p.c.B, std::max(1, (4 * ctas + p.nk - 1) / p.nk)) : 1;
   p.chunk_q = p.c.causal ? std::min(p.c.H * p.c.B, std::max(1, (4 * ctas + p.nq - 1) / p.nq)) : 1;

@@ -566,8 +566,10 @@ __device__ __forceinline__ BwdItem bwd_item(const BwdParams& p, int i) {
 template <int P>
 struct BwdCfg {
   static constexpr int kHeld = 2 * 128 * P * 2, kStream = 2 * 64 * P * 2, kStage = kStream + 1024;
-  static constexpr int kSets = P == 64 ? 2 : 1;      // accumulators: an item's results are stored while the next one computes
-  static constexpr uint32_t kAcc = 256;              // tensor memory: two buffers of scores and dP (64 columns each), accumulators
+  // Tensor memory: buffers of scores and dP (64 columns each), then the accumulators.  A third buffer, where it fits, lets a tile
+  // be multiplied before either group is done with its own: without it a group waits for two products and two hand-overs.
+  static constexpr int kBuf = P == 64 ? 3 : 2;
+  static constexpr uint32_t kAcc = kBuf * 128;
   static constexpr int smem(int stages, int held, int pitch, int reach) {
     return held * kHeld + stages * kStage + 2 * pitch * 4 + 8 * ((2 * reach + 4) & ~3) * 4 + 1024 + 512;
   }
@@ -655,7 +657,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
   const int width = (2 * p.c.reach + 4) & ~3;        // floats of a warp's row of sums
   const uint32_t ssums = sbias + 2u * p.c.pitch * 4u, bars = ssums + 8u * width * 4u;
   const uint32_t item_full = bars, item_empty = bars + 32, h_full = bars + 64, h_empty = bars + 80, b_full = bars + 96, b_empty = bars + 112;
-  const uint32_t s_full = bars + 128, pd_full = bars + 144, acc_full = bars + 160, acc_empty = bars + 176, full = bars + 192, empty = bars + 256;
+  const uint32_t s_full = bars + 128, pd_full = bars + 152, acc_full = bars + 176, acc_empty = bars + 184, full = bars + 192, empty = bars + 256;
   uint8_t* gen = smem_raw + (sheld - raw);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (bars + 320 - sheld));
   volatile int* queue = reinterpret_cast<volatile int*>(gen + (bars + 336 - sheld));
@@ -673,12 +675,14 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       mbar_init(h_empty + 8 * i, 1);
       mbar_init(b_full + 8 * i, 1);
       mbar_init(b_empty + 8 * i, 8);
-      mbar_init(s_full + 8 * i, 1);
-      mbar_init(pd_full + 8 * i, 4);
-      mbar_init(acc_full + 8 * i, 1);
-      mbar_init(acc_empty + 8 * i, 8);
       mbar_init(g_sync + 8 * i, 4);
     }
+    for (int i = 0; i < Cfg::kBuf; ++i) {
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(pd_full + 8 * i, 4);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 8);
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(full + 8 * i, 1);
       mbar_init(empty + 8 * i, 1);
@@ -784,16 +788,16 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       id = __shfl_sync(0xffffffffu, after, 0);
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer: scores at most two tiles ahead of the products that read what became of them ----------------
+    // ---------------- MMA issuer: scores at most kBuf tiles ahead of the products that read what became of them ----------------
     struct Work { int q, tiles, keys; };
     Work even{0, 0, 0}, odd{0, 0, 0};                  // the live item of an even or odd number
     uint32_t sa = 0, sb = 0, na = 0, nb = 0;           // live items and tiles: scores (a) and products (b)
     int ta = 0, tb = 0;
-    uint32_t ra = 0, ra_phase = 0, rb = 0;             // ring slots
+    uint32_t ra = 0, ra_phase = 0, rb = 0, ba = 0, bb = 0, bb_phase = 0;   // ring slots, tensor memory buffers
     bool ok = true, in_a = false, end = false;
     while (ok) {
       const bool pending = na != nb;
-      bool step_a = !end && na - nb < 2u && sa - sb < (uint32_t)p.held;   // (a third live item would overwrite the first's place)
+      bool step_a = !end && na - nb < (uint32_t)Cfg::kBuf && sa - sb < (uint32_t)p.held;   // (a third live item would overwrite the first's place)
       if (step_a && !in_a) {
         // the next live item, without waiting while products are due
         if (pending && !__all_sync(0xffffffffu, mbar_try(item_full + 8 * (taken & 3u), (taken >> 2) & 1u))) step_a = false;
@@ -820,37 +824,38 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         ok = ok && __all_sync(0xffffffffu, mbar_wait(full + 8 * ra, ra_phase, 56));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t x = ring + ra * Cfg::kStage, hd = sheld + hb * Cfg::kHeld, ts = tmem + (na & 1u) * 128u;
+        const uint32_t x = ring + ra * Cfg::kStage, hd = sheld + hb * Cfg::kHeld, ts = tmem + ba * 128u;
         if (w.q && w.keys - ta * 64 < 64) zero_rows<P, 64>(gen + (x - sheld), w.keys - ta * 64, lane);
         if (flash::elect_one()) {
           mma_rows<P, 64>(ts, hd, x);
           mma_rows<P, 64>(ts + 64u, hd + Cfg::kHeld / 2, x + Cfg::kStream / 2);
-          umma_commit(s_full + 8 * (na & 1u));
+          umma_commit(s_full + 8 * ba);
         }
         __syncwarp();
         if (++ra == (uint32_t)p.stages) { ra = 0; ra_phase ^= 1u; }
+        if (++ba == (uint32_t)Cfg::kBuf) ba = 0;
         ++na;
         if (++ta == w.tiles) { in_a = false; ++sa; }
       } else {
         const Work w = sb & 1u ? odd : even;
-        const uint32_t set = Cfg::kSets == 2 ? sb & 1u : 0u, sp = Cfg::kSets == 2 ? sb >> 1 : sb;
-        ok = __all_sync(0xffffffffu, mbar_wait(pd_full + 8 * (nb & 1u), (nb >> 1) & 1u, 57));
-        if (ok && tb == 0) ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * set, (sp & 1u) ^ 1u, 58));
+        ok = __all_sync(0xffffffffu, mbar_wait(pd_full + 8 * bb, bb_phase, 57));
+        if (ok && tb == 0) ok = __all_sync(0xffffffffu, mbar_wait(acc_empty, (sb & 1u) ^ 1u, 58));
         if (!ok) break;
         tc_fence_after();
         const bool last = tb == w.tiles - 1;
         if (flash::elect_one()) {
-          const uint32_t x = ring + rb * Cfg::kStage, ts = tmem + (nb & 1u) * 128u, acc = tmem + Cfg::kAcc + set * 2u * P;
+          const uint32_t x = ring + rb * Cfg::kStage, ts = tmem + bb * 128u, acc = tmem + Cfg::kAcc;
           mma_weighted<P, 64>(acc, ts + 64u, x, tb > 0);                                               // dK += ds Q, dQ += ds K
           if (!w.q) mma_weighted<P, 64>(acc + (uint32_t)P, ts, x + Cfg::kStream / 2, tb > 0);          // dV += softmax dOUT
           umma_commit(empty + 8 * rb);
           if (last) {
             umma_commit(h_empty + 8 * (p.held == 2 ? sb & 1u : 0u));
-            umma_commit(acc_full + 8 * set);
+            umma_commit(acc_full);
           }
         }
         __syncwarp();
         if (++rb == (uint32_t)p.stages) rb = 0;
+        if (++bb == (uint32_t)Cfg::kBuf) { bb = 0; bb_phase ^= 1u; }
         ++nb;
         if (++tb == w.tiles) { tb = 0; ++sb; }
       }
@@ -858,12 +863,12 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
   } else {
     // ---------------- element warps ----------------
     const int q = warp & 3, g = (warp - 2) >> 2, rt = q * 32 + lane;
-    const uint32_t lanes = (uint32_t)(q * 32) << 16, ts = tmem + lanes + g * 128u;
+    const uint32_t lanes = (uint32_t)(q * 32) << 16;
     const int blocks = (p.c.J + 63) >> 6, reach = p.c.reach, entries = 2 * reach + 1;
     float* group_sums = reinterpret_cast<float*>(gen + (ssums - sheld)) + g * 4 * width;
     float* sums = group_sums + ((warp - 2) & 3) * width;
     const int in_group = ((warp - 2) & 3) * 32 + lane;
-    uint32_t n = 0, live = 0, run = 0, st = 0, st_phase = 0;
+    uint32_t n = 0, live = 0, run = 0, st = 0, st_phase = 0, bf = 0, bf_phase = 0;
     bool ok = true, have = false;
     BwdItem prev;
     float below = 0.f, above = 0.f;                    // sums outside the varying part of the bias
@@ -887,14 +892,13 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       }
     };
     auto finish = [&](const BwdItem& it, uint32_t s) {
-      const uint32_t set = Cfg::kSets == 2 ? s & 1u : 0u, sp = Cfg::kSets == 2 ? s >> 1 : s;
-      ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * set, sp & 1u, 59));
+      ok = __all_sync(0xffffffffu, mbar_wait(acc_full, s & 1u, 59));
       if (!ok) return;
       tc_fence_after();
-      store(it, tmem + Cfg::kAcc + set * 2u * P, false);
+      store(it, tmem + Cfg::kAcc, false);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty + 8 * set);
+      if (lane == 0) mbar_arrive(acc_empty);
     };
     auto add = [&](int rel, float v) {
       if (rel <= -reach) below += v;
@@ -957,10 +961,11 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         if ((int)(n & 1u) == g) {
           ok = __all_sync(0xffffffffu, mbar_wait(b_full + 8 * bb, (run >> 1) & 1u, 60)) &&
                __all_sync(0xffffffffu, mbar_wait(full + 8 * st, st_phase, 60)) &&
-               __all_sync(0xffffffffu, mbar_wait(s_full + 8 * g, (n >> 1) & 1u, 60));
+               __all_sync(0xffffffffu, mbar_wait(s_full + 8 * bf, bf_phase, 60));
           if (!ok) break;
           tc_fence_after();
           const float* bias = bias_s + bb * p.c.pitch;
+          const uint32_t ts = tmem + lanes + bf * 128u;
           if (w.q) {
             const int k0 = t * 64, pos0 = w.first + w.t * 128 + q * 32, lo = k0 - pos0 - 31, hi = k0 + 63 - pos0;
             const bool near = hi > -reach && lo < reach;
@@ -1005,7 +1010,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
           attn::tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(pd_full + 8 * g);
+          if (lane == 0) mbar_arrive(pd_full + 8 * bf);
           if (due) {
             finish(prev, live - 1u);
             if (!ok) break;
@@ -1013,6 +1018,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
           }
         }
         if (++st == (uint32_t)p.stages) { st = 0; st_phase ^= 1u; }
+        if (++bf == (uint32_t)Cfg::kBuf) { bf = 0; bf_phase ^= 1u; }
         ++t;
         if (--left == 0) {
           t = w.t0;
