@@ -1600,7 +1600,7 @@ template <int P>
 int rel_fwd(cudaStream_t s, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, rel::FwdParams& p) {
   using Cfg = rel::FwdCfg<P>;
   constexpr int kMostPitch = (2 * kRelMaxReach + 1 + 2 * rel::kPad + 3) / 4 * 4;
-  static_assert(2 * (Cfg::kTiles + 2 * kMostPitch * 4 + 1024 + 256 + 1024) <= 233472, "two CTAs of the attention forward kernel per SM");
+  static_assert(2 * (Cfg::smem(kMostPitch) + 1024) <= 233472, "two CTAs of the attention forward kernel per SM");
   // Two CTAs per SM, but the machine may place one on each SM first: within a budget there is one for every SM of it.
   const int ctas = sm_count() < device_sms() ? sm_count() : 2 * sm_count();
   p.chunk = p.c.causal ? std::min(p.units, std::max(1, (4 * ctas + p.nq - 1) / p.nq)) : 1;
@@ -1616,7 +1616,7 @@ int launch_rel_tiles_fwd(cudaStream_t s, Proj q, Proj k, Proj v, RelTables t, Pr
   if (!g_encode) return fail(SB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   std::string why;
   CUtensorMap mq, mk, mv;
-  if (!rel_map(q, 128, &mq, &why) || !rel_map(k, 128, &mk, &why) || !rel_map(v, 128, &mv, &why))
+  if (!rel_map(q, 128, &mq, &why) || !rel_map(k, 64, &mk, &why) || !rel_map(v, 64, &mv, &why))
     return fail(SB_ERR_UNSUPPORTED, "relative attention, operands: " + why);
   rel::FwdParams p;
   p.c = rel_common(q, k, t, span);

@@ -150,7 +150,7 @@ __device__ __forceinline__ void store_features(sb_half* ptr, long long sP, const
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------
-constexpr int kFwdThreads = 192;                     // producer warp, MMA warp, four softmax warps
+constexpr int kFwdThreads = 224;                     // producer warp, two MMA warps, four softmax warps
 
 struct FwdParams {
   Common c;
@@ -173,20 +173,21 @@ __device__ __forceinline__ Item item_of(const FwdParams& p, int i) {
   it.first = first_of(p.c, it.b);
   it.keys = keys_of(p.c, it.b);
   if (p.c.causal) it.keys = max(0, min(it.keys, it.first + min(p.c.J, it.t * 128 + 128)));
-  it.tiles = (it.keys + 127) >> 7;
+  it.tiles = (it.keys + 63) >> 6;
   return it;
 }
 
+// Tiles of 64 keys.  Tensor memory: two buffers of scores (64 columns each), which their exponentials overwrite, then the output.
 // Shared memory of a CTA (two per SM): query tiles, the ring of key and value tiles, two rows of biases, barriers.
 template <int P>
 struct FwdCfg {
-  static constexpr int kTile = 128 * P * 2;
+  static constexpr int kN = 64;
+  static constexpr uint32_t kO = 2 * kN;
+  static constexpr int kQTile = 128 * P * 2, kTile = kN * P * 2;
   static constexpr int kQ = P == 64 ? 2 : 1;         // query tiles (the next item's is fetched early)
-  static constexpr int kRing = P == 64 ? 4 : 2;
-  static constexpr int kTiles = (kQ + kRing) * kTile;
-  static constexpr bool kAlias = P == 128;           // the exponentials overwrite their scores
-  static constexpr uint32_t kPm = kAlias ? 0 : 128, kO = kAlias ? 128 : 192;   // tensor memory columns; scores at 0
-  static int smem(int pitch) { return kTiles + 2 * pitch * 4 + 1024 + 256; }
+  static constexpr int kRing = P == 64 ? 8 : 4;
+  static constexpr int kTiles = kQ * kQTile + kRing * kTile;
+  static constexpr int smem(int pitch) { return kTiles + 2 * pitch * 4 + 1024 + 320; }
 };
 
 // A row's state: reference of its exponentials, their sum so far.
@@ -223,13 +224,13 @@ __device__ __noinline__ void rescale(uint32_t to, uint32_t tp, bool started, int
   attn::tmem_st_wait();
 }
 
-// A thread's row of 128 scores, 32 columns at a time while the next 32 are on their way: exponentials against the row's
-// reference as 16-bit pairs into tensor memory (where they may overwrite scores already read).  The reference lags behind the
+// A thread's row of 64 scores, 32 columns at a time while the next 32 are on their way: exponentials against the row's
+// reference as 16-bit pairs, which overwrite scores already read.  `settled` waits for the output.  The reference lags behind the
 // maximum by at most 2^kLazy; a chunk that exceeds it makes it rise before its own exponentials are taken.
 // NEAR: the bias varies, bp[c] is column c's; else it is `flat`.  MASK: columns from lim on are hidden.
-template <int P, bool NEAR, bool MASK>
-__device__ __forceinline__ void row_tile(uint32_t s, uint32_t tp, uint32_t to, bool started, const float* bp, float flat, int lim, float c2,
-                                         Row& row) {
+template <int P, bool NEAR, bool MASK, class Settled>
+__device__ __forceinline__ void row_tile(uint32_t s, uint32_t to, bool started, const float* bp, float flat, int lim, float c2, Row& row,
+                                         Settled&& settled) {
   float2 sum = make_float2(0.f, 0.f);
   const float2 c22 = make_float2(c2, c2);
   auto chunk = [&](int c, uint32_t* r, uint32_t* coming) {
@@ -261,7 +262,8 @@ __device__ __forceinline__ void row_tile(uint32_t s, uint32_t tp, uint32_t to, b
         sum.x *= f;
         sum.y *= f;
         attn::tmem_ld_wait32(coming);                    // (a call moves registers)
-        rescale<P>(to, tp, started, c, f);
+        settled();
+        rescale<P>(to, s, started, c, f);
       }
     }
     const float ref = row.m == -INFINITY ? 0.f : row.m;
@@ -275,38 +277,34 @@ __device__ __forceinline__ void row_tile(uint32_t s, uint32_t tp, uint32_t to, b
       sum = add2(sum, x);
       w[e >> 1] = flash::pack2(x.x, x.y);
     }
-    tmem_st16(tp + c * 16, w);
+    tmem_st16(s + c * 16, w);
   };
   uint32_t ra[32], rb[32];
   tmem_ld32_nowait(s, ra);
-#pragma unroll 1
-  for (int c = 0; c < 4; c += 2) {
-    attn::tmem_ld_wait32(ra);
-    tmem_ld32_nowait(s + c * 32 + 32, rb);
-    chunk(c, ra, rb);
-    attn::tmem_ld_wait32(rb);
-    if (c == 0) tmem_ld32_nowait(s + 64, ra);
-    chunk(c + 1, rb, ra);
-  }
+  attn::tmem_ld_wait32(ra);
+  tmem_ld32_nowait(s + 32, rb);
+  chunk(0, ra, rb);
+  attn::tmem_ld_wait32(rb);
+  chunk(1, rb, ra);
   row.l += sum.x + sum.y;
 }
 
-// One CTA: 128 queries of one unit against its keys in tiles of 128; two CTAs per SM, so that one's tensor and copy work runs
-// beside the other's softmax.  Tensor memory: scores [128 x 128], their exponentials as 16-bit pairs (the second product's
-// operand comes from there) and the output [128 x P].  Softmax warps: thread = row, exponentials against a reference that may
-// lag 2^8 behind the maximum; only beyond is the output rescaled.
+// One CTA: 128 queries of one unit against its keys; two CTAs per SM.  Scores are multiplied a tile ahead of the softmax, by a
+// warp of their own: with one warp for both products and one buffer, issuing and handing over took most of the time (B=2,
+// L=4096: 140 us of 270 without any softmax).  Exponentials go back into tensor memory as 16-bit pairs, where the second product
+// takes them from.  Softmax warps: thread = row.
 template <int P>
 __global__ void __launch_bounds__(kFwdThreads, 2)
 rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                const __grid_constant__ FwdParams p) {
   using Cfg = FwdCfg<P>;
-  constexpr int kRing = Cfg::kRing, kQ = Cfg::kQ;
+  constexpr int kRing = Cfg::kRing, kQ = Cfg::kQ, N = Cfg::kN;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
-  const uint32_t sq = (raw + 1023u) & ~1023u, ring = sq + kQ * Cfg::kTile;
+  const uint32_t sq = (raw + 1023u) & ~1023u, ring = sq + kQ * Cfg::kQTile;
   const uint32_t sbias = sq + Cfg::kTiles, bars = sbias + 2u * p.c.pitch * 4u;
-  const uint32_t q_full = bars, q_empty = bars + 16, s_full = bars + 32, p_full = bars + 40, p_free = bars + 48, o_empty = bars + 56;
-  const uint32_t b_full = bars + 64, b_empty = bars + 80, kv_full = bars + 96, kv_empty = kv_full + 8 * kRing;
+  const uint32_t q_full = bars, q_empty = bars + 16, s_full = bars + 32, p_full = bars + 48, o_empty = bars + 64;
+  const uint32_t b_full = bars + 80, b_empty = bars + 96, p_free = bars + 112, kv_full = bars + 128, kv_empty = kv_full + 8 * kRing;
   uint8_t* gen = smem_raw + (sq - raw);
   const float* bias_s = reinterpret_cast<const float*>(gen + (sbias - sq));
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (kv_empty + 8 * kRing - sq));
@@ -318,10 +316,10 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       mbar_init(q_empty + 8 * i, 1);
       mbar_init(b_full + 8 * i, 1);
       mbar_init(b_empty + 8 * i, 4);
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_full + 8 * i, 4);
+      mbar_init(p_free + 8 * i, 1);
     }
-    mbar_init(s_full, 1);
-    mbar_init(p_full, 4);
-    mbar_init(p_free, 1);
     mbar_init(o_empty, 4);
     for (int i = 0; i < kRing; ++i) {
       mbar_init(kv_full + 8 * i, 1);
@@ -356,8 +354,8 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
            __all_sync(0xffffffffu, mbar_wait(b_empty + 8 * bb, ((it >> 1) & 1u) ^ 1u, 41));
       if (!ok) break;
       if (lane == 0) {
-        mbar_expect_tx(q_full + 8 * qb, Cfg::kTile);
-        load_rows<P, 128>(sq + qb * Cfg::kTile, &tmQ, q_full + 8 * qb, w.t * 128, w.h, w.b);
+        mbar_expect_tx(q_full + 8 * qb, Cfg::kQTile);
+        load_rows<P, 128>(sq + qb * Cfg::kQTile, &tmQ, q_full + 8 * qb, w.t * 128, w.h, w.b);
         mbar_expect_tx(b_full + 8 * bb, p.c.pitch * 4);
         bulk_load(sbias + bb * p.c.pitch * 4, p.c.bias_rows + (long long)w.h * p.c.pitch, p.c.pitch * 4, b_full + 8 * bb);
       }
@@ -369,62 +367,57 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         if (!ok) break;
         if (lane == 0) {
           mbar_expect_tx(kv_full + 8 * s, Cfg::kTile);
-          load_rows<P, 128>(ring + s * Cfg::kTile, i & 1 ? &tmV : &tmK, kv_full + 8 * s, (i >> 1) * 128, hk, w.b);
+          load_rows<P, N>(ring + s * Cfg::kTile, i & 1 ? &tmV : &tmK, kv_full + 8 * s, (i >> 1) * N, hk, w.b);
         }
         __syncwarp();
       }
       ++it;
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    uint32_t it = 0, n = 0, x = 0;                       // x: ring uses before this item
+    // ---------------- MMA issuer of scores, a tile ahead of the softmax ----------------
+    uint32_t it = 0, n = 0;                              // ring uses are 2 n (keys) and 2 n + 1 (values)
     bool ok = true;
     for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
       const Item w = item_of(p, item);
       if (w.tiles == 0) continue;
       const uint32_t qb = it % kQ;
-      auto slot_full = [&](uint32_t use) {
-        ok = __all_sync(0xffffffffu, mbar_wait(kv_full + 8 * (use % kRing), (use / kRing) & 1u, 42));
+      ok = __all_sync(0xffffffffu, mbar_wait(q_full + 8 * qb, (it / kQ) & 1u, 42));
+      for (int i = 0; i < w.tiles && ok; ++i, ++n) {
+        const uint32_t s = 2 * n % kRing, sb = n & 1u;
+        ok = __all_sync(0xffffffffu, mbar_wait(kv_full + 8 * s, (2 * n / kRing) & 1u, 42) && mbar_wait(p_free + 8 * sb, ((n >> 1) & 1u) ^ 1u, 42));
+        if (!ok) break;
         tc_fence_after();
-        return ok;
-      };
-      auto scores = [&](int i) {
-        const uint32_t use = x + 2u * i, s = use % kRing;
-        if (!slot_full(use)) return;
         if (flash::elect_one()) {
-          mma_rows<P, 128>(tmem, sq + qb * Cfg::kTile, ring + s * Cfg::kTile);
-          umma_commit(s_full);
+          mma_rows<P, N>(tmem + sb * N, sq + qb * Cfg::kQTile, ring + s * Cfg::kTile);
+          umma_commit(s_full + 8 * sb);
           umma_commit(kv_empty + 8 * s);
           if (i == w.tiles - 1) umma_commit(q_empty + 8 * qb);
         }
         __syncwarp();
-      };
-      ok = __all_sync(0xffffffffu, mbar_wait(q_full + 8 * qb, (it / kQ) & 1u, 42));
-      if (!ok) break;
-      scores(0);
-      for (int i = 0; i < w.tiles && ok; ++i, ++n) {
-        ok = __all_sync(0xffffffffu, mbar_wait(p_full, n & 1u, 43));   // the scores have been read, their exponentials written
+      }
+      ++it;
+    }
+  } else if (warp == 2) {
+    // ---------------- MMA issuer of the output ----------------
+    uint32_t it = 0, n = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
+      const Item w = item_of(p, item);
+      if (w.tiles == 0) continue;
+      for (int i = 0; i < w.tiles; ++i, ++n) {
+        const uint32_t s = (2 * n + 1) % kRing, sb = n & 1u;
+        ok = __all_sync(0xffffffffu, mbar_wait(kv_full + 8 * s, ((2 * n + 1) / kRing) & 1u, 43));
+        if (ok && w.keys - i * N < N) zero_rows<P, N>(gen + (ring - sq) + s * Cfg::kTile, w.keys - i * N, lane);
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(p_full + 8 * sb, (n >> 1) & 1u, 43) && (i > 0 || mbar_wait(o_empty, (it & 1u) ^ 1u, 44)));
         if (!ok) break;
         tc_fence_after();
-        if (!Cfg::kAlias && i + 1 < w.tiles) scores(i + 1);
-        if (!ok) break;
-        const uint32_t use = x + 2u * i + 1u, s = use % kRing;
-        if (!slot_full(use)) break;
-        if (w.keys - i * 128 < 128) zero_rows<P, 128>(gen + (ring - sq) + s * Cfg::kTile, w.keys - i * 128, lane);
-        if (i == 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(o_empty, (it & 1u) ^ 1u, 44));
-          if (!ok) break;
-          tc_fence_after();
-        }
         if (flash::elect_one()) {
-          mma_weighted<P, 128>(tmem + Cfg::kO, tmem + Cfg::kPm, ring + s * Cfg::kTile, i > 0);
+          mma_weighted<P, N>(tmem + Cfg::kO, tmem + sb * N, ring + s * Cfg::kTile, i > 0);
           umma_commit(kv_empty + 8 * s);
-          umma_commit(p_free);
+          umma_commit(p_free + 8 * sb);
         }
         __syncwarp();
-        if (Cfg::kAlias && i + 1 < w.tiles) scores(i + 1);
       }
-      x += 2u * w.tiles;
       ++it;
     }
   } else {
@@ -432,7 +425,7 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     const int q = warp & 3;
     const int rt = q * 32 + lane;
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
-    const uint32_t ts = tmem + lanes, tp = ts + Cfg::kPm, to = ts + Cfg::kO;
+    const uint32_t to = tmem + lanes + Cfg::kO;
     uint32_t n = 0, it = 0;
     bool ok = true;
     for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
@@ -449,36 +442,37 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         if (!ok) break;
       }
       for (int kb = 0; kb < w.tiles; ++kb, ++n) {
-        const int lim = mine - kb * 128;
-        const int rel0 = kb * 128 - pos;                 // relative position of the first column
-        const int lo = kb * 128 - (w.first + w.t * 128 + q * 32 + 31), hi = kb * 128 + 127 - (w.first + w.t * 128 + q * 32);
+        const int lim = mine - kb * N;
+        const int rel0 = kb * N - pos;                 // relative position of the first column
+        const int lo = kb * N - (w.first + w.t * 128 + q * 32 + 31), hi = kb * N + N - 1 - (w.first + w.t * 128 + q * 32);
+        const uint32_t sb = n & 1u, ts = tmem + lanes + sb * N;
         const bool near = hi > -p.c.reach && lo < p.c.reach;
-        const bool mask = __any_sync(0xffffffffu, lim < 128);
-        // outside the varying part, a place in the row where 128 entries have the end's value
+        const bool mask = __any_sync(0xffffffffu, lim < N);
+        // outside the varying part, a place in the row where N entries have the end's value
         const float* bp = bias + (near ? rel0 + p.c.reach + kPad : lo >= p.c.reach ? kPad + 2 * p.c.reach : 0);
         const float flat = bp[0];
-        ok = __all_sync(0xffffffffu, mbar_wait(s_full, n & 1u, 46));
+        ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * sb, (n >> 1) & 1u, 46));
         if (!ok) break;
         tc_fence_after();
-        if (n > 0) {                                     // the previous output product has read its exponentials
-          ok = __all_sync(0xffffffffu, mbar_wait(p_free, (n - 1u) & 1u, 47));
-          if (!ok) break;
+        auto settled = [&] {                             // every product so far is in the output
+          ok = kb == 0 || __all_sync(0xffffffffu, mbar_wait(p_free + 8 * ((n - 1u) & 1u), ((n - 1u) >> 1) & 1u, 47));
           tc_fence_after();
-        }
-        if (mask) row_tile<P, true, true>(ts, tp, to, kb > 0, bp, 0.f, lim, p.c.c2, state);
-        else if (near) row_tile<P, true, false>(ts, tp, to, kb > 0, bp, 0.f, lim, p.c.c2, state);
-        else row_tile<P, false, false>(ts, tp, to, kb > 0, bp, flat, lim, p.c.c2, state);
+        };
+        if (mask) row_tile<P, true, true>(ts, to, kb > 0, bp, 0.f, lim, p.c.c2, state, settled);
+        else if (near) row_tile<P, true, false>(ts, to, kb > 0, bp, 0.f, lim, p.c.c2, state, settled);
+        else row_tile<P, false, false>(ts, to, kb > 0, bp, flat, lim, p.c.c2, state, settled);
+        if (!ok) break;
         attn::tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
+        if (lane == 0) mbar_arrive(p_full + 8 * sb);
       }
       if (!ok) break;
       sb_half* out = reinterpret_cast<sb_half*>(p.out.p) + (long long)w.h * p.out.sH + (long long)w.b * p.out.sB + (long long)j * p.out.sR;
       const float inv = state.l > 0.f ? 1.f / state.l : 0.f;
       if (w.tiles > 0) {
         if (lane == 0) mbar_arrive(b_empty + 8 * bb);
-        ok = __all_sync(0xffffffffu, mbar_wait(p_free, (n - 1u) & 1u, 47));
+        ok = __all_sync(0xffffffffu, mbar_wait(p_free + 8 * ((n - 1u) & 1u), ((n - 1u) >> 1) & 1u, 47));
         if (!ok) break;
         tc_fence_after();
       }
@@ -515,7 +509,7 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------
-constexpr int kBwdThreads = 320;                     // producer warp, MMA warp, two groups of four element warps
+constexpr int kBwdThreads = 352;                     // producer warp, two MMA warps, two groups of four element warps
 constexpr int kRecord = 192;                         // floats of 64 query rows: log2-sum-exps, D, weights of the table's sums
 
 struct BwdParams {
@@ -661,14 +655,14 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
   uint8_t* gen = smem_raw + (sheld - raw);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (bars + 320 - sheld));
   volatile int* queue = reinterpret_cast<volatile int*>(gen + (bars + 336 - sheld));
-  const uint32_t g_sync = bars + 352;
+  const uint32_t g_sync = bars + 352, buf_free = bars + 368;
   const float* bias_s = reinterpret_cast<const float*>(gen + (sbias - sheld));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) {
       mbar_init(item_full + 8 * i, 1);
-      mbar_init(item_empty + 8 * i, 9);
+      mbar_init(item_empty + 8 * i, 10);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(h_full + 8 * i, 1);
@@ -680,6 +674,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     for (int i = 0; i < Cfg::kBuf; ++i) {
       mbar_init(s_full + 8 * i, 1);
       mbar_init(pd_full + 8 * i, 4);
+      mbar_init(buf_free + 8 * i, 1);
     }
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, 8);
@@ -788,86 +783,67 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       id = __shfl_sync(0xffffffffu, after, 0);
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer: scores at most kBuf tiles ahead of the products that read what became of them ----------------
-    struct Work { int q, tiles, keys; };
-    Work even{0, 0, 0}, odd{0, 0, 0};                  // the live item of an even or odd number
-    uint32_t sa = 0, sb = 0, na = 0, nb = 0;           // live items and tiles: scores (a) and products (b)
-    int ta = 0, tb = 0;
-    uint32_t ra = 0, ra_phase = 0, rb = 0, ba = 0, bb = 0, bb_phase = 0;   // ring slots, tensor memory buffers
-    bool ok = true, in_a = false, end = false;
-    while (ok) {
-      const bool pending = na != nb;
-      bool step_a = !end && na - nb < (uint32_t)Cfg::kBuf && sa - sb < (uint32_t)p.held;   // (a third live item would overwrite the first's place)
-      if (step_a && !in_a) {
-        // the next live item, without waiting while products are due
-        if (pending && !__all_sync(0xffffffffu, mbar_try(item_full + 8 * (taken & 3u), (taken >> 2) & 1u))) step_a = false;
-        else {
-          BwdItem w;
-          if (!take(&w, &ok)) {
-            end = true;
-          } else if (w.tiles > 0) {
-            (sa & 1u ? odd : even) = Work{w.q ? 1 : 0, w.tiles, w.keys};
-            in_a = true;
-            ta = 0;
-          }
-          continue;
-        }
-      }
-      if (!step_a && !pending) {
-        if (end) break;
-        continue;                                       // (not reached: with nothing pending the next item may start)
-      }
-      if (step_a) {
-        const Work w = sa & 1u ? odd : even;
-        const uint32_t hb = p.held == 2 ? sa & 1u : 0u, hp = p.held == 2 ? sa >> 1 : sa;
-        if (ta == 0) ok = __all_sync(0xffffffffu, mbar_wait(h_full + 8 * hb, hp & 1u, 56));
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(full + 8 * ra, ra_phase, 56));
+    // ---------------- MMA issuer of scores and dP ----------------
+    uint32_t live = 0, st = 0, st_phase = 0, bf = 0, bf_phase = 1;
+    bool ok = true;
+    BwdItem w;
+    while (ok && take(&w, &ok)) {
+      if (w.tiles == 0) continue;
+      const uint32_t hb = p.held == 2 ? live & 1u : 0u, hp = p.held == 2 ? live >> 1 : live, hd = sheld + hb * Cfg::kHeld;
+      ok = __all_sync(0xffffffffu, mbar_wait(h_full + 8 * hb, hp & 1u, 56));
+      for (int i = 0; i < w.tiles && ok; ++i) {
+        ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * st, st_phase, 56) && mbar_wait(buf_free + 8 * bf, bf_phase, 56));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t x = ring + ra * Cfg::kStage, hd = sheld + hb * Cfg::kHeld, ts = tmem + ba * 128u;
-        if (w.q && w.keys - ta * 64 < 64) zero_rows<P, 64>(gen + (x - sheld), w.keys - ta * 64, lane);
+        const uint32_t x = ring + st * Cfg::kStage, ts = tmem + bf * 128u;
+        if (w.q && w.keys - i * 64 < 64) zero_rows<P, 64>(gen + (x - sheld), w.keys - i * 64, lane);
         if (flash::elect_one()) {
           mma_rows<P, 64>(ts, hd, x);
           mma_rows<P, 64>(ts + 64u, hd + Cfg::kHeld / 2, x + Cfg::kStream / 2);
-          umma_commit(s_full + 8 * ba);
+          umma_commit(s_full + 8 * bf);
         }
         __syncwarp();
-        if (++ra == (uint32_t)p.stages) { ra = 0; ra_phase ^= 1u; }
-        if (++ba == (uint32_t)Cfg::kBuf) ba = 0;
-        ++na;
-        if (++ta == w.tiles) { in_a = false; ++sa; }
-      } else {
-        const Work w = sb & 1u ? odd : even;
-        ok = __all_sync(0xffffffffu, mbar_wait(pd_full + 8 * bb, bb_phase, 57));
-        if (ok && tb == 0) ok = __all_sync(0xffffffffu, mbar_wait(acc_empty, (sb & 1u) ^ 1u, 58));
+        if (++st == (uint32_t)p.stages) { st = 0; st_phase ^= 1u; }
+        if (++bf == (uint32_t)Cfg::kBuf) { bf = 0; bf_phase ^= 1u; }
+      }
+      ++live;
+    }
+  } else if (warp == 2) {
+    // ---------------- MMA issuer of the products that read what became of them ----------------
+    uint32_t live = 0, st = 0, bf = 0, bf_phase = 0;
+    bool ok = true;
+    BwdItem w;
+    while (ok && take(&w, &ok)) {
+      if (w.tiles == 0) continue;
+      for (int i = 0; i < w.tiles; ++i) {
+        ok = __all_sync(0xffffffffu, mbar_wait(pd_full + 8 * bf, bf_phase, 57) && (i > 0 || mbar_wait(acc_empty, (live & 1u) ^ 1u, 58)));
         if (!ok) break;
         tc_fence_after();
-        const bool last = tb == w.tiles - 1;
         if (flash::elect_one()) {
-          const uint32_t x = ring + rb * Cfg::kStage, ts = tmem + bb * 128u, acc = tmem + Cfg::kAcc;
-          mma_weighted<P, 64>(acc, ts + 64u, x, tb > 0);                                               // dK += ds Q, dQ += ds K
-          if (!w.q) mma_weighted<P, 64>(acc + (uint32_t)P, ts, x + Cfg::kStream / 2, tb > 0);          // dV += softmax dOUT
-          umma_commit(empty + 8 * rb);
-          if (last) {
-            umma_commit(h_empty + 8 * (p.held == 2 ? sb & 1u : 0u));
+          const uint32_t x = ring + st * Cfg::kStage, ts = tmem + bf * 128u, acc = tmem + Cfg::kAcc;
+          mma_weighted<P, 64>(acc, ts + 64u, x, i > 0);                                               // dK += ds Q, dQ += ds K
+          if (!w.q) mma_weighted<P, 64>(acc + (uint32_t)P, ts, x + Cfg::kStream / 2, i > 0);          // dV += softmax dOUT
+          umma_commit(empty + 8 * st);
+          umma_commit(buf_free + 8 * bf);
+          if (i == w.tiles - 1) {
+            umma_commit(h_empty + 8 * (p.held == 2 ? live & 1u : 0u));
             umma_commit(acc_full);
           }
         }
         __syncwarp();
-        if (++rb == (uint32_t)p.stages) rb = 0;
-        if (++bb == (uint32_t)Cfg::kBuf) { bb = 0; bb_phase ^= 1u; }
-        ++nb;
-        if (++tb == w.tiles) { tb = 0; ++sb; }
+        if (++st == (uint32_t)p.stages) st = 0;
+        if (++bf == (uint32_t)Cfg::kBuf) { bf = 0; bf_phase ^= 1u; }
       }
+      ++live;
     }
   } else {
     // ---------------- element warps ----------------
-    const int q = warp & 3, g = (warp - 2) >> 2, rt = q * 32 + lane;
+    const int q = warp & 3, g = (warp - 3) >> 2, rt = q * 32 + lane;
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
     const int blocks = (p.c.J + 63) >> 6, reach = p.c.reach, entries = 2 * reach + 1;
     float* group_sums = reinterpret_cast<float*>(gen + (ssums - sheld)) + g * 4 * width;
-    float* sums = group_sums + ((warp - 2) & 3) * width;
-    const int in_group = ((warp - 2) & 3) * 32 + lane;
+    float* sums = group_sums + ((warp - 3) & 3) * width;
+    const int in_group = ((warp - 3) & 3) * 32 + lane;
     uint32_t n = 0, live = 0, run = 0, st = 0, st_phase = 0, bf = 0, bf_phase = 0;
     bool ok = true, have = false;
     BwdItem prev;
