@@ -72,7 +72,6 @@ _T = ctypes.POINTER(SbTensor)
 _D = ctypes.POINTER(SbDropout)
 _PP = ctypes.POINTER(c_void_p)
 _SZ = ctypes.c_size_t
-_R, _RB, _AS = ctypes.POINTER(SbRotation), ctypes.POINTER(SbRelativeBias), ctypes.POINTER(SbAttentionSpan)
 
 #: every exported symbol with (restype, argtypes); the CPU test suite checks the
 #: library exports exactly these
@@ -103,13 +102,14 @@ SIGNATURES = {
                         ctypes.c_size_t]),
     'sb_einsum_fused': (c_int, [c_void_p, c_char_p, _T, c_char_p, _T, c_char_p, _T, c_float, ctypes.POINTER(SbEpilogue)]),
     'sb_einsum_last_impl': (c_int, []),
-    'sb_query_key_norm_rotation': (c_int, [c_void_p] + [_T] * 7 + [_R]),
+    # (structures of these go over as packed bytes or by reference: building ctypes objects took longer than the kernels)
+    'sb_query_key_norm_rotation': (c_int, [c_void_p] * 9),
     'sb_query_key_norm_scratch_bytes': (_SZ, []),
-    'sb_backward_query_key_norm_rotation': (c_int, [c_void_p, c_void_p, _SZ] + [_T] * 11 + [_R]),
-    'sb_relative_attention': (c_int, [c_void_p, c_void_p, _SZ, _T, _T, _T, _RB, _T, _T, _AS]),
-    'sb_relative_attention_scratch_bytes': (c_int, [_T, _T, _T, _RB, ctypes.POINTER(_SZ)]),
-    'sb_backward_relative_attention': (c_int, [c_void_p, c_void_p, _SZ, _T, _T, _T, _T, _RB] + [_T] * 6 + [_AS]),
-    'sb_backward_relative_attention_scratch_bytes': (c_int, [_T, _T, _T, _T, _RB, ctypes.POINTER(_SZ)]),
+    'sb_backward_query_key_norm_rotation': (c_int, [c_void_p, c_void_p, _SZ] + [c_void_p] * 12),
+    'sb_relative_attention': (c_int, [c_void_p, c_void_p, _SZ] + [c_void_p] * 7),
+    'sb_relative_attention_scratch_bytes': (c_int, [c_void_p] * 4 + [ctypes.POINTER(_SZ)]),
+    'sb_backward_relative_attention': (c_int, [c_void_p, c_void_p, _SZ] + [c_void_p] * 12),
+    'sb_backward_relative_attention_scratch_bytes': (c_int, [c_void_p] * 5 + [ctypes.POINTER(_SZ)]),
     'sb_device_error': (c_int, [c_void_p, ctypes.POINTER(c_int)]),
     'sb_device_error_reset': (c_int, [c_void_p]),
     'sb_mma_peak_probe': (c_int, [c_void_p, c_int, c_int, ctypes.POINTER(ctypes.c_double)]),

@@ -10,6 +10,7 @@ import bisect
 import contextlib
 import ctypes
 import functools
+import struct
 import threading
 
 import torch
@@ -326,34 +327,67 @@ def set_sm_budget(n_sms):
 _PAIRING = {'halves': _lib.SB_PAIR_HALVES, 'adjacent': _lib.SB_PAIR_ADJACENT}
 
 
-def _here(*tensors):
-    """All operands of a call are CUDA tensors of one device; returns it as the current one for the call."""
-    _check_cuda(*tensors)
-    dev = tensors[0].device
-    for t in tensors:
-        if t.device != dev:
-            raise ValueError(f'operands on {dev} and on {t.device}')
-    return torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else contextlib.nullcontext()
+# SbTensor, SbRotation, SbRelativeBias and SbAttentionSpan as packed bytes
+_TENSOR, _ROTATION, _BIAS, _SPAN = (struct.Struct(f) for f in ('Pi4x10q', 'diif4x', 'PiiP', 'fiPP'))
+_half_libs = {}
+
+
+def _packed(t):
+    """SbTensor of a tensor, or NULL."""
+    if t is None:
+        return None
+    shape, stride = t.shape, t.stride()
+    n = len(shape)
+    if n == 4:
+        return _TENSOR.pack(t.data_ptr(), 4, *shape, 0, *stride, 0)
+    if n > _lib.SB_MAX_DIMS:
+        raise ValueError(f'at most {_lib.SB_MAX_DIMS} dimensions, got {n}')
+    fill = (0,) * (_lib.SB_MAX_DIMS - n)
+    return _TENSOR.pack(t.data_ptr(), n, *shape, *fill, *stride, *fill)
+
+
+def _operands(half, others=()):
+    """Checks what a call's tensors have in common: CUDA tensors of one device, one 16-bit storage type (``half``).  Returns the
+    library of that type, the device's index, and a context in which it is the current device."""
+    dev, dt = half[0].get_device(), half[0].dtype
+    for t in half:
+        if t.get_device() != dev or dev < 0:
+            _check_cuda(t)
+            raise ValueError(f'operands on {half[0].device} and on {t.device}')
+        if t.dtype is not dt:
+            raise TypeError(f'operands mix {dt} and {t.dtype}')
+    for t in others:
+        if t.get_device() != dev:
+            _check_cuda(t)
+            raise ValueError(f'operands on {half[0].device} and on {t.device}')
+    lib = _half_libs.get(dt)
+    if lib is None:
+        if dt not in (torch.float16, torch.bfloat16):
+            raise TypeError(f'expected float16 or bfloat16, got {dt}')
+        lib = _half_libs[dt] = _lib.load(dt)
+    return lib, dev, _NOTHING if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
+_NOTHING = contextlib.nullcontext()
 
 
 def _int32(t, what):
-    if t.dtype != torch.int32:
+    if t.dtype is not torch.int32:
         raise TypeError(f'{what} are int32, got {t.dtype}')
 
 
-def _scratch(nbytes, device):
+def _scratch(nbytes, like):
     """Device memory of one call, from torch's allocator: calls on several streams, and graphs that were captured with
     them, have their own."""
-    if nbytes == 0:
-        return None, ctypes.c_void_p(None)
-    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return t, ctypes.c_void_p(t.data_ptr())
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 def _rotation(q, base, rotary, pairing, eps):
-    r = _lib.SbRotation()
-    r.base, r.rotary, r.pairing, r.eps = float(base), q.shape[0] if rotary is None else int(rotary), _PAIRING[pairing], float(eps)
-    return ctypes.byref(r)
+    return _ROTATION.pack(base, q.shape[0] if rotary is None else rotary, _PAIRING[pairing], eps)
 
 
 def query_key_norm_rotation(q, k, q_gain, k_gain, positions, q_out, k_out, base=10000.0, rotary=None, pairing='halves', eps=1e-6):
@@ -361,25 +395,26 @@ def query_key_norm_rotation(q, k, q_gain, k_gain, positions, q_out, k_out, base=
     rotation of the first ``rotary`` features (None: all) by the tokens' int32 ``positions`` [B,J]; one pass over both.
     ``pairing``: 'halves' turns features i and i + rotary/2 together, 'adjacent' 2i and 2i+1.  ``k``, ``k_gain`` and ``k_out``
     may be None.  An output may be its input."""
-    some = _given(q, k, q_gain, k_gain, q_out, k_out)
-    with _here(*some, positions):
-        _half(*some); _int32(positions, 'positions')
-        check(_cur().sb_query_key_norm_rotation(_stream(), _d(q), _opt(k), _d(q_gain), _opt(k_gain), _d(positions), _d(q_out),
-                                                _opt(k_out), _rotation(q, base, rotary, pairing, eps)))
+    _int32(positions, 'positions')
+    lib, dev, here = _operands([q, q_gain, q_out] + _given(k, k_gain, k_out), (positions,))
+    with here:
+        _lib.check(lib.sb_query_key_norm_rotation(
+            torch._C._cuda_getCurrentRawStream(dev), _packed(q), _packed(k), _packed(q_gain), _packed(k_gain), _packed(positions),
+            _packed(q_out), _packed(k_out), _rotation(q, base, rotary, pairing, eps)), lib)
 
 
 def backward_query_key_norm_rotation(dq_out, dk_out, q, k, q_gain, k_gain, positions, dq, dk, dq_gain, dk_gain, base=10000.0,
                                      rotary=None, pairing='halves', eps=1e-6):
     """Gradients of ``query_key_norm_rotation`` with respect to q, k and the gains, from those of its outputs."""
-    some = _given(dq_out, dk_out, q, k, q_gain, k_gain, dq, dk, dq_gain, dk_gain)
-    with _here(*some, positions):
-        _half(*some); _int32(positions, 'positions')
-        lib = _cur()
+    _int32(positions, 'positions')
+    lib, dev, here = _operands([dq_out, q, q_gain, dq, dq_gain] + _given(dk_out, k, k_gain, dk, dk_gain), (positions,))
+    with here:
         nbytes = lib.sb_query_key_norm_scratch_bytes()
-        keep, ptr = _scratch(nbytes, q.device)
-        check(lib.sb_backward_query_key_norm_rotation(
-            _stream(), ptr, nbytes, _d(dq_out), _opt(dk_out), _d(q), _opt(k), _d(q_gain), _opt(k_gain), _d(positions), _d(dq),
-            _opt(dk), _d(dq_gain), _opt(dk_gain), _rotation(q, base, rotary, pairing, eps)))
+        scratch = _scratch(nbytes, q)
+        _lib.check(lib.sb_backward_query_key_norm_rotation(
+            torch._C._cuda_getCurrentRawStream(dev), scratch.data_ptr(), nbytes, _packed(dq_out), _packed(dk_out), _packed(q),
+            _packed(k), _packed(q_gain), _packed(k_gain), _packed(positions), _packed(dq), _packed(dk), _packed(dq_gain),
+            _packed(dk_gain), _rotation(q, base, rotary, pairing, eps)), lib)
 
 
 class RelativeBuckets:
@@ -391,6 +426,7 @@ class RelativeBuckets:
         self.starts = tuple(int(s) for s in starts)
         self.bidirectional = bool(bidirectional)
         self._array = (ctypes.c_int32 * len(self.starts))(*self.starts)
+        self._at = ctypes.addressof(self._array)
 
     def __len__(self):
         """Entries of a table of biases."""
@@ -423,30 +459,27 @@ def relative_buckets(num_buckets=32, max_distance=128, bidirectional=True):
 
 
 def _relative_bias(table, buckets):
-    b = _lib.SbRelativeBias()
-    b.table = ctypes.pointer(tensor_desc(table))
-    b.n, b.bidirectional = len(buckets.starts), 1 if buckets.bidirectional else 0
-    b.starts = ctypes.cast(buckets._array, ctypes.POINTER(ctypes.c_int32))
-    return ctypes.byref(b)
+    """SbRelativeBias; its table's descriptor lies in memory of the thread, which the call reads before it returns."""
+    place = getattr(_tls, 'table', None)
+    if place is None:
+        place = _tls.table = ctypes.create_string_buffer(_TENSOR.size)
+    place.raw = _packed(table)
+    return _BIAS.pack(ctypes.addressof(place), len(buckets.starts), 1 if buckets.bidirectional else 0, buckets._at)
 
 
 def _span(q, scale, causal, lengths, first):
-    s = _lib.SbAttentionSpan()
-    s.scale, s.causal = float(scale), 1 if causal else 0
     for name, t in (('lengths', lengths), ('first', first)):
-        if t is None:
-            continue
-        _int32(t, name)
-        if tuple(t.shape) != (q.shape[2],) or not t.is_contiguous():
-            raise ValueError(f'{name} is one contiguous int32 per sample ({q.shape[2]}), got {tuple(t.shape)}')
-        setattr(s, name, t.data_ptr())
-    return ctypes.byref(s)
+        if t is not None:
+            _int32(t, name)
+            if t.shape != q.shape[2:3] or not t.is_contiguous():
+                raise ValueError(f'{name} is one contiguous int32 per sample ({q.shape[2]}), got {tuple(t.shape)}')
+    return _SPAN.pack(scale, 1 if causal else 0, _address(lengths) or 0, _address(first) or 0)
 
 
 def _rows(t):
-    if t is not None and t.dtype != torch.float32:
+    if t is not None and t.dtype is not torch.float32:
         raise TypeError(f'lse is float32, got {t.dtype}')
-    return _opt(t)
+    return _packed(t)
 
 
 def relative_attention(q, k, v, table, out, lse=None, *, buckets, scale, causal=False, lengths=None, first=None):
@@ -454,28 +487,27 @@ def relative_attention(q, k, v, table, out, lse=None, *, buckets, scale, causal=
     a multiple of G; ``table`` [len(buckets),H]; ``lse``: float32 [H,B,J], the rows' log-sum-exp, which the backward pass
     needs.  ``lengths``: int32 [B], keys of each sample; ``first``: int32 [B], position of a sample's first query on the
     keys' axis (None: 0); ``causal``: queries see no keys behind their position.  A query that sees nothing gives 0."""
-    half = [q, k, v, table, out]
-    with _here(*half, *_given(lse, lengths, first)):
-        _half(*half)
-        lib, bias, nbytes = _cur(), _relative_bias(table, buckets), ctypes.c_size_t(0)
-        span, rows = _span(q, scale, causal, lengths, first), _rows(lse)
-        dq, dk, dv = _d(q), _d(k), _d(v)
-        check(lib.sb_relative_attention_scratch_bytes(dq, dk, dv, bias, ctypes.byref(nbytes)))
-        keep, ptr = _scratch(nbytes.value, q.device)
-        check(lib.sb_relative_attention(_stream(), ptr, nbytes.value, dq, dk, dv, bias, _d(out), rows, span))
+    lib, dev, here = _operands((q, k, v, table, out), _given(lse, lengths, first))
+    span, rows = _span(q, scale, causal, lengths, first), _rows(lse)
+    with here:
+        bias, nbytes, q_, k_, v_ = _relative_bias(table, buckets), ctypes.c_size_t(0), _packed(q), _packed(k), _packed(v)
+        _lib.check(lib.sb_relative_attention_scratch_bytes(q_, k_, v_, bias, nbytes), lib)
+        scratch = _scratch(nbytes.value, q)
+        _lib.check(lib.sb_relative_attention(torch._C._cuda_getCurrentRawStream(dev), _address(scratch), nbytes.value, q_, k_, v_, bias,
+                                             _packed(out), rows, span), lib)
 
 
 def backward_relative_attention(dout, q, k, v, table, out, lse, dq, dk, dv, dtable, *, buckets, scale, causal=False, lengths=None,
                                 first=None):
     """Gradients of ``relative_attention`` with respect to q, k, v and the table, from that of its output, its output and its
     ``lse``.  The same call gives the same bits."""
-    half = [dout, q, k, v, table, out, dq, dk, dv, dtable]
-    with _here(*half, lse, *_given(lengths, first)):
-        _half(*half)
-        lib, bias, nbytes = _cur(), _relative_bias(table, buckets), ctypes.c_size_t(0)
-        span, rows = _span(q, scale, causal, lengths, first), _rows(lse)
-        dg, d1, d2, d3 = _d(dout), _d(q), _d(k), _d(v)
-        check(lib.sb_backward_relative_attention_scratch_bytes(dg, d1, d2, d3, bias, ctypes.byref(nbytes)))
-        keep, ptr = _scratch(nbytes.value, q.device)
-        check(lib.sb_backward_relative_attention(_stream(), ptr, nbytes.value, dg, d1, d2, d3, bias, _d(out), rows, _d(dq), _d(dk),
-                                                 _d(dv), _d(dtable), span))
+    lib, dev, here = _operands((dout, q, k, v, table, out, dq, dk, dv, dtable), _given(lse, lengths, first))
+    span, rows = _span(q, scale, causal, lengths, first), _rows(lse)
+    with here:
+        bias, nbytes = _relative_bias(table, buckets), ctypes.c_size_t(0)
+        g_, q_, k_, v_ = _packed(dout), _packed(q), _packed(k), _packed(v)
+        _lib.check(lib.sb_backward_relative_attention_scratch_bytes(g_, q_, k_, v_, bias, nbytes), lib)
+        scratch = _scratch(nbytes.value, q)
+        _lib.check(lib.sb_backward_relative_attention(
+            torch._C._cuda_getCurrentRawStream(dev), _address(scratch), nbytes.value, g_, q_, k_, v_, bias, _packed(out), rows,
+            _packed(dq), _packed(dk), _packed(dv), _packed(dtable), span), lib)
