@@ -1611,7 +1611,7 @@ int rel_fwd(cudaStream_t s, const CUtensorMap& mq, const CUtensorMap& mk, const 
 
 }  // namespace
 
-int launch_rel_tiles_fwd(cudaStream_t s, Proj q, Proj k, Proj v, RelTables t, Proj out, RelRows lse, const RelSpan& span) {
+int launch_rel_tiles_fwd(cudaStream_t s, Proj q, Proj k, Proj v, RelTables t, int* next, Proj out, RelRows lse, const RelSpan& span) {
   std::call_once(g_encode_once, load_encode);
   if (!g_encode) return fail(SB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   std::string why;
@@ -1623,6 +1623,7 @@ int launch_rel_tiles_fwd(cudaStream_t s, Proj q, Proj k, Proj v, RelTables t, Pr
   p.nq = (q.R + 127) / 128;
   p.units = q.H * q.B;
   p.items = p.units * p.nq;
+  p.next = next;
   p.out = out;
   p.lse = lse;
   return q.P <= 64 ? rel_fwd<64>(s, mq, mk, mv, p) : rel_fwd<128>(s, mq, mk, mv, p);

@@ -118,8 +118,8 @@ constexpr int kRelMaxHead = 128;
 struct RelTables { const float* rows; int pitch, reach; };
 // What tensor maps can address: unit-stride features, 16-byte multiples everywhere else.
 bool rel_direct(const Proj& x);
-// The tcgen05 kernels; q, k, v are rel_direct.
-int launch_rel_tiles_fwd(cudaStream_t s, Proj q, Proj k, Proj v, RelTables t, Proj out, RelRows lse, const RelSpan& span);
+// The tcgen05 kernels; q, k, v are rel_direct.  `next`: a zero in device memory.
+int launch_rel_tiles_fwd(cudaStream_t s, Proj q, Proj k, Proj v, RelTables t, int* next, Proj out, RelRows lse, const RelSpan& span);
 // Backward: `records` [B][H][ceil(J / 64)][192]: of 64 query rows the log-sum-exps in units of log2 (+inf: row without keys, or
 // none), D and the weight (0 or 1) of the row in the table's sums; `partial` [H][B * ceil(J / 128) * 2][2 * reach + 1] sums of
 // score gradients by relative position; `next`: a zero.

@@ -13,7 +13,7 @@
 
 namespace rel {
 
-constexpr int kPad = 160;                            // 128 columns and the 32 rows of a warp
+constexpr int kPad = 96;                             // 64 columns and the 32 rows of a warp
 constexpr float kLazy = 8.f;                         // log2 units a row's reference may lag behind its maximum
 
 struct Common {
@@ -149,6 +149,51 @@ __device__ __forceinline__ void store_features(sb_half* ptr, long long sP, const
   }
 }
 
+// ---- work items ------------------------------------------------------------------------------------------------
+// Items come from a counter in memory, so that long ones do not hold up others (which item runs where changes nothing in its
+// results).  The producer warp works out an item's sizes, once, and hands them to the other warps through kSlots places in shared
+// memory: 48 bytes each, {kind, b, h, t}, {first, keys, tiles, each}, {t0}; kind < 0 ends.
+constexpr int kSlots = 4;
+struct Item {
+  int kind, b, h, t;
+  int first, keys, tiles, each;
+  int t0;
+};
+__device__ __forceinline__ void write_item(uint8_t* slot, const Item& w) {
+  reinterpret_cast<int4*>(slot)[0] = make_int4(w.kind, w.b, w.h, w.t);
+  reinterpret_cast<int4*>(slot)[1] = make_int4(w.first, w.keys, w.tiles, w.each);
+  reinterpret_cast<int*>(slot)[8] = w.t0;
+}
+__device__ __forceinline__ void read_item(const uint8_t* slot, Item* w) {
+  const int4 a = reinterpret_cast<const int4*>(slot)[0], b = reinterpret_cast<const int4*>(slot)[1];
+  w->kind = a.x; w->b = a.y; w->h = a.z; w->t = a.w;
+  w->first = b.x; w->keys = b.y; w->tiles = b.z; w->each = b.w;
+  w->t0 = reinterpret_cast<const int*>(slot)[8];
+}
+// The next item for a consuming warp; false at the end, or with *ok = false when a wait ran out.
+__device__ __forceinline__ bool take_item(const uint8_t* slots, uint32_t full, uint32_t empty, uint32_t* taken, int lane, Item* w, bool* ok) {
+  const uint32_t s = *taken & (kSlots - 1u);
+  *ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * s, (*taken / kSlots) & 1u, 51));
+  if (!*ok) return false;
+  read_item(slots + 48 * s, w);
+  __syncwarp();
+  if (lane == 0) mbar_arrive(empty + 8 * s);
+  ++*taken;
+  return w->kind >= 0;
+}
+// The producer's side: publishes item `w` (or the end).
+__device__ __forceinline__ bool put_item(uint8_t* slots, uint32_t full, uint32_t empty, uint32_t* put, int lane, const Item& w) {
+  const uint32_t s = *put & (kSlots - 1u);
+  if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ((*put / kSlots) & 1u) ^ 1u, 52))) return false;
+  if (lane == 0) {
+    write_item(slots + 48 * s, w);
+    mbar_arrive(full + 8 * s);
+  }
+  __syncwarp();
+  ++*put;
+  return true;
+}
+
 // ---- forward ---------------------------------------------------------------------------------------------------
 constexpr int kFwdThreads = 224;                     // producer warp, two MMA warps, four softmax warps
 
@@ -156,15 +201,16 @@ struct FwdParams {
   Common c;
   int nq, units, chunk;                              // query tiles of a unit; units = H * B; units taken together
   int items;
+  int* next;                                         // work queue
   Proj out;
   RelRows lse;
 };
 
 // The i-th work item: a tile of queries of one head and sample.  Units go in chunks, and within a chunk the last tiles first:
 // with a causal span these are the long ones, and one head's keys stay in L2 while its tiles are worked on.
-struct Item { int b, h, t, first, keys, tiles; };
-__device__ __forceinline__ Item item_of(const FwdParams& p, int i) {
+__device__ __forceinline__ Item fwd_item(const FwdParams& p, int i) {
   Item it;
+  it.kind = 0; it.each = it.t0 = 0;
   const int per = p.chunk * p.nq, c = i / per, r = i % per;
   const int here = min(p.chunk, p.units - c * p.chunk), unit = c * p.chunk + r % here;
   it.t = p.nq - 1 - r / here;
@@ -187,7 +233,7 @@ struct FwdCfg {
   static constexpr int kQ = P == 64 ? 2 : 1;         // query tiles (the next item's is fetched early)
   static constexpr int kRing = P == 64 ? 8 : 4;
   static constexpr int kTiles = kQ * kQTile + kRing * kTile;
-  static constexpr int smem(int pitch) { return kTiles + 2 * pitch * 4 + 1024 + 320; }
+  static constexpr int smem(int pitch) { return kTiles + 2 * pitch * 4 + 1024 + 128 + 16 * kRing + 16 * kSlots + 48 * kSlots + 16; }
 };
 
 // A row's state: reference of its exponentials, their sum so far.
@@ -304,10 +350,11 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   const uint32_t sq = (raw + 1023u) & ~1023u, ring = sq + kQ * Cfg::kQTile;
   const uint32_t sbias = sq + Cfg::kTiles, bars = sbias + 2u * p.c.pitch * 4u;
   const uint32_t q_full = bars, q_empty = bars + 16, s_full = bars + 32, p_full = bars + 48, o_empty = bars + 64;
-  const uint32_t b_full = bars + 80, b_empty = bars + 96, p_free = bars + 112, kv_full = bars + 128, kv_empty = kv_full + 8 * kRing;
+  const uint32_t b_full = bars + 80, b_empty = bars + 96, p_free = bars + 112, kv_full = bars + 128, kv_empty = kv_full + 8 * kRing, item_full = kv_empty + 8 * kRing, item_empty = item_full + 8 * kSlots;
   uint8_t* gen = smem_raw + (sq - raw);
   const float* bias_s = reinterpret_cast<const float*>(gen + (sbias - sq));
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (kv_empty + 8 * kRing - sq));
+  uint8_t* slots = gen + (item_empty + 8 * kSlots - sq);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(slots + 48 * kSlots);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -321,6 +368,10 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       mbar_init(p_free + 8 * i, 1);
     }
     mbar_init(o_empty, 4);
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(item_full + 8 * i, 1);
+      mbar_init(item_empty + 8 * i, 6);
+    }
     for (int i = 0; i < kRing; ++i) {
       mbar_init(kv_full + 8 * i, 1);
       mbar_init(kv_empty + 8 * i, 1);
@@ -342,12 +393,22 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   grid_dependency_sync();
 
   // `it` counts the items that see a key, n their key tiles
+  uint32_t taken = 0;
+  auto take = [&](Item* w, bool* ok) { return take_item(slots, item_full, item_empty, &taken, lane, w, ok); };
   if (warp == 0) {
     // ---------------- producer: queries and biases of the item, then its keys and values in turn ----------------
-    uint32_t it = 0, x = 0;
+    uint32_t it = 0, x = 0, put = 0;
     bool ok = true;
-    for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
-      const Item w = item_of(p, item);
+    int id = blockIdx.x;
+    while (ok) {
+      int after = 0;
+      if (lane == 0 && id < p.items) after = atomicAdd(p.next, 1) + (int)gridDim.x;
+      Item w;
+      w.kind = -1;
+      if (id < p.items) w = fwd_item(p, id);
+      ok = put_item(slots, item_full, item_empty, &put, lane, w);
+      if (!ok || id >= p.items) break;
+      id = __shfl_sync(0xffffffffu, after, 0);
       if (w.tiles == 0) continue;
       const uint32_t qb = it % kQ, bb = it & 1u;
       ok = __all_sync(0xffffffffu, mbar_wait(q_empty + 8 * qb, ((it / kQ) & 1u) ^ 1u, 41)) &&
@@ -377,8 +438,8 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     // ---------------- MMA issuer of scores, a tile ahead of the softmax ----------------
     uint32_t it = 0, n = 0;                              // ring uses are 2 n (keys) and 2 n + 1 (values)
     bool ok = true;
-    for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
-      const Item w = item_of(p, item);
+    Item w;
+    while (ok && take(&w, &ok)) {
       if (w.tiles == 0) continue;
       const uint32_t qb = it % kQ;
       ok = __all_sync(0xffffffffu, mbar_wait(q_full + 8 * qb, (it / kQ) & 1u, 42));
@@ -401,8 +462,8 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     // ---------------- MMA issuer of the output ----------------
     uint32_t it = 0, n = 0;
     bool ok = true;
-    for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
-      const Item w = item_of(p, item);
+    Item w;
+    while (ok && take(&w, &ok)) {
       if (w.tiles == 0) continue;
       for (int i = 0; i < w.tiles; ++i, ++n) {
         const uint32_t s = (2 * n + 1) % kRing, sb = n & 1u;
@@ -428,8 +489,8 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     const uint32_t to = tmem + lanes + Cfg::kO;
     uint32_t n = 0, it = 0;
     bool ok = true;
-    for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
-      const Item w = item_of(p, item);
+    Item w;
+    while (ok && take(&w, &ok)) {
       const int j = w.t * 128 + rt, pos = w.first + j;
       const bool row = j < p.c.J;
       int mine = w.keys;                                 // keys that this row sees
@@ -441,13 +502,12 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         ok = __all_sync(0xffffffffu, mbar_wait(b_full + 8 * bb, (it >> 1) & 1u, 45));
         if (!ok) break;
       }
-      for (int kb = 0; kb < w.tiles; ++kb, ++n) {
-        const int lim = mine - kb * N;
-        const int rel0 = kb * N - pos;                 // relative position of the first column
-        const int lo = kb * N - (w.first + w.t * 128 + q * 32 + 31), hi = kb * N + N - 1 - (w.first + w.t * 128 + q * 32);
+      // columns of the tile that this row sees, the fewest of the warp's rows, the relative position of the first column at this
+      // row, and the lowest of the warp's block (its highest is lo + N + 30)
+      int lim = mine, least = __reduce_min_sync(0xffffffffu, mine), rel0 = -pos, lo = -(w.first + w.t * 128 + q * 32 + 31);
+      for (int kb = 0; kb < w.tiles; ++kb, ++n, lim -= N, least -= N, rel0 += N, lo += N) {
         const uint32_t sb = n & 1u, ts = tmem + lanes + sb * N;
-        const bool near = hi > -p.c.reach && lo < p.c.reach;
-        const bool mask = __any_sync(0xffffffffu, lim < N);
+        const bool near = lo + N + 30 > -p.c.reach && lo < p.c.reach, mask = least < N;
         // outside the varying part, a place in the row where N entries have the end's value
         const float* bp = bias + (near ? rel0 + p.c.reach + kPad : lo >= p.c.reach ? kPad + 2 * p.c.reach : 0);
         const float flat = bp[0];
@@ -526,26 +586,22 @@ struct BwdParams {
 };
 
 // An item holds one pair of 128-row tiles and streams pairs of 64-row tiles past it: (K, V) held and (Q, dOUT) of every query
-// head that shares them streamed, or (Q, dOUT) held and (K, V) streamed.  `b`, `h`, `t`: the held tile.
-struct BwdItem {
-  bool q;
-  int b, h, t, first, keys;
-  int tiles, each, t0;                               // streamed tiles: `each` from t0 on, for each head in turn
-};
-__device__ __forceinline__ BwdItem bwd_item(const BwdParams& p, int i) {
-  BwdItem it;
-  it.q = i >= p.first_q;
-  if (it.q) i -= p.first_q;
-  const int rows = it.q ? p.nq : p.nk, heads = it.q ? p.c.H : p.c.G, chunk = it.q ? p.chunk_q : p.chunk_k;
+// head that shares them streamed (kind 0), or (Q, dOUT) held and (K, V) streamed (kind 1).  `b`, `h`, `t`: the held tile;
+// `tiles` streamed ones, `each` from t0 on for each head in turn.
+__device__ __forceinline__ Item bwd_item(const BwdParams& p, int i) {
+  Item it;
+  it.kind = i >= p.first_q ? 1 : 0;
+  if (it.kind) i -= p.first_q;
+  const int rows = it.kind ? p.nq : p.nk, heads = it.kind ? p.c.H : p.c.G, chunk = it.kind ? p.chunk_q : p.chunk_k;
   const int per = chunk * rows, c = i / per, r = i % per;
   const int here = min(chunk, heads * p.c.B - c * chunk), unit = c * chunk + r % here;
-  it.t = it.q ? rows - 1 - r / here : r / here;      // long ones first where the span is causal
+  it.t = it.kind ? rows - 1 - r / here : r / here;   // long ones first where the span is causal
   it.b = unit / heads;
   it.h = unit % heads;
   it.first = first_of(p.c, it.b);
   it.keys = keys_of(p.c, it.b);
   it.t0 = 0;
-  if (it.q) {
+  if (it.kind) {
     if (p.c.causal) it.keys = max(0, min(it.keys, it.first + min(p.c.J, it.t * 128 + 128)));
     it.each = it.tiles = (it.keys + 63) >> 6;
   } else {
@@ -565,12 +621,12 @@ struct BwdCfg {
   static constexpr int kBuf = P == 64 ? 3 : 2;
   static constexpr uint32_t kAcc = kBuf * 128;
   static constexpr int smem(int stages, int held, int pitch, int reach) {
-    return held * kHeld + stages * kStage + 2 * pitch * 4 + 8 * ((2 * reach + 4) & ~3) * 4 + 1024 + 512;
+    return held * kHeld + stages * kStage + 2 * pitch * 4 + 8 * ((2 * reach + 4) & ~3) * 4 + 1024 + 400 + 48 * kSlots;
   }
 };
 
 // Scores and dP of a thread's row of 64 columns -> exponentials and score gradients, 16-bit pairs over the columns they came
-// from, 16 columns at a time while the next 16 are on their way.  Column c has the bias bp[c] (key tiles: bp[-c]; NEAR) or `flat`.
+// from, 32 columns at a time.  Column c has the bias bp[c] (key tiles: bp[-c]; NEAR) or `flat`.
 // What differs between the two kinds of items: in key tiles (KEYS) a thread is a key, log-sum-exps and D change along columns
 // (L, D in shared memory), visible columns are c >= lim; in query tiles a thread is a query and visible columns are c < lim.
 // `emit` gets every score gradient, `block` is told after each 32 columns.
@@ -578,20 +634,26 @@ template <bool KEYS, bool NEAR, bool MASK, class Emit, class Block>
 __device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float flat, const float* L, const float* D, float lse, float dsum,
                                           int lim, float c2, Emit&& emit, Block&& block) {
   const float2 c22 = make_float2(c2, c2), minus = make_float2(-1.f, -1.f);
-  auto chunk = [&](int c, uint32_t* s, uint32_t* g) {
-    uint32_t pm[8], dm[8];
+#pragma unroll 1
+  for (int c = 0; c < 2; ++c) {
+    uint32_t s[32], g[32], dm[16], pm[16];
+    tmem_ld32_nowait(ts + c * 32, s);
+    tmem_ld32_nowait(ts + 64 + c * 32, g);
+    const float* bc = bp + (KEYS ? -c * 32 : c * 32);
+    attn::tmem_ld_wait32(s);
+    attn::tmem_ld_wait32(g);
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
+    for (int e = 0; e < 32; e += 4) {
       float4 l4 = make_float4(lse, lse, lse, lse), d4 = make_float4(dsum, dsum, dsum, dsum);
       if (KEYS) {
-        l4 = *reinterpret_cast<const float4*>(L + c * 16 + e);
-        d4 = *reinterpret_cast<const float4*>(D + c * 16 + e);
+        l4 = *reinterpret_cast<const float4*>(L + c * 32 + e);
+        d4 = *reinterpret_cast<const float4*>(D + c * 32 + e);
       }
 #pragma unroll
       for (int x = 0; x < 4; x += 2) {
-        const int i = e + x, col = c * 16 + i;
+        const int i = e + x, col = c * 32 + i;
         const float2 l = x ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y), d = x ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
-        const float2 b = NEAR ? (KEYS ? make_float2(bp[-col], bp[-col - 1]) : make_float2(bp[col], bp[col + 1])) : make_float2(flat, flat);
+        const float2 b = NEAR ? (KEYS ? make_float2(bc[-i], bc[-i - 1]) : make_float2(bc[i], bc[i + 1])) : make_float2(flat, flat);
         float2 pr = fma2(pair(s, i), c22, fma2(l, minus, b));
         pr.x = attn::ex2_approx(pr.x);
         pr.y = attn::ex2_approx(pr.y);
@@ -601,35 +663,19 @@ __device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float fl
           pr = make_float2(seen0 ? pr.x : 0.f, seen1 ? pr.y : 0.f);
           ds = make_float2(seen0 ? ds.x : 0.f, seen1 ? ds.y : 0.f);
         }
-        emit((c & 1) * 16 + i, ds.x);
-        emit((c & 1) * 16 + i + 1, ds.y);
+        emit(i, ds.x);
+        emit(i + 1, ds.y);
         if (KEYS) pm[i >> 1] = flash::pack2(pr.x, pr.y);
         dm[i >> 1] = flash::pack2(ds.x, ds.y);
       }
     }
-    if (KEYS) tmem_st8(ts + c * 8, pm);
-    tmem_st8(ts + 64 + c * 8, dm);
-  };
-  uint32_t sa[16], ga[16], sb[16], gb[16];
-  tmem_ld16(ts, sa);
-  tmem_ld16(ts + 64, ga);
-#pragma unroll 1
-  for (int c = 0; c < 4; c += 2) {
-    tmem_wait16(sa, ga);
-    tmem_ld16(ts + c * 16 + 16, sb);
-    tmem_ld16(ts + 64 + c * 16 + 16, gb);
-    chunk(c, sa, ga);
-    tmem_wait16(sb, gb);
-    if (c == 0) {
-      tmem_ld16(ts + 32, sa);
-      tmem_ld16(ts + 96, ga);
-    }
-    chunk(c + 1, sb, gb);
-    block(c >> 1);
+    if (KEYS) tmem_st16(ts + c * 16, pm);
+    tmem_st16(ts + 64 + c * 16, dm);
+    block(c);
   }
 }
 
-// One CTA per SM, work items from a queue (which item runs where changes nothing in its results).  The two groups of element
+// One CTA per SM.  The two groups of element
 // warps take the streamed tiles in turn: while one turns scores and dP into exponentials and score gradients, the tensor cores
 // multiply for the other.  Both results go back into tensor memory, where the second products take them from.  Everything is
 // computed twice, once per kind of item; the alternative, dQ summed over key tiles in memory, needs atomics whose order
@@ -654,13 +700,13 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
   const uint32_t s_full = bars + 128, pd_full = bars + 152, acc_full = bars + 176, acc_empty = bars + 184, full = bars + 192, empty = bars + 256;
   uint8_t* gen = smem_raw + (sheld - raw);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (bars + 320 - sheld));
-  volatile int* queue = reinterpret_cast<volatile int*>(gen + (bars + 336 - sheld));
+  uint8_t* slots = gen + (bars + 400 - sheld);
   const uint32_t g_sync = bars + 352, buf_free = bars + 368;
   const float* bias_s = reinterpret_cast<const float*>(gen + (sbias - sheld));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kSlots; ++i) {
       mbar_init(item_full + 8 * i, 1);
       mbar_init(item_empty + 8 * i, 10);
     }
@@ -699,42 +745,24 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   grid_dependency_sync();
 
-  // Consumers read every item of the queue in turn.
   uint32_t taken = 0;
-  auto take = [&](BwdItem* it, bool* ok) {
-    const uint32_t s = taken & 3u;
-    *ok = __all_sync(0xffffffffu, mbar_wait(item_full + 8 * s, (taken >> 2) & 1u, 51));
-    if (!*ok) return false;
-    const int id = queue[s];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(item_empty + 8 * s);
-    ++taken;
-    if (id >= p.items) return false;
-    *it = bwd_item(p, id);
-    return true;
-  };
+  auto take = [&](Item* w, bool* ok) { return take_item(slots, item_full, item_empty, &taken, lane, w, ok); };
 
   if (warp == 0) {
     // ---------------- producer ----------------
     // live: items with tiles; run: tiles of one head in an item, which share a row of biases
-    uint32_t seq = 0, live = 0, run = 0, st = 0, st_phase = 1;
+    uint32_t put = 0, live = 0, run = 0, st = 0, st_phase = 1;
     const int rep = p.c.H / p.c.G, blocks = (p.c.J + 63) >> 6;
     bool ok = true;
     int id = blockIdx.x;
     while (ok) {
       int after = 0;
       if (lane == 0 && id < p.items) after = atomicAdd(p.next, 1) + (int)gridDim.x;
-      const uint32_t s = seq & 3u;
-      ok = __all_sync(0xffffffffu, mbar_wait(item_empty + 8 * s, ((seq >> 2) & 1u) ^ 1u, 52));
-      if (!ok) break;
-      if (lane == 0) {
-        queue[s] = id;
-        mbar_arrive(item_full + 8 * s);
-      }
-      __syncwarp();
-      ++seq;
-      if (id >= p.items) break;
-      const BwdItem w = bwd_item(p, id);
+      Item w;
+      w.kind = -1;
+      if (id < p.items) w = bwd_item(p, id);
+      ok = put_item(slots, item_full, item_empty, &put, lane, w);
+      if (!ok || id >= p.items) break;
       if (w.tiles > 0) {
         const uint32_t hb = p.held == 2 ? live & 1u : 0u, hp = p.held == 2 ? live >> 1 : live;
         ok = __all_sync(0xffffffffu, mbar_wait(h_empty + 8 * hb, (hp & 1u) ^ 1u, 53));
@@ -742,13 +770,13 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         if (lane == 0) {
           const uint32_t d = sheld + hb * Cfg::kHeld;
           mbar_expect_tx(h_full + 8 * hb, Cfg::kHeld);
-          load_rows<P, 128>(d, w.q ? &tmQh : &tmKh, h_full + 8 * hb, w.t * 128, w.h, w.b);
-          load_rows<P, 128>(d + Cfg::kHeld / 2, w.q ? &tmGh : &tmVh, h_full + 8 * hb, w.t * 128, w.h, w.b);
+          load_rows<P, 128>(d, w.kind ? &tmQh : &tmKh, h_full + 8 * hb, w.t * 128, w.h, w.b);
+          load_rows<P, 128>(d + Cfg::kHeld / 2, w.kind ? &tmGh : &tmVh, h_full + 8 * hb, w.t * 128, w.h, w.b);
         }
         __syncwarp();
         ++live;
       }
-      int head = w.q ? w.h : w.h * rep, t = w.t0, left = w.each;
+      int head = w.kind ? w.h : w.h * rep, t = w.t0, left = w.each;
       for (int i = 0; i < w.tiles && ok; ++i) {
         if (left == w.each) {
           const uint32_t bb = run & 1u;
@@ -765,8 +793,8 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         if (!ok) break;
         if (lane == 0) {
           const uint32_t d = ring + st * Cfg::kStage, bar = full + 8 * st;
-          mbar_expect_tx(bar, Cfg::kStream + (w.q ? 0 : 512));
-          if (w.q) {
+          mbar_expect_tx(bar, Cfg::kStream + (w.kind ? 0 : 512));
+          if (w.kind) {
             load_rows<P, 64>(d, &tmKs, bar, t * 64, w.h / rep, w.b);
             load_rows<P, 64>(d + Cfg::kStream / 2, &tmVs, bar, t * 64, w.h / rep, w.b);
           } else {
@@ -786,7 +814,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     // ---------------- MMA issuer of scores and dP ----------------
     uint32_t live = 0, st = 0, st_phase = 0, bf = 0, bf_phase = 1;
     bool ok = true;
-    BwdItem w;
+    Item w;
     while (ok && take(&w, &ok)) {
       if (w.tiles == 0) continue;
       const uint32_t hb = p.held == 2 ? live & 1u : 0u, hp = p.held == 2 ? live >> 1 : live, hd = sheld + hb * Cfg::kHeld;
@@ -796,7 +824,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         if (!ok) break;
         tc_fence_after();
         const uint32_t x = ring + st * Cfg::kStage, ts = tmem + bf * 128u;
-        if (w.q && w.keys - i * 64 < 64) zero_rows<P, 64>(gen + (x - sheld), w.keys - i * 64, lane);
+        if (w.kind && w.keys - i * 64 < 64) zero_rows<P, 64>(gen + (x - sheld), w.keys - i * 64, lane);
         if (flash::elect_one()) {
           mma_rows<P, 64>(ts, hd, x);
           mma_rows<P, 64>(ts + 64u, hd + Cfg::kHeld / 2, x + Cfg::kStream / 2);
@@ -812,7 +840,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     // ---------------- MMA issuer of the products that read what became of them ----------------
     uint32_t live = 0, st = 0, bf = 0, bf_phase = 0;
     bool ok = true;
-    BwdItem w;
+    Item w;
     while (ok && take(&w, &ok)) {
       if (w.tiles == 0) continue;
       for (int i = 0; i < w.tiles; ++i) {
@@ -822,7 +850,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         if (flash::elect_one()) {
           const uint32_t x = ring + st * Cfg::kStage, ts = tmem + bf * 128u, acc = tmem + Cfg::kAcc;
           mma_weighted<P, 64>(acc, ts + 64u, x, i > 0);                                               // dK += ds Q, dQ += ds K
-          if (!w.q) mma_weighted<P, 64>(acc + (uint32_t)P, ts, x + Cfg::kStream / 2, i > 0);          // dV += softmax dOUT
+          if (!w.kind) mma_weighted<P, 64>(acc + (uint32_t)P, ts, x + Cfg::kStream / 2, i > 0);          // dV += softmax dOUT
           umma_commit(empty + 8 * st);
           umma_commit(buf_free + 8 * bf);
           if (i == w.tiles - 1) {
@@ -846,28 +874,28 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     const int in_group = ((warp - 3) & 3) * 32 + lane;
     uint32_t n = 0, live = 0, run = 0, st = 0, st_phase = 0, bf = 0, bf_phase = 0;
     bool ok = true, have = false;
-    BwdItem prev;
+    Item prev;
     float below = 0.f, above = 0.f;                    // sums outside the varying part of the bias
     // An item's results: dK (group 0) and dV (group 1) of a key, or dQ of a query, 32 features in turn.
-    auto store = [&](const BwdItem& it, uint32_t acc, bool zero) {
+    auto store = [&](const Item& it, uint32_t acc, bool zero) {
       const int r = it.t * 128 + rt;
-      const Proj& o = it.q ? p.dq : g ? p.dv : p.dk;
+      const Proj& o = it.kind ? p.dq : g ? p.dv : p.dk;
       sb_half* out = reinterpret_cast<sb_half*>(o.p) + (long long)it.h * o.sH + (long long)it.b * o.sB + (long long)r * o.sR;
-      const float f = it.q || !g ? p.scale : 1.f;
+      const float f = it.kind || !g ? p.scale : 1.f;
 #pragma unroll 1
-      for (int c = it.q ? g : 0; c < P / 32; c += it.q ? 2 : 1) {
+      for (int c = it.kind ? g : 0; c < P / 32; c += it.kind ? 2 : 1) {
         uint32_t v[32];
         if (!zero) {
-          tmem_ld32_nowait(acc + lanes + (it.q || !g ? 0u : (uint32_t)P) + c * 32, v);
+          tmem_ld32_nowait(acc + lanes + (it.kind || !g ? 0u : (uint32_t)P) + c * 32, v);
           attn::tmem_ld_wait32(v);
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = 0u;
         }
-        if (r < (it.q ? p.c.J : p.c.K) && c * 32 < p.c.P) store_features(out + c * 32 * o.sP, o.sP, v, f, min(32, p.c.P - c * 32));
+        if (r < (it.kind ? p.c.J : p.c.K) && c * 32 < p.c.P) store_features(out + c * 32 * o.sP, o.sP, v, f, min(32, p.c.P - c * 32));
       }
     };
-    auto finish = [&](const BwdItem& it, uint32_t s) {
+    auto finish = [&](const Item& it, uint32_t s) {
       ok = __all_sync(0xffffffffu, mbar_wait(acc_full, s & 1u, 59));
       if (!ok) return;
       tc_fence_after();
@@ -892,7 +920,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       return ok;
     };
     // the group's sums of a query tile to memory
-    auto flush = [&](const BwdItem& it) {
+    auto flush = [&](const Item& it) {
       const float lo = warp_sum(below), hi = warp_sum(above);
       below = above = 0.f;
       if (lane == 0) {
@@ -912,48 +940,55 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       }
       group_sync();
     };
-    BwdItem w;
+    Item w;
     while (ok && take(&w, &ok)) {
       if (w.tiles == 0) {
         store(w, 0u, true);
-        if (w.q) flush(w);
+        if (w.kind) flush(w);
         continue;
       }
       const int r = w.t * 128 + rt;                    // query or key of this thread
       float lse = INFINITY, dsum = 0.f, weight = 1.f;
-      if (w.q && r < p.c.J) {
+      if (w.kind && r < p.c.J) {
         const float* rec = p.records + (((long long)w.b * p.c.H + w.h) * blocks + (r >> 6)) * kRecord + (r & 63);
         lse = rec[0];
         dsum = rec[64];
         weight = rec[128];
       }
       const bool weighted = __any_sync(0xffffffffu, weight != 1.f);
-      int mine = w.keys;
-      if (w.q && p.c.causal) mine = min(mine, w.first + r + 1);
       bool due = have;                                 // the previous item's results are still to be stored
-      int t = w.t0, left = w.each;
+      // Per streamed tile, all moving by 64: relative position of this thread's first column, lowest of the warp's block (its
+      // highest is lo + 94), the thread's bound on visible columns and the block's tightest.
+      const int step = w.kind ? 64 : -64;
+      int rel = w.kind ? -(w.first + r) : r - (w.first + w.t0 * 64), lim;
+      if (w.kind) lim = p.c.causal ? min(w.keys, w.first + r + 1) : w.keys;
+      else lim = r < w.keys ? (p.c.causal ? rel : -(1 << 30)) : 1 << 30;
+      const int rel0 = rel, lim0 = lim, lo0 = __shfl_sync(0xffffffffu, rel, w.kind ? 31 : 0) - (w.kind ? 0 : 63);
+      const int tight0 = w.kind ? __reduce_min_sync(0xffffffffu, lim) : __reduce_max_sync(0xffffffffu, lim);
+      const bool moves = w.kind || p.c.causal;
+      int lo = lo0, tight = tight0, left = w.each;
+      const float* bias = bias_s;
       for (int i = 0; i < w.tiles; ++i, ++n) {
-        const uint32_t bb = run & 1u;
+        if (left == w.each) {
+          ok = __all_sync(0xffffffffu, mbar_wait(b_full + 8 * (run & 1u), (run >> 1) & 1u, 60));
+          if (!ok) break;
+          bias = bias_s + (run & 1u) * p.c.pitch;
+        }
         if ((int)(n & 1u) == g) {
-          ok = __all_sync(0xffffffffu, mbar_wait(b_full + 8 * bb, (run >> 1) & 1u, 60)) &&
-               __all_sync(0xffffffffu, mbar_wait(full + 8 * st, st_phase, 60)) &&
-               __all_sync(0xffffffffu, mbar_wait(s_full + 8 * bf, bf_phase, 60));
+          const bool near = lo + 94 > -reach && lo < reach;
+          // outside the varying part, a place in the row where the 64 entries in use have the end's value
+          const float* bp = bias + (near ? rel + reach + kPad : (lo >= reach ? kPad + 2 * reach : 0) + (w.kind ? 0 : 64));
+          const uint32_t ts = tmem + lanes + bf * 128u;
+          ok = __all_sync(0xffffffffu, (w.kind || mbar_wait(full + 8 * st, st_phase, 60)) && mbar_wait(s_full + 8 * bf, bf_phase, 60));
           if (!ok) break;
           tc_fence_after();
-          const float* bias = bias_s + bb * p.c.pitch;
-          const uint32_t ts = tmem + lanes + bf * 128u;
-          if (w.q) {
-            const int k0 = t * 64, pos0 = w.first + w.t * 128 + q * 32, lo = k0 - pos0 - 31, hi = k0 + 63 - pos0;
-            const bool near = hi > -reach && lo < reach;
-            const int lim = mine - k0;
-            const bool mask = __any_sync(0xffffffffu, lim < 64);
-            // outside the varying part, a place in the row where 64 entries have the end's value
-            const float* bp = bias + (near ? k0 - (w.first + r) + reach + kPad : lo >= reach ? kPad + 2 * reach : 0);
+          if (w.kind) {
+            const bool mask = tight < 64;
             if (near || mask || weighted) {
               float up = 0.f, down = 0.f;              // diagonals `lane` and `lane - 32` of a block
               auto block = [&](int c) {
-                add(k0 + 32 * c - pos0 + lane, up);
-                add(k0 + 32 * c - pos0 + lane - 32, down);
+                add(lo + 31 + 32 * c + lane, up);
+                add(lo - 1 + 32 * c + lane, down);
                 up = down = 0.f;
               };
               auto sum = [&](int e, float ds) {
@@ -971,15 +1006,10 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
               (lo >= reach ? above : below) += sum.x + sum.y;
             }
           } else {
-            const int pos0 = w.first + t * 64, lo = w.t * 128 + q * 32 - pos0 - 63, hi = w.t * 128 + q * 32 + 31 - pos0;
-            const bool near = hi > -reach && lo < reach;
-            const int lim = r < w.keys ? (p.c.causal ? r - pos0 : 0) : 64;
-            const bool mask = __any_sync(0xffffffffu, lim > 0);
             const float* L = reinterpret_cast<const float*>(gen + (ring - sheld) + st * Cfg::kStage + Cfg::kStream);
-            const float* bp = bias + (near ? r - pos0 + reach + kPad : lo >= reach ? kPad + 2 * reach + 64 : 64);
             auto none = [](int, float) {};
             auto after = [](int) {};
-            if (mask) turn_tile<true, true, true>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
+            if (tight > 0) turn_tile<true, true, true>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
             else if (near) turn_tile<true, true, false>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
             else turn_tile<true, false, false>(ts, bp, bp[0], L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
           }
@@ -995,12 +1025,14 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         }
         if (++st == (uint32_t)p.stages) { st = 0; st_phase ^= 1u; }
         if (++bf == (uint32_t)Cfg::kBuf) { bf = 0; bf_phase ^= 1u; }
-        ++t;
+        rel += step;
+        lo += step;
+        if (moves) { lim -= 64; tight -= 64; }
         if (--left == 0) {
-          t = w.t0;
+          rel = rel0; lo = lo0; lim = lim0; tight = tight0;
           left = w.each;
           __syncwarp();
-          if (lane == 0) mbar_arrive(b_empty + 8 * bb);
+          if (lane == 0) mbar_arrive(b_empty + 8 * (run & 1u));
           ++run;
         }
       }
@@ -1009,7 +1041,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         finish(prev, live - 1u);
         if (!ok) break;
       }
-      if (w.q) flush(w);
+      if (w.kind) flush(w);
       prev = w;
       have = true;
       ++live;

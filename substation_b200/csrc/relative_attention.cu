@@ -11,7 +11,7 @@ namespace sb {
 namespace {
 
 constexpr int kMaxP = kRelMaxHead;
-constexpr int kRelPad = 160;                        // as the tile kernels' kPad
+constexpr int kRelPad = 96;                         // as the tile kernels' kPad
 constexpr float kHidden = -8.507059173023462e37f;   // -2^126: entries at or below hide their keys
 
 struct Starts { int s[kRelMaxBuckets]; };
@@ -50,8 +50,9 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
 // rows[h][i] = log2(e) * bias of head h at relative position i - kRelPad - reach, which stays at its end values beyond the reach.
 // Finite biases stay finite, so that a row of nothing but the lowest ones still has a maximum.
 __global__ void __launch_bounds__(256)
-expand_bias_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, float* rows, int pitch, int reach) {
+expand_bias_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, float* rows, int pitch, int reach, int* next) {
   grid_dependency_sync();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *next = 0;   // the work queue of the kernel that follows
   const int i = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
   if (i >= pitch) return;
   const int rel = max(-reach, min(reach, i - kRelPad - reach));
@@ -387,10 +388,9 @@ join_splits_kernel(const __grid_constant__ FewParams p) {
 // What the backward pass knows of 64 query rows (RelBackward in ops.h); four threads a row.  `vec`: both tensors have unit-stride
 // features in 16-byte pieces; else lanes run along rows.
 __global__ void __launch_bounds__(256)
-row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, float* records, int* next, int vec) {
+row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, float* records, int vec) {
   __shared__ float part[4][64];
   grid_dependency_sync();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *next = 0;
   const int blocks = (a.J + 63) / 64;
   const long long all = (long long)a.H * a.B * blocks;
   for (long long it = blockIdx.x; it < all; it += gridDim.x) {
@@ -477,8 +477,8 @@ AttnArgs attn_args(const Proj& q, const Proj& k, const Proj& v, const RelBias& b
   for (int i = 0; i < bias.n; ++i) st->s[i] = bias.starts[i];
   return a;
 }
-// Scratch: rows of biases, then a packed copy of each operand that tensor maps cannot address.
-struct Plan { int pitch, reach; size_t at[4], bytes; };
+// Scratch: rows of biases, a packed copy of each operand that tensor maps cannot address, the work queue's counter.
+struct Plan { int pitch, reach; size_t at[4], next, bytes; };
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 size_t packed_bytes(const Proj& x) { return align256(2 * (size_t)((x.P + 7) / 8 * 8) * x.H * x.B * x.R); }
 Plan plan_of(std::initializer_list<const Proj*> operands, int heads, const RelBias& bias) {
@@ -491,6 +491,8 @@ Plan plan_of(std::initializer_list<const Proj*> operands, int heads, const RelBi
     p.at[i++] = p.bytes;
     if (!rel_direct(*x)) p.bytes += packed_bytes(*x);
   }
+  p.next = p.bytes;
+  p.bytes += 256;
   return p;
 }
 // x becomes the copy at `at`.
@@ -508,7 +510,8 @@ int pack(cudaStream_t s, void* scratch, size_t at, Proj* x) {
 int direct_or_packed(cudaStream_t s, void* scratch, size_t at, Proj* x) { return rel_direct(*x) ? SB_OK : pack(s, scratch, at, x); }
 int expand_bias(cudaStream_t s, const AttnArgs& a, const Starts& st, void* scratch, const Plan& pl, RelTables* t) {
   t->rows = reinterpret_cast<float*>(scratch); t->pitch = pl.pitch; t->reach = pl.reach;
-  SB_LAUNCH_OK(launch_k(expand_bias_kernel, dim3((pl.pitch + 255) / 256, a.H), 256, 0, s, a, st, reinterpret_cast<float*>(scratch), pl.pitch, pl.reach));
+  SB_LAUNCH_OK(launch_k(expand_bias_kernel, dim3((pl.pitch + 255) / 256, a.H), 256, 0, s, a, st, reinterpret_cast<float*>(scratch), pl.pitch, pl.reach,
+                        reinterpret_cast<int*>(reinterpret_cast<char*>(scratch) + pl.next)));
   return SB_OK;
 }
 
@@ -581,20 +584,19 @@ int launch_rel_attn_fwd(cudaStream_t s, void* scratch, Proj q, Proj k, Proj v, c
   SB_TRY(direct_or_packed(s, scratch, pl.at[0], &q));
   SB_TRY(direct_or_packed(s, scratch, pl.at[1], &k));
   SB_TRY(direct_or_packed(s, scratch, pl.at[2], &v));
-  return launch_rel_tiles_fwd(s, q, k, v, t, out, lse, span);
+  return launch_rel_tiles_fwd(s, q, k, v, t, reinterpret_cast<int*>(reinterpret_cast<char*>(scratch) + pl.next), out, lse, span);
 }
 
 namespace {
-// and for the backward pass records, sums and the queue's counter
-struct BwdPlan { Plan p; size_t records, partial, next, bytes; int rows; };
+// and for the backward pass records and sums
+struct BwdPlan { Plan p; size_t records, partial, bytes; int rows; };
 BwdPlan bwd_plan(const Proj& dout, const Proj& q, const Proj& k, const Proj& v, const RelBias& bias) {
   BwdPlan b;
   b.p = plan_of({&dout, &q, &k, &v}, q.H, bias);
   b.rows = q.B * ((q.R + 127) / 128) * 2;
   b.records = b.p.bytes;
   b.partial = b.records + align256(sizeof(float) * 192 * (size_t)q.H * q.B * ((q.R + 63) / 64));
-  b.next = b.partial + align256(sizeof(float) * (size_t)q.H * b.rows * (2 * b.p.reach + 1));
-  b.bytes = b.next + 256;
+  b.bytes = b.partial + align256(sizeof(float) * (size_t)q.H * b.rows * (2 * b.p.reach + 1));
   return b;
 }
 }  // namespace
@@ -616,10 +618,10 @@ int launch_rel_attn_bwd(cudaStream_t s, void* scratch, Proj dout, Proj q, Proj k
     return x.sP == 1 && x.P % 8 == 0 && !((x.sH | x.sB | x.sR) & 7) && !(reinterpret_cast<uintptr_t>(x.p) & 15u);
   };
   float* records = reinterpret_cast<float*>(base + pl.records);
-  int* next = reinterpret_cast<int*>(base + pl.next);
+  int* next = reinterpret_cast<int*>(base + pl.p.next);
   const long long blocks = (long long)a.H * a.B * ((a.J + 63) / 64);
   SB_LAUNCH_OK(launch_k(row_records_kernel, (unsigned)std::min<long long>(blocks, 8 * usable_sms(device_facts().sms)), 256, 0, s, a, st, records,
-                        next, pieces(dout) && pieces(out) ? 1 : 0));
+                        pieces(dout) && pieces(out) ? 1 : 0));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[0], &dout));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[1], &q));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[2], &k));
