@@ -42,13 +42,29 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-// D (+)= A * B with A in tensor memory (16-bit pairs, a row per lane)
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+// D (+)= A * B, A in shared memory or (ts) in tensor memory as 16-bit pairs, a row per lane.  The whole warp comes here and one
+// thread issues (`on`): inside a branch of one thread the operands were moved to uniform registers for each instruction, 70
+// clocks apart whatever its size.
+__device__ __forceinline__ void umma_ss(uint32_t on, uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-      ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+      "{\n .reg .pred p, e;\n setp.ne.b32 e, %5, 0;\n setp.ne.b32 p, %4, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+      ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
 }
+__device__ __forceinline__ void umma_ts(uint32_t on, uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n setp.ne.b32 e, %5, 0;\n setp.ne.b32 p, %4, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+      ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
+}
+__device__ __forceinline__ void commit_if(uint32_t on, uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar), "r"(on) : "memory");
+}
+// A value that all lanes hold, as the compiler can see.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {   // (no wait)
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -104,22 +120,22 @@ __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, 
 }
 // D[128 x N] = A rows [128 x P] times B rows [N x P], over the features
 template <int P, int N>
-__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b) {
+__device__ __forceinline__ void mma_rows(uint32_t on, uint32_t d, uint32_t a, uint32_t b) {
   const uint32_t idesc = (1u << 4) | SB_IDESC_AB_FMT | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
   const uint64_t da = make_desc(a, 16u, 1024u), db = make_desc(b, 16u, 1024u);
 #pragma unroll
   for (int k = 0; k < P / 16; ++k)
-    umma_f16(d, da + (uint64_t)((k >> 2) * (128 * 8) + (k & 3) * 2), db + (uint64_t)((k >> 2) * (N * 8) + (k & 3) * 2), idesc,
+    umma_ss(on, d, da + (uint64_t)((k >> 2) * (128 * 8) + (k & 3) * 2), db + (uint64_t)((k >> 2) * (N * 8) + (k & 3) * 2), idesc,
              k > 0 ? 1u : 0u);
 }
 // D[128 x P] (+)= S[128 x K] * B, S in tensor memory and B [K rows x P features] in shared memory
 template <int P, int K>
-__device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t s, uint32_t b, bool accumulate) {
+__device__ __forceinline__ void mma_weighted(uint32_t on, uint32_t d, uint32_t s, uint32_t b, bool accumulate) {
   const uint32_t idesc = (1u << 4) | SB_IDESC_AB_FMT | (1u << 16) | ((uint32_t)(P >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
   const uint64_t db = make_desc(b, (uint32_t)(K * 128), 1024u);
 #pragma unroll
   for (int k = 0; k < K / 16; ++k)
-    umma_f16_ts(d, s + (uint32_t)(k * 8), db + (uint64_t)(k * 128), idesc, (accumulate || k > 0) ? 1u : 0u);
+    umma_ts(on, d, s + (uint32_t)(k * 8), db + (uint64_t)(k * 128), idesc, (accumulate || k > 0) ? 1u : 0u);
 }
 // Rows from `valid` on of a [ROWS x P] tile become zeros: 0 * what stands behind a sequence's end must be 0.
 template <int P, int ROWS>
@@ -389,7 +405,7 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  const uint32_t tmem = uniform(*reinterpret_cast<volatile uint32_t*>(tmem_slot));
   grid_dependency_sync();
 
   // `it` counts the items that see a key, n their key tiles
@@ -436,6 +452,7 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer of scores, a tile ahead of the softmax ----------------
+    const uint32_t on = flash::elect_one() ? 1u : 0u;
     uint32_t it = 0, n = 0;                              // ring uses are 2 n (keys) and 2 n + 1 (values)
     bool ok = true;
     Item w;
@@ -443,41 +460,38 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       if (w.tiles == 0) continue;
       const uint32_t qb = it % kQ;
       ok = __all_sync(0xffffffffu, mbar_wait(q_full + 8 * qb, (it / kQ) & 1u, 42));
-      for (int i = 0; i < w.tiles && ok; ++i, ++n) {
+      const int tiles = uniform(w.tiles);
+      for (int i = 0; i < tiles && ok; ++i, ++n) {
         const uint32_t s = 2 * n % kRing, sb = n & 1u;
         ok = __all_sync(0xffffffffu, mbar_wait(kv_full + 8 * s, (2 * n / kRing) & 1u, 42) && mbar_wait(p_free + 8 * sb, ((n >> 1) & 1u) ^ 1u, 42));
         if (!ok) break;
         tc_fence_after();
-        if (flash::elect_one()) {
-          mma_rows<P, N>(tmem + sb * N, sq + qb * Cfg::kQTile, ring + s * Cfg::kTile);
-          umma_commit(s_full + 8 * sb);
-          umma_commit(kv_empty + 8 * s);
-          if (i == w.tiles - 1) umma_commit(q_empty + 8 * qb);
-        }
-        __syncwarp();
+        mma_rows<P, N>(on, tmem + sb * N, sq + qb * Cfg::kQTile, ring + s * Cfg::kTile);
+        commit_if(on, s_full + 8 * sb);
+        commit_if(on, kv_empty + 8 * s);
+        if (i == tiles - 1) commit_if(on, q_empty + 8 * qb);
       }
       ++it;
     }
   } else if (warp == 2) {
     // ---------------- MMA issuer of the output ----------------
+    const uint32_t on = flash::elect_one() ? 1u : 0u;
     uint32_t it = 0, n = 0;
     bool ok = true;
     Item w;
     while (ok && take(&w, &ok)) {
       if (w.tiles == 0) continue;
-      for (int i = 0; i < w.tiles; ++i, ++n) {
+      const int tiles = uniform(w.tiles);
+      for (int i = 0; i < tiles; ++i, ++n) {
         const uint32_t s = (2 * n + 1) % kRing, sb = n & 1u;
         ok = __all_sync(0xffffffffu, mbar_wait(kv_full + 8 * s, ((2 * n + 1) / kRing) & 1u, 43));
         if (ok && w.keys - i * N < N) zero_rows<P, N>(gen + (ring - sq) + s * Cfg::kTile, w.keys - i * N, lane);
         ok = ok && __all_sync(0xffffffffu, mbar_wait(p_full + 8 * sb, (n >> 1) & 1u, 43) && (i > 0 || mbar_wait(o_empty, (it & 1u) ^ 1u, 44)));
         if (!ok) break;
         tc_fence_after();
-        if (flash::elect_one()) {
-          mma_weighted<P, N>(tmem + Cfg::kO, tmem + sb * N, ring + s * Cfg::kTile, i > 0);
-          umma_commit(kv_empty + 8 * s);
-          umma_commit(p_free + 8 * sb);
-        }
-        __syncwarp();
+        mma_weighted<P, N>(on, tmem + Cfg::kO, tmem + sb * N, ring + s * Cfg::kTile, i > 0);
+        commit_if(on, kv_empty + 8 * s);
+        commit_if(on, p_free + 8 * sb);
       }
       ++it;
     }
@@ -742,7 +756,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  const uint32_t tmem = uniform(*reinterpret_cast<volatile uint32_t*>(tmem_slot));
   grid_dependency_sync();
 
   uint32_t taken = 0;
@@ -812,6 +826,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer of scores and dP ----------------
+    const uint32_t on = flash::elect_one() ? 1u : 0u;
     uint32_t live = 0, st = 0, st_phase = 0, bf = 0, bf_phase = 1;
     bool ok = true;
     Item w;
@@ -819,18 +834,16 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       if (w.tiles == 0) continue;
       const uint32_t hb = p.held == 2 ? live & 1u : 0u, hp = p.held == 2 ? live >> 1 : live, hd = sheld + hb * Cfg::kHeld;
       ok = __all_sync(0xffffffffu, mbar_wait(h_full + 8 * hb, hp & 1u, 56));
-      for (int i = 0; i < w.tiles && ok; ++i) {
+      const int tiles = uniform(w.tiles);
+      for (int i = 0; i < tiles && ok; ++i) {
         ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * st, st_phase, 56) && mbar_wait(buf_free + 8 * bf, bf_phase, 56));
         if (!ok) break;
         tc_fence_after();
         const uint32_t x = ring + st * Cfg::kStage, ts = tmem + bf * 128u;
         if (w.kind && w.keys - i * 64 < 64) zero_rows<P, 64>(gen + (x - sheld), w.keys - i * 64, lane);
-        if (flash::elect_one()) {
-          mma_rows<P, 64>(ts, hd, x);
-          mma_rows<P, 64>(ts + 64u, hd + Cfg::kHeld / 2, x + Cfg::kStream / 2);
-          umma_commit(s_full + 8 * bf);
-        }
-        __syncwarp();
+        mma_rows<P, 64>(on, ts, hd, x);
+        mma_rows<P, 64>(on, ts + 64u, hd + Cfg::kHeld / 2, x + Cfg::kStream / 2);
+        commit_if(on, s_full + 8 * bf);
         if (++st == (uint32_t)p.stages) { st = 0; st_phase ^= 1u; }
         if (++bf == (uint32_t)Cfg::kBuf) { bf = 0; bf_phase ^= 1u; }
       }
@@ -838,27 +851,26 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     }
   } else if (warp == 2) {
     // ---------------- MMA issuer of the products that read what became of them ----------------
+    const uint32_t on = flash::elect_one() ? 1u : 0u;
     uint32_t live = 0, st = 0, bf = 0, bf_phase = 0;
     bool ok = true;
     Item w;
     while (ok && take(&w, &ok)) {
       if (w.tiles == 0) continue;
-      for (int i = 0; i < w.tiles; ++i) {
+      const int tiles = uniform(w.tiles), kind = uniform(w.kind);
+      for (int i = 0; i < tiles; ++i) {
         ok = __all_sync(0xffffffffu, mbar_wait(pd_full + 8 * bf, bf_phase, 57) && (i > 0 || mbar_wait(acc_empty, (live & 1u) ^ 1u, 58)));
         if (!ok) break;
         tc_fence_after();
-        if (flash::elect_one()) {
-          const uint32_t x = ring + st * Cfg::kStage, ts = tmem + bf * 128u, acc = tmem + Cfg::kAcc;
-          mma_weighted<P, 64>(acc, ts + 64u, x, i > 0);                                               // dK += ds Q, dQ += ds K
-          if (!w.kind) mma_weighted<P, 64>(acc + (uint32_t)P, ts, x + Cfg::kStream / 2, i > 0);          // dV += softmax dOUT
-          umma_commit(empty + 8 * st);
-          umma_commit(buf_free + 8 * bf);
-          if (i == w.tiles - 1) {
-            umma_commit(h_empty + 8 * (p.held == 2 ? live & 1u : 0u));
-            umma_commit(acc_full);
-          }
+        const uint32_t x = ring + st * Cfg::kStage, ts = tmem + bf * 128u, acc = tmem + Cfg::kAcc;
+        mma_weighted<P, 64>(on, acc, ts + 64u, x, i > 0);                                               // dK += ds Q, dQ += ds K
+        if (!kind) mma_weighted<P, 64>(on, acc + (uint32_t)P, ts, x + Cfg::kStream / 2, i > 0);         // dV += softmax dOUT
+        commit_if(on, empty + 8 * st);
+        commit_if(on, buf_free + 8 * bf);
+        if (i == tiles - 1) {
+          commit_if(on, h_empty + 8 * (p.held == 2 ? live & 1u : 0u));
+          commit_if(on, acc_full);
         }
-        __syncwarp();
         if (++st == (uint32_t)p.stages) st = 0;
         if (++bf == (uint32_t)Cfg::kBuf) { bf = 0; bf_phase ^= 1u; }
       }

@@ -104,4 +104,15 @@ def attention(q, k, v, table, buckets, scale, causal=False, lengths=None, first=
     bound['dq'] = scale * torch.einsum('hbjk,phbk->phbj', rounded, kk.abs()) + end(r['dq'])
     bound['dtable'] = end(r['dtable'])
     bound['dtable'].index_add_(0, bucket.flatten(), off.permute(1, 2, 3, 0).reshape(-1, H))
+    # How far the table's gradient may stray although its sums are 32 bits: D comes from the output, whose P numbers are rounded
+    # once themselves and are sums of rounded exponentials.  A rounding is uniform in +-half |x| at most, of variance
+    # (half x)^2 / 3, and they are independent: var D = sum_p dout^2 half^2 / 3 (out^2 + sum_k p^2 v^2), and D's error enters bucket
+    # n with the probability of its keys.  Rows whose keys share a bucket do not take part.
+    var = half ** 2 / 3 * torch.einsum('phbj,phbj->hbj', g * g, r['out'] ** 2 + torch.einsum('hbjk,phbk->phbj', p * p, vv * vv))
+    stray = torch.zeros(H, dtype=torch.float64, device=dev)
+    for n in range(len(buckets)):
+        mass = (p * (bucket == n)).sum(-1)
+        mass[(bucket == n).masked_fill(~seen, True).all(-1).expand_as(mass)] = 0.0
+        stray += (mass ** 2 * var).sum((1, 2))
+    r['dtable_stray'] = float(stray.sum()) ** 0.5
     return r, bound

@@ -261,7 +261,8 @@ def test_attention_backward(case, dtype):
     for name in got:
         size = want[name].norm()
         if size > 1e-3 * bound[name].norm() and K > 1:
-            assert (got[name].double() - want[name]).norm() <= 1e-2 * size, name
+            stray = 3 * want['dtable_stray'] if name == 'dtable' else 0.0        # (three standard deviations, see the reference)
+            assert (got[name].double() - want[name]).norm() <= 1e-2 * size + stray, name
 
 
 @pytest.mark.parametrize('dtype', BOTH)
