@@ -28,12 +28,12 @@ struct AttnArgs {
   int J, K, H, G, B, P;
 };
 
-__device__ __forceinline__ int bucket_of(const AttnArgs& a, const Starts& st, int rel) {
+__device__ __forceinline__ int bucket_of(const AttnArgs& a, const int* starts, int rel) {
   const int d = rel > 0 ? (a.bidirectional ? rel : 0) : -rel;
   int lo = 0, hi = a.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (st.s[mid] <= d) lo = mid; else hi = mid - 1;
+    if (starts[mid] <= d) lo = mid; else hi = mid - 1;
   }
   return lo + (a.bidirectional && rel > 0 ? a.n : 0);
 }
@@ -56,7 +56,7 @@ expand_bias_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
   const int i = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
   if (i >= pitch) return;
   const int rel = max(-reach, min(reach, i - kRelPad - reach));
-  const float b = sb_h2f(a.table[bucket_of(a, st, rel) * a.t_sN + h * a.t_sH]);
+  const float b = sb_h2f(a.table[bucket_of(a, st.s, rel) * a.t_sN + h * a.t_sH]);
   rows[(long long)h * pitch + i] = b <= kHidden ? -INFINITY : b * 1.4426950408889634f;
 }
 
@@ -201,13 +201,7 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
   }
   __syncthreads();
   auto bias_at = [&](int rel, int h) {
-    const int d = rel > 0 ? (a.bidirectional ? rel : 0) : -rel;
-    int l = 0, u = a.n - 1;
-    while (l < u) {
-      const int mid = (l + u + 1) >> 1;
-      if (starts[mid] <= d) l = mid; else u = mid - 1;
-    }
-    const float v = sb_h2f(a.table[(l + (a.bidirectional && rel > 0 ? a.n : 0)) * a.t_sN + h * a.t_sH]);
+    const float v = sb_h2f(a.table[bucket_of(a, starts, rel) * a.t_sN + h * a.t_sH]);
     return v <= kHidden ? -INFINITY : v * 1.4426950408889634f;
   };
 #pragma unroll
@@ -390,77 +384,83 @@ join_splits_kernel(const __grid_constant__ FewParams p) {
 __global__ void __launch_bounds__(256)
 row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, float* records, int vec) {
   __shared__ float part[4][64];
+  __shared__ int starts[kRelMaxBuckets];
   grid_dependency_sync();
-  const int blocks = (a.J + 63) / 64;
-  const long long all = (long long)a.H * a.B * blocks;
-  for (long long it = blockIdx.x; it < all; it += gridDim.x) {
-    const int j0 = (int)(it % blocks) * 64, h = (int)(it / blocks % a.H), b = (int)(it / blocks / a.H);
-    const int row = vec ? threadIdx.x >> 2 : threadIdx.x & 63, i = vec ? threadIdx.x & 3 : threadIdx.x >> 6;
-    float sum = 0.f;
-    if (j0 + row < a.J) {
-      const sb_half* g = row_of(a.g, h, b, j0 + row);
-      const sb_half* o = row_of(a.o, h, b, j0 + row);
-      if (vec) {
-        for (int p = i * 8; p < a.P; p += 32) {
+  for (int i = threadIdx.x; i < a.n; i += 256) starts[i] = st.s[i];
+  const int blocks = (a.J + 63) / 64, it = blockIdx.x;
+  const int j0 = it % blocks * 64, h = it / blocks % a.H, b = it / blocks / a.H;
+  const int row = vec ? threadIdx.x >> 2 : threadIdx.x & 63, i = vec ? threadIdx.x & 3 : threadIdx.x >> 6;
+  float sum = 0.f;
+  if (j0 + row < a.J) {
+    const sb_half* g = row_of(a.g, h, b, j0 + row);
+    const sb_half* o = row_of(a.o, h, b, j0 + row);
+    if (vec) {
+#pragma unroll
+      for (int c = 0; c < kMaxP / 32; ++c) {
+        const int p = i * 8 + c * 32;
+        if (p < a.P) {
           float x[8], y[8];
           unpack8(*reinterpret_cast<const uint4*>(g + p), x);
           unpack8(*reinterpret_cast<const uint4*>(o + p), y);
 #pragma unroll
           for (int e = 0; e < 8; ++e) sum = fmaf(x[e], y[e], sum);
         }
-      } else {
-        for (int p = i; p < a.P; p += 4) sum = fmaf(sb_h2f(g[p * a.g.sP]), sb_h2f(o[p * a.o.sP]), sum);
       }
+    } else {
+#pragma unroll 4
+      for (int p = i; p < a.P; p += 4) sum = fmaf(sb_h2f(g[p * a.g.sP]), sb_h2f(o[p * a.o.sP]), sum);
     }
-    __syncthreads();
-    part[i][row] = sum;
-    __syncthreads();
-    if (threadIdx.x < 64) {
-      const int j = j0 + threadIdx.x;
-      float lse = INFINITY, weight = 0.f;
-      if (j < a.J) {
-        lse = a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] * 1.4426950408889634f;
-        if (lse == -INFINITY) lse = INFINITY;
-        const int pos = first_of(a, b) + j;
-        int n = keys_of(a, b);
-        if (a.causal) n = max(0, min(n, pos + 1));
-        // a row's score gradients sum to zero, so a row whose keys all share a bucket adds nothing to the table: its sum would
-        // only be what D, from the rounded output, is off by
-        if (n > 0 && bucket_of(a, st, -pos) != bucket_of(a, st, n - 1 - pos)) weight = 1.f;
-      }
-      float* r = records + it * 192 + threadIdx.x;
-      r[0] = lse;
-      r[64] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
-      r[128] = weight;
+  }
+  part[i][row] = sum;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int j = j0 + threadIdx.x;
+    float lse = INFINITY, weight = 0.f;
+    if (j < a.J) {
+      lse = a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] * 1.4426950408889634f;
+      if (lse == -INFINITY) lse = INFINITY;
+      const int pos = first_of(a, b) + j;
+      int n = keys_of(a, b);
+      if (a.causal) n = max(0, min(n, pos + 1));
+      // a row's score gradients sum to zero, so a row whose keys all share a bucket adds nothing to the table: its sum would
+      // only be what D, from the rounded output, is off by
+      if (n > 0 && bucket_of(a, starts, -pos) != bucket_of(a, starts, n - 1 - pos)) weight = 1.f;
     }
+    float* r = records + it * 192ll + threadIdx.x;
+    r[0] = lse;
+    r[64] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+    r[128] = weight;
   }
 }
 
-// dtable[n,h] = the head's sums over the relative positions of bucket n; one block each, in a fixed order.
-__global__ void __launch_bounds__(128)
+// dtable[n,h] = the head's sums over the relative positions of bucket n; one block each, in a fixed order: lanes along as many
+// positions as the bucket has, up to 32, and along rows of sums beside that.
+__global__ void __launch_bounds__(256)
 table_finish_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const float* partial, int rows, int reach,
                     sb_half* out, long long sN, long long sH) {
-  __shared__ float part[4];
+  __shared__ float part[8];
   grid_dependency_sync();
   const int n = blockIdx.x, h = blockIdx.y, entries = 2 * reach + 1;
   const bool behind = n >= a.n;
   const int i = behind ? n - a.n : n;
-  // distances [lo, hi]; without `bidirectional` every key behind the query has distance 0
-  int lo = st.s[i], hi = i + 1 < a.n ? st.s[i + 1] - 1 : reach;
-  if (behind) lo = max(lo, 1);
-  hi = min(hi, reach);
-  int from = behind ? reach + lo : reach - hi, to = behind ? reach + hi : reach - lo;
-  if (!a.bidirectional && lo == 0 && hi >= 0) to = 2 * reach;
-  const int run = max(0, to - from + 1);
+  // distances lo .. hi; without `bidirectional` every key behind the query has distance 0
+  const int lo = behind ? max(st.s[i], 1) : st.s[i], hi = i + 1 < a.n ? min(st.s[i + 1] - 1, reach) : reach;
+  const int from = behind ? reach + lo : reach - hi;
+  const int to = behind ? reach + hi : !a.bidirectional && lo == 0 && hi >= 0 ? 2 * reach : reach - lo;
+  const int run = to - from + 1;
+  int across = 1;
+  while (across < run && across < 32) across *= 2;
+  const int lane = threadIdx.x & 31, each = 32 / across, r0 = (threadIdx.x >> 5) * each + lane / across;
   const float* base = partial + (long long)h * rows * entries + from;
-  const long long all = (long long)rows * run;
   float s = 0.f;
-#pragma unroll 4
-  for (long long e = threadIdx.x; e < all; e += 128) s += base[e / run * entries + e % run];
+  for (int c = lane % across; c < run; c += across)
+#pragma unroll 8
+    for (int r = r0; r < rows; r += 8 * each) s += base[(long long)r * entries + c];
   s = group_sum<32>(s);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  if (lane == 0) part[threadIdx.x >> 5] = s;
   __syncthreads();
-  if (threadIdx.x == 0) out[n * sN + h * sH] = sb_f2h((part[0] + part[1]) + (part[2] + part[3]));
+  if (threadIdx.x == 0)
+    out[n * sN + h * sH] = sb_f2h(((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7])));
 }
 
 AttnArgs attn_args(const Proj& q, const Proj& k, const Proj& v, const RelBias& bias, const Proj& out, const RelRows& lse, const RelSpan& span,
@@ -620,15 +620,14 @@ int launch_rel_attn_bwd(cudaStream_t s, void* scratch, Proj dout, Proj q, Proj k
   float* records = reinterpret_cast<float*>(base + pl.records);
   int* next = reinterpret_cast<int*>(base + pl.p.next);
   const long long blocks = (long long)a.H * a.B * ((a.J + 63) / 64);
-  SB_LAUNCH_OK(launch_k(row_records_kernel, (unsigned)std::min<long long>(blocks, 8 * usable_sms(device_facts().sms)), 256, 0, s, a, st, records,
-                        pieces(dout) && pieces(out) ? 1 : 0));
+  SB_LAUNCH_OK(launch_k(row_records_kernel, (unsigned)blocks, 256, 0, s, a, st, records, pieces(dout) && pieces(out) ? 1 : 0));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[0], &dout));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[1], &q));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[2], &k));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[3], &v));
   float* partial = reinterpret_cast<float*>(base + pl.partial);
   SB_TRY(launch_rel_tiles_bwd(s, dout, q, k, v, t, RelBackward{records, partial, next}, dq, dk, dv, span));
-  SB_LAUNCH_OK(launch_k(table_finish_kernel, dim3(a.buckets, a.H), 128, 0, s, a, st, partial, pl.rows, pl.p.reach,
+  SB_LAUNCH_OK(launch_k(table_finish_kernel, dim3(a.buckets, a.H), 256, 0, s, a, st, partial, pl.rows, pl.p.reach,
                         reinterpret_cast<sb_half*>(dtable), dt_sN, dt_sH));
   return SB_OK;
 }
