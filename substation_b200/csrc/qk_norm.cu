@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 #include "ops.h"
 
@@ -217,8 +218,10 @@ norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ T
 
 // Any strides, any head size, lanes along tokens (what head-first projections have side by side).  Warp w of a block has the
 // pairs w, w + 8, .. of features (rotary pairs, then neighbours), SLOTS at most, of TOKENS tokens per lane, and keeps their
-// angles in registers while the block walks its heads; a row's sums go through shared memory.
-template <int SLOTS, int TOKENS, bool BWD>
+// angles in registers while the block walks its heads; a row's sums go through shared memory.  Off: the type that holds a
+// feature's offset, 32 bits wherever a head's features span less than 2^31 elements (64-bit products of strides were most of the
+// instructions).
+template <int SLOTS, int TOKENS, bool BWD, class Off>
 __global__ void __launch_bounds__(256)
 norm_strided_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Turns turns) {
   __shared__ float2 part[2][8][32 * TOKENS];
@@ -228,61 +231,77 @@ norm_strided_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ 
   const int chunks = (a.x[w].H + a.chunk - 1) / a.chunk, stride = a.blocks[w] / chunks;
   const int h_from = mine % chunks * a.chunk, h_to = min(a.x[w].H, h_from + a.chunk);
   const float inv = 1.f / (float)a.P;
-  const sb_half* X = reinterpret_cast<const sb_half*>(a.x[w].p);
-  const sb_half* G = reinterpret_cast<const sb_half*>(a.g[w].p);
-  sb_half* Y = reinterpret_cast<sb_half*>(a.y[w].p);
-  // features of slot i: f (always there where the slot is) and f2
-  auto first = [&](int i) { const int u = warp + 8 * i; return u < pairs ? (a.pairing == SB_PAIR_HALVES ? u : 2 * u) : 2 * u; };
-  auto second = [&](int i) { const int u = warp + 8 * i; return u < pairs && a.pairing == SB_PAIR_HALVES ? u + pairs : 2 * u + 1; };
+  // the two features of each slot: number (that of the first where there is none), gain (then 0), place in x, g and y
+  int feature[SLOTS][2];
+  Off xo[SLOTS][2], go[SLOTS][2], yo[SLOTS][2];
   float gain[SLOTS][2], sum[SLOTS][2];
+  uint32_t there = 0;
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
-    const bool there = warp + 8 * i < slots;
-    gain[i][0] = there ? sb_h2f(a.gain[w][first(i)]) : 0.f;
-    gain[i][1] = there && second(i) < a.P ? sb_h2f(a.gain[w][second(i)]) : 0.f;
-    sum[i][0] = sum[i][1] = 0.f;
+    const int u = warp + 8 * i;
+    const bool halves = u < pairs && a.pairing == SB_PAIR_HALVES;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int f = halves ? u + e * pairs : 2 * u + e;
+      const bool is = u < slots && f < a.P;
+      there |= (is ? 1u : 0u) << (2 * i + e);
+      feature[i][e] = is ? f : 0;
+      gain[i][e] = is ? sb_h2f(a.gain[w][f]) : 0.f;
+      xo[i][e] = (Off)(feature[i][e] * a.x[w].sP);
+      go[i][e] = BWD ? (Off)(feature[i][e] * a.g[w].sP) : 0;
+      yo[i][e] = (Off)(feature[i][e] * a.y[w].sP);
+      sum[i][e] = 0.f;
+    }
   }
   int turnstile = 0;
   for (int t = mine / chunks; t < a.tiles; t += stride) {
-    int token[TOKENS];
     bool live[TOKENS];
     float2 ang[SLOTS][TOKENS];
-    long long ox[TOKENS], og[TOKENS], oy[TOKENS];
+    const sb_half *X[TOKENS], *G[TOKENS];
+    sb_half* Y[TOKENS];
 #pragma unroll
     for (int k = 0; k < TOKENS; ++k) {
-      token[k] = t * 32 * TOKENS + k * 32 + lane;
-      live[k] = token[k] < a.tokens;
-      const int tc = live[k] ? token[k] : 0, pos = position(a, tc);
+      const int token = t * 32 * TOKENS + k * 32 + lane;
+      live[k] = token < a.tokens;
+      const int tc = live[k] ? token : 0, pos = position(a, tc);
 #pragma unroll
       for (int i = 0; i < SLOTS; ++i) ang[i][k] = warp + 8 * i < pairs ? cos_sin(pos, turns.t[warp + 8 * i]) : make_float2(1.f, 0.f);
-      ox[k] = token_offset(a.x[w], tc, a.J);
-      og[k] = BWD ? token_offset(a.g[w], tc, a.J) : 0;
-      oy[k] = token_offset(a.y[w], tc, a.J);
+      X[k] = reinterpret_cast<const sb_half*>(a.x[w].p) + token_offset(a.x[w], tc, a.J) + h_from * a.x[w].sH;
+      G[k] = BWD ? reinterpret_cast<const sb_half*>(a.g[w].p) + token_offset(a.g[w], tc, a.J) + h_from * a.g[w].sH : nullptr;
+      Y[k] = reinterpret_cast<sb_half*>(a.y[w].p) + token_offset(a.y[w], tc, a.J) + h_from * a.y[w].sH;
     }
     for (int h = h_from; h < h_to; ++h, turnstile ^= 1) {
-      sb_half xr[SLOTS][TOKENS][2], gr[SLOTS][TOKENS][2];
+      float x[SLOTS][TOKENS][2], g[SLOTS][TOKENS][2];
 #pragma unroll
-      for (int i = 0; i < SLOTS; ++i)
+      for (int k = 0; k < TOKENS; ++k) {
 #pragma unroll
-        for (int k = 0; k < TOKENS; ++k)
+        for (int i = 0; i < SLOTS; ++i)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int f = e ? second(i) : first(i);
-            const bool there = live[k] && warp + 8 * i < slots && f < a.P;
-            xr[i][k][e] = there ? X[ox[k] + h * a.x[w].sH + f * a.x[w].sP] : sb_f2h(0.f);
-            if (BWD) gr[i][k][e] = there ? G[og[k] + h * a.g[w].sH + f * a.g[w].sP] : sb_f2h(0.f);
+            const bool is = (there >> (2 * i + e)) & 1u;      // (a feature that is not there reads the first and counts 0)
+            const float v = sb_h2f(X[k][xo[i][e]]);
+            x[i][k][e] = is ? v : 0.f;
+            if (BWD) {
+              const float d = sb_h2f(G[k][go[i][e]]);
+              g[i][k][e] = is ? d : 0.f;
+            }
           }
+        X[k] += a.x[w].sH;
+        if (BWD) G[k] += a.g[w].sH;
+      }
       float sq[TOKENS], dot[TOKENS];
 #pragma unroll
       for (int k = 0; k < TOKENS; ++k) {
         sq[k] = dot[k] = 0.f;
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i) {
-          const float u = sb_h2f(xr[i][k][0]), v = sb_h2f(xr[i][k][1]);
+          const float u = x[i][k][0], v = x[i][k][1];
           sq[k] = fmaf(u, u, fmaf(v, v, sq[k]));
           if (BWD) {
-            const float c = ang[i][k].x, s = ang[i][k].y, p = sb_h2f(gr[i][k][0]), q = sb_h2f(gr[i][k][1]);
-            dot[k] = fmaf((p * c + q * s) * gain[i][0], u, fmaf((q * c - p * s) * gain[i][1], v, dot[k]));
+            const float c = ang[i][k].x, s = ang[i][k].y, p = g[i][k][0], q = g[i][k][1];
+            g[i][k][0] = p * c + q * s;                       // turned back
+            g[i][k][1] = q * c - p * s;
+            dot[k] = fmaf(g[i][k][0] * gain[i][0], u, fmaf(g[i][k][1] * gain[i][1], v, dot[k]));
           }
         }
         part[turnstile][warp][k * 32 + lane] = make_float2(sq[k], dot[k]);
@@ -295,29 +314,29 @@ norm_strided_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ 
         for (int i = 0; i < 8; ++i) {
           const float2 s = part[turnstile][i][k * 32 + lane];
           sq[k] += s.x;
-          dot[k] += s.y;
+          if (BWD) dot[k] += s.y;
         }
         const float rs = rsqrtf(fmaf(sq[k], inv, a.eps)), mean = dot[k] * rs * inv;
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i) {
-          const float c = ang[i][k].x, s = ang[i][k].y;
-          float u = sb_h2f(xr[i][k][0]) * rs, v = sb_h2f(xr[i][k][1]) * rs;
+          float u = x[i][k][0] * rs, v = x[i][k][1] * rs;
           if (!BWD) {
-            const float p = u * gain[i][0], q = v * gain[i][1];
+            const float c = ang[i][k].x, s = ang[i][k].y, p = u * gain[i][0], q = v * gain[i][1];
             u = p * c - q * s;
             v = q * c + p * s;
           } else {
-            const float y = sb_h2f(gr[i][k][0]), z = sb_h2f(gr[i][k][1]), p = y * c + z * s, q = z * c - y * s;
-            sum[i][0] = fmaf(p, u, sum[i][0]);
-            sum[i][1] = fmaf(q, v, sum[i][1]);
+            const float p = g[i][k][0], q = g[i][k][1];
+            if (live[k]) {                                    // (what lies behind the last token is token 0 again)
+              sum[i][0] = fmaf(p, u, sum[i][0]);
+              sum[i][1] = fmaf(q, v, sum[i][1]);
+            }
             u = rs * (p * gain[i][0] - u * mean);
             v = rs * (q * gain[i][1] - v * mean);
           }
-          if (live[k] && warp + 8 * i < slots) {
-            Y[oy[k] + h * a.y[w].sH + first(i) * a.y[w].sP] = sb_f2h(u);
-            if (second(i) < a.P) Y[oy[k] + h * a.y[w].sH + second(i) * a.y[w].sP] = sb_f2h(v);
-          }
+          if (live[k] && ((there >> (2 * i)) & 1u)) Y[k][yo[i][0]] = sb_f2h(u);
+          if (live[k] && ((there >> (2 * i + 1)) & 1u)) Y[k][yo[i][1]] = sb_f2h(v);
         }
+        Y[k] += a.y[w].sH;
       }
     }
   }
@@ -326,8 +345,7 @@ norm_strided_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ 
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const float v = warp_sum(sum[i][e]);
-      const int f = e ? second(i) : first(i);
-      if (lane == 0 && warp + 8 * i < slots && f < a.P) a.partial[w][(long long)mine * a.P + f] = v;
+      if (lane == 0 && ((there >> (2 * i + e)) & 1u)) a.partial[w][(long long)mine * a.P + feature[i][e]] = v;
     }
 }
 
@@ -411,7 +429,11 @@ int launch_strided(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) 
     const int each = BWD && chunks > 0 ? std::max(1, std::min(a.tiles, kMaxPartials / chunks)) : a.tiles;
     a.blocks[w] = rows[w] = chunks * each;
   }
-  SB_LAUNCH_OK(launch_k(norm_strided_kernel<SLOTS, TOKENS, BWD>, a.blocks[0] + a.blocks[1], 256, 0, s, a, turns_of(rot)));
+  bool narrow = true;
+  for (int w = 0; w < 2; ++w)
+    for (const Proj* v : {&a.x[w], &a.y[w], &a.g[w]}) narrow = narrow && std::llabs(v->sP) < (1ll << 31) / kNormMaxHead;
+  auto kernel = narrow ? norm_strided_kernel<SLOTS, TOKENS, BWD, int> : norm_strided_kernel<SLOTS, TOKENS, BWD, long long>;
+  SB_LAUNCH_OK(launch_k(kernel, a.blocks[0] + a.blocks[1], 256, 0, s, a, turns_of(rot)));
   return SB_OK;
 }
 template <bool BWD>

@@ -105,6 +105,7 @@ struct FewCfg {
 struct FewParams {
   AttnArgs a;
   int rows, blocks, splits, reach;                   // rows of a key head, blocks of 16 of them
+  int before, behind;                                // buckets of far keys
   float* partial;                                    // [B][G][rows][splits][P + 2]: output, reference, sum; null with one share
 };
 
@@ -139,6 +140,7 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
   constexpr int kKeys = Cfg::kKeys, kStages = Cfg::kStages, kSteps = P / 16, kTiles = kKeys / 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int starts[kRelMaxBuckets];
+  __shared__ uint16_t map[2 * kRelMaxReach + 2];
   const AttnArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_sync();
@@ -155,20 +157,27 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
   const sb_half* kp = row_of(a.k, hk, b, 0);
   const sb_half* vp = row_of(a.v, hk, b, 0);
 
-  // piece i of this warp into its slot: 16-byte chunk c of row r at c ^ (r & 7)
+  // piece i of this warp into its slot: 16-byte chunk c of row r at c ^ (r & 7); a lane has one c and every kStep-th row
+  constexpr int kStep = 32 / (P / 8);
+  const int fr = lane / (P / 8), fc = lane % (P / 8), bytes = max(0, min(16, (a.P - fc * 8) * 2));
+  const sb_half* fk = kp + (long long)(k_from + warp * kKeys + fr) * a.k.sR + (bytes > 0 ? fc * 8 : 0);
+  const sb_half* fv = vp + (long long)(k_from + warp * kKeys + fr) * a.v.sR + (bytes > 0 ? fc * 8 : 0);
+  int left = k_to - (k_from + warp * kKeys) - fr, slot = 0;
   auto fetch = [&](int i) {
     if (i < mine) {
-      const int k0 = k_from + (warp + 4 * i) * kKeys;
-      const uint32_t slot = ring + (i % kStages) * 2 * Cfg::kHalf;
+      const uint32_t at = ring + slot * 2 * Cfg::kHalf;
 #pragma unroll
-      for (int x = lane; x < kKeys * (P / 8); x += 32) {
-        const int r = x / (P / 8), c = x % (P / 8), k = min(k0 + r, a.K - 1);
-        const int bytes = k0 + r < k_to ? max(0, min(16, (a.P - c * 8) * 2)) : 0;
-        const int from = bytes > 0 ? c * 8 : 0;
-        const uint32_t d = slot + r * (P * 2) + ((c ^ (r & 7)) << 4);
-        cp_async16(d, kp + (long long)k * a.k.sR + from, bytes);
-        cp_async16(d + Cfg::kHalf, vp + (long long)k * a.v.sR + from, bytes);
+      for (int x = 0; x < kKeys / kStep; ++x) {
+        const int r = fr + x * kStep;
+        const bool there = x * kStep < left;                 // (a row that is not there is read as no bytes of the first one)
+        const uint32_t d = at + r * (P * 2) + ((fc ^ (r & 7)) << 4);
+        cp_async16(d, there ? fk + (long long)(x * kStep) * a.k.sR : kp, there ? bytes : 0);
+        cp_async16(d + Cfg::kHalf, there ? fv + (long long)(x * kStep) * a.v.sR : vp, there ? bytes : 0);
       }
+      fk += (long long)(4 * kKeys) * a.k.sR;
+      fv += (long long)(4 * kKeys) * a.v.sR;
+      left -= 4 * kKeys;
+      if (++slot == kStages) slot = 0;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -199,15 +208,21 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
         qf[s][y * 2 + x] = pack_pair(u, v);
       }
   }
-  __syncthreads();
-  auto bias_at = [&](int rel, int h) {
-    const float v = sb_h2f(a.table[bucket_of(a, starts, rel) * a.t_sN + h * a.t_sH]);
+  auto bias_of = [&](int bucket, int h) {
+    const float v = sb_h2f(a.table[bucket * a.t_sN + h * a.t_sH]);
     return v <= kHidden ? -INFINITY : v * 1.4426950408889634f;
   };
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    lo[x] = bias_at(-p.reach, head[x]);
-    hi[x] = bias_at(p.reach, head[x]);
+    lo[x] = bias_of(p.before, head[x]);
+    hi[x] = bias_of(p.behind, head[x]);
+  }
+  __syncthreads();
+  // buckets of the relative positions within reach, where this CTA's keys have any
+  const int pos_lo = first, pos_hi = first + a.J - 1;
+  if (k_to - 1 - pos_lo > -p.reach && k_from - pos_hi < p.reach) {
+    for (int i = threadIdx.x; i <= 2 * p.reach; i += kFewThreads) map[i] = (uint16_t)bucket_of(a, starts, i - p.reach);
+    __syncthreads();
   }
   const float c2 = a.scale * 1.4426950408889634f;
   float o[P / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -215,7 +230,6 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
   for (int i = 0; i < P / 8; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-  const int pos_lo = first, pos_hi = first + a.J - 1;
 
   for (int i = 0; i < mine; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
@@ -240,18 +254,29 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
       }
     // biases, what is hidden, maxima
     const bool near = k0 + kKeys - 1 - pos_lo > -p.reach && k0 - pos_hi < p.reach;
-    const bool after = k0 - pos_hi >= p.reach;
+    const bool after = k0 - pos_hi >= p.reach, whole = k0 + kKeys <= k_to && !(a.causal && k0 + kKeys - 1 > pos_lo);
     float mx[2] = {-INFINITY, -INFINITY};
+    if (!near && whole) {
+      const float flat[2] = {after ? hi[0] : lo[0], after ? hi[1] : lo[1]};
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t)
+      for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int x = e >> 1, k = k0 + t * 8 + (lane & 3) * 2 + (e & 1);
-        const float bias = near ? bias_at(k - pos[x], head[x]) : after ? hi[x] : lo[x];
-        const bool seen = k < k_to && !(a.causal && k > pos[x]);
-        s[t][e] = seen ? fmaf(s[t][e], c2, bias) : -INFINITY;
-        mx[x] = fmaxf(mx[x], s[t][e]);
-      }
+        for (int e = 0; e < 4; ++e) {
+          s[t][e] = fmaf(s[t][e], c2, flat[e >> 1]);
+          mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
+        }
+    } else {
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int x = e >> 1, k = k0 + t * 8 + (lane & 3) * 2 + (e & 1), rel = k - pos[x];
+          const float bias = rel <= -p.reach ? lo[x] : rel >= p.reach ? hi[x] : bias_of(map[rel + p.reach], head[x]);
+          const bool seen = k < k_to && !(a.causal && rel > 0);
+          s[t][e] = seen ? fmaf(s[t][e], c2, bias) : -INFINITY;
+          mx[x] = fmaxf(mx[x], s[t][e]);
+        }
+    }
     bool raise = false;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -387,8 +412,9 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
   __shared__ int starts[kRelMaxBuckets];
   grid_dependency_sync();
   for (int i = threadIdx.x; i < a.n; i += 256) starts[i] = st.s[i];
-  const int blocks = (a.J + 63) / 64, it = blockIdx.x;
-  const int j0 = it % blocks * 64, h = it / blocks % a.H, b = it / blocks / a.H;
+  // blocks that run together share tokens, whose heads usually lie side by side
+  const int blocks = (a.J + 63) / 64, h = blockIdx.x % a.H, block = blockIdx.x / a.H % blocks, b = blockIdx.x / a.H / blocks;
+  const int j0 = block * 64;
   const int row = vec ? threadIdx.x >> 2 : threadIdx.x & 63, i = vec ? threadIdx.x & 3 : threadIdx.x >> 6;
   float sum = 0.f;
   if (j0 + row < a.J) {
@@ -426,7 +452,7 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
       // only be what D, from the rounded output, is off by
       if (n > 0 && bucket_of(a, starts, -pos) != bucket_of(a, starts, n - 1 - pos)) weight = 1.f;
     }
-    float* r = records + it * 192ll + threadIdx.x;
+    float* r = records + (((long long)b * a.H + h) * blocks + block) * 192 + threadIdx.x;
     r[0] = lse;
     r[64] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
     r[128] = weight;
@@ -575,6 +601,10 @@ int launch_rel_attn_fwd(cudaStream_t s, void* scratch, Proj q, Proj k, Proj v, c
     p.blocks = (p.rows + 15) / 16;
     p.splits = f.splits;
     p.reach = std::max(1, bias.starts[bias.n - 1]);
+    p.before = bias.n - 1;
+    p.behind = 0;
+    if (bias.bidirectional) p.behind = 2 * bias.n - 1;
+    else while (p.behind + 1 < bias.n && bias.starts[p.behind + 1] <= 0) ++p.behind;
     p.partial = f.splits > 1 ? reinterpret_cast<float*>(scratch) : nullptr;
     return q.P <= 64 ? launch_few<64>(s, p, st) : launch_few<128>(s, p, st);
   }
