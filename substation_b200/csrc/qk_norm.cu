@@ -15,9 +15,9 @@ constexpr int kDepth = 4;              // rows that a thread of the pieces kerne
 constexpr int kMaxPairs = kNormMaxHead / 2;
 constexpr int kMaxPartials = 1184;     // rows of partial sums of a gain's gradient: eight blocks of 148 SMs
 
-// Turns per position of pair i: base^(-2i/rotary) / (2 pi).  Angles are counted in turns and reduced to a fraction of one in
-// 64 bits: a position of 2^31 then still has 22 bits behind the binary point.
-struct Turns { double t[kMaxPairs]; };
+// Turns per position of pair i, base^(-2i/rotary) / (2 pi), as a fraction of 2^64: the product with a position, of any sign, wraps
+// around as turns do, and its top half is the angle to 2^-32 of a turn however far out the position is.
+struct Turns { unsigned long long t[kMaxPairs]; };
 
 struct NormArgs {
   Proj x[2], g[2], y[2];               // queries, keys: input, gradient of the output (backward), result
@@ -31,18 +31,21 @@ struct NormArgs {
   float eps;
 };
 
-__device__ __forceinline__ float2 cos_sin(int pos, double turns_per_position) {
-  const double t = (double)pos * turns_per_position;
+__device__ __forceinline__ float2 cos_sin(int pos, unsigned long long turns_per_position) {
+  const unsigned long long t = (unsigned long long)(long long)pos * turns_per_position;
   float s, c;
-  sincospif(2.f * (float)(t - rint(t)), &s, &c);
+  sincospif((float)(int)(t >> 32) * 4.656612873077393e-10f, &s, &c);   // halves of a turn: 2^-31
   return make_float2(c, s);
 }
-__device__ __forceinline__ int position(const NormArgs& a, int token) {
-  return a.pos[(long long)(token / a.J) * a.pos_sB + (long long)(token % a.J) * a.pos_sJ];
+struct Place { int b, j; };
+__device__ __forceinline__ Place place_of(const NormArgs& a, int token) {
+  Place p;
+  p.b = token / a.J;
+  p.j = token - p.b * a.J;
+  return p;
 }
-__device__ __forceinline__ long long token_offset(const Proj& v, int token, int J) {
-  return (long long)(token / J) * v.sB + (long long)(token % J) * v.sR;
-}
+__device__ __forceinline__ int position(const NormArgs& a, Place p) { return a.pos[p.b * a.pos_sB + p.j * a.pos_sJ]; }
+__device__ __forceinline__ long long token_offset(const Proj& v, Place p) { return p.b * v.sB + p.j * v.sR; }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -59,7 +62,7 @@ __global__ void __launch_bounds__(256, 2)
 norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Turns turns) {
   constexpr int kGroups = 256 / LANES, kPieces = BWD ? 4 : 2;
   extern __shared__ uint4 smem[];                             // ring [kDepth][kPieces][256], frequencies, angles [2][tile][pairs]
-  double* freq = reinterpret_cast<double*>(smem + kDepth * kPieces * 256);
+  unsigned long long* freq = reinterpret_cast<unsigned long long*>(smem + kDepth * kPieces * 256);
   float2* cs = reinterpret_cast<float2*>(freq + a.rotary / 2);
   grid_dependency_sync();
   const int pairs = a.rotary / 2, turned = a.rotary / 16, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
@@ -74,6 +77,10 @@ norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ T
   uint4* slots = smem + threadIdx.x;
   const uint32_t slots_at = (uint32_t)__cvta_generic_to_shared(slots);
 
+  if (!on)                                                    // (what no copy writes stays 0)
+    for (int i = 0; i < kDepth * kPieces; ++i) slots[i * 256] = make_uint4(0u, 0u, 0u, 0u);
+  const long long x_step = across * vx.sH, g_step = across * vg.sH, y_step = across * vy.sH;
+
   // the row that is fetched next
   int ft = mine, fh = first_head, fslot = 0;
   const sb_half *fx = nullptr, *fg = nullptr;
@@ -82,20 +89,21 @@ norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ T
     const int token = ft * a.tile + tok;
     flive = on && ft < a.tiles && token < a.tokens && first_head < heads;
     if (flive) {
-      fx = reinterpret_cast<const sb_half*>(vx.p) + token_offset(vx, token, a.J);
-      if (BWD) fg = reinterpret_cast<const sb_half*>(vg.p) + token_offset(vg, token, a.J);
+      const Place p = place_of(a, token);
+      fx = reinterpret_cast<const sb_half*>(vx.p) + token_offset(vx, p) + first_head * vx.sH;
+      if (BWD) fg = reinterpret_cast<const sb_half*>(vg.p) + token_offset(vg, p) + first_head * vg.sH;
     }
   };
   auto fetch = [&] {
     if (flive) {
       const uint32_t d = slots_at + fslot * kPieces * 4096;
-      const sb_half* s = fx + fh * vx.sH;
-      cp_async16(d, s + f0);
-      cp_async16(d + 4096, s + f1);
+      cp_async16(d, fx + f0);
+      cp_async16(d + 4096, fx + f1);
+      fx += x_step;
       if (BWD) {
-        s = fg + fh * vg.sH;
-        cp_async16(d + 2 * 4096, s + f0);
-        cp_async16(d + 3 * 4096, s + f1);
+        cp_async16(d + 2 * 4096, fg + f0);
+        cp_async16(d + 3 * 4096, fg + f1);
+        fg += g_step;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -121,12 +129,15 @@ norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ T
   float sum[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) sum[e] = 0.f;
+  const uint32_t by_pairs = 0xffffffffu / max(pairs, 1) + 1u;   // (i < 2^16: the quotient's high half is exact)
   int slot = 0, buffer = 0;
   for (int t = mine; t < a.tiles; t += a.blocks[w], buffer ^= 1) {
     const int t0 = t * a.tile, token = t0 + tok;
     float2* table = cs + buffer * a.tile * pairs;             // (two in turn: one barrier a tile)
-    for (int i = threadIdx.x; i < a.tile * pairs; i += 256)
-      if (t0 + i / pairs < a.tokens) table[i] = cos_sin(position(a, t0 + i / pairs), freq[i % pairs]);
+    for (int i = threadIdx.x; i < a.tile * pairs; i += 256) {
+      const int k = pairs > 1 ? (int)__umulhi((uint32_t)i, by_pairs) : i;
+      if (t0 + k < a.tokens) table[i] = cos_sin(position(a, place_of(a, t0 + k)), freq[i - k * pairs]);
+    }
     __syncthreads();
     const bool live = token < a.tokens;
     // halves: the angles of pairs (f0 + e, f1 + e); adjacent: four of the first piece, four of the second
@@ -144,24 +155,24 @@ norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ T
         q = y * ang[e].x + x * s;
       }
     };
-    sb_half* py = reinterpret_cast<sb_half*>(vy.p) + (live ? token_offset(vy, token, a.J) : 0);
-    for (int h = first_head; h < heads; h += across) {
+    sb_half* py = reinterpret_cast<sb_half*>(vy.p) + (live ? token_offset(vy, place_of(a, token)) : 0) + first_head * vy.sH;
+    for (int h = first_head; h < heads; h += across, py += y_step) {
       fetch();
       asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
       const uint4* in = slots + slot * kPieces * 256;
       if (++slot == kDepth) slot = 0;
       if (!live) continue;
       float u[8], v[8], p[8], q[8], sq = 0.f, dot = 0.f;
-      unpack8(on ? in[0] : make_uint4(0u, 0u, 0u, 0u), u);
-      unpack8(on ? in[256] : make_uint4(0u, 0u, 0u, 0u), v);
+      unpack8(in[0], u);
+      unpack8(in[256], v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) sq = fmaf(u[e], u[e], fmaf(v[e], v[e], sq));
       if (BWD) {
-        unpack8(on ? in[512] : make_uint4(0u, 0u, 0u, 0u), p);
-        unpack8(on ? in[768] : make_uint4(0u, 0u, 0u, 0u), q);
+        unpack8(in[512], p);
+        unpack8(in[768], q);
         turn(p, q, -1.f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) dot = fmaf(p[e] * gf[0][e], u[e], fmaf(q[e] * gf[1][e], v[e], dot));
+        for (int e = 0; e < 8; ++e) dot = fmaf(p[e] * u[e], gf[0][e], fmaf(q[e] * v[e], gf[1][e], dot));
       }
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) {
@@ -177,20 +188,18 @@ norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ T
         }
         turn(u, v, 1.f);
       } else {
-        const float mean = dot * rs * inv;                    // of g gain n
+        const float k = -dot * rs * rs * rs * inv;            // dx = rs g gain - x rs^3 mean(g gain x)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float nu = u[e] * rs, nv = v[e] * rs;
-          sum[e] = fmaf(p[e], nu, sum[e]);
-          sum[8 + e] = fmaf(q[e], nv, sum[8 + e]);
-          u[e] = rs * (p[e] * gf[0][e] - nu * mean);
-          v[e] = rs * (q[e] * gf[1][e] - nv * mean);
+          sum[e] = fmaf(p[e] * u[e], rs, sum[e]);
+          sum[8 + e] = fmaf(q[e] * v[e], rs, sum[8 + e]);
+          u[e] = fmaf(p[e] * gf[0][e], rs, u[e] * k);
+          v[e] = fmaf(q[e] * gf[1][e], rs, v[e] * k);
         }
       }
       if (on) {
-        sb_half* d = py + h * vy.sH;
-        *reinterpret_cast<uint4*>(d + f0) = pack8(u);
-        *reinterpret_cast<uint4*>(d + f1) = pack8(v);
+        *reinterpret_cast<uint4*>(py + f0) = pack8(u);
+        *reinterpret_cast<uint4*>(py + f1) = pack8(v);
       }
     }
   }
@@ -263,12 +272,13 @@ norm_strided_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ 
     for (int k = 0; k < TOKENS; ++k) {
       const int token = t * 32 * TOKENS + k * 32 + lane;
       live[k] = token < a.tokens;
-      const int tc = live[k] ? token : 0, pos = position(a, tc);
+      const Place tc = place_of(a, live[k] ? token : 0);
+      const int pos = position(a, tc);
 #pragma unroll
       for (int i = 0; i < SLOTS; ++i) ang[i][k] = warp + 8 * i < pairs ? cos_sin(pos, turns.t[warp + 8 * i]) : make_float2(1.f, 0.f);
-      X[k] = reinterpret_cast<const sb_half*>(a.x[w].p) + token_offset(a.x[w], tc, a.J) + h_from * a.x[w].sH;
-      G[k] = BWD ? reinterpret_cast<const sb_half*>(a.g[w].p) + token_offset(a.g[w], tc, a.J) + h_from * a.g[w].sH : nullptr;
-      Y[k] = reinterpret_cast<sb_half*>(a.y[w].p) + token_offset(a.y[w], tc, a.J) + h_from * a.y[w].sH;
+      X[k] = reinterpret_cast<const sb_half*>(a.x[w].p) + token_offset(a.x[w], tc) + h_from * a.x[w].sH;
+      G[k] = BWD ? reinterpret_cast<const sb_half*>(a.g[w].p) + token_offset(a.g[w], tc) + h_from * a.g[w].sH : nullptr;
+      Y[k] = reinterpret_cast<sb_half*>(a.y[w].p) + token_offset(a.y[w], tc) + h_from * a.y[w].sH;
     }
     for (int h = h_from; h < h_to; ++h, turnstile ^= 1) {
       float x[SLOTS][TOKENS][2], g[SLOTS][TOKENS][2];
@@ -372,8 +382,13 @@ const Turns& turns_of(const Rotation& r) {
   static thread_local double base = 0.0;
   static thread_local int rotary = -1;
   if (base != r.base || rotary != r.rotary) {
-    for (int i = 0; i < kMaxPairs; ++i)
-      t.t[i] = 2 * i < r.rotary ? std::pow(r.base, -2.0 * i / r.rotary) / 6.283185307179586476925286766559 : 0.0;
+    for (int i = 0; i < kMaxPairs; ++i) {
+      t.t[i] = 0;
+      if (2 * i >= r.rotary) continue;
+      const long double turns = std::pow((long double)r.base, -2.0L * i / r.rotary) / 6.283185307179586476925286766559L;
+      const long double scaled = std::ldexp(turns - std::floor(turns), 64);
+      t.t[i] = scaled < 18446744073709551615.0L ? (unsigned long long)scaled : ~0ull;
+    }
     base = r.base;
     rotary = r.rotary;
   }
@@ -411,7 +426,7 @@ int launch_pieces(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
   const int most = std::min(2 * sms, kMaxPartials), heads = a.x[0].H + a.x[1].H;
   for (int w = 0; w < 2; ++w)
     a.blocks[w] = rows[w] = a.x[w].H > 0 ? std::min(a.tiles, std::max(1, (int)(most * (long long)a.x[w].H / heads))) : 0;
-  const size_t smem = kDepth * (BWD ? 4 : 2) * 4096 + sizeof(double) * (a.rotary / 2) + 2 * sizeof(float2) * a.tile * (a.rotary / 2);
+  const size_t smem = kDepth * (BWD ? 4 : 2) * 4096 + sizeof(unsigned long long) * (a.rotary / 2) + 2 * sizeof(float2) * a.tile * (a.rotary / 2);
   auto kernel = a.pairing == SB_PAIR_HALVES ? norm_pieces_kernel<LANES, BWD, true> : norm_pieces_kernel<LANES, BWD, false>;
   SB_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), 100 * 1024));
   SB_LAUNCH_OK(launch_k(kernel, a.blocks[0] + a.blocks[1], 256, smem, s, a, turns_of(rot)));
@@ -422,7 +437,7 @@ int launch_strided(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) 
   const int sms = usable_sms(device_facts().sms), heads = a.x[0].H + a.x[1].H;
   a.tiles = (a.tokens + 32 * TOKENS - 1) / (32 * TOKENS);
   // up to eight heads a block, which share the angles; fewer where SMs would be without a block
-  for (a.chunk = 8; a.chunk > 1 && (long long)a.tiles * ((heads + a.chunk - 1) / a.chunk) < 2 * sms; a.chunk /= 2) {}
+  for (a.chunk = 8; a.chunk > 1 && (long long)a.tiles * ((heads + a.chunk - 1) / a.chunk) < sms; a.chunk /= 2) {}
   for (int w = 0; w < 2; ++w) {
     const int chunks = (a.x[w].H + a.chunk - 1) / a.chunk;
     // (every chunk has the same number of blocks; the backward pass bounds their number by its rows of sums)
