@@ -231,7 +231,7 @@ norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ T
 // feature's offset, 32 bits wherever a head's features span less than 2^31 elements (64-bit products of strides were most of the
 // instructions).
 template <int SLOTS, int TOKENS, bool BWD, class Off>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, SLOTS <= 4 ? 2 : 1)
 norm_strided_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Turns turns) {
   __shared__ float2 part[2][8][32 * TOKENS];
   grid_dependency_sync();
@@ -421,11 +421,11 @@ int launch_pieces(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
   const int sms = usable_sms(device_facts().sms), groups = 256 / LANES;
   for (a.tile = groups / 4; a.tile > 1 && (a.tokens + a.tile - 1) / a.tile < sms; a.tile /= 2) {}
   a.tiles = (a.tokens + a.tile - 1) / a.tile;
-  // Two blocks an SM at a time, the queries' and the keys' share of them by their heads; the backward pass has room for the sums
-  // of so many.
-  const int most = std::min(2 * sms, kMaxPartials), heads = a.x[0].H + a.x[1].H;
+  // Two blocks an SM at a time; the backward pass has room for the sums of so many.  A tile costs its heads and, for angles and
+  // barriers, about as much as six more, and so queries and keys share the blocks.
+  const int most = std::min(2 * sms, kMaxPartials), cost[2] = {a.x[0].H + 6, a.x[1].H > 0 ? a.x[1].H + 6 : 0};
   for (int w = 0; w < 2; ++w)
-    a.blocks[w] = rows[w] = a.x[w].H > 0 ? std::min(a.tiles, std::max(1, (int)(most * (long long)a.x[w].H / heads))) : 0;
+    a.blocks[w] = rows[w] = cost[w] ? std::min(a.tiles, std::max(1, (most * cost[w] + (w ? cost[0] + cost[1] - 1 : 0)) / (cost[0] + cost[1]))) : 0;
   const size_t smem = kDepth * (BWD ? 4 : 2) * 4096 + sizeof(unsigned long long) * (a.rotary / 2) + 2 * sizeof(float2) * a.tile * (a.rotary / 2);
   auto kernel = a.pairing == SB_PAIR_HALVES ? norm_pieces_kernel<LANES, BWD, true> : norm_pieces_kernel<LANES, BWD, false>;
   SB_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), 100 * 1024));
@@ -463,7 +463,7 @@ int launch_norm(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
     if (a.P <= 128) return launch_pieces<8, BWD>(s, a, rot, rows);
     return launch_pieces<16, BWD>(s, a, rot, rows);
   }
-  return a.P <= 64 ? launch_strided<4, 2, BWD>(s, a, rot, rows) : a.P <= 128 ? launch_strided<8, 1, BWD>(s, a, rot, rows)
+  return a.P <= 64 ? launch_strided<4, 1, BWD>(s, a, rot, rows) : a.P <= 128 ? launch_strided<8, 1, BWD>(s, a, rot, rows)
                                                                              : launch_strided<16, 1, BWD>(s, a, rot, rows);
 }
 
