@@ -1635,17 +1635,20 @@ template <int P>
 int rel_bwd(cudaStream_t s, const CUtensorMap (&m)[8], rel::BwdParams& p) {
   using Cfg = rel::BwdCfg<P>;
   constexpr int kMost = 232448;
-  // Two held pairs let an item's tiles arrive while the one before computes; they go first where the sums' rows leave no room,
-  // then streamed pairs beyond those that scores run ahead.
-  for (p.held = 2; p.held > 1 && Cfg::smem(Cfg::kBuf, p.held, p.c.pitch, p.c.reach) > kMost; --p.held) {}
-  for (p.stages = 6; p.stages > Cfg::kBuf && Cfg::smem(p.stages, p.held, p.c.pitch, p.c.reach) > kMost; --p.stages) {}
-  static_assert(Cfg::smem(Cfg::kBuf, 1, 2 * kRelMaxReach + 4 + 2 * rel::kPad, kRelMaxReach) <= kMost, "shared memory of the attention backward kernel");
+  // Two held pairs let an item's tiles arrive while the one before computes, two sets of sums save a barrier per query tile.  The sets
+  // and then the held pairs give way where the sums' rows are long, then streamed pairs beyond those that scores run ahead.
+  auto need = [&] { return Cfg::smem(p.stages, p.held, p.sets, p.c.pitch, p.c.reach); };
+  p.stages = Cfg::kBuf; p.held = 2; p.sets = 2;
+  if (need() > kMost) p.sets = 1;
+  if (need() > kMost) p.held = 1;
+  while (p.stages < 6 && Cfg::smem(p.stages + 1, p.held, p.sets, p.c.pitch, p.c.reach) <= kMost) ++p.stages;
+  static_assert(Cfg::smem(Cfg::kBuf, 1, 1, 2 * kRelMaxReach + 4 + 2 * rel::kPad, kRelMaxReach) <= kMost, "shared memory of the attention backward kernel");
   const int ctas = sm_count();
   p.chunk_k = p.c.causal ? std::min(p.c.G * p.c.B, std::max(1, (4 * ctas + p.nk - 1) / p.nk)) : 1;
   p.chunk_q = p.c.causal ? std::min(p.c.H * p.c.B, std::max(1, (4 * ctas + p.nq - 1) / p.nq)) : 1;
   SB_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(rel::rel_bwd_kernel<P>), kMost));
   SB_LAUNCH_OK(launch_k(rel::rel_bwd_kernel<P>, (unsigned)std::min(p.items, ctas), rel::kBwdThreads,
-                        Cfg::smem(p.stages, p.held, p.c.pitch, p.c.reach), s, m[0], m[1], m[2], m[3], m[4], m[5], m[6], m[7], p));
+                        need(), s, m[0], m[1], m[2], m[3], m[4], m[5], m[6], m[7], p));
   return SB_OK;
 }
 

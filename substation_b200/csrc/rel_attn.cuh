@@ -573,6 +573,7 @@ struct BwdParams {
   int first_q, items;                                // items below first_q: dK and dV of a key tile; the others: dQ of a query tile
   int chunk_k, chunk_q;
   int stages, held;                                  // ring of streamed pairs; held pairs (1 or 2)
+  int sets;                                          // rows of sums per warp (1 or 2)
   float scale;
   const float* records;                              // [B][H][ceil(J / 64)][kRecord]
   float* partial;                                    // [H][B * nq * 2][2 * reach + 1]
@@ -610,13 +611,13 @@ __device__ __forceinline__ Item bwd_item(const BwdParams& p, int i) {
 
 template <int P>
 struct BwdCfg {
-  static constexpr int kHeld = 2 * 128 * P * 2, kStream = 2 * 64 * P * 2, kStage = kStream + 1024;
+  static constexpr int kHeld = 2 * 128 * P * 2 + 2048, kStream = 2 * 64 * P * 2, kStage = kStream + 1024;   // tiles and records
   // Tensor memory: buffers of scores and dP (64 columns each), then the accumulators.  A third buffer, where it fits, lets a tile
   // be multiplied before either group is done with its own: without it a group waits for two products and two hand-overs.
   static constexpr int kBuf = P == 64 ? 3 : 2;
   static constexpr uint32_t kAcc = kBuf * 128;
-  static constexpr int smem(int stages, int held, int pitch, int reach) {
-    return held * kHeld + stages * kStage + 2 * pitch * 4 + 8 * ((2 * reach + 4) & ~3) * 4 + 1024 + 400 + 48 * kSlots;
+  static constexpr int smem(int stages, int held, int sets, int pitch, int reach) {
+    return held * kHeld + stages * kStage + 2 * pitch * 4 + sets * 8 * ((2 * reach + 4) & ~3) * 4 + 1024 + 400 + 48 * kSlots;
   }
 };
 
@@ -690,7 +691,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
   const uint32_t sheld = (raw + 1023u) & ~1023u, ring = sheld + p.held * Cfg::kHeld;
   const uint32_t sbias = ring + p.stages * Cfg::kStage;
   const int width = (2 * p.c.reach + 4) & ~3;        // floats of a warp's row of sums
-  const uint32_t ssums = sbias + 2u * p.c.pitch * 4u, bars = ssums + 8u * width * 4u;
+  const uint32_t ssums = sbias + 2u * p.c.pitch * 4u, bars = ssums + p.sets * 8u * width * 4u;
   const uint32_t item_full = bars, item_empty = bars + 32, h_full = bars + 64, h_empty = bars + 80, b_full = bars + 96, b_empty = bars + 112;
   const uint32_t s_full = bars + 128, pd_full = bars + 152, acc_full = bars + 176, acc_empty = bars + 184, full = bars + 192, empty = bars + 256;
   uint8_t* gen = smem_raw + (sheld - raw);
@@ -732,7 +733,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
   }
   {
     float* sums = reinterpret_cast<float*>(gen + (ssums - sheld));
-    for (int i = threadIdx.x; i < 8 * width; i += kBwdThreads) sums[i] = 0.f;
+    for (int i = threadIdx.x; i < p.sets * 8 * width; i += kBwdThreads) sums[i] = 0.f;
   }
   tc_fence_before();
   __syncthreads();
@@ -764,9 +765,11 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         if (!ok) break;
         if (lane == 0) {
           const uint32_t d = sheld + hb * Cfg::kHeld;
-          mbar_expect_tx(h_full + 8 * hb, Cfg::kHeld);
+          const int rows = min(2, blocks - w.t * 2) * kRecord * 4;   // bytes of a query tile's records
+          mbar_expect_tx(h_full + 8 * hb, 512 * P + (w.kind ? rows : 0));
           load_rows<P, 128>(d, w.kind ? &tmQh : &tmKh, h_full + 8 * hb, w.t * 128, w.h, w.b);
-          load_rows<P, 128>(d + Cfg::kHeld / 2, w.kind ? &tmGh : &tmVh, h_full + 8 * hb, w.t * 128, w.h, w.b);
+          load_rows<P, 128>(d + 256 * P, w.kind ? &tmGh : &tmVh, h_full + 8 * hb, w.t * 128, w.h, w.b);
+          if (w.kind) bulk_load(d + 512 * P, p.records + (((long long)w.b * p.c.H + w.h) * blocks + w.t * 2) * kRecord, rows, h_full + 8 * hb);
         }
         __syncwarp();
         ++live;
@@ -823,7 +826,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         const uint32_t x = ring + st * Cfg::kStage, ts = tmem + bf * 128u;
         if (w.kind && w.keys - i * 64 < 64) zero_rows<P, 64>(gen + (x - sheld), w.keys - i * 64, lane);
         mma_rows<P, 64>(on, ts, hd, x);
-        mma_rows<P, 64>(on, ts + 64u, hd + Cfg::kHeld / 2, x + Cfg::kStream / 2);
+        mma_rows<P, 64>(on, ts + 64u, hd + 256 * P, x + Cfg::kStream / 2);
         commit_if(on, s_full + 8 * bf);
         if (++st == (uint32_t)p.stages) { st = 0; st_phase ^= 1u; }
         if (++bf == (uint32_t)Cfg::kBuf) { bf = 0; bf_phase ^= 1u; }
@@ -861,9 +864,10 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     // ---------------- element warps ----------------
     const int q = warp & 3, g = (warp - 3) >> 2, rt = q * 32 + lane;
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
-    const int blocks = (p.c.J + 63) >> 6, reach = p.c.reach, entries = 2 * reach + 1;
-    float* group_sums = reinterpret_cast<float*>(gen + (ssums - sheld)) + g * 4 * width;
+    const int reach = p.c.reach, entries = 2 * reach + 1;
+    float* group_sums = reinterpret_cast<float*>(gen + (ssums - sheld)) + g * 4 * width;   // with a second set 8 rows behind
     float* sums = group_sums + ((warp - 3) & 3) * width;
+    int other_set = p.sets == 2 ? 8 * width : 0;
     const int in_group = ((warp - 3) & 3) * 32 + lane;
     uint32_t n = 0, live = 0, run = 0, st = 0, st_phase = 0, bf = 0, bf_phase = 0;
     bool ok = true, have = false;
@@ -912,7 +916,8 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       ++syncs;
       return ok;
     };
-    // the group's sums of a query tile to memory
+    // The group's sums of a query tile to memory.  The rows are left at zero for the next but one such item; with one set it
+    // is the next one, and everybody has to be done with them.
     auto flush = [&](const Item& it) {
       const float lo = warp_sum(below), hi = warp_sum(above);
       below = above = 0.f;
@@ -931,7 +936,10 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         }
         out[i] = v;
       }
-      group_sync();
+      group_sums += other_set;
+      sums += other_set;
+      other_set = -other_set;
+      if (p.sets == 1) group_sync();
     };
     Item w;
     while (ok && take(&w, &ok)) {
@@ -942,32 +950,43 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       }
       const int r = w.t * 128 + rt;                    // query or key of this thread
       float lse = INFINITY, dsum = 0.f, weight = 1.f;
-      if (w.kind && r < p.c.J) {
-        const float* rec = p.records + (((long long)w.b * p.c.H + w.h) * blocks + (r >> 6)) * kRecord + (r & 63);
-        lse = rec[0];
-        dsum = rec[64];
-        weight = rec[128];
+      if (w.kind) {
+        const uint32_t hb = p.held == 2 ? live & 1u : 0u, hp = p.held == 2 ? live >> 1 : live;
+        ok = __all_sync(0xffffffffu, mbar_wait(h_full + 8 * hb, hp & 1u, 60));
+        if (!ok) break;
+        if (r < p.c.J) {
+          const float* rec = reinterpret_cast<const float*>(gen + hb * Cfg::kHeld + 512 * P) + (rt >> 6) * kRecord + (rt & 63);
+          lse = rec[0];
+          dsum = rec[64];
+          weight = rec[128];
+        }
       }
       const bool weighted = __any_sync(0xffffffffu, weight != 1.f);
       bool due = have;                                 // the previous item's results are still to be stored
-      // Per streamed tile, all moving by 64: relative position of this thread's first column, lowest of the warp's block (its
-      // highest is lo + 94), the thread's bound on visible columns and the block's tightest.
-      const int step = w.kind ? 64 : -64;
-      int rel = w.kind ? -(w.first + r) : r - (w.first + w.t0 * 64), lim;
-      if (w.kind) lim = p.c.causal ? min(w.keys, w.first + r + 1) : w.keys;
-      else lim = r < w.keys ? (p.c.causal ? rel : -(1 << 30)) : 1 << 30;
-      const int rel0 = rel, lim0 = lim, lo0 = __shfl_sync(0xffffffffu, rel, w.kind ? 31 : 0) - (w.kind ? 0 : 63);
-      const int tight0 = w.kind ? __reduce_min_sync(0xffffffffu, lim) : __reduce_max_sync(0xffffffffu, lim);
-      const bool moves = w.kind || p.c.causal;
-      int lo = lo0, tight = tight0, left = w.each;
-      const float* bias = bias_s;
-      for (int i = 0; i < w.tiles; ++i, ++n) {
-        if (left == w.each) {
-          ok = __all_sync(0xffffffffu, mbar_wait(b_full + 8 * (run & 1u), (run >> 1) & 1u, 60));
-          if (!ok) break;
-          bias = bias_s + (run & 1u) * p.c.pitch;
-        }
-        if ((int)(n & 1u) == g) {
+      // At the first streamed tile of a run, all moving by 64 a tile: relative position of this thread's first column, lowest of
+      // the warp's block (its highest is lo + 94), the thread's bound on visible columns and the block's tightest.
+      const int step = w.kind ? 64 : -64, moves = w.kind || p.c.causal ? 64 : 0;
+      int lim0;
+      const int rel0 = w.kind ? -(w.first + r) : r - (w.first + w.t0 * 64);
+      if (w.kind) lim0 = p.c.causal ? min(w.keys, w.first + r + 1) : w.keys;
+      else lim0 = r < w.keys ? (p.c.causal ? rel0 : -(1 << 30)) : 1 << 30;
+      const int lo0 = __shfl_sync(0xffffffffu, rel0, w.kind ? 31 : 0) - (w.kind ? 0 : 63);
+      const int tight0 = w.kind ? __reduce_min_sync(0xffffffffu, lim0) : __reduce_max_sync(0xffffffffu, lim0);
+      for (int done = 0; done < w.tiles && ok; done += w.each) {
+        const float* bias = bias_s + (run & 1u) * p.c.pitch;
+        ok = __all_sync(0xffffffffu, mbar_wait(b_full + 8 * (run & 1u), (run >> 1) & 1u, 60));
+        // this group's tiles of the run: every second one
+        const int skip = (n & 1u) == (uint32_t)g ? 0 : 1;
+        n += w.each;
+        auto advance = [&](uint32_t by) {
+          st += by;
+          if (st >= (uint32_t)p.stages) { st -= p.stages; st_phase ^= 1u; }
+          bf += by;
+          if (bf >= (uint32_t)Cfg::kBuf) { bf -= Cfg::kBuf; bf_phase ^= 1u; }
+        };
+        if (skip) advance(1);
+        int rel = rel0 + skip * step, lo = lo0 + skip * step, lim = lim0 - skip * moves, tight = tight0 - skip * moves, i = skip;
+        for (; i < w.each && ok; i += 2) {
           const bool near = lo + 94 > -reach && lo < reach;
           // outside the varying part, a place in the row where the 64 entries in use have the end's value
           const float* bp = bias + (near ? rel + reach + kPad : (lo >= reach ? kPad + 2 * reach : 0) + (w.kind ? 0 : 64));
@@ -1015,19 +1034,15 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
             if (!ok) break;
             due = false;
           }
+          advance(i + 2 <= w.each ? 2 : 1);
+          rel += 2 * step;
+          lo += 2 * step;
+          lim -= 2 * moves;
+          tight -= 2 * moves;
         }
-        if (++st == (uint32_t)p.stages) { st = 0; st_phase ^= 1u; }
-        if (++bf == (uint32_t)Cfg::kBuf) { bf = 0; bf_phase ^= 1u; }
-        rel += step;
-        lo += step;
-        if (moves) { lim -= 64; tight -= 64; }
-        if (--left == 0) {
-          rel = rel0; lo = lo0; lim = lim0; tight = tight0;
-          left = w.each;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(b_empty + 8 * (run & 1u));
-          ++run;
-        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b_empty + 8 * (run & 1u));
+        ++run;
       }
       if (!ok) break;
       if (due) {
