@@ -1631,9 +1631,9 @@ int launch_rel_tiles_fwd(cudaStream_t s, Proj q, Proj k, Proj v, RelTables t, in
 
 namespace {
 
-template <int P>
+template <int P, bool BOTH>
 int rel_bwd(cudaStream_t s, const CUtensorMap (&m)[8], rel::BwdParams& p) {
-  using Cfg = rel::BwdCfg<P>;
+  using Cfg = rel::BwdCfg<P, BOTH>;
   constexpr int kMost = 232448;
   // Two held pairs let an item's tiles arrive while the one before computes, two sets of sums save a barrier per query tile.  The sets
   // and then the held pairs give way where the sums' rows are long, then streamed pairs beyond those that scores run ahead.
@@ -1646,9 +1646,9 @@ int rel_bwd(cudaStream_t s, const CUtensorMap (&m)[8], rel::BwdParams& p) {
   const int ctas = sm_count();
   p.chunk_k = p.c.causal ? std::min(p.c.G * p.c.B, std::max(1, (4 * ctas + p.nk - 1) / p.nk)) : 1;
   p.chunk_q = p.c.causal ? std::min(p.c.H * p.c.B, std::max(1, (4 * ctas + p.nq - 1) / p.nq)) : 1;
-  SB_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(rel::rel_bwd_kernel<P>), kMost));
-  SB_LAUNCH_OK(launch_k(rel::rel_bwd_kernel<P>, (unsigned)std::min(p.items, ctas), rel::kBwdThreads,
-                        need(), s, m[0], m[1], m[2], m[3], m[4], m[5], m[6], m[7], p));
+  SB_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(rel::rel_bwd_kernel<P, BOTH>), kMost));
+  SB_LAUNCH_OK(launch_k(rel::rel_bwd_kernel<P, BOTH>, (unsigned)std::min(p.items, ctas), rel::kBwdThreads, need(), s, m[0], m[1], m[2], m[3], m[4],
+                        m[5], m[6], m[7], p));
   return SB_OK;
 }
 
@@ -1673,7 +1673,10 @@ int launch_rel_tiles_bwd(cudaStream_t s, Proj dout, Proj q, Proj k, Proj v, RelT
   p.scale = span.scale;
   p.records = w.records; p.partial = w.partial; p.next = w.next;
   p.dq = dq; p.dk = dk; p.dv = dv;
-  return q.P <= 64 ? rel_bwd<64>(s, m, p) : rel_bwd<128>(s, m, p);
+  // Units of one tile each way give all three gradients in one item; with shared key heads dQ would have to be stored per head.
+  const bool both = q.P <= 64 && p.nq == 1 && p.nk == 1 && q.H == k.H;
+  if (both) p.items = p.first_q;
+  return both ? rel_bwd<64, true>(s, m, p) : q.P <= 64 ? rel_bwd<64, false>(s, m, p) : rel_bwd<128, false>(s, m, p);
 }
 
 int gemm_device_error(cudaStream_t s, int* code) {

@@ -118,6 +118,14 @@ __device__ __forceinline__ void mma_weighted(uint32_t on, uint32_t d, uint32_t s
   for (int k = 0; k < K / 16; ++k)
     umma_ts(on, d, s + (uint32_t)(k * 8), db + (uint64_t)(k * 128), idesc, (accumulate || k > 0) ? 1u : 0u);
 }
+// D[128 x P] = S^T * B, S [128 x 128] in shared memory as two boxes of 64 columns, summed over its rows, B [128 rows x P features]
+template <int P>
+__device__ __forceinline__ void mma_transposed(uint32_t on, uint32_t d, uint32_t s, uint32_t b) {
+  const uint32_t idesc = (1u << 4) | SB_IDESC_AB_FMT | (1u << 15) | (1u << 16) | ((uint32_t)(P >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+  const uint64_t da = make_desc(s, 16384u, 1024u), db = make_desc(b, 16384u, 1024u);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) umma_ss(on, d, da + (uint64_t)(k * 128), db + (uint64_t)(k * 128), idesc, k > 0 ? 1u : 0u);
+}
 // Rows from `valid` on of a [ROWS x P] tile become zeros: 0 * what stands behind a sequence's end must be 0.
 template <int P, int ROWS>
 __device__ __forceinline__ void zero_rows(uint8_t* tile, int valid, int lane) {
@@ -584,9 +592,10 @@ struct BwdParams {
 // An item holds one pair of 128-row tiles and streams pairs of 64-row tiles past it: (K, V) held and (Q, dOUT) of every query
 // head that shares them streamed (kind 0), or (Q, dOUT) held and (K, V) streamed (kind 1).  `b`, `h`, `t`: the held tile;
 // `tiles` streamed ones, `each` from t0 on for each head in turn.
+template <bool BOTH>
 __device__ __forceinline__ Item bwd_item(const BwdParams& p, int i) {
   Item it;
-  it.kind = i >= p.first_q ? 1 : 0;
+  it.kind = !BOTH && i >= p.first_q ? 1 : 0;
   if (it.kind) i -= p.first_q;
   const int rows = it.kind ? p.nq : p.nk, heads = it.kind ? p.c.H : p.c.G, chunk = it.kind ? p.chunk_q : p.chunk_k;
   const int per = chunk * rows, c = i / per, r = i % per;
@@ -602,22 +611,27 @@ __device__ __forceinline__ Item bwd_item(const BwdParams& p, int i) {
     it.each = it.tiles = (it.keys + 63) >> 6;
   } else {
     const int all = (p.c.J + 63) >> 6;
-    if (p.c.causal) it.t0 = min(all, max(0, it.t * 128 - it.first) >> 6);
+    if (p.c.causal && !BOTH) it.t0 = min(all, max(0, it.t * 128 - it.first) >> 6);
     it.each = it.t * 128 < it.keys ? all - it.t0 : 0;
     it.tiles = it.each * (p.c.H / p.c.G);
   }
   return it;
 }
 
-template <int P>
+// BOTH: units of one tile of queries and one of keys, each key head with one query head: an item gives all three gradients and
+// everything is computed once.  dQ needs score gradients with the keys as the summed index, so they go to shared memory as
+// well ([128 keys x 128 queries], 32 KB).
+template <int P, bool BOTH>
 struct BwdCfg {
+  static_assert(P == 64 || !BOTH, "tensor memory has no room for a third accumulator of 128 columns");
   static constexpr int kHeld = 2 * 128 * P * 2 + 2048, kStream = 2 * 64 * P * 2, kStage = kStream + 1024;   // tiles and records
+  static constexpr int kStaged = BOTH ? 32768 : 0;
   // Tensor memory: buffers of scores and dP (64 columns each), then the accumulators.  A third buffer, where it fits, lets a tile
   // be multiplied before either group is done with its own: without it a group waits for two products and two hand-overs.
-  static constexpr int kBuf = P == 64 ? 3 : 2;
-  static constexpr uint32_t kAcc = kBuf * 128;
+  static constexpr int kBuf = P == 64 && !BOTH ? 3 : 2;
+  static constexpr uint32_t kAcc = P == 64 ? 384 : 256, kAccQ = 256;
   static constexpr int smem(int stages, int held, int sets, int pitch, int reach) {
-    return held * kHeld + stages * kStage + 2 * pitch * 4 + sets * 8 * ((2 * reach + 4) & ~3) * 4 + 1024 + 400 + 48 * kSlots;
+    return held * kHeld + stages * kStage + kStaged + 2 * pitch * 4 + sets * 8 * ((2 * reach + 4) & ~3) * 4 + 1024 + 400 + 48 * kSlots;
   }
 };
 
@@ -625,10 +639,10 @@ struct BwdCfg {
 // from, 32 columns at a time.  Column c has the bias bp[c] (key tiles: bp[-c]; NEAR) or `flat`.
 // What differs between the two kinds of items: in key tiles (KEYS) a thread is a key, log-sum-exps and D change along columns
 // (L, D in shared memory), visible columns are c >= lim; in query tiles a thread is a query and visible columns are c < lim.
-// `emit` gets every score gradient, `block` is told after each 32 columns.
+// `emit` gets every score gradient, `block` is told after each 32 columns; `staged`: where the row goes in shared memory too.
 template <bool KEYS, bool NEAR, bool MASK, class Emit, class Block>
 __device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float flat, const float* L, const float* D, float lse, float dsum,
-                                          int lim, float c2, Emit&& emit, Block&& block) {
+                                          int lim, float c2, Emit&& emit, Block&& block, uint8_t* staged = nullptr, int row7 = 0) {
   const float2 c22 = make_float2(c2, c2), minus = make_float2(-1.f, -1.f);
 #pragma unroll 1
   for (int c = 0; c < 2; ++c) {
@@ -667,6 +681,11 @@ __device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float fl
     }
     if (KEYS) tmem_st16(ts + c * 16, pm);
     tmem_st16(ts + 64 + c * 16, dm);
+    if (staged) {                                        // (a row of 128 bytes, 16-byte piece i at i ^ (row & 7))
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        *reinterpret_cast<uint4*>(staged + (((c * 4 + v) ^ row7) << 4)) = make_uint4(dm[4 * v], dm[4 * v + 1], dm[4 * v + 2], dm[4 * v + 3]);
+    }
     block(c);
   }
 }
@@ -674,22 +693,22 @@ __device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float fl
 // One CTA per SM.  The two groups of element
 // warps take the streamed tiles in turn: while one turns scores and dP into exponentials and score gradients, the tensor cores
 // multiply for the other.  Both results go back into tensor memory, where the second products take them from.  Everything is
-// computed twice, once per kind of item; the alternative, dQ summed over key tiles in memory, needs atomics whose order
+// computed twice, once per kind of item (but for BOTH); the alternative, dQ summed over key tiles in memory, needs atomics whose order
 // changes the result, or a partial dQ for every key tile.
 // The table's gradient: a score gradient belongs to its relative position, a diagonal of the tile.  A warp moves each column of
 // its 32 x 32 blocks so that lane l holds diagonals l and l - 32 (one shuffle a column), adds the sums of a block to its own row
 // of sums over relative positions, and a group of warps adds up its four rows per item.  Tiles outside the varying part of the
 // bias have one sum.  Everything in a fixed order.
-template <int P>
+template <int P, bool BOTH>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__ CUtensorMap tmGh, const __grid_constant__ CUtensorMap tmKh,
                const __grid_constant__ CUtensorMap tmVh, const __grid_constant__ CUtensorMap tmQs, const __grid_constant__ CUtensorMap tmGs,
                const __grid_constant__ CUtensorMap tmKs, const __grid_constant__ CUtensorMap tmVs, const __grid_constant__ BwdParams p) {
-  using Cfg = BwdCfg<P>;
+  using Cfg = BwdCfg<P, BOTH>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t sheld = (raw + 1023u) & ~1023u, ring = sheld + p.held * Cfg::kHeld;
-  const uint32_t sbias = ring + p.stages * Cfg::kStage;
+  const uint32_t staged = ring + p.stages * Cfg::kStage, sbias = staged + Cfg::kStaged;
   const int width = (2 * p.c.reach + 4) & ~3;        // floats of a warp's row of sums
   const uint32_t ssums = sbias + 2u * p.c.pitch * 4u, bars = ssums + p.sets * 8u * width * 4u;
   const uint32_t item_full = bars, item_empty = bars + 32, h_full = bars + 64, h_empty = bars + 80, b_full = bars + 96, b_empty = bars + 112;
@@ -697,7 +716,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
   uint8_t* gen = smem_raw + (sheld - raw);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (bars + 320 - sheld));
   uint8_t* slots = gen + (bars + 400 - sheld);
-  const uint32_t g_sync = bars + 352, buf_free = bars + 368;
+  const uint32_t g_sync = bars + 352, buf_free = bars + 368, q_free = bars + 392;
   const float* bias_s = reinterpret_cast<const float*>(gen + (sbias - sheld));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -720,6 +739,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     }
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, 8);
+    mbar_init(q_free, 1);
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(full + 8 * i, 1);
       mbar_init(empty + 8 * i, 1);
@@ -756,7 +776,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       if (lane == 0 && id < p.items) after = atomicAdd(p.next, 1) + (int)gridDim.x;
       Item w;
       w.kind = -1;
-      if (id < p.items) w = bwd_item(p, id);
+      if (id < p.items) w = bwd_item<BOTH>(p, id);
       ok = put_item(slots, item_full, item_empty, &put, lane, w);
       if (!ok || id >= p.items) break;
       if (w.tiles > 0) {
@@ -791,14 +811,14 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         if (!ok) break;
         if (lane == 0) {
           const uint32_t d = ring + st * Cfg::kStage, bar = full + 8 * st;
-          mbar_expect_tx(bar, Cfg::kStream + (w.kind ? 0 : 512));
+          mbar_expect_tx(bar, Cfg::kStream + (w.kind ? 0 : BOTH ? 768 : 512));
           if (w.kind) {
             load_rows<P, 64>(d, &tmKs, bar, t * 64, w.h / rep, w.b);
             load_rows<P, 64>(d + Cfg::kStream / 2, &tmVs, bar, t * 64, w.h / rep, w.b);
           } else {
             load_rows<P, 64>(d, &tmQs, bar, t * 64, head, w.b);
             load_rows<P, 64>(d + Cfg::kStream / 2, &tmGs, bar, t * 64, head, w.b);
-            bulk_load(d + Cfg::kStream, p.records + (((long long)w.b * p.c.H + head) * blocks + t) * kRecord, 512, bar);
+            bulk_load(d + Cfg::kStream, p.records + (((long long)w.b * p.c.H + head) * blocks + t) * kRecord, BOTH ? 768 : 512, bar);
           }
         }
         __syncwarp();
@@ -825,6 +845,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         tc_fence_after();
         const uint32_t x = ring + st * Cfg::kStage, ts = tmem + bf * 128u;
         if (w.kind && w.keys - i * 64 < 64) zero_rows<P, 64>(gen + (x - sheld), w.keys - i * 64, lane);
+        if (BOTH && i == 0 && w.keys < 128) zero_rows<P, 128>(gen + (hd - sheld), w.keys, lane);
         mma_rows<P, 64>(on, ts, hd, x);
         mma_rows<P, 64>(on, ts + 64u, hd + 256 * P, x + Cfg::kStream / 2);
         commit_if(on, s_full + 8 * bf);
@@ -849,6 +870,10 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         const uint32_t x = ring + st * Cfg::kStage, ts = tmem + bf * 128u, acc = tmem + Cfg::kAcc;
         mma_weighted<P, 64>(on, acc, ts + 64u, x, i > 0);                                               // dK += ds Q, dQ += ds K
         if (!kind) mma_weighted<P, 64>(on, acc + (uint32_t)P, ts, x + Cfg::kStream / 2, i > 0);         // dV += softmax dOUT
+        if (BOTH && i == tiles - 1) {                      // dQ = ds K, over the item's keys
+          mma_transposed<P>(on, tmem + Cfg::kAccQ, staged, sheld + (p.held == 2 ? live & 1u : 0u) * Cfg::kHeld);
+          commit_if(on, q_free);
+        }
         commit_if(on, empty + 8 * st);
         commit_if(on, buf_free + 8 * bf);
         if (i == tiles - 1) {
@@ -874,29 +899,30 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     Item prev;
     float below = 0.f, above = 0.f;                    // sums outside the varying part of the bias
     // An item's results: dK (group 0) and dV (group 1) of a key, or dQ of a query, 32 features in turn.
-    auto store = [&](const Item& it, uint32_t acc, bool zero) {
+    auto store = [&](const Item& it, bool queries, uint32_t acc, bool zero) {
       const int r = it.t * 128 + rt;
-      const Proj& o = it.kind ? p.dq : g ? p.dv : p.dk;
+      const Proj& o = queries ? p.dq : g ? p.dv : p.dk;
       sb_half* out = reinterpret_cast<sb_half*>(o.p) + (long long)it.h * o.sH + (long long)it.b * o.sB + (long long)r * o.sR;
-      const float f = it.kind || !g ? p.scale : 1.f;
+      const float f = queries || !g ? p.scale : 1.f;
 #pragma unroll 1
-      for (int c = it.kind ? g : 0; c < P / 32; c += it.kind ? 2 : 1) {
+      for (int c = queries ? g : 0; c < P / 32; c += queries ? 2 : 1) {
         uint32_t v[32];
         if (!zero) {
-          tmem_ld32_nowait(acc + lanes + (it.kind || !g ? 0u : (uint32_t)P) + c * 32, v);
+          tmem_ld32_nowait(acc + lanes + (queries || !g ? 0u : (uint32_t)P) + c * 32, v);
           attn::tmem_ld_wait32(v);
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = 0u;
         }
-        if (r < (it.kind ? p.c.J : p.c.K) && c * 32 < p.c.P) store_features(out + c * 32 * o.sP, o.sP, v, f, min(32, p.c.P - c * 32));
+        if (r < (queries ? p.c.J : p.c.K) && c * 32 < p.c.P) store_features(out + c * 32 * o.sP, o.sP, v, f, min(32, p.c.P - c * 32));
       }
     };
     auto finish = [&](const Item& it, uint32_t s) {
       ok = __all_sync(0xffffffffu, mbar_wait(acc_full, s & 1u, 59));
       if (!ok) return;
       tc_fence_after();
-      store(it, tmem + Cfg::kAcc, false);
+      store(it, it.kind != 0, tmem + Cfg::kAcc, false);
+      if (BOTH) store(it, true, tmem + Cfg::kAccQ, false);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(acc_empty);
@@ -944,8 +970,9 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     Item w;
     while (ok && take(&w, &ok)) {
       if (w.tiles == 0) {
-        store(w, 0u, true);
-        if (w.kind) flush(w);
+        store(w, w.kind != 0, 0u, true);
+        if (BOTH) store(w, true, 0u, true);
+        if (BOTH || w.kind) flush(w);
         continue;
       }
       const int r = w.t * 128 + rt;                    // query or key of this thread
@@ -994,7 +1021,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
           ok = __all_sync(0xffffffffu, (w.kind || mbar_wait(full + 8 * st, st_phase, 60)) && mbar_wait(s_full + 8 * bf, bf_phase, 60));
           if (!ok) break;
           tc_fence_after();
-          if (w.kind) {
+          if (!BOTH && w.kind) {
             const bool mask = tight < 64;
             if (near || mask || weighted) {
               float up = 0.f, down = 0.f;              // diagonals `lane` and `lane - 32` of a block
@@ -1019,11 +1046,39 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
             }
           } else {
             const float* L = reinterpret_cast<const float*>(gen + (ring - sheld) + st * Cfg::kStage + Cfg::kStream);
-            auto none = [](int, float) {};
-            auto after = [](int) {};
-            if (tight > 0) turn_tile<true, true, true>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
-            else if (near) turn_tile<true, true, false>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
-            else turn_tile<true, false, false>(ts, bp, bp[0], L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
+            if (BOTH) {
+              // the diagonals of a block run the other way: lane l gets those of key - query = l and l - 32
+              float up = 0.f, down = 0.f;
+              auto block = [&](int c) {
+                add(lo + 63 - 32 * c + lane, up);
+                add(lo + 31 - 32 * c + lane, down);
+                up = down = 0.f;
+              };
+              auto sum = [&](int e, float ds) {
+                const float v = __shfl_sync(0xffffffffu, ds, e + lane);
+                if (lane + e < 32) up += v;
+                else down += v;
+              };
+              const float* W = L + 128;
+              int half = 0;
+              auto weigh = [&](int e, float ds) { sum(e, ds * W[half + e]); };
+              auto next = [&](int c) { block(c); half = 32; };
+              const bool some = __any_sync(0xffffffffu, W[lane] != 1.f || W[lane + 32] != 1.f);
+              if (live > 0) {                            // the last item's product is done with its score gradients
+                ok = __all_sync(0xffffffffu, mbar_wait(q_free, (live - 1u) & 1u, 62));
+                if (!ok) break;
+              }
+              uint8_t* row = gen + (staged - sheld) + i * 16384 + rt * 128;
+              if (tight > 0 || some) turn_tile<true, true, true>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, weigh, next, row, rt & 7);
+              else turn_tile<true, true, false>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, sum, block, row, rt & 7);
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            } else {
+              auto none = [](int, float) {};
+              auto after = [](int) {};
+              if (tight > 0) turn_tile<true, true, true>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
+              else if (near) turn_tile<true, true, false>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
+              else turn_tile<true, false, false>(ts, bp, bp[0], L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
+            }
           }
           attn::tmem_st_wait();
           tc_fence_before();
@@ -1049,7 +1104,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         finish(prev, live - 1u);
         if (!ok) break;
       }
-      if (w.kind) flush(w);
+      if (BOTH || w.kind) flush(w);
       prev = w;
       have = true;
       ++live;

@@ -441,7 +441,7 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
   __syncthreads();
   if (threadIdx.x < 64) {
     const int j = j0 + threadIdx.x;
-    float lse = INFINITY, weight = 0.f;
+    float lse = INFINITY, weight = 1.f;
     if (j < a.J) {
       lse = a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] * 1.4426950408889634f;
       if (lse == -INFINITY) lse = INFINITY;
@@ -450,7 +450,7 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
       if (a.causal) n = max(0, min(n, pos + 1));
       // a row's score gradients sum to zero, so a row whose keys all share a bucket adds nothing to the table: its sum would
       // only be what D, from the rounded output, is off by
-      if (n > 0 && bucket_of(a, starts, -pos) != bucket_of(a, starts, n - 1 - pos)) weight = 1.f;
+      if (n <= 0 || bucket_of(a, starts, -pos) == bucket_of(a, starts, n - 1 - pos)) weight = 0.f;
     }
     float* r = records + (((long long)b * a.H + h) * blocks + block) * 192 + threadIdx.x;
     r[0] = lse;
