@@ -154,6 +154,39 @@ __device__ __forceinline__ void store_features(sb_half* ptr, long long sP, const
   }
 }
 
+// 32 accumulator columns of a warp's 32 rows -> alpha * value, 16-bit: the first `features` of the first `rows` rows, at
+// ptr[row * sR + feature * sP], by way of 2 KB of shared memory.  Four lanes write 64 bytes of a row; a thread writing its own row
+// meets 32 lines with each instruction, which for short sequences took as long as all the rest (backward at B=96, L=128: 83 -> 77 us);
+// where an item has many tiles the registers that this takes cost more (B=8, L=512: 80 -> 83 us).
+constexpr int kStoreBytes = 2048;
+__device__ __forceinline__ void store_rows(uint8_t* mem, sb_half* ptr, long long sR, long long sP, const uint32_t* r, float alpha, int features,
+                                           int rows, int lane) {
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {                          // 16-byte piece v of row `lane` at v ^ (lane / 2 & 3)
+    uint4 o;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = flash::pack2(__uint_as_float(r[v * 8 + 2 * e]) * alpha, __uint_as_float(r[v * 8 + 2 * e + 1]) * alpha);
+    *reinterpret_cast<uint4*>(mem + lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4)) = o;
+  }
+  __syncwarp();
+  if (sP == 1 && ((reinterpret_cast<uintptr_t>(ptr) | (uintptr_t)(2 * sR)) & 15u) == 0 && (features & 7) == 0) {
+    const int piece = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = i * 8 + (lane >> 2);
+      if (row < rows && piece * 8 < features)
+        *reinterpret_cast<uint4*>(ptr + row * sR + piece * 8) = *reinterpret_cast<const uint4*>(mem + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
+    }
+  } else if (lane < rows) {
+    const sb_half* row = reinterpret_cast<const sb_half*>(mem + lane * 64);
+    sb_half* out = ptr + lane * sR;
+#pragma unroll 1
+    for (int f = 0; f < features; ++f, out += sP) *out = row[(((f >> 3) ^ ((lane >> 1) & 3)) << 3) + (f & 7)];
+  }
+  __syncwarp();
+}
+
 // ---- work items ------------------------------------------------------------------------------------------------
 // Items come from a counter in memory, so that long ones do not hold up others (which item runs where changes nothing in its
 // results).  The producer warp works out an item's sizes, once, and hands them to the other warps through kSlots places in shared
@@ -631,7 +664,7 @@ struct BwdCfg {
   static constexpr int kBuf = P == 64 && !BOTH ? 3 : 2;
   static constexpr uint32_t kAcc = P == 64 ? 384 : 256, kAccQ = 256;
   static constexpr int smem(int stages, int held, int sets, int pitch, int reach) {
-    return held * kHeld + stages * kStage + kStaged + 2 * pitch * 4 + sets * 8 * ((2 * reach + 4) & ~3) * 4 + 1024 + 400 + 48 * kSlots;
+    return held * kHeld + stages * kStage + kStaged + (BOTH ? 8 * kStoreBytes : 0) + 2 * pitch * 4 + sets * 8 * ((2 * reach + 4) & ~3) * 4 + 1024 + 400 + 48 * kSlots;
   }
 };
 
@@ -708,7 +741,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t sheld = (raw + 1023u) & ~1023u, ring = sheld + p.held * Cfg::kHeld;
-  const uint32_t staged = ring + p.stages * Cfg::kStage, sbias = staged + Cfg::kStaged;
+  const uint32_t staged = ring + p.stages * Cfg::kStage, sstore = staged + Cfg::kStaged, sbias = sstore + (BOTH ? 8 * kStoreBytes : 0);
   const int width = (2 * p.c.reach + 4) & ~3;        // floats of a warp's row of sums
   const uint32_t ssums = sbias + 2u * p.c.pitch * 4u, bars = ssums + p.sets * 8u * width * 4u;
   const uint32_t item_full = bars, item_empty = bars + 32, h_full = bars + 64, h_empty = bars + 80, b_full = bars + 96, b_empty = bars + 112;
@@ -914,7 +947,11 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = 0u;
         }
-        if (r < (queries ? p.c.J : p.c.K) && c * 32 < p.c.P) store_features(out + c * 32 * o.sP, o.sP, v, f, min(32, p.c.P - c * 32));
+        const int rows = queries ? p.c.J : p.c.K;
+        if (BOTH && c * 32 < p.c.P)
+          store_rows(gen + (sstore - sheld) + (warp - 3) * kStoreBytes, out + c * 32 * o.sP - lane * o.sR, o.sR, o.sP, v, f, min(32, p.c.P - c * 32),
+                     rows - r + lane, lane);
+        if (!BOTH && r < rows && c * 32 < p.c.P) store_features(out + c * 32 * o.sP, o.sP, v, f, min(32, p.c.P - c * 32));
       }
     };
     auto finish = [&](const Item& it, uint32_t s) {
