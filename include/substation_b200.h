@@ -353,7 +353,7 @@ int sb_backward_query_key_norm_rotation(void* stream, void* scratch, size_t scra
  * their positions; starts[i] is the smallest distance in bucket i (host memory, starts[0] = 0, not decreasing; of several
  * buckets that start together only the last is met).  With `bidirectional`, keys before the query and at its place use
  * buckets 0 .. n-1 and keys behind it n .. 2n-1; without, keys behind it count as distance 0.  table: [2n or n, H].  At most
- * 256 buckets a direction, and the last one starts at a distance of at most 832.  An entry of -inf, or one at or below
+ * 512 buckets a direction, and the last one starts at a distance of at most 832.  An entry of -inf, or one at or below
  * -2^126 (which only bfloat16 has), hides the keys of its bucket. */
 typedef struct sb_relative_bias {
   const sb_tensor* table;

@@ -111,7 +111,7 @@ int launch_qk_norm_bwd(cudaStream_t s, void* scratch, Proj dq_out, Proj dk_out, 
 struct RelBias { const void* table; long long sN, sH; int n, bidirectional; const int32_t* starts; };
 struct RelSpan { float scale; int causal; const int* lengths; const int* first; };
 struct RelRows { float* p; long long sH, sB, sJ; };   // float32 [H,B,J]
-constexpr int kRelMaxBuckets = 256;                   // of one direction
+constexpr int kRelMaxBuckets = 512;                   // of one direction
 constexpr int kRelMaxReach = 832;                     // first distance of the last bucket
 constexpr int kRelMaxHead = 128;
 // Rows of biases over relative positions in units of log2, one per head (expand_bias_kernel); first distance of the last bucket.

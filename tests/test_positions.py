@@ -155,7 +155,7 @@ def _attention_call(backward=False, **kw):
     (dict(table=_t([4, 4])), 1, '[buckets, heads]'),
     (dict(both=0), 1, '[buckets, heads]'),
     (dict(n=0), 1, 'at least one'),
-    (dict(starts=[0] * 257, table=_t([514, 4])), 3, 'at most 256'),
+    (dict(starts=[0] * 513, table=_t([1026, 4])), 3, 'at most 512'),
     (dict(starts=[1, 2, 3, 4]), 1, 'distance 0'),
     (dict(starts=[0, 3, 2, 4]), 1, 'decrease'),
     (dict(starts=[0, 1, 2, 833]), 3, 'at most 832'),

@@ -197,6 +197,10 @@ ATTENTION_CASES = [
     (80, 4, 2, 2, 3, 333, 'PHBJ', 32, 128, True, False, None, [100, 330]),
     (24, 2, 2, 2, 4, 70, 'BJHP', 32, 128, False, True, [70, 9], [66, 5]),
     (64, 24, 1, 2, 1, 700, 'BJHP', 64, 512, False, True, [700, 699], [699, 698]),
+    # as many buckets as there may be, up to the last distance
+    (64, 2, 2, 1, 900, 900, 'BJHP', 512, 832, False, True, None, None),
+    (128, 4, 4, 1, 2, 1700, 'BJHP', 1024, 832, True, False, None, [850]),
+    (128, 2, 2, 1, 150, 1000, 'BJHP', 512, 832, True, False, None, [850]),
 ]
 
 
