@@ -375,7 +375,8 @@ typedef struct sb_attention_span {
  * q, out: [P,H,B,J]; k, v: [P,G,B,K], H a multiple of G (head h reads h / (H/G)); P at most 128; lse: float32 [H,B,J] or
  * NULL.  A query that sees no key gives out = 0 and lse = -inf.  Scores are not stored anywhere; exponentials are rounded to 16
  * bits where they meet v, sums are fp32.  Few queries against many keys are split along the keys and joined by a second kernel.
- * scratch: sb_relative_attention_scratch_bytes() for the same operands (may be 0), 16-byte aligned, as above. */
+ * out overlaps none of the inputs.  scratch: sb_relative_attention_scratch_bytes() for the same operands (may be 0), 16-byte
+ * aligned, as above. */
 int sb_relative_attention(void* stream, void* scratch, size_t scratch_bytes, const sb_tensor* q, const sb_tensor* k,
                           const sb_tensor* v, const sb_relative_bias* bias, const sb_tensor* out, const sb_tensor* lse,
                           const sb_attention_span* span);
@@ -385,8 +386,8 @@ int sb_relative_attention_scratch_bytes(const sb_tensor* q, const sb_tensor* k, 
  *   D = sum_p dout out,  ds = softmax * (sum_p dout v - D),  dv = sum_{j} softmax dout,  dk = scale sum_j ds q,
  *   dq = scale sum_k ds k,  dtable[n,h] = sum of ds over the batch's pairs in bucket n.
  * dk and dv of shared heads are sums over the query heads, and 0 behind a sample's length; every element of the five outputs
- * is written.  Sums run in a fixed order: the same call gives the same bits.  No counterpart in the reference, which has
- * neither positions nor padding. */
+ * is written, and they overlap none of the inputs.  Sums run in a fixed order: the same call gives the same bits.  No
+ * counterpart in the reference, which has neither positions nor padding. */
 int sb_backward_relative_attention(void* stream, void* scratch, size_t scratch_bytes, const sb_tensor* dout,
                                    const sb_tensor* q, const sb_tensor* k, const sb_tensor* v,
                                    const sb_relative_bias* bias, const sb_tensor* out, const sb_tensor* lse,

@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -320,6 +321,7 @@ int relative_operands(const sb_tensor* q, const sb_tensor* k, const sb_tensor* v
   for (const Proj* x : {pq, pk})
     if (x->P < 1 || x->H < 1 || x->B < 1 || x->R < 1) return fail(SB_ERR_ARG, "relative attention: every extent must be positive");
   if (pq->H % pk->H) return fail(SB_ERR_ARG, "relative attention: the query heads are not a multiple of the key heads");
+  if (pq->H > 65535) return fail(SB_ERR_UNSUPPORTED, "relative attention: more than 65535 heads");
   if (pq->P > kRelMaxHead)
     return fail(SB_ERR_UNSUPPORTED, "relative attention: heads of " + std::to_string(pq->P) + " features, at most " + std::to_string(kRelMaxHead));
   const long long units = (long long)pq->H * pq->B;
@@ -362,6 +364,14 @@ int to_lse(const sb_tensor* t, const sb_tensor* q, RelRows* o) {
   return SB_OK;
 }
 
+// Outputs are written while other tiles of the inputs are still to be read.
+int apart(std::initializer_list<const void*> outputs, std::initializer_list<const void*> inputs) {
+  for (const void* o : outputs)
+    for (const void* i : inputs)
+      if (o == i) return fail(SB_ERR_ARG, "relative attention: an output lies in an input's place");
+  return SB_OK;
+}
+
 int check_scratch(const void* scratch, size_t have, size_t need) {
   if (need == 0) return SB_OK;
   if (!scratch || have < need) return fail(SB_ERR_ARG, "relative attention: scratch is missing or too small");
@@ -390,6 +400,7 @@ extern "C" int sb_relative_attention(void* stream, void* scratch, size_t scratch
   RelRows rows;
   SB_TRY(relative_operands(q, k, v, bias, &pq, &pk, &pv, &rb));
   SB_TRY(to_projection_out(out, q, "relative attention.out", &po));
+  SB_TRY(apart({po.p}, {pq.p, pk.p, pv.p, rb.table}));
   SB_TRY(to_lse(lse, q, &rows));
   if (lse) SB_TRY(distinct(lse, "relative attention.lse"));
   SB_TRY(to_span(span, &sp));
@@ -428,6 +439,7 @@ extern "C" int sb_backward_relative_attention(void* stream, void* scratch, size_
   SB_TRY(to_projection_out(dk, k, "relative attention.dk", &ok));
   SB_TRY(to_projection_out(dv, v, "relative attention.dv", &ov));
   SB_TRY(check_tensor(dtable, 2, "relative attention.dtable"));
+  SB_TRY(apart({oq.p, ok.p, ov.p, dtable->ptr}, {pg.p, pq.p, pk.p, pv.p, po.p, rb.table, rows.p}));
   SB_TRY(same_shape(bias->table, dtable, "relative attention.dtable"));
   SB_TRY(distinct(dtable, "relative attention.dtable"));
   SB_TRY(to_span(span, &sp));

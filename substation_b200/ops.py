@@ -424,6 +424,8 @@ class RelativeBuckets:
 
     def __init__(self, starts, bidirectional=True):
         self.starts = tuple(int(s) for s in starts)
+        if any(not 0 <= s < 1 << 31 for s in self.starts):
+            raise ValueError('distances are from 0 to 2^31 - 1')
         self.bidirectional = bool(bidirectional)
         self._array = (ctypes.c_int32 * len(self.starts))(*self.starts)
         self._at = ctypes.addressof(self._array)

@@ -41,6 +41,9 @@ def test_bucket_refusals():
         with pytest.raises(ValueError):
             ops.relative_buckets(*args)
     assert ops.relative_buckets(32, 128) is ops.relative_buckets(32, 128)
+    for starts in ([0, -1], [0, 1 << 31]):
+        with pytest.raises(ValueError):
+            ops.RelativeBuckets(starts)
 
 
 # ---- refusals --------------------------------------------------------------------------------------------------------
@@ -97,6 +100,12 @@ def test_norm_refusals(kw, status, fragment):
     assert st == status and fragment in text, (st, text)
 
 
+def test_attention_output_in_an_inputs_place():
+    for name in ('q', 'k', 'v'):
+        st, text = _attention_call(**{name: _t([64, 4, 2, 8] if name == 'q' else [64, 2, 2, 12], ptr=0x90000)})
+        assert st == 1 and 'place' in text
+
+
 def test_norm_backward_refusals():
     lib = _lib.load()
     r = _lib.SbRotation()
@@ -117,8 +126,9 @@ def test_norm_backward_refusals():
 
 def _attention_call(backward=False, **kw):
     a = dict(q=_t([64, 4, 2, 8]), k=_t([64, 2, 2, 12]), v=_t([64, 2, 2, 12]), table=_t([8, 4]), starts=[0, 1, 2, 4], n=None, both=1,
-             out=_t([64, 4, 2, 8], ptr=0x90000), lse=_t([4, 2, 8]), scale=1.0, lengths=None, first=None, dtable=_t([8, 4]),
-             dout=_t([64, 4, 2, 8]), dk=_t([64, 2, 2, 12]), scratch=0x1000, room=1 << 40, span=True)
+             out=_t([64, 4, 2, 8], ptr=0x90000), lse=_t([4, 2, 8]), scale=1.0, lengths=None, first=None, dtable=_t([8, 4], ptr=0xa0000),
+             dout=_t([64, 4, 2, 8]), dq=_t([64, 4, 2, 8], ptr=0xb0000), dk=_t([64, 2, 2, 12], ptr=0xc0000),
+             dv=_t([64, 2, 2, 12], ptr=0xd0000), scratch=0x1000, room=1 << 40, span=True)
     a.update(kw)
     bias = _lib.SbRelativeBias()
     starts = (ctypes.c_int32 * max(1, len(a['starts'])))(*a['starts'])
@@ -132,8 +142,8 @@ def _attention_call(backward=False, **kw):
     sp = ctypes.byref(span) if a['span'] else None
     if backward:
         st = lib.sb_backward_relative_attention(None, a['scratch'], a['room'], opt(a['dout']), opt(a['q']), opt(a['k']), opt(a['v']),
-                                                ctypes.byref(bias), opt(a['out']), opt(a['lse']), opt(a['q']), opt(a['dk']),
-                                                opt(a['v']), opt(a['dtable']), sp)
+                                                ctypes.byref(bias), opt(a['out']), opt(a['lse']), opt(a['dq']), opt(a['dk']),
+                                                opt(a['dv']), opt(a['dtable']), sp)
     else:
         st = lib.sb_relative_attention(None, a['scratch'], a['room'], opt(a['q']), opt(a['k']), opt(a['v']), ctypes.byref(bias),
                                        opt(a['out']), opt(a['lse']), sp)
@@ -161,6 +171,7 @@ def _attention_call(backward=False, **kw):
     (dict(starts=[0, 1, 2, 833]), 3, 'at most 832'),
     (dict(out=_t([64, 4, 2, 9])), 1, 'extent mismatch'),
     (dict(lse=_t([4, 2, 9])), 1, 'extent mismatch'),
+    (dict(q=_t([64, 65536, 2, 8]), out=_t([64, 65536, 2, 8], ptr=0x90000), dout=_t([64, 65536, 2, 8]), table=_t([8, 65536])), 3, '65535'),
     (dict(scale=math.nan), 1, 'finite'),
     (dict(scale=-1.0), 1, 'negative'),
     (dict(lengths=0x1002), 5, 'int32'),
@@ -174,9 +185,11 @@ def test_attention_refusals(backward, kw, status, fragment):
 
 @pytest.mark.parametrize('kw,status,fragment', [
     (dict(lse=None), 1, 'lse'),
-    (dict(dtable=_t([8, 5])), 1, 'extent mismatch'),
-    (dict(dtable=_t([8, 4], [0, 1])), 1, 'zero stride'),
-    (dict(dk=_t([64, 2, 2, 12], [1, 64, 0, 128])), 1, 'zero stride'),
+    (dict(dtable=_t([8, 5], ptr=0xa0000)), 1, 'extent mismatch'),
+    (dict(dq=_t([64, 4, 2, 8])), 1, 'place'),
+    (dict(dv=_t([64, 2, 2, 12], ptr=0x90000)), 1, 'place'),
+    (dict(dtable=_t([8, 4], [0, 1], ptr=0xa0000)), 1, 'zero stride'),
+    (dict(dk=_t([64, 2, 2, 12], [1, 64, 0, 128], ptr=0xc0000)), 1, 'zero stride'),
     (dict(dout=_t([64, 4, 2, 9])), 1, 'extent mismatch'),
     (dict(scratch=None), 1, 'scratch'),
     (dict(room=16), 1, 'scratch'),
