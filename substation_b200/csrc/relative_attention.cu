@@ -271,8 +271,9 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int x = e >> 1, k = k0 + t * 8 + (lane & 3) * 2 + (e & 1), rel = k - pos[x];
-          const float bias = rel <= -p.reach ? lo[x] : rel >= p.reach ? hi[x] : bias_of(map[rel + p.reach], head[x]);
+          // (a key behind this CTA's last may be within reach of the query when none of the CTA's is, and then there is no map)
           const bool seen = k < k_to && !(a.causal && rel > 0);
+          const float bias = rel <= -p.reach ? lo[x] : rel >= p.reach ? hi[x] : seen ? bias_of(map[rel + p.reach], head[x]) : 0.f;
           s[t][e] = seen ? fmaf(s[t][e], c2, bias) : -INFINITY;
           mx[x] = fmaxf(mx[x], s[t][e]);
         }

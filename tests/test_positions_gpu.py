@@ -432,6 +432,25 @@ def test_calls_on_two_streams_and_captured_ones():
         assert all(torch.equal(a[n], b[n]) for n in a)
 
 
+@pytest.mark.parametrize('P', [64, 128])
+@pytest.mark.parametrize('behind', [0, 5, 15])
+def test_few_queries_far_behind_the_last_key(P, behind):
+    """The last key is just beyond the buckets' reach, the places behind it, up to a whole piece, would be within."""
+    ops = _ops()
+    gen = torch.Generator(device=DEV).manual_seed(behind)
+    B, H, G, J, K = 3, 4, 2, 3, 300
+    q, k, v = (_make((P, h, B, n), 'BJHP', torch.float16, gen) for h, n in ((H, J), (G, K), (G, K)))
+    b = ops.relative_buckets(32, 128, True)
+    table = torch.randn(32, H, generator=gen, device=DEV).half()
+    lengths = torch.tensor([1, 257, 289], dtype=torch.int32, device=DEV)
+    how = dict(buckets=b, scale=P ** -0.5, lengths=lengths, first=lengths - 1 + b.starts[-1] + behind)
+    out, lse = _nan((P, H, B, J), 'BJHP', torch.float16), torch.empty(H, B, J, device=DEV)
+    ops.relative_attention(q, k, v, table, out, lse, **how)
+    want, bound = ref.attention(q, k, v, table, half=HALF[torch.float16], **how)
+    _within(out, want['out'], bound['out'], 'out')
+    assert ((lse - want['lse']).abs() <= 1e-5 * (1 + want['lse'].abs())).all()
+
+
 def test_few_queries_agree_with_many():
     """The last queries of a causal sequence, one call for all or a call for the last ones against the cache."""
     ops = _ops()
