@@ -438,10 +438,11 @@ int launch_strided(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) 
   a.tiles = (a.tokens + 32 * TOKENS - 1) / (32 * TOKENS);
   // up to eight heads a block, which share the angles; fewer where SMs would be without a block
   for (a.chunk = 8; a.chunk > 1 && (long long)a.tiles * ((heads + a.chunk - 1) / a.chunk) < sms; a.chunk /= 2) {}
+  if (BWD) a.chunk = std::max({a.chunk, (a.x[0].H + kMaxPartials - 1) / kMaxPartials, (a.x[1].H + kMaxPartials - 1) / kMaxPartials});
   for (int w = 0; w < 2; ++w) {
     const int chunks = (a.x[w].H + a.chunk - 1) / a.chunk;
     // (every chunk has the same number of blocks; the backward pass bounds their number by its rows of sums)
-    const int each = BWD && chunks > 0 ? std::max(1, std::min(a.tiles, kMaxPartials / chunks)) : a.tiles;
+    const int each = BWD && chunks > 0 ? std::min(a.tiles, kMaxPartials / chunks) : a.tiles;
     a.blocks[w] = rows[w] = chunks * each;
   }
   bool narrow = true;

@@ -58,6 +58,7 @@ NORM_CASES = [
     (16, 5, 2, 4, 9, 'BJHP', 'JBHP', 16, 'halves'),
     (256, 2, 1, 2, 33, 'BJHP', 'BHJP', 256, 'halves'),
     (80, 12, 4, 2, 40, 'BJHP', 'BJHP', 80, 'halves'),
+    (2, 9600, 20000, 1, 2, 'BJHP', 'BJHP', 2, 'halves'),    # more heads than rows of partial sums for eight of them each
     (96, 4, 4, 2, 21, 'BJHP', 'BJHP', 32, 'adjacent'),
     (64, 12, 12, 3, 24, 'PHBJ', 'PHBJ', 32, 'adjacent'),
     (64, 12, 4, 3, 25, 'PHBJ', 'BJHP', 64, 'halves'),
