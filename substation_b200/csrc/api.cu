@@ -236,7 +236,8 @@ int norm_operands(const sb_tensor* q, const sb_tensor* k, const sb_tensor* q_gai
   if (pq->P < 1 || pq->H < 1) return fail(SB_ERR_ARG, "norm.q: no features or no heads");
   if (pq->P > kNormMaxHead)
     return fail(SB_ERR_UNSUPPORTED, "norm: heads of " + std::to_string(pq->P) + " features, at most " + std::to_string(kNormMaxHead));
-  if ((long long)pq->B * pq->R > 0x7fffffffLL) return fail(SB_ERR_UNSUPPORTED, "norm: more than 2^31-1 tokens");
+  // (the kernels count tokens in whole tiles and grids, past the last one)
+  if ((long long)pq->B * pq->R > 1LL << 30) return fail(SB_ERR_UNSUPPORTED, "norm: more than 2^30 tokens");
   if ((long long)pq->H + pk->H > 65535) return fail(SB_ERR_UNSUPPORTED, "norm: more than 65535 heads");
   SB_TRY(check_tensor(positions, 2, "norm.positions"));
   if (positions->size[0] != pq->B || positions->size[1] != pq->R)
@@ -324,8 +325,9 @@ int relative_operands(const sb_tensor* q, const sb_tensor* k, const sb_tensor* v
   if (pq->H > 65535) return fail(SB_ERR_UNSUPPORTED, "relative attention: more than 65535 heads");
   if (pq->P > kRelMaxHead)
     return fail(SB_ERR_UNSUPPORTED, "relative attention: heads of " + std::to_string(pq->P) + " features, at most " + std::to_string(kRelMaxHead));
+  // (first is held to 2^29 in size, so that its sums with places in a sequence and tiles behind its end stay within 32 bits)
   const long long units = (long long)pq->H * pq->B;
-  if (units * ((pq->R + 63) / 64) > 0x1fffffffLL || units * ((pk->R + 63) / 64) > 0x1fffffffLL || pq->R > 0x3fffffff || pk->R > 0x3fffffff)
+  if (units * ((pq->R + 63) / 64) > 0x1fffffffLL || units * ((pk->R + 63) / 64) > 0x1fffffffLL || pq->R > 1 << 28 || pk->R > 1 << 28)
     return fail(SB_ERR_UNSUPPORTED, "relative attention: too many heads, samples and rows");
   if (!bias || !bias->table || !bias->starts) return fail(SB_ERR_ARG, "relative attention: null bias, table or starts");
   const int n = bias->n;

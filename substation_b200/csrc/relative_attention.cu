@@ -48,7 +48,7 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
 }
 
 // rows[h][i] = log2(e) * bias of head h at relative position i - kRelPad - reach, which stays at its end values beyond the reach.
-// Finite biases stay finite, so that a row of nothing but the lowest ones still has a maximum.
+// Biases of up to 2^127 in size stay finite, so that a row of nothing but float16's lowest still has a maximum.
 __global__ void __launch_bounds__(256)
 expand_bias_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, float* rows, int pitch, int reach, int* next) {
   grid_dependency_sync();

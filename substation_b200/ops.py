@@ -453,9 +453,8 @@ def relative_buckets(num_buckets=32, max_distance=128, bidirectional=True):
     if max_distance <= exact:
         raise ValueError(f'max_distance {max_distance} has to exceed the {exact} distances with a bucket each')
     steps, starts, d = n - exact, list(range(exact)), exact
-    for i in range(steps):
-        while d ** steps * exact ** i < max_distance ** i * exact ** steps:   # log(d/exact) / log(max/exact) < i / steps
-            d += 1
+    for i in range(steps):      # the first d with log(d/exact) / log(max/exact) >= i / steps
+        d = bisect.bisect_left(range(max_distance + 1), max_distance ** i * exact ** steps, lo=d, key=lambda e: e ** steps * exact ** i)
         starts.append(d)
     return RelativeBuckets(starts, bidirectional)
 

@@ -41,6 +41,7 @@ def test_bucket_refusals():
         with pytest.raises(ValueError):
             ops.relative_buckets(*args)
     assert ops.relative_buckets(32, 128) is ops.relative_buckets(32, 128)
+    assert ops.relative_buckets(32, 10 ** 9).bucket(-10 ** 8) == 15     # (far borders are searched, not counted to)
     for starts in ([0, -1], [0, 1 << 31]):
         with pytest.raises(ValueError):
             ops.RelativeBuckets(starts)
@@ -94,6 +95,7 @@ def _norm_call(**kw):
     (dict(rot=False), 1, 'null rotation'),
     (dict(q=_t([320, 4, 2, 8]), qo=_t([320, 4, 2, 8]), qg=_t([320]), k=None, kg=None, ko=None), 3, 'at most 256'),
     (dict(q=_t([64, 4, 65536, 65536], [0] * 4), k=None, kg=None, ko=None), 3, 'tokens'),
+    (dict(q=_t([64, 4, 32768, 32769], [0] * 4), k=None, kg=None, ko=None), 3, 'tokens'),
 ])
 def test_norm_refusals(kw, status, fragment):
     st, text = _norm_call(**kw)
@@ -172,6 +174,7 @@ def _attention_call(backward=False, **kw):
     (dict(out=_t([64, 4, 2, 9])), 1, 'extent mismatch'),
     (dict(lse=_t([4, 2, 9])), 1, 'extent mismatch'),
     (dict(q=_t([64, 65536, 2, 8]), out=_t([64, 65536, 2, 8], ptr=0x90000), dout=_t([64, 65536, 2, 8]), table=_t([8, 65536])), 3, '65535'),
+    (dict(k=_t([64, 2, 2, (1 << 28) + 1]), v=_t([64, 2, 2, (1 << 28) + 1])), 3, 'too many'),
     (dict(scale=math.nan), 1, 'finite'),
     (dict(scale=-1.0), 1, 'negative'),
     (dict(lengths=0x1002), 5, 'int32'),
