@@ -760,7 +760,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(h_full + 8 * i, 1);
-      mbar_init(h_empty + 8 * i, 1);
+      mbar_init(h_empty + 8 * i, 9);                   // the products, and the element warps, which read records
       mbar_init(b_full + 8 * i, 1);
       mbar_init(b_empty + 8 * i, 8);
       mbar_init(g_sync + 8 * i, 4);
@@ -1026,6 +1026,8 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         }
       }
       const bool weighted = __any_sync(0xffffffffu, weight != 1.f);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(h_empty + 8 * (p.held == 2 ? live & 1u : 0u));   // (a group without a tile may come here last)
       bool due = have;                                 // the previous item's results are still to be stored
       // At the first streamed tile of a run, all moving by 64 a tile: relative position of this thread's first column, lowest of
       // the warp's block (its highest is lo + 94), the thread's bound on visible columns and the block's tightest.
