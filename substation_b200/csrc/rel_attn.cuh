@@ -135,17 +135,23 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int valid, int lane) {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
 }
-// 32 accumulator columns -> alpha * value, 16-bit, the first n of them, at ptr[p * sP]
+// 32 accumulator columns -> alpha * value, 16-bit, the first n of them, at ptr[p * sP].  A thread writes its own row, whole sectors
+// at a time where the row allows it.
 __device__ __forceinline__ void store_features(sb_half* ptr, long long sP, const uint32_t* r, float alpha, int n) {
-  if (sP == 1 && (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0 && (n & 7) == 0) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(ptr);
+  if (sP == 1 && (at & 15u) == 0 && (n & 7) == 0) {
+    uint32_t o[16];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      uint4 o;
-      uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+    for (int e = 0; e < 16; ++e) o[e] = flash::pack2(__uint_as_float(r[2 * e]) * alpha, __uint_as_float(r[2 * e + 1]) * alpha);
+    if ((at & 31u) == 0 && n == 32) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = flash::pack2(__uint_as_float(r[v * 8 + 2 * e]) * alpha, __uint_as_float(r[v * 8 + 2 * e + 1]) * alpha);
-      if (v * 8 < n) reinterpret_cast<uint4*>(ptr)[v] = o;
+      for (int v = 0; v < 2; ++v)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(ptr + v * 16), "r"(o[8 * v]), "r"(o[8 * v + 1]), "r"(o[8 * v + 2]),
+                     "r"(o[8 * v + 3]), "r"(o[8 * v + 4]), "r"(o[8 * v + 5]), "r"(o[8 * v + 6]), "r"(o[8 * v + 7]) : "memory");
+    } else {
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        if (v * 8 < n) reinterpret_cast<uint4*>(ptr)[v] = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
     }
   } else {
 #pragma unroll
