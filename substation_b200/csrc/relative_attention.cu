@@ -49,15 +49,21 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
 
 // rows[h][i] = log2(e) * bias of head h at relative position i - kRelPad - reach, which stays at its end values beyond the reach.
 // Biases of up to 2^127 in size stay finite, so that a row of nothing but float16's lowest still has a maximum.
+// Block `part` of expand_blocks() for the head.
+struct Expand { float* rows; int pitch, reach; int* next; };   // next: the work queue of the kernel that follows
+__host__ __device__ constexpr int expand_blocks(int pitch) { return (pitch + 255) / 256; }
+__device__ __forceinline__ void expand_part(const AttnArgs& a, const int* starts, const Expand& x, int h, int part) {
+  if (h == 0 && part == 0 && threadIdx.x == 0) *x.next = 0;
+  const int i = part * 256 + threadIdx.x;
+  if (i >= x.pitch) return;
+  const int rel = max(-x.reach, min(x.reach, i - kRelPad - x.reach));
+  const float b = sb_h2f(a.table[bucket_of(a, starts, rel) * a.t_sN + h * a.t_sH]);
+  x.rows[(long long)h * x.pitch + i] = b <= kHidden ? -INFINITY : b * 1.4426950408889634f;
+}
 __global__ void __launch_bounds__(256)
-expand_bias_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, float* rows, int pitch, int reach, int* next) {
+expand_bias_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const __grid_constant__ Expand x) {
   grid_dependency_sync();
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *next = 0;   // the work queue of the kernel that follows
-  const int i = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
-  if (i >= pitch) return;
-  const int rel = max(-reach, min(reach, i - kRelPad - reach));
-  const float b = sb_h2f(a.table[bucket_of(a, st.s, rel) * a.t_sN + h * a.t_sH]);
-  rows[(long long)h * pitch + i] = b <= kHidden ? -INFINITY : b * 1.4426950408889634f;
+  expand_part(a, st.s, x, blockIdx.y, blockIdx.x);
 }
 
 // [P,H,B,R] of any strides -> [B][H][R][Pp], which tensor maps can address; 64 rows of one head and sample a block.
@@ -405,58 +411,74 @@ join_splits_kernel(const __grid_constant__ FewParams p) {
   if (lane == 0 && a.lse.p) a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] = sum > 0.f ? (mm + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 }
 
-// What the backward pass knows of 64 query rows (RelBackward in ops.h); four threads a row.  `vec`: both tensors have unit-stride
-// features in 16-byte pieces; else lanes run along rows.
+// What the backward pass knows of 64 query rows (RelBackward in ops.h), four threads a row, and in the blocks behind those the rows
+// of biases.  `vec`: both tensors have unit-stride features in 16-byte pieces; else lanes run along rows.  Everything is
+// asked for before anything is waited for: one trip to memory a block.
 __global__ void __launch_bounds__(256)
-row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, float* records, int vec) {
+row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const __grid_constant__ Expand x, float* records, int vec,
+                   int record_blocks) {
   __shared__ float part[4][64];
   __shared__ int starts[kRelMaxBuckets];
   grid_dependency_sync();
-  for (int i = threadIdx.x; i < a.n; i += 256) starts[i] = st.s[i];
+  if ((int)blockIdx.x >= record_blocks) {
+    const int i = blockIdx.x - record_blocks, parts = expand_blocks(x.pitch);
+    expand_part(a, st.s, x, i / parts, i % parts);
+    return;
+  }
   // blocks that run together share tokens, whose heads usually lie side by side
   const int blocks = (a.J + 63) / 64, h = blockIdx.x % a.H, block = blockIdx.x / a.H % blocks, b = blockIdx.x / a.H / blocks;
-  const int j0 = block * 64;
-  const int row = vec ? threadIdx.x >> 2 : threadIdx.x & 63, i = vec ? threadIdx.x & 3 : threadIdx.x >> 6;
-  float sum = 0.f;
-  if (j0 + row < a.J) {
-    const sb_half* g = row_of(a.g, h, b, j0 + row);
-    const sb_half* o = row_of(a.o, h, b, j0 + row);
-    if (vec) {
+  const int row = vec ? threadIdx.x >> 2 : threadIdx.x & 63, i = vec ? threadIdx.x & 3 : threadIdx.x >> 6, j = block * 64 + row;
+  const bool live = j < a.J;
+  const sb_half* g = row_of(a.g, h, b, live ? j : 0);
+  const sb_half* o = row_of(a.o, h, b, live ? j : 0);
+  uint4 gv[kMaxP / 32], ov[kMaxP / 32];
+  if (vec)
 #pragma unroll
-      for (int c = 0; c < kMaxP / 32; ++c) {
-        const int p = i * 8 + c * 32;
-        if (p < a.P) {
-          float x[8], y[8];
-          unpack8(*reinterpret_cast<const uint4*>(g + p), x);
-          unpack8(*reinterpret_cast<const uint4*>(o + p), y);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sum = fmaf(x[e], y[e], sum);
-        }
+    for (int c = 0; c < kMaxP / 32; ++c) {
+      const int p = i * 8 + c * 32;
+      gv[c] = ov[c] = make_uint4(0u, 0u, 0u, 0u);
+      if (p < a.P) {
+        gv[c] = *reinterpret_cast<const uint4*>(g + p);
+        ov[c] = *reinterpret_cast<const uint4*>(o + p);
       }
-    } else {
-#pragma unroll 4
-      for (int p = i; p < a.P; p += 4) sum = fmaf(sb_h2f(g[p * a.g.sP]), sb_h2f(o[p * a.o.sP]), sum);
     }
+  float lse = 0.f;
+  int n = 0, pos = 0;
+  if (i == 0) {
+    lse = a.lse.p[h * a.lse.sH + b * a.lse.sB + (live ? j : 0) * a.lse.sJ];
+    n = keys_of(a, b);
+    pos = first_of(a, b) + j;
   }
-  part[i][row] = sum;
+  for (int y = threadIdx.x; y < a.n; y += 256) starts[y] = st.s[y];
   __syncthreads();
-  if (threadIdx.x < 64) {
-    const int j = j0 + threadIdx.x;
-    float lse = INFINITY, weight = 1.f;
-    if (j < a.J) {
-      lse = a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] * 1.4426950408889634f;
-      if (lse == -INFINITY) lse = INFINITY;
-      const int pos = first_of(a, b) + j;
-      int n = keys_of(a, b);
-      if (a.causal) n = max(0, min(n, pos + 1));
-      // a row's score gradients sum to zero, so a row whose keys all share a bucket adds nothing to the table: its sum would
-      // only be what D, from the rounded output, is off by
-      if (n <= 0 || bucket_of(a, starts, -pos) == bucket_of(a, starts, n - 1 - pos)) weight = 0.f;
+  float sum = 0.f;
+  if (vec) {
+#pragma unroll
+    for (int c = 0; c < kMaxP / 32; ++c) {
+      float u[8], v[8];
+      unpack8(gv[c], u);
+      unpack8(ov[c], v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = fmaf(u[e], v[e], sum);
     }
-    float* r = records + (((long long)b * a.H + h) * blocks + block) * 192 + threadIdx.x;
-    r[0] = lse;
-    r[64] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
-    r[128] = weight;
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+  } else {
+#pragma unroll 4
+    for (int p = i; p < a.P; p += 4) sum = fmaf(sb_h2f(g[p * a.g.sP]), sb_h2f(o[p * a.o.sP]), sum);
+    part[i][row] = sum;
+    __syncthreads();
+    if (i == 0) sum = (part[0][row] + part[1][row]) + (part[2][row] + part[3][row]);
+  }
+  if (i == 0) {
+    if (a.causal) n = max(0, min(n, pos + 1));
+    // a row's score gradients sum to zero, so a row whose keys all share a bucket adds nothing to the table: its sum would
+    // only be what D, from the rounded output, is off by
+    const bool alike = n <= 0 || bucket_of(a, starts, -pos) == bucket_of(a, starts, n - 1 - pos);
+    float* r = records + (((long long)b * a.H + h) * blocks + block) * 192 + row;
+    r[0] = live && lse != -INFINITY ? lse * 1.4426950408889634f : INFINITY;
+    r[64] = live ? sum : 0.f;
+    r[128] = live && alike ? 0.f : 1.f;
   }
 }
 
@@ -535,12 +557,10 @@ int pack(cudaStream_t s, void* scratch, size_t at, Proj* x) {
   return SB_OK;
 }
 int direct_or_packed(cudaStream_t s, void* scratch, size_t at, Proj* x) { return rel_direct(*x) ? SB_OK : pack(s, scratch, at, x); }
-int expand_bias(cudaStream_t s, const AttnArgs& a, const Starts& st, void* scratch, const Plan& pl, RelTables* t) {
-  t->rows = reinterpret_cast<float*>(scratch); t->pitch = pl.pitch; t->reach = pl.reach;
-  SB_LAUNCH_OK(launch_k(expand_bias_kernel, dim3((pl.pitch + 255) / 256, a.H), 256, 0, s, a, st, reinterpret_cast<float*>(scratch), pl.pitch, pl.reach,
-                        reinterpret_cast<int*>(reinterpret_cast<char*>(scratch) + pl.next)));
-  return SB_OK;
+Expand expansion(void* scratch, const Plan& pl) {
+  return {reinterpret_cast<float*>(scratch), pl.pitch, pl.reach, reinterpret_cast<int*>(reinterpret_cast<char*>(scratch) + pl.next)};
 }
+RelTables tables_of(const Expand& x) { return {x.rows, x.pitch, x.reach}; }
 
 }  // namespace
 
@@ -610,12 +630,12 @@ int launch_rel_attn_fwd(cudaStream_t s, void* scratch, Proj q, Proj k, Proj v, c
     return q.P <= 64 ? launch_few<64>(s, p, st) : launch_few<128>(s, p, st);
   }
   const Plan pl = plan_of({&q, &k, &v}, q.H, bias);
-  RelTables t;
-  SB_TRY(expand_bias(s, a, st, scratch, pl, &t));
+  const Expand x = expansion(scratch, pl);
+  SB_LAUNCH_OK(launch_k(expand_bias_kernel, dim3(expand_blocks(x.pitch), a.H), 256, 0, s, a, st, x));
   SB_TRY(direct_or_packed(s, scratch, pl.at[0], &q));
   SB_TRY(direct_or_packed(s, scratch, pl.at[1], &k));
   SB_TRY(direct_or_packed(s, scratch, pl.at[2], &v));
-  return launch_rel_tiles_fwd(s, q, k, v, t, reinterpret_cast<int*>(reinterpret_cast<char*>(scratch) + pl.next), out, lse, span);
+  return launch_rel_tiles_fwd(s, q, k, v, tables_of(x), x.next, out, lse, span);
 }
 
 namespace {
@@ -643,21 +663,20 @@ int launch_rel_attn_bwd(cudaStream_t s, void* scratch, Proj dout, Proj q, Proj k
   a.g = dout;
   const BwdPlan pl = bwd_plan(dout, q, k, v, bias);
   char* base = reinterpret_cast<char*>(scratch);
-  RelTables t;
-  SB_TRY(expand_bias(s, a, st, scratch, pl.p, &t));
+  const Expand x = expansion(scratch, pl.p);
   auto pieces = [](const Proj& x) {
     return x.sP == 1 && x.P % 8 == 0 && !((x.sH | x.sB | x.sR) & 7) && !(reinterpret_cast<uintptr_t>(x.p) & 15u);
   };
   float* records = reinterpret_cast<float*>(base + pl.records);
-  int* next = reinterpret_cast<int*>(base + pl.p.next);
-  const long long blocks = (long long)a.H * a.B * ((a.J + 63) / 64);
-  SB_LAUNCH_OK(launch_k(row_records_kernel, (unsigned)blocks, 256, 0, s, a, st, records, pieces(dout) && pieces(out) ? 1 : 0));
+  const int blocks = a.H * a.B * ((a.J + 63) / 64);
+  SB_LAUNCH_OK(launch_k(row_records_kernel, (unsigned)(blocks + a.H * expand_blocks(x.pitch)), 256, 0, s, a, st, x, records,
+                        pieces(dout) && pieces(out) ? 1 : 0, blocks));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[0], &dout));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[1], &q));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[2], &k));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[3], &v));
   float* partial = reinterpret_cast<float*>(base + pl.partial);
-  SB_TRY(launch_rel_tiles_bwd(s, dout, q, k, v, t, RelBackward{records, partial, next}, dq, dk, dv, span));
+  SB_TRY(launch_rel_tiles_bwd(s, dout, q, k, v, tables_of(x), RelBackward{records, partial, x.next}, dq, dk, dv, span));
   SB_LAUNCH_OK(launch_k(table_finish_kernel, dim3(a.buckets, a.H), 256, 0, s, a, st, partial, pl.rows, pl.p.reach,
                         reinterpret_cast<sb_half*>(dtable), dt_sN, dt_sH));
   return SB_OK;
