@@ -411,22 +411,22 @@ join_splits_kernel(const __grid_constant__ FewParams p) {
   if (lane == 0 && a.lse.p) a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] = sum > 0.f ? (mm + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 }
 
-// What the backward pass knows of 64 query rows (RelBackward in ops.h), four threads a row, and in the blocks behind those the rows
+// What the backward pass knows of 64 query rows (RelBackward in ops.h), four threads a row, and in the blocks before those the rows
 // of biases.  `vec`: both tensors have unit-stride features in 16-byte pieces; else lanes run along rows.  Everything is
 // asked for before anything is waited for: one trip to memory a block.
 __global__ void __launch_bounds__(256)
 row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const __grid_constant__ Expand x, float* records, int vec,
-                   int record_blocks) {
+                   int expanding) {
   __shared__ float part[4][64];
-  __shared__ int starts[kRelMaxBuckets];
   grid_dependency_sync();
-  if ((int)blockIdx.x >= record_blocks) {
-    const int i = blockIdx.x - record_blocks, parts = expand_blocks(x.pitch);
-    expand_part(a, st.s, x, i / parts, i % parts);
+  const int it = (int)blockIdx.x - expanding;
+  if (it < 0) {
+    const int parts = expand_blocks(x.pitch);
+    expand_part(a, st.s, x, blockIdx.x / parts, blockIdx.x % parts);
     return;
   }
   // blocks that run together share tokens, whose heads usually lie side by side
-  const int blocks = (a.J + 63) / 64, h = blockIdx.x % a.H, block = blockIdx.x / a.H % blocks, b = blockIdx.x / a.H / blocks;
+  const int blocks = (a.J + 63) / 64, h = it % a.H, block = it / a.H % blocks, b = it / a.H / blocks;
   const int row = vec ? threadIdx.x >> 2 : threadIdx.x & 63, i = vec ? threadIdx.x & 3 : threadIdx.x >> 6, j = block * 64 + row;
   const bool live = j < a.J;
   const sb_half* g = row_of(a.g, h, b, live ? j : 0);
@@ -449,8 +449,6 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
     n = keys_of(a, b);
     pos = first_of(a, b) + j;
   }
-  for (int y = threadIdx.x; y < a.n; y += 256) starts[y] = st.s[y];
-  __syncthreads();
   float sum = 0.f;
   if (vec) {
 #pragma unroll
@@ -474,7 +472,10 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
     if (a.causal) n = max(0, min(n, pos + 1));
     // a row's score gradients sum to zero, so a row whose keys all share a bucket adds nothing to the table: its sum would
     // only be what D, from the rounded output, is off by
-    const bool alike = n <= 0 || bucket_of(a, starts, -pos) == bucket_of(a, starts, n - 1 - pos);
+    // (seldom; most rows have keys on both sides or, of the far ones, before and within the reach, and need no search)
+    const int lo = -pos, hi = n - 1 - pos, last = st.s[a.n - 1];
+    const bool sides = (a.bidirectional && lo <= 0 && hi > 0) || (last > 0 && lo <= -last && hi > -last);
+    const bool alike = n <= 0 || (!sides && bucket_of(a, st.s, lo) == bucket_of(a, st.s, hi));
     float* r = records + (((long long)b * a.H + h) * blocks + block) * 192 + row;
     r[0] = live && lse != -INFINITY ? lse * 1.4426950408889634f : INFINITY;
     r[64] = live ? sum : 0.f;
@@ -484,10 +485,10 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
 
 // dtable[n,h] = the head's sums over the relative positions of bucket n; one block each, in a fixed order: lanes along as many
 // positions as the bucket has, up to 32, and along rows of sums beside that.
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(512)
 table_finish_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const float* partial, int rows, int reach,
                     sb_half* out, long long sN, long long sH) {
-  __shared__ float part[8];
+  __shared__ float part[16];
   grid_dependency_sync();
   const int n = blockIdx.x, h = blockIdx.y, entries = 2 * reach + 1;
   const bool behind = n >= a.n;
@@ -504,12 +505,14 @@ table_finish_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   float s = 0.f;
   for (int c = lane % across; c < run; c += across)
 #pragma unroll 8
-    for (int r = r0; r < rows; r += 8 * each) s += base[(long long)r * entries + c];
+    for (int r = r0; r < rows; r += 16 * each) s += base[(long long)r * entries + c];
   s = group_sum<32>(s);
   if (lane == 0) part[threadIdx.x >> 5] = s;
   __syncthreads();
-  if (threadIdx.x == 0)
-    out[n * sN + h * sH] = sb_f2h(((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7])));
+  if (threadIdx.x < 32) {
+    s = group_sum<16>(part[threadIdx.x & 15]);
+    if (threadIdx.x == 0) out[n * sN + h * sH] = sb_f2h(s);
+  }
 }
 
 AttnArgs attn_args(const Proj& q, const Proj& k, const Proj& v, const RelBias& bias, const Proj& out, const RelRows& lse, const RelSpan& span,
@@ -668,16 +671,16 @@ int launch_rel_attn_bwd(cudaStream_t s, void* scratch, Proj dout, Proj q, Proj k
     return x.sP == 1 && x.P % 8 == 0 && !((x.sH | x.sB | x.sR) & 7) && !(reinterpret_cast<uintptr_t>(x.p) & 15u);
   };
   float* records = reinterpret_cast<float*>(base + pl.records);
-  const int blocks = a.H * a.B * ((a.J + 63) / 64);
-  SB_LAUNCH_OK(launch_k(row_records_kernel, (unsigned)(blocks + a.H * expand_blocks(x.pitch)), 256, 0, s, a, st, x, records,
-                        pieces(dout) && pieces(out) ? 1 : 0, blocks));
+  const int expanding = a.H * expand_blocks(x.pitch);
+  SB_LAUNCH_OK(launch_k(row_records_kernel, (unsigned)(expanding + a.H * a.B * ((a.J + 63) / 64)), 256, 0, s, a, st, x, records,
+                        pieces(dout) && pieces(out) ? 1 : 0, expanding));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[0], &dout));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[1], &q));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[2], &k));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[3], &v));
   float* partial = reinterpret_cast<float*>(base + pl.partial);
   SB_TRY(launch_rel_tiles_bwd(s, dout, q, k, v, tables_of(x), RelBackward{records, partial, x.next}, dq, dk, dv, span));
-  SB_LAUNCH_OK(launch_k(table_finish_kernel, dim3(a.buckets, a.H), 256, 0, s, a, st, partial, pl.rows, pl.p.reach,
+  SB_LAUNCH_OK(launch_k(table_finish_kernel, dim3(a.buckets, a.H), 512, 0, s, a, st, partial, pl.rows, pl.p.reach,
                         reinterpret_cast<sb_half*>(dtable), dt_sN, dt_sH));
   return SB_OK;
 }
