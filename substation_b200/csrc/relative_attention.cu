@@ -414,6 +414,7 @@ join_splits_kernel(const __grid_constant__ FewParams p) {
 // What the backward pass knows of 64 query rows (RelBackward in ops.h), four threads a row, and in the blocks before those the rows
 // of biases.  `vec`: both tensors have unit-stride features in 16-byte pieces; else lanes run along rows.  Everything is
 // asked for before anything is waited for: one trip to memory a block.
+template <int P>
 __global__ void __launch_bounds__(256)
 row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const __grid_constant__ Expand x, float* records, int vec,
                    int expanding) {
@@ -431,10 +432,10 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
   const bool live = j < a.J;
   const sb_half* g = row_of(a.g, h, b, live ? j : 0);
   const sb_half* o = row_of(a.o, h, b, live ? j : 0);
-  uint4 gv[kMaxP / 32], ov[kMaxP / 32];
+  uint4 gv[P / 32], ov[P / 32];
   if (vec)
 #pragma unroll
-    for (int c = 0; c < kMaxP / 32; ++c) {
+    for (int c = 0; c < P / 32; ++c) {
       const int p = i * 8 + c * 32;
       gv[c] = ov[c] = make_uint4(0u, 0u, 0u, 0u);
       if (p < a.P) {
@@ -452,7 +453,7 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
   float sum = 0.f;
   if (vec) {
 #pragma unroll
-    for (int c = 0; c < kMaxP / 32; ++c) {
+    for (int c = 0; c < P / 32; ++c) {
       float u[8], v[8];
       unpack8(gv[c], u);
       unpack8(ov[c], v);
@@ -672,7 +673,7 @@ int launch_rel_attn_bwd(cudaStream_t s, void* scratch, Proj dout, Proj q, Proj k
   };
   float* records = reinterpret_cast<float*>(base + pl.records);
   const int expanding = a.H * expand_blocks(x.pitch);
-  SB_LAUNCH_OK(launch_k(row_records_kernel, (unsigned)(expanding + a.H * a.B * ((a.J + 63) / 64)), 256, 0, s, a, st, x, records,
+  SB_LAUNCH_OK(launch_k(q.P <= 64 ? row_records_kernel<64> : row_records_kernel<128>, (unsigned)(expanding + a.H * a.B * ((a.J + 63) / 64)), 256, 0, s, a, st, x, records,
                         pieces(dout) && pieces(out) ? 1 : 0, expanding));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[0], &dout));
   SB_TRY(direct_or_packed(s, scratch, pl.p.at[1], &q));
