@@ -226,127 +226,173 @@ norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ T
 }
 
 // Any strides, any head size, lanes along tokens (what head-first projections have side by side).  Warp w of a block has the
-// pairs w, w + 8, .. of features (rotary pairs, then neighbours), SLOTS at most, of TOKENS tokens per lane, and keeps their
-// angles in registers while the block walks its heads; a row's sums go through shared memory.  Off: the type that holds a
-// feature's offset, 32 bits wherever a head's features span less than 2^31 elements (64-bit products of strides were most of the
-// instructions).
-template <int SLOTS, int TOKENS, bool BWD, class Off>
-__global__ void __launch_bounds__(256, SLOTS <= 4 ? 2 : 1)
+// pairs w, w + WARPS, .. of features (rotary pairs, then neighbours), SLOTS at most, of TOKENS tokens per lane, and keeps their
+// angles in registers while the block walks its heads; a row's sums go through shared memory.  The next head's elements are on
+// their way meanwhile, as long as registers last.  TOKENS = 2: tokens side by side in memory, in 32-bit words.  Off: the type that
+// holds a feature's offset, 32 bits wherever a head's features span less than 2^31 elements (64-bit products of strides were most
+// of the instructions).
+template <int TOKENS> struct Elements;                        // of one feature: TOKENS tokens
+template <> struct Elements<1> {
+  sb_half h;
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = sb_h2f(h); }
+  __device__ __forceinline__ static Elements of(const float (&v)[1]) { return {sb_f2h(v[0])}; }
+};
+template <> struct Elements<2> {
+  sb_half2 h;
+  __device__ __forceinline__ void get(float (&v)[2]) const {
+    const float2 f = sb_h22f2(h);
+    v[0] = f.x;
+    v[1] = f.y;
+  }
+  __device__ __forceinline__ static Elements of(const float (&v)[2]) { return {sb_f2h2(v[0], v[1])}; }
+};
+template <int WARPS, int SLOTS, int TOKENS, bool BWD, class Off>
+__global__ void __launch_bounds__(32 * WARPS, 16 / WARPS)
 norm_strided_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Turns turns) {
-  __shared__ float2 part[2][8][32 * TOKENS];
+  using El = Elements<TOKENS>;
+  constexpr bool kAhead = SLOTS <= 4;
+  __shared__ float2 part[2][WARPS][32 * TOKENS];
   grid_dependency_sync();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pairs = a.rotary / 2, slots = (a.P + 1) / 2;
   const int w = (int)blockIdx.x < a.blocks[0] ? 0 : 1, mine = (int)blockIdx.x - (w ? a.blocks[0] : 0);
   const int chunks = (a.x[w].H + a.chunk - 1) / a.chunk, stride = a.blocks[w] / chunks;
   const int h_from = mine % chunks * a.chunk, h_to = min(a.x[w].H, h_from + a.chunk);
   const float inv = 1.f / (float)a.P;
-  // the two features of each slot: number (that of the first where there is none), gain (then 0), place in x, g and y
-  int feature[SLOTS][2];
+  // the two features of each slot: place in x, g and y (of the first where there is none), gain (then 0)
   Off xo[SLOTS][2], go[SLOTS][2], yo[SLOTS][2];
   float gain[SLOTS][2], sum[SLOTS][2];
   uint32_t there = 0;
+  auto feature = [&](int i, int e) {
+    const int u = warp + WARPS * i;
+    return u < pairs && a.pairing == SB_PAIR_HALVES ? u + e * pairs : 2 * u + e;
+  };
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
-    const int u = warp + 8 * i;
-    const bool halves = u < pairs && a.pairing == SB_PAIR_HALVES;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int f = halves ? u + e * pairs : 2 * u + e;
-      const bool is = u < slots && f < a.P;
+      const bool is = warp + WARPS * i < slots && feature(i, e) < a.P;
+      const int f = is ? feature(i, e) : 0;
       there |= (is ? 1u : 0u) << (2 * i + e);
-      feature[i][e] = is ? f : 0;
       gain[i][e] = is ? sb_h2f(a.gain[w][f]) : 0.f;
-      xo[i][e] = (Off)(feature[i][e] * a.x[w].sP);
-      go[i][e] = BWD ? (Off)(feature[i][e] * a.g[w].sP) : 0;
-      yo[i][e] = (Off)(feature[i][e] * a.y[w].sP);
+      xo[i][e] = (Off)(f * a.x[w].sP);
+      go[i][e] = BWD ? (Off)(f * a.g[w].sP) : 0;
+      yo[i][e] = (Off)(f * a.y[w].sP);
       sum[i][e] = 0.f;
     }
   }
   int turnstile = 0;
   for (int t = mine / chunks; t < a.tiles; t += stride) {
-    bool live[TOKENS];
+    const int token = (t * 32 + lane) * TOKENS;               // (two of them are of one sample and both there, or neither)
+    const bool live = token < a.tokens;
+    const Place at = place_of(a, live ? token : 0);
+    const sb_half* X = reinterpret_cast<const sb_half*>(a.x[w].p) + token_offset(a.x[w], at) + h_from * a.x[w].sH;
+    const sb_half* G = BWD ? reinterpret_cast<const sb_half*>(a.g[w].p) + token_offset(a.g[w], at) + h_from * a.g[w].sH : nullptr;
+    sb_half* Y = reinterpret_cast<sb_half*>(a.y[w].p) + token_offset(a.y[w], at) + h_from * a.y[w].sH;
+    El x[SLOTS][2], g[SLOTS][2], x_next[SLOTS][2], g_next[SLOTS][2];
+    auto load = [&](El (&lx)[SLOTS][2], El (&lg)[SLOTS][2]) { // (a feature that is not there reads the first and counts 0)
+#pragma unroll
+      for (int i = 0; i < SLOTS; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          lx[i][e] = *reinterpret_cast<const El*>(X + xo[i][e]);
+          if (BWD) lg[i][e] = *reinterpret_cast<const El*>(G + go[i][e]);
+        }
+      X += a.x[w].sH;
+      if (BWD) G += a.g[w].sH;
+    };
+    if (kAhead) load(x_next, g_next);
     float2 ang[SLOTS][TOKENS];
-    const sb_half *X[TOKENS], *G[TOKENS];
-    sb_half* Y[TOKENS];
 #pragma unroll
     for (int k = 0; k < TOKENS; ++k) {
-      const int token = t * 32 * TOKENS + k * 32 + lane;
-      live[k] = token < a.tokens;
-      const Place tc = place_of(a, live[k] ? token : 0);
-      const int pos = position(a, tc);
+      const int pos = position(a, Place{at.b, at.j + (live ? k : 0)});
 #pragma unroll
-      for (int i = 0; i < SLOTS; ++i) ang[i][k] = warp + 8 * i < pairs ? cos_sin(pos, turns.t[warp + 8 * i]) : make_float2(1.f, 0.f);
-      X[k] = reinterpret_cast<const sb_half*>(a.x[w].p) + token_offset(a.x[w], tc) + h_from * a.x[w].sH;
-      G[k] = BWD ? reinterpret_cast<const sb_half*>(a.g[w].p) + token_offset(a.g[w], tc) + h_from * a.g[w].sH : nullptr;
-      Y[k] = reinterpret_cast<sb_half*>(a.y[w].p) + token_offset(a.y[w], tc) + h_from * a.y[w].sH;
+      for (int i = 0; i < SLOTS; ++i) ang[i][k] = warp + WARPS * i < pairs ? cos_sin(pos, turns.t[warp + WARPS * i]) : make_float2(1.f, 0.f);
     }
-    for (int h = h_from; h < h_to; ++h, turnstile ^= 1) {
-      float x[SLOTS][TOKENS][2], g[SLOTS][TOKENS][2];
+    // features (2 of a slot, of all tokens) as numbers, and gradients turned back
+    auto numbers = [&](int i, float (&u)[TOKENS], float (&v)[TOKENS], float (&p)[TOKENS], float (&q)[TOKENS]) {
+      x[i][0].get(u);
+      x[i][1].get(v);
+      if (BWD) {
+        g[i][0].get(p);
+        g[i][1].get(q);
+      }
 #pragma unroll
       for (int k = 0; k < TOKENS; ++k) {
+        if (!((there >> (2 * i)) & 1u)) u[k] = p[k] = 0.f;
+        if (!((there >> (2 * i + 1)) & 1u)) v[k] = q[k] = 0.f;
+        if (BWD) {
+          const float c = ang[i][k].x, s = ang[i][k].y, y = p[k], z = q[k];
+          p[k] = y * c + z * s;
+          q[k] = z * c - y * s;
+        }
+      }
+    };
+#pragma unroll 1
+    for (int h = h_from; h < h_to; ++h, turnstile ^= 1, Y += a.y[w].sH) {
+      if (kAhead) {
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const bool is = (there >> (2 * i + e)) & 1u;      // (a feature that is not there reads the first and counts 0)
-            const float v = sb_h2f(X[k][xo[i][e]]);
-            x[i][k][e] = is ? v : 0.f;
-            if (BWD) {
-              const float d = sb_h2f(G[k][go[i][e]]);
-              g[i][k][e] = is ? d : 0.f;
-            }
+            x[i][e] = x_next[i][e];
+            if (BWD) g[i][e] = g_next[i][e];
           }
-        X[k] += a.x[w].sH;
-        if (BWD) G[k] += a.g[w].sH;
+        if (h + 1 < h_to) load(x_next, g_next);
+      } else {
+        load(x, g);
       }
       float sq[TOKENS], dot[TOKENS];
 #pragma unroll
-      for (int k = 0; k < TOKENS; ++k) {
-        sq[k] = dot[k] = 0.f;
+      for (int k = 0; k < TOKENS; ++k) sq[k] = dot[k] = 0.f;
 #pragma unroll
-        for (int i = 0; i < SLOTS; ++i) {
-          const float u = x[i][k][0], v = x[i][k][1];
-          sq[k] = fmaf(u, u, fmaf(v, v, sq[k]));
-          if (BWD) {
-            const float c = ang[i][k].x, s = ang[i][k].y, p = g[i][k][0], q = g[i][k][1];
-            g[i][k][0] = p * c + q * s;                       // turned back
-            g[i][k][1] = q * c - p * s;
-            dot[k] = fmaf(g[i][k][0] * gain[i][0], u, fmaf(g[i][k][1] * gain[i][1], v, dot[k]));
-          }
+      for (int i = 0; i < SLOTS; ++i) {
+        float u[TOKENS], v[TOKENS], p[TOKENS], q[TOKENS];
+        numbers(i, u, v, p, q);
+#pragma unroll
+        for (int k = 0; k < TOKENS; ++k) {
+          sq[k] = fmaf(u[k], u[k], fmaf(v[k], v[k], sq[k]));
+          if (BWD) dot[k] = fmaf(p[k] * gain[i][0], u[k], fmaf(q[k] * gain[i][1], v[k], dot[k]));
         }
-        part[turnstile][warp][k * 32 + lane] = make_float2(sq[k], dot[k]);
       }
+#pragma unroll
+      for (int k = 0; k < TOKENS; ++k) part[turnstile][warp][lane * TOKENS + k] = make_float2(sq[k], dot[k]);
       __syncthreads();
+      float rs[TOKENS], mean[TOKENS];
 #pragma unroll
       for (int k = 0; k < TOKENS; ++k) {
         sq[k] = dot[k] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 s = part[turnstile][i][k * 32 + lane];
+        for (int i = 0; i < WARPS; ++i) {
+          const float2 s = part[turnstile][i][lane * TOKENS + k];
           sq[k] += s.x;
           if (BWD) dot[k] += s.y;
         }
-        const float rs = rsqrtf(fmaf(sq[k], inv, a.eps)), mean = dot[k] * rs * inv;
+        rs[k] = rsqrtf(fmaf(sq[k], inv, a.eps));
+        mean[k] = dot[k] * rs[k] * inv;
+      }
 #pragma unroll
-        for (int i = 0; i < SLOTS; ++i) {
-          float u = x[i][k][0] * rs, v = x[i][k][1] * rs;
+      for (int i = 0; i < SLOTS; ++i) {
+        float u[TOKENS], v[TOKENS], p[TOKENS], q[TOKENS];
+        numbers(i, u, v, p, q);
+#pragma unroll
+        for (int k = 0; k < TOKENS; ++k) {
+          u[k] *= rs[k];
+          v[k] *= rs[k];
           if (!BWD) {
-            const float c = ang[i][k].x, s = ang[i][k].y, p = u * gain[i][0], q = v * gain[i][1];
-            u = p * c - q * s;
-            v = q * c + p * s;
+            const float c = ang[i][k].x, s = ang[i][k].y, y = u[k] * gain[i][0], z = v[k] * gain[i][1];
+            u[k] = y * c - z * s;
+            v[k] = z * c + y * s;
           } else {
-            const float p = g[i][k][0], q = g[i][k][1];
-            if (live[k]) {                                    // (what lies behind the last token is token 0 again)
-              sum[i][0] = fmaf(p, u, sum[i][0]);
-              sum[i][1] = fmaf(q, v, sum[i][1]);
+            if (live) {                                       // (what lies behind the last token is token 0 again)
+              sum[i][0] = fmaf(p[k], u[k], sum[i][0]);
+              sum[i][1] = fmaf(q[k], v[k], sum[i][1]);
             }
-            u = rs * (p * gain[i][0] - u * mean);
-            v = rs * (q * gain[i][1] - v * mean);
+            u[k] = rs[k] * (p[k] * gain[i][0] - u[k] * mean[k]);
+            v[k] = rs[k] * (q[k] * gain[i][1] - v[k] * mean[k]);
           }
-          if (live[k] && ((there >> (2 * i)) & 1u)) Y[k][yo[i][0]] = sb_f2h(u);
-          if (live[k] && ((there >> (2 * i + 1)) & 1u)) Y[k][yo[i][1]] = sb_f2h(v);
         }
-        Y[k] += a.y[w].sH;
+        if (live && ((there >> (2 * i)) & 1u)) *reinterpret_cast<El*>(Y + yo[i][0]) = El::of(u);
+        if (live && ((there >> (2 * i + 1)) & 1u)) *reinterpret_cast<El*>(Y + yo[i][1]) = El::of(v);
       }
     }
   }
@@ -355,7 +401,7 @@ norm_strided_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ 
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const float v = warp_sum(sum[i][e]);
-      if (lane == 0 && ((there >> (2 * i + e)) & 1u)) a.partial[w][(long long)mine * a.P + feature[i][e]] = v;
+      if (lane == 0 && ((there >> (2 * i + e)) & 1u)) a.partial[w][(long long)mine * a.P + feature(i, e)] = v;
     }
 }
 
@@ -432,12 +478,20 @@ int launch_pieces(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
   SB_LAUNCH_OK(launch_k(kernel, a.blocks[0] + a.blocks[1], 256, smem, s, a, turns_of(rot)));
   return SB_OK;
 }
-template <int SLOTS, int TOKENS, bool BWD>
+template <int WARPS, int SLOTS, int TOKENS, bool BWD>
 int launch_strided(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
-  const int sms = usable_sms(device_facts().sms), heads = a.x[0].H + a.x[1].H;
+  const int resident = 16 / WARPS * usable_sms(device_facts().sms);
   a.tiles = (a.tokens + 32 * TOKENS - 1) / (32 * TOKENS);
-  // up to eight heads a block, which share the angles; fewer where SMs would be without a block
-  for (a.chunk = 8; a.chunk > 1 && (long long)a.tiles * ((heads + a.chunk - 1) / a.chunk) < sms; a.chunk /= 2) {}
+  // Up to eight heads a block, which share its angles and everything else that a block begins with, about as much as two more
+  // heads; what matters is how often the SMs are filled with blocks.
+  long long least = 0;
+  for (int c = 8; c >= 1; --c) {
+    const long long blocks = (long long)a.tiles * ((a.x[0].H + c - 1) / c + (a.x[1].H + c - 1) / c), cost = (blocks + resident - 1) / resident * (c + 2);
+    if (c == 8 || cost < least) {
+      least = cost;
+      a.chunk = c;
+    }
+  }
   if (BWD) a.chunk = std::max({a.chunk, (a.x[0].H + kMaxPartials - 1) / kMaxPartials, (a.x[1].H + kMaxPartials - 1) / kMaxPartials});
   for (int w = 0; w < 2; ++w) {
     const int chunks = (a.x[w].H + a.chunk - 1) / a.chunk;
@@ -448,8 +502,8 @@ int launch_strided(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) 
   bool narrow = true;
   for (int w = 0; w < 2; ++w)
     for (const Proj* v : {&a.x[w], &a.y[w], &a.g[w]}) narrow = narrow && std::llabs(v->sP) < (1ll << 31) / kNormMaxHead;
-  auto kernel = narrow ? norm_strided_kernel<SLOTS, TOKENS, BWD, int> : norm_strided_kernel<SLOTS, TOKENS, BWD, long long>;
-  SB_LAUNCH_OK(launch_k(kernel, a.blocks[0] + a.blocks[1], 256, 0, s, a, turns_of(rot)));
+  auto kernel = narrow ? norm_strided_kernel<WARPS, SLOTS, TOKENS, BWD, int> : norm_strided_kernel<WARPS, SLOTS, TOKENS, BWD, long long>;
+  SB_LAUNCH_OK(launch_k(kernel, a.blocks[0] + a.blocks[1], 32 * WARPS, 0, s, a, turns_of(rot)));
   return SB_OK;
 }
 template <bool BWD>
@@ -464,8 +518,14 @@ int launch_norm(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
     if (a.P <= 128) return launch_pieces<8, BWD>(s, a, rot, rows);
     return launch_pieces<16, BWD>(s, a, rot, rows);
   }
-  return a.P <= 64 ? launch_strided<4, 1, BWD>(s, a, rot, rows) : a.P <= 128 ? launch_strided<8, 1, BWD>(s, a, rot, rows)
-                                                                             : launch_strided<16, 1, BWD>(s, a, rot, rows);
+  // tokens in twos where they lie side by side in 32-bit words
+  bool twos = a.J % 2 == 0;
+  for (int w = 0; w < 2; ++w)
+    for (const Proj* v : {&a.x[w], &a.y[w], &a.g[w]})
+      twos = twos && (v->p == nullptr || (v->sR == 1 && !((v->sP | v->sH | v->sB) & 1) && !(reinterpret_cast<uintptr_t>(v->p) & 3u)));
+  if (a.P <= 64) return twos ? launch_strided<8, 4, 2, BWD>(s, a, rot, rows) : launch_strided<8, 4, 1, BWD>(s, a, rot, rows);
+  if (a.P <= 128) return twos ? launch_strided<16, 4, 2, BWD>(s, a, rot, rows) : launch_strided<16, 4, 1, BWD>(s, a, rot, rows);
+  return launch_strided<16, 8, 1, BWD>(s, a, rot, rows);
 }
 
 }  // namespace
