@@ -250,7 +250,7 @@ template <int WARPS, int SLOTS, int TOKENS, bool BWD, class Off>
 __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS)
 norm_strided_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Turns turns) {
   using El = Elements<TOKENS>;
-  constexpr bool kAhead = SLOTS <= 4;
+  constexpr bool kAhead = SLOTS <= 4 && !(BWD && TOKENS == 2);   // (no registers left there: 19.2 us with, 18.4 without)
   __shared__ float2 part[2][WARPS][32 * TOKENS];
   grid_dependency_sync();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pairs = a.rotary / 2, slots = (a.P + 1) / 2;
