@@ -96,21 +96,25 @@ pack_rows_kernel(const Proj x, sb_half* dst, int Pp, int along_rows) {
 // The rows of a key head are the queries of all heads that share it, J for each.  A CTA takes 16 of them (one mma.sync tile) and a
 // share of the keys; its four warps walk pieces of those keys in turn, each with a ring of its own filled by cp.async (which
 // also puts zeros behind a sequence's end), softmax state and accumulator, joined at the end.  With more than one share, a
-// second kernel joins those.  Bound by reading keys and values once: tcgen05's smallest tile would be 64 or 128 rows for the
-// one to 16 there are, and the matrix work here is a few percent of the time.
+// second kernel joins those.  Bound by reading keys and values once (B=16, 16 heads on 8, 8192 keys of 128 features: 72 us, 87 % of the
+// copy bandwidth); tcgen05's smallest tile would be 64 or 128 rows for the one to 16 there are, and the matrix work here
+// is a few percent of the time.
 constexpr int kFewThreads = 128;
 template <int P>
 struct FewCfg {
   static constexpr int kKeys = P == 64 ? 32 : 16;    // of a piece
   static constexpr int kStages = 3;
   static constexpr int kHalf = kKeys * P * 2;        // bytes of a piece's keys
-  static constexpr int kWarp = kStages * 2 * kHalf;
-  static constexpr int kSmem = 4 * kWarp;
-  static_assert(4 * (16 * P + 32) * 4 <= kSmem, "results of the warps in the rings' place");
+  // A ring has a slot for each of its warp's pieces, up to kStages: short shares leave room for more CTAs.
+  static constexpr int slots(int share) { return share <= 4 * kKeys ? 1 : share <= 8 * kKeys ? 2 : kStages; }
+  static constexpr int smem(int share) {
+    const int rings = 4 * slots(share) * 2 * kHalf, results = 4 * (16 * P + 32) * 4;
+    return rings > results ? rings : results;
+  }
 };
 struct FewParams {
   AttnArgs a;
-  int rows, blocks, splits, reach;                   // rows of a key head, blocks of 16 of them
+  int rows, blocks, splits, reach, slots;            // rows of a key head, blocks of 16 of them; slots of a ring
   int before, behind;                                // buckets of far keys
   float* partial;                                    // [B][G][rows][splits][P + 2]: output, reference, sum; null with one share
 };
@@ -139,6 +143,7 @@ __device__ __forceinline__ uint32_t pack_pair(float x, float y) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+__host__ __device__ constexpr int share_of(int keys, int splits) { return ((keys + splits - 1) / splits + 31) & ~31; }
 template <int P>
 __global__ void __launch_bounds__(kFewThreads)
 few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ Starts st) {
@@ -156,10 +161,10 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
   // keys that some row of the sample sees, and this CTA's share of them
   int keys = keys_of(a, b);
   if (a.causal) keys = max(0, min(keys, first + a.J));
-  const int share = ((keys + p.splits - 1) / p.splits + 31) & ~31;
+  const int share = share_of(keys, p.splits);
   const int k_from = min(keys, split * share), k_to = min(keys, k_from + share);
   const int pieces = (k_to - k_from + kKeys - 1) / kKeys, mine = pieces > warp ? (pieces - warp + 3) >> 2 : 0;
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * Cfg::kWarp;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * p.slots * 2 * Cfg::kHalf;
   const sb_half* kp = row_of(a.k, hk, b, 0);
   const sb_half* vp = row_of(a.v, hk, b, 0);
 
@@ -224,9 +229,9 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
     hi[x] = bias_of(p.behind, head[x]);
   }
   __syncthreads();
-  // buckets of the relative positions within reach, where this CTA's keys have any
+  // buckets of the relative positions within reach, where this CTA's pieces have any
   const int pos_lo = first, pos_hi = first + a.J - 1;
-  if (k_to - 1 - pos_lo > -p.reach && k_from - pos_hi < p.reach) {
+  if (k_from + pieces * kKeys - 1 - pos_lo > -p.reach && k_from - pos_hi < p.reach) {
     for (int i = threadIdx.x; i <= 2 * p.reach; i += kFewThreads) map[i] = (uint16_t)bucket_of(a, starts, i - p.reach);
     __syncthreads();
   }
@@ -258,32 +263,37 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
         mma16816(s[t], qf[c], f[0], f[1]);
         mma16816(s[t + 1], qf[c], f[2], f[3]);
       }
-    // biases, what is hidden, maxima
+    // biases, what is hidden, maxima.  (All loads of biases unconditional: a branch for each waits for each)
     const bool near = k0 + kKeys - 1 - pos_lo > -p.reach && k0 - pos_hi < p.reach;
     const bool after = k0 - pos_hi >= p.reach, whole = k0 + kKeys <= k_to && !(a.causal && k0 + kKeys - 1 > pos_lo);
     float mx[2] = {-INFINITY, -INFINITY};
-    if (!near && whole) {
-      const float flat[2] = {after ? hi[0] : lo[0], after ? hi[1] : lo[1]};
+    const float flat[2] = {after ? hi[0] : lo[0], after ? hi[1] : lo[1]};
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[t][e] = fmaf(s[t][e], c2, near ? 0.f : flat[e >> 1]);
+    if (near) {
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[t][e] = fmaf(s[t][e], c2, flat[e >> 1]);
-          mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
-        }
-    } else {
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int x = e >> 1, k = k0 + t * 8 + (lane & 3) * 2 + (e & 1), rel = k - pos[x];
-          // (a key behind this CTA's last may be within reach of the query when none of the CTA's is, and then there is no map)
-          const bool seen = k < k_to && !(a.causal && rel > 0);
-          const float bias = rel <= -p.reach ? lo[x] : rel >= p.reach ? hi[x] : seen ? bias_of(map[rel + p.reach], head[x]) : 0.f;
-          s[t][e] = seen ? fmaf(s[t][e], c2, bias) : -INFINITY;
-          mx[x] = fmaxf(mx[x], s[t][e]);
+          const int x = e >> 1, rel = k0 + t * 8 + (lane & 3) * 2 + (e & 1) - pos[x];
+          s[t][e] += bias_of(map[max(-p.reach, min(p.reach, rel)) + p.reach], head[x]);
         }
     }
+    if (!whole) {
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = k0 + t * 8 + (lane & 3) * 2 + (e & 1);
+          if (k >= k_to || (a.causal && k > pos[e >> 1])) s[t][e] = -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
     bool raise = false;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -576,13 +586,20 @@ bool piecewise(const Proj& x) {
   return (x.sP == 1 || x.P == 1) && !(reinterpret_cast<uintptr_t>(x.p) & 15u) && ok(x.H, x.sH) && ok(x.B, x.sB) && ok(x.R, x.sR);
 }
 
-// The forward pass with few queries: how many shares the keys are cut into, 0 when the tile kernel is to run.
+// The forward pass with few queries: how many shares the keys are cut into, 0 when the tile kernel is to run.  The tile kernel has an
+// item for 128 queries of one head, which walks the keys alone at 0.7 us per 64 of them; here 16 rows of all heads that share keys
+// walk as many shares of the keys as there is room for.  So they are few when their CTAs do not fill the SMs and there are keys to
+// share out (8 heads of 64, 256 queries, 4096 keys: 27 against 54 us here; 64 queries and keys: 8.2 against 7.2), and beyond that
+// when there are not more CTAs than items: every key is read as often (64 x 16 heads, one query, 512 keys: 38 against 41 us), with
+// heads that share keys less often (64 x 16 heads on 8, 4096 keys: 84 against 225); with more than four queries the tensor cores
+// of the tile kernel outweigh that (16 queries, 512 keys: 52 against 41).
 int few_splits(const Proj& q, const Proj& k) {
-  const long long rows = (long long)(q.H / k.H) * q.R;
-  if (rows > 64) return 0;
-  const long long ctas = (long long)k.B * k.H * ((rows + 15) / 16);
-  // about four CTAs for each of 148 SMs, at least 256 keys a share
-  return (int)std::max<long long>(1, std::min<long long>({(592 + ctas - 1) / ctas, (k.R + 255) / 256, 64}));
+  const long long blocks = ((long long)(q.H / k.H) * q.R + 15) / 16, ctas = blocks * k.B * k.H, items = (long long)q.B * q.H * ((q.R + 127) / 128);
+  const bool idle = ctas <= 148 && (blocks == 1 || k.R >= 1024);
+  if (!idle && ctas * (q.R > 4 ? 2 : 1) > items) return 0;
+  // two CTAs for each of 148 SMs and no more, which would wait for those (16 x 16 heads on 8, 8192 keys of 128 features, 128 CTAs: two
+  // shares 87 us, four 97, five 114), at least 256 keys a share
+  return (int)std::max<long long>(1, std::min<long long>({296 / ctas, (k.R + 255) / 256, 64}));
 }
 struct FewPlan { int splits; size_t k, v, bytes; };
 FewPlan few_plan(const Proj& q, const Proj& k, const Proj& v) {
@@ -597,10 +614,12 @@ FewPlan few_plan(const Proj& q, const Proj& k, const Proj& v) {
 }
 
 template <int P>
-int launch_few(cudaStream_t s, const FewParams& p, const Starts& st) {
-  SB_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(few_queries_kernel<P>), FewCfg<P>::kSmem));
+int launch_few(cudaStream_t s, FewParams& p, const Starts& st) {
+  const int share = share_of(p.a.K, p.splits);
+  p.slots = FewCfg<P>::slots(share);
+  SB_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(few_queries_kernel<P>), FewCfg<P>::smem(1 << 30)));
   const long long units = (long long)p.a.B * p.a.G;
-  SB_LAUNCH_OK(launch_k(few_queries_kernel<P>, (unsigned)(units * p.blocks * p.splits), kFewThreads, FewCfg<P>::kSmem, s, p, st));
+  SB_LAUNCH_OK(launch_k(few_queries_kernel<P>, (unsigned)(units * p.blocks * p.splits), kFewThreads, FewCfg<P>::smem(share), s, p, st));
   if (p.splits > 1)
     SB_LAUNCH_OK(launch_k(join_splits_kernel<P>, (unsigned)((units * p.rows + 3) / 4), 128, 0, s, p));
   return SB_OK;

@@ -198,6 +198,13 @@ ATTENTION_CASES = [
     (80, 4, 2, 2, 3, 333, 'PHBJ', 32, 128, True, False, None, [100, 330]),
     (24, 2, 2, 2, 4, 70, 'BJHP', 32, 128, False, True, [70, 9], [66, 5]),
     (64, 24, 1, 2, 1, 700, 'BJHP', 64, 512, False, True, [700, 699], [699, 698]),
+    # many queries, few heads and long keys: split along the keys as well
+    (64, 2, 1, 1, 150, 1100, 'BJHP', 32, 128, True, False, [1090], [900]),
+    (128, 2, 2, 2, 40, 2100, 'BJHP', 32, 128, False, True, [2100, 700], [2060, 500]),
+    (40, 3, 3, 1, 333, 1300, 'PHBJ', 16, 64, True, True, None, [967]),
+    # many single tokens, and as many again with shared keys
+    (64, 4, 4, 50, 1, 70, 'BJHP', 32, 128, False, True, None, [69] * 50),
+    (64, 8, 4, 50, 3, 90, 'BJHP', 32, 128, True, False, list(range(41, 91)), [20] * 50),
     # as many buckets as there may be, up to the last distance
     (64, 2, 2, 1, 900, 900, 'BJHP', 512, 832, False, True, None, None),
     (128, 4, 4, 1, 2, 1700, 'BJHP', 1024, 832, True, False, None, [850]),
