@@ -329,6 +329,7 @@ _PAIRING = {'halves': _lib.SB_PAIR_HALVES, 'adjacent': _lib.SB_PAIR_ADJACENT}
 
 # SbTensor, SbRotation, SbRelativeBias and SbAttentionSpan as packed bytes
 _TENSOR, _ROTATION, _BIAS, _SPAN = (struct.Struct(f) for f in ('Pi4x10q', 'diif4x', 'PiiP', 'fiPP'))
+_pack, _size, _stride, _data_ptr = _TENSOR.pack, torch.Tensor.size, torch.Tensor.stride, torch.Tensor.data_ptr
 _half_libs = {}
 
 
@@ -336,10 +337,18 @@ def _packed(t):
     """SbTensor of a tensor, or NULL."""
     if t is None:
         return None
-    shape, stride = t.shape, t.stride()
+    shape, stride = _size(t), _stride(t)
     n = len(shape)
-    if n == 4:
-        return _TENSOR.pack(t.data_ptr(), 4, *shape, 0, *stride, 0)
+    if n == 4:                  # (names for each: unpacking into the call takes longer)
+        a, b, c, d = shape
+        e, f, g, h = stride
+        return _pack(_data_ptr(t), 4, a, b, c, d, 0, e, f, g, h, 0)
+    if n == 2:
+        a, b = shape
+        e, f = stride
+        return _pack(_data_ptr(t), 2, a, b, 0, 0, 0, e, f, 0, 0, 0)
+    if n == 1:
+        return _pack(_data_ptr(t), 1, shape[0], 0, 0, 0, 0, stride[0], 0, 0, 0, 0)
     if n > _lib.SB_MAX_DIMS:
         raise ValueError(f'at most {_lib.SB_MAX_DIMS} dimensions, got {n}')
     fill = (0,) * (_lib.SB_MAX_DIMS - n)
