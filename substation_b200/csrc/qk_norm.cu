@@ -1,5 +1,11 @@
 // Norms of query and key heads and their rotation by position, forward and backward (sb_query_key_norm_rotation and
 // sb_backward_query_key_norm_rotation; formulas in the header).  A row is one head of one token.
+//
+//   forward   y = R(pos) (gain x rs),   rs = (mean x^2 + eps)^(-1/2)
+//   backward  g = R(-pos) dy,   dgain = sum g x rs,   dx = rs g gain - x rs^3 mean(g gain x)
+//
+// A few operations per element: all of it is bound by bytes, each element read once and written once, and for small calls by the
+// launch.  Everything is 32 bits between load and store, with one rounding at the end.
 
 #include <algorithm>
 #include <cmath>
@@ -56,7 +62,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 // their angles into shared memory, and its groups of threads walk the query (or key) heads of a token each.  Rows are fetched
 // kDepth ahead into a ring that belongs to the thread alone, so that nothing has to be waited for but the copy itself; as
 // registers they held half as many bytes in flight.  In the backward pass sum x^2 and sum g gain x are all that a row needs
-// from its other threads; the gains' gradients stay in registers until the block's last tile.
+// from its other threads; the gains' gradients stay in registers until the block's last tile.  Copy bandwidth reached: backward,
+// B=4, L=4096, 32 + 8 heads of 128 (503 MB): 104 us, 74 %; forward, B=8, L=512, 16 + 16 heads of 64 (33.6 MB): 9.8 us, 52 %, of
+// which about 3 are launch and the first tile's way; a single token for each of 8 samples: 3.7 us.
 template <int LANES, bool BWD, bool HALVES>
 __global__ void __launch_bounds__(256, 2)
 norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Turns turns) {
@@ -230,7 +238,8 @@ norm_pieces_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ T
 // angles in registers while the block walks its heads; a row's sums go through shared memory.  The next head's elements are on
 // their way meanwhile, as long as registers last.  TOKENS = 2: tokens side by side in memory, in 32-bit words.  Off: the type that
 // holds a feature's offset, 32 bits wherever a head's features span less than 2^31 elements (64-bit products of strides were most
-// of the instructions).
+// of the instructions).  Forward, B=12, L=200, 12 + 12 heads of 64, head-first (14.7 MB): 8.2 us, 27 % of the copy bandwidth, one wave
+// of blocks that are chains of as many heads as each has (11.9 us with single tokens, eight heads a block, no head on its way).
 template <int TOKENS> struct Elements;                        // of one feature: TOKENS tokens
 template <> struct Elements<1> {
   sb_half h;
@@ -405,7 +414,107 @@ norm_strided_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ 
     }
 }
 
-// out[p] = sum of the blocks' rows in a fixed order: 32 threads a column take every 32nd row, then a tree.
+// Features side by side, but off the 16-byte grid or with pairs that pieces do not hold: a warp per row, a lane per pair (SLOTS of them,
+// 32 apart), kRows heads of a token at a time, whose elements are all asked for before any is used.  Angles stay for a token's heads.
+// Bound by the 64 bytes of its loads: B=8, L=512, 16 + 16 heads of 64, one element off the grid: 24.6 us (pieces on the grid 9.8; lanes
+// along tokens 113, each of which touches 32 rows with a load).
+template <int SLOTS, bool BWD>
+__global__ void __launch_bounds__(256, 2)
+norm_rows_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Turns turns) {
+  constexpr int kRows = SLOTS == 1 ? 4 : SLOTS == 2 ? 2 : 1;
+  __shared__ float part[BWD ? 8 * kNormMaxHead : 1];
+  grid_dependency_sync();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pairs = a.rotary / 2, slots = (a.P + 1) / 2;
+  const int w = (int)blockIdx.x < a.blocks[0] ? 0 : 1, mine = (int)blockIdx.x - (w ? a.blocks[0] : 0), heads = a.x[w].H;
+  const float inv = 1.f / (float)a.P;
+  int f[SLOTS][2];                                            // -1: not there
+  float gain[SLOTS][2], sum[SLOTS][2];
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int u = lane + 32 * i, n = u < pairs && a.pairing == SB_PAIR_HALVES ? u + e * pairs : 2 * u + e;
+      f[i][e] = u < slots && n < a.P ? n : -1;
+      gain[i][e] = f[i][e] >= 0 ? sb_h2f(a.gain[w][f[i][e]]) : 0.f;
+      sum[i][e] = 0.f;
+    }
+  for (int token = mine * 8 + warp; token < a.tokens; token += a.blocks[w] * 8) {
+    const Place at = place_of(a, token);
+    const sb_half* X = reinterpret_cast<const sb_half*>(a.x[w].p) + token_offset(a.x[w], at);
+    const sb_half* G = BWD ? reinterpret_cast<const sb_half*>(a.g[w].p) + token_offset(a.g[w], at) : nullptr;
+    sb_half* Y = reinterpret_cast<sb_half*>(a.y[w].p) + token_offset(a.y[w], at);
+    const int pos = position(a, at);
+    float2 ang[SLOTS];
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) ang[i] = lane + 32 * i < pairs ? cos_sin(pos, turns.t[lane + 32 * i]) : make_float2(1.f, 0.f);
+    for (int h0 = 0; h0 < heads; h0 += kRows) {
+      float x[kRows][SLOTS][2], g[kRows][SLOTS][2];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const bool is = f[i][e] >= 0 && h0 + r < heads;
+            x[r][i][e] = is ? sb_h2f(X[(h0 + r) * a.x[w].sH + f[i][e]]) : 0.f;
+            if (BWD) g[r][i][e] = is ? sb_h2f(G[(h0 + r) * a.g[w].sH + f[i][e]]) : 0.f;
+          }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        float sq = 0.f, dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) {
+          const float u = x[r][i][0], v = x[r][i][1];
+          sq = fmaf(u, u, fmaf(v, v, sq));
+          if (BWD) {
+            const float c = ang[i].x, s = ang[i].y, p = g[r][i][0], q = g[r][i][1];
+            g[r][i][0] = p * c + q * s;                       // turned back
+            g[r][i][1] = q * c - p * s;
+            dot = fmaf(g[r][i][0] * gain[i][0], u, fmaf(g[r][i][1] * gain[i][1], v, dot));
+          }
+        }
+        sq = group_sum<32>(sq);
+        if (BWD) dot = group_sum<32>(dot);
+        const float rs = rsqrtf(fmaf(sq, inv, a.eps)), mean = BWD ? dot * rs * inv : 0.f;
+        if (h0 + r >= heads) continue;                        // (the same for the whole warp)
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) {
+          float u = x[r][i][0] * rs, v = x[r][i][1] * rs;
+          if (!BWD) {
+            const float c = ang[i].x, s = ang[i].y, p = u * gain[i][0], q = v * gain[i][1];
+            u = p * c - q * s;
+            v = q * c + p * s;
+          } else {
+            const float p = g[r][i][0], q = g[r][i][1];
+            sum[i][0] = fmaf(p, u, sum[i][0]);
+            sum[i][1] = fmaf(q, v, sum[i][1]);
+            u = rs * (p * gain[i][0] - u * mean);
+            v = rs * (q * gain[i][1] - v * mean);
+          }
+          if (f[i][0] >= 0) Y[(h0 + r) * a.y[w].sH + f[i][0]] = sb_f2h(u);
+          if (f[i][1] >= 0) Y[(h0 + r) * a.y[w].sH + f[i][1]] = sb_f2h(v);
+        }
+      }
+    }
+  }
+  if (BWD) {
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (f[i][e] >= 0) part[warp * a.P + f[i][e]] = sum[i][e];
+    __syncthreads();
+    for (int p = threadIdx.x; p < a.P; p += 256) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += part[i * a.P + p];
+      a.partial[w][(long long)mine * a.P + p] = v;
+    }
+  }
+}
+
+// out[p] = sum of the blocks' rows in a fixed order: 32 threads a column take every 32nd row, then a tree.  Latency alone: 2.9 us for
+// 296 rows of 64.
 __global__ void __launch_bounds__(1024)
 gain_finish_kernel(const float* q_partial, const float* k_partial, int q_rows, int k_rows, int P, sb_half* q, sb_half* k) {
   __shared__ float part[32][33];
@@ -478,6 +587,15 @@ int launch_pieces(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
   SB_LAUNCH_OK(launch_k(kernel, a.blocks[0] + a.blocks[1], 256, smem, s, a, turns_of(rot)));
   return SB_OK;
 }
+template <int SLOTS, bool BWD>
+int launch_rows(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
+  a.tiles = (a.tokens + 7) / 8;
+  const long long most = std::min(4 * usable_sms(device_facts().sms), kMaxPartials), heads = a.x[0].H + a.x[1].H;
+  for (int w = 0; w < 2; ++w)    // queries and keys share the blocks by their heads
+    a.blocks[w] = rows[w] = a.x[w].H ? (int)std::min<long long>(a.tiles, std::max(1ll, most * a.x[w].H / heads)) : 0;
+  SB_LAUNCH_OK(launch_k(norm_rows_kernel<SLOTS, BWD>, a.blocks[0] + a.blocks[1], 256, 0, s, a, turns_of(rot)));
+  return SB_OK;
+}
 template <int WARPS, int SLOTS, int TOKENS, bool BWD>
 int launch_strided(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
   const int resident = 16 / WARPS * usable_sms(device_facts().sms);
@@ -518,6 +636,11 @@ int launch_norm(cudaStream_t s, NormArgs& a, const Rotation& rot, int* rows) {
     if (a.P <= 128) return launch_pieces<8, BWD>(s, a, rot, rows);
     return launch_pieces<16, BWD>(s, a, rot, rows);
   }
+  // features side by side
+  bool side = true;
+  for (int w = 0; w < 2; ++w)
+    for (const Proj* v : {&a.x[w], &a.y[w], &a.g[w]}) side = side && (v->p == nullptr || v->sP == 1);
+  if (side) return a.P <= 64 ? launch_rows<1, BWD>(s, a, rot, rows) : a.P <= 128 ? launch_rows<2, BWD>(s, a, rot, rows) : launch_rows<4, BWD>(s, a, rot, rows);
   // tokens in twos where they lie side by side in 32-bit words
   bool twos = a.J % 2 == 0;
   for (int w = 0; w < 2; ++w)

@@ -58,7 +58,12 @@ NORM_CASES = [
     (16, 5, 2, 4, 9, 'BJHP', 'JBHP', 16, 'halves'),
     (256, 2, 1, 2, 33, 'BJHP', 'BHJP', 256, 'halves'),
     (80, 12, 4, 2, 40, 'BJHP', 'BJHP', 80, 'halves'),
-    (2, 9600, 20000, 1, 2, 'BJHP', 'BJHP', 2, 'halves'),    # more heads than rows of partial sums for eight of them each
+    (80, 6, 3, 2, 33, 'BJHP', 'BHJP', 40, 'halves'),        # pairs that no two pieces hold
+    (31, 5, 2, 3, 20, 'BJHP', 'BJHP', 30, 'adjacent'),
+    (130, 3, 9, 2, 41, 'BJHP', 'BHJP', 66, 'halves'),
+    (90, 4, 2, 2, 150, 'PHBJ', 'BHPJ', 90, 'adjacent'),     # tokens in twos, sixteen warps
+    (2, 9600, 20000, 1, 2, 'PHBJ', 'PHBJ', 2, 'halves'),    # more heads than rows of partial sums for eight of them each
+    (2, 9600, 20000, 1, 2, 'BJHP', 'BJHP', 2, 'halves'),
     (96, 4, 4, 2, 21, 'BJHP', 'BJHP', 32, 'adjacent'),
     (64, 12, 12, 3, 24, 'PHBJ', 'PHBJ', 32, 'adjacent'),
     (64, 12, 4, 3, 25, 'PHBJ', 'BJHP', 64, 'halves'),
