@@ -43,8 +43,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 // D (+)= A * B, A in shared memory or (ts) in tensor memory as 16-bit pairs, a row per lane.  The whole warp comes here and one
-// thread issues (`on`): inside a branch of one thread the operands were moved to uniform registers for each instruction, 70
-// clocks apart whatever its size.
+// thread issues (`on`), so that the operands are the warp's and not a branch's.
 __device__ __forceinline__ void umma_ss(uint32_t on, uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n .reg .pred p, e;\n setp.ne.b32 e, %5, 0;\n setp.ne.b32 p, %4, 0;\n"
@@ -379,10 +378,13 @@ __device__ __forceinline__ void row_tile(uint32_t s, uint32_t to, bool started, 
   row.l += sum.x + sum.y;
 }
 
-// One CTA: 128 queries of one unit against its keys; two CTAs per SM.  Scores are multiplied a tile ahead of the softmax, by a
-// warp of their own: with one warp for both products and one buffer, issuing and handing over took most of the time (B=2,
-// L=4096: 140 us of 270 without any softmax).  Exponentials go back into tensor memory as 16-bit pairs, where the second product
-// takes them from.  Softmax warps: thread = row.
+// One CTA: 128 queries of one unit against its keys, one pass with running references and sums; two CTAs per SM.  Scores are
+// multiplied a tile ahead of the softmax, by a warp of their own: with one warp for both products and one buffer, issuing and
+// handing over took most of the time.  Exponentials go back into tensor memory as 16-bit pairs (rounded once, as an operand of the
+// second product has to be), where that product takes them from.  Softmax warps: thread = row.
+// B=2, L=4096, 16 heads of 64 (137 GFLOP): 244 us, 34 % of the measured matrix rate; B=8, L=512: 27 us; B=2, L=2000 causal, 16 heads
+// of 128 on 4: 55 us.  Bound by the softmax warps, of which a scheduler has two: exponentials keep their unit busy for 53 % of the
+// time (without any 20 % less), half of it per tile of 64 columns is waiting for one's own results; without softmax 140 us.
 template <int P>
 __global__ void __launch_bounds__(kFwdThreads, 2)
 rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -729,11 +731,15 @@ __device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float fl
   }
 }
 
-// One CTA per SM.  The two groups of element
-// warps take the streamed tiles in turn: while one turns scores and dP into exponentials and score gradients, the tensor cores
-// multiply for the other.  Both results go back into tensor memory, where the second products take them from.  Everything is
+// One CTA per SM.  The two groups of element warps take the streamed tiles in turn: while one turns scores and dP into
+// exponentials and score gradients, the tensor cores multiply for the other.  Both results go back into tensor memory as 16-bit
+// pairs, rounded once as operands have to be, where the second products take them from.  Everything is
 // computed twice, once per kind of item (but for BOTH); the alternative, dQ summed over key tiles in memory, needs atomics whose order
 // changes the result, or a partial dQ for every key tile.
+// B=2, L=4096, 16 heads of 64 (344 GFLOP, of which 481 are multiplied): 658 us, 32 % of the measured matrix rate; B=2, L=2000 causal, 16
+// heads of 128 on 4: 203 us; B=8, L=512: 77 us; BOTH at B=96, L=128: 74 us, bound by its items' beginnings and ends.  Without element
+// work 410 us, without products 599: the element warps' instructions, two warps per scheduler.  A third group (128 registers a
+// thread) took 694 us, scores from tensor memory 630 at best.
 // The table's gradient: a score gradient belongs to its relative position, a diagonal of the tile.  A warp moves each column of
 // its 32 x 32 blocks so that lane l holds diagonals l and l - 32 (one shuffle a column), adds the sums of a block to its own row
 // of sums over relative positions, and a group of warps adds up its four rows per item.  Tiles outside the varying part of the

@@ -49,7 +49,7 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
 
 // rows[h][i] = log2(e) * bias of head h at relative position i - kRelPad - reach, which stays at its end values beyond the reach.
 // Biases of up to 2^127 in size stay finite, so that a row of nothing but float16's lowest still has a maximum.
-// Block `part` of expand_blocks() for the head.
+// Block `part` of expand_blocks() for the head.  A launch and a search among the starts: 1.9 us alone, whatever the size.
 struct Expand { float* rows; int pitch, reach; int* next; };   // next: the work queue of the kernel that follows
 __host__ __device__ constexpr int expand_blocks(int pitch) { return (pitch + 255) / 256; }
 __device__ __forceinline__ void expand_part(const AttnArgs& a, const int* starts, const Expand& x, int h, int part) {
@@ -66,30 +66,75 @@ expand_bias_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
   expand_part(a, st.s, x, blockIdx.y, blockIdx.x);
 }
 
-// [P,H,B,R] of any strides -> [B][H][R][Pp], which tensor maps can address; 64 rows of one head and sample a block.
-__global__ void __launch_bounds__(256)
-pack_rows_kernel(const Proj x, sb_half* dst, int Pp, int along_rows) {
-  __shared__ sb_half tile[64][kMaxP + 2];
+// Copies of operands that tensor maps cannot address: [P,H,B,R] of any strides -> [B][H][R][Pp], up to four of them in a launch.  A
+// block turns 64 rows of one head and sample over in shared memory: words of two rows where rows lie side by side in them, else
+// elements along rows or along features, 16 of them on their way per thread, and 16-byte pieces out.  B=8, L=512, three operands of
+// 16 heads of 64 (50 MB): 13 us head-first, 15 feature-innermost off the 16-byte grid (26 and 40 with one load after the other and a
+// launch each); bound by the rounds of loads that its blocks wait for.
+enum { kPackTwos, kPackRows, kPackFeatures };
+struct PackJobs {
+  struct { Proj x; sb_half* dst; int mode; int first; } job[4];   // first: its first block
+  int n, blocks;
+};
+__global__ void __launch_bounds__(256, 5)
+pack_rows_kernel(const __grid_constant__ PackJobs jobs) {
+  constexpr int kPitch = kMaxP + 8;                            // (pieces aligned, rows four banks apart)
+  __shared__ __align__(16) sb_half tile[64][kPitch];
   grid_dependency_sync();
-  const int blocks = (x.R + 63) / 64;
-  const long long all = (long long)x.H * x.B * blocks;
-  for (long long it = blockIdx.x; it < all; it += gridDim.x) {
-    const int r0 = (int)(it % blocks) * 64, h = (int)(it / blocks % x.H), b = (int)(it / blocks / x.H), n = min(64, x.R - r0);
-    const sb_half* src = row_of(x, h, b, r0);
-    __syncthreads();
-    if (along_rows) {
-      const int r = threadIdx.x & 63;
-      if (r < n)
-        for (int p = threadIdx.x >> 6; p < x.P; p += 4) tile[r][p] = src[p * x.sP + r * x.sR];
-    } else {
-      for (int r = threadIdx.x >> 5; r < n; r += 8)
-        for (int p = threadIdx.x & 31; p < x.P; p += 32) tile[r][p] = src[p * x.sP + r * x.sR];
+  int n = 0;
+  while (n + 1 < jobs.n && (int)blockIdx.x >= jobs.job[n + 1].first) ++n;
+  const Proj& x = jobs.job[n].x;
+  const int blocks = (x.R + 63) / 64, it = blockIdx.x - jobs.job[n].first, mode = jobs.job[n].mode;
+  const int r0 = it % blocks * 64, h = it / blocks % x.H, b = it / blocks / x.H, rows = min(64, x.R - r0), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int Pp = (x.P + 7) / 8 * 8;
+  const sb_half* src = row_of(x, h, b, r0);
+  if (mode == kPackTwos) {                                    // a warp: 16 rows of four features
+    const int r = (warp & 3) * 16 + (lane & 7) * 2, f = (warp >> 2) * 4 + (lane >> 3);
+    const sb_half* at = src + f * x.sP + r;
+    if (r < rows)
+      for (int p0 = f; p0 < x.P; p0 += 64) {
+        sb_half2 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k, at += 8 * x.sP)
+          if (p0 + k * 8 < x.P) v[k] = *reinterpret_cast<const sb_half2*>(at);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const sb_half* e = reinterpret_cast<const sb_half*>(&v[k]);
+          if (p0 + k * 8 < x.P) tile[r][p0 + k * 8] = e[0];
+          if (p0 + k * 8 < x.P) tile[r + 1][p0 + k * 8] = e[1];
+        }
+      }
+  } else if (mode == kPackRows) {                             // a warp: 16 rows of two features
+    const int r = (warp & 3) * 16 + (lane & 15), f = (warp >> 2) * 2 + (lane >> 4);
+    const sb_half* at = src + f * x.sP + r * x.sR;
+    if (r < rows)
+      for (int p0 = f; p0 < x.P; p0 += 64) {
+        sb_half v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k, at += 4 * x.sP)
+          if (p0 + k * 4 < x.P) v[k] = *at;
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (p0 + k * 4 < x.P) tile[r][p0 + k * 4] = v[k];
+      }
+  } else {                                                    // a warp: 32 features of a row
+    const int f = (warp & 1) * 32 + lane, w = warp >> 1;
+    for (int p = f; p < x.P; p += 64) {
+      const sb_half* at = src + p * x.sP + w * x.sR;
+      sb_half v[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k, at += 4 * x.sR)
+        if (w + k * 4 < rows) v[k] = *at;
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (w + k * 4 < rows) tile[w + k * 4][p] = v[k];
     }
-    __syncthreads();
-    sb_half* d = dst + (((long long)b * x.H + h) * x.R + r0) * Pp;
-    for (int r = threadIdx.x >> 5; r < n; r += 8)
-      for (int p = threadIdx.x & 31; p < x.P; p += 32) d[(long long)r * Pp + p] = tile[r][p];
   }
+  __syncthreads();
+  sb_half* d = jobs.job[n].dst + (((long long)b * x.H + h) * x.R + r0) * Pp;
+  const int pieces = Pp / 8;
+  for (int i = threadIdx.x; i < rows * pieces; i += 256)
+    *reinterpret_cast<uint4*>(d + i * 8) = *reinterpret_cast<const uint4*>(&tile[i / pieces][i % pieces * 8]);
 }
 
 // ---- few queries ------------------------------------------------------------------------------------------------
@@ -387,7 +432,8 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
   }
 }
 
-// One warp per row joins its shares.
+// One warp per row joins its shares: with weights exp(reference - highest reference), sums and outputs add up.  Latency: 4 us for 512 rows
+// of 128 features in two shares.
 template <int P>
 __global__ void __launch_bounds__(128)
 join_splits_kernel(const __grid_constant__ FewParams p) {
@@ -422,8 +468,9 @@ join_splits_kernel(const __grid_constant__ FewParams p) {
 }
 
 // What the backward pass knows of 64 query rows (RelBackward in ops.h), four threads a row, and in the blocks before those the rows
-// of biases.  `vec`: both tensors have unit-stride features in 16-byte pieces; else lanes run along rows.  Everything is
-// asked for before anything is waited for: one trip to memory a block.
+// of biases.  `vec`: both tensors have unit-stride features in 16-byte pieces; else lanes run along rows.  Bound by reading dout and out
+// once (B=96, L=128, 16 heads of 64, 50 MB: 11 us, 70 % of the copy bandwidth), so everything is asked for before anything is
+// waited for: one trip to memory a block (18 us with a barrier before the sums and another trip behind it).
 template <int P>
 __global__ void __launch_bounds__(256)
 row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const __grid_constant__ Expand x, float* records, int vec,
@@ -495,7 +542,8 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
 }
 
 // dtable[n,h] = the head's sums over the relative positions of bucket n; one block each, in a fixed order: lanes along as many
-// positions as the bucket has, up to 32, and along rows of sums beside that.
+// positions as the bucket has, up to 32, and along rows of sums beside that.  Latency: 5 us for 64 rows and 32 buckets of 16 heads (B=8,
+// L=512), 8.6 for 128 rows whose buckets reach 472 positions (B=2, L=4096; 11 with 256 threads).
 __global__ void __launch_bounds__(512)
 table_finish_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const float* partial, int rows, int reach,
                     sb_half* out, long long sN, long long sH) {
@@ -558,19 +606,34 @@ Plan plan_of(std::initializer_list<const Proj*> operands, int heads, const RelBi
   p.bytes += 256;
   return p;
 }
-// x becomes the copy at `at`.
-int pack(cudaStream_t s, void* scratch, size_t at, Proj* x) {
+// x becomes a copy at `at`, which launch_pack() makes.
+void pack(PackJobs* jobs, void* scratch, size_t at, Proj* x) {
   const int Pp = (x->P + 7) / 8 * 8;
   auto mag = [](long long v) { return v < 0 ? -v : v; };
-  sb_half* dst = reinterpret_cast<sb_half*>(reinterpret_cast<char*>(scratch) + at);
-  const long long blocks = (long long)x->H * x->B * ((x->R + 63) / 64);
-  SB_LAUNCH_OK(launch_k(pack_rows_kernel, (unsigned)std::min<long long>(blocks, 8 * usable_sms(device_facts().sms)), 256, 0, s, *x, dst, Pp,
-                        x->R > 1 && mag(x->sR) < mag(x->sP) ? 1 : 0));
-  x->p = dst;
+  auto& j = jobs->job[jobs->n++];
+  j.x = *x;
+  j.dst = reinterpret_cast<sb_half*>(reinterpret_cast<char*>(scratch) + at);
+  j.first = jobs->blocks;
+  j.mode = x->sR == 1 && x->R % 2 == 0 && !((x->sP | x->sH | x->sB) & 1) && !(reinterpret_cast<uintptr_t>(x->p) & 3u) ? kPackTwos
+           : x->R > 1 && mag(x->sR) < mag(x->sP) ? kPackRows : kPackFeatures;
+  jobs->blocks += x->H * x->B * ((x->R + 63) / 64);
+  x->p = j.dst;
   x->sP = 1; x->sR = Pp; x->sH = (long long)Pp * x->R; x->sB = x->sH * x->H;
+}
+int launch_pack(cudaStream_t s, const PackJobs& jobs) {
+  if (jobs.n > 0) SB_LAUNCH_OK(launch_k(pack_rows_kernel, (unsigned)jobs.blocks, 256, 0, s, jobs));
   return SB_OK;
 }
-int direct_or_packed(cudaStream_t s, void* scratch, size_t at, Proj* x) { return rel_direct(*x) ? SB_OK : pack(s, scratch, at, x); }
+// Copies what tensor maps cannot address.
+int pack_indirect(cudaStream_t s, void* scratch, const size_t* at, std::initializer_list<Proj*> operands) {
+  PackJobs jobs;
+  memset(&jobs, 0, sizeof(jobs));
+  for (Proj* x : operands) {
+    if (!rel_direct(*x)) pack(&jobs, scratch, *at, x);
+    ++at;
+  }
+  return launch_pack(s, jobs);
+}
 Expand expansion(void* scratch, const Plan& pl) {
   return {reinterpret_cast<float*>(scratch), pl.pitch, pl.reach, reinterpret_cast<int*>(reinterpret_cast<char*>(scratch) + pl.next)};
 }
@@ -636,8 +699,11 @@ int launch_rel_attn_fwd(cudaStream_t s, void* scratch, Proj q, Proj k, Proj v, c
   AttnArgs a = attn_args(q, k, v, bias, out, lse, span, &st);
   if (few_splits(q, k)) {
     const FewPlan f = few_plan(q, k, v);
-    if (!piecewise(k)) SB_TRY(pack(s, scratch, f.k, &k));
-    if (!piecewise(v)) SB_TRY(pack(s, scratch, f.v, &v));
+    PackJobs jobs;
+    memset(&jobs, 0, sizeof(jobs));
+    if (!piecewise(k)) pack(&jobs, scratch, f.k, &k);
+    if (!piecewise(v)) pack(&jobs, scratch, f.v, &v);
+    SB_TRY(launch_pack(s, jobs));
     FewParams p;
     a.k = k; a.v = v;
     p.a = a;
@@ -655,9 +721,7 @@ int launch_rel_attn_fwd(cudaStream_t s, void* scratch, Proj q, Proj k, Proj v, c
   const Plan pl = plan_of({&q, &k, &v}, q.H, bias);
   const Expand x = expansion(scratch, pl);
   SB_LAUNCH_OK(launch_k(expand_bias_kernel, dim3(expand_blocks(x.pitch), a.H), 256, 0, s, a, st, x));
-  SB_TRY(direct_or_packed(s, scratch, pl.at[0], &q));
-  SB_TRY(direct_or_packed(s, scratch, pl.at[1], &k));
-  SB_TRY(direct_or_packed(s, scratch, pl.at[2], &v));
+  SB_TRY(pack_indirect(s, scratch, pl.at, {&q, &k, &v}));
   return launch_rel_tiles_fwd(s, q, k, v, tables_of(x), x.next, out, lse, span);
 }
 
@@ -694,10 +758,7 @@ int launch_rel_attn_bwd(cudaStream_t s, void* scratch, Proj dout, Proj q, Proj k
   const int expanding = a.H * expand_blocks(x.pitch);
   SB_LAUNCH_OK(launch_k(q.P <= 64 ? row_records_kernel<64> : row_records_kernel<128>, (unsigned)(expanding + a.H * a.B * ((a.J + 63) / 64)), 256, 0, s, a, st, x, records,
                         pieces(dout) && pieces(out) ? 1 : 0, expanding));
-  SB_TRY(direct_or_packed(s, scratch, pl.p.at[0], &dout));
-  SB_TRY(direct_or_packed(s, scratch, pl.p.at[1], &q));
-  SB_TRY(direct_or_packed(s, scratch, pl.p.at[2], &k));
-  SB_TRY(direct_or_packed(s, scratch, pl.p.at[3], &v));
+  SB_TRY(pack_indirect(s, scratch, pl.p.at, {&dout, &q, &k, &v}));
   float* partial = reinterpret_cast<float*>(base + pl.partial);
   SB_TRY(launch_rel_tiles_bwd(s, dout, q, k, v, tables_of(x), RelBackward{records, partial, x.next}, dq, dk, dv, span));
   SB_LAUNCH_OK(launch_k(table_finish_kernel, dim3(a.buckets, a.H), 512, 0, s, a, st, partial, pl.rows, pl.p.reach,
