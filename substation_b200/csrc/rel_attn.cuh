@@ -161,8 +161,8 @@ __device__ __forceinline__ void store_features(sb_half* ptr, long long sP, const
 
 // 32 accumulator columns of a warp's 32 rows -> alpha * value, 16-bit: the first `features` of the first `rows` rows, at
 // ptr[row * sR + feature * sP], by way of 2 KB of shared memory.  Four lanes write 64 bytes of a row; a thread writing its own row
-// meets 32 lines with each instruction, which for short sequences took as long as all the rest (backward at B=96, L=128: 83 -> 77 us);
-// where an item has many tiles the registers that this takes cost more (B=8, L=512: 80 -> 83 us).
+// meets 32 lines with each instruction, which counts where items are short (training at B=96, L=128: 121 us with threads' own rows, 116
+// so); elsewhere the registers that this takes cost more (forward at B=16, L=384: 28.6 -> 29.9 us).
 constexpr int kStoreBytes = 2048;
 __device__ __forceinline__ void store_rows(uint8_t* mem, sb_half* ptr, long long sR, long long sP, const uint32_t* r, float alpha, int features,
                                            int rows, int lane) {

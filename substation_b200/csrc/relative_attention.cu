@@ -141,7 +141,7 @@ pack_rows_kernel(const __grid_constant__ PackJobs jobs) {
 // The rows of a key head are the queries of all heads that share it, J for each.  A CTA takes 16 of them (one mma.sync tile) and a
 // share of the keys; its four warps walk pieces of those keys in turn, each with a ring of its own filled by cp.async (which
 // also puts zeros behind a sequence's end), softmax state and accumulator, joined at the end.  With more than one share, a
-// second kernel joins those.  Bound by reading keys and values once (B=16, 16 heads on 8, 8192 keys of 128 features: 72 us, 87 % of the
+// second kernel joins those.  Bound by reading keys and values once (B=16, 32 heads on 8, 8192 keys of 128 features: 72 us, 87 % of the
 // copy bandwidth); tcgen05's smallest tile would be 64 or 128 rows for the one to 16 there are, and the matrix work here
 // is a few percent of the time.
 constexpr int kFewThreads = 128;
@@ -660,7 +660,7 @@ int few_splits(const Proj& q, const Proj& k) {
   const long long blocks = ((long long)(q.H / k.H) * q.R + 15) / 16, ctas = blocks * k.B * k.H, items = (long long)q.B * q.H * ((q.R + 127) / 128);
   const bool idle = ctas <= 148 && (blocks == 1 || k.R >= 1024);
   if (!idle && ctas * (q.R > 4 ? 2 : 1) > items) return 0;
-  // two CTAs for each of 148 SMs and no more, which would wait for those (16 x 16 heads on 8, 8192 keys of 128 features, 128 CTAs: two
+  // two CTAs for each of 148 SMs and no more, which would wait for those (B=16, 16 heads on 8, 8192 keys of 128 features, 128 CTAs: two
   // shares 87 us, four 97, five 114), at least 256 keys a share
   return (int)std::max<long long>(1, std::min<long long>({296 / ctas, (k.R + 255) / 256, 64}));
 }
