@@ -991,9 +991,10 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       ++syncs;
       return ok;
     };
-    // The group's sums of a query tile to memory.  The rows are left at zero for the next but one such item; with one set it
+    // The group's sums of a query tile to memory, to row `place`: 0 for the item's even tiles, 1 for its odd ones, whichever group had
+    // them (that depends on the items before).  The rows are left at zero for the next but one such item; with one set it
     // is the next one, and everybody has to be done with them.
-    auto flush = [&](const Item& it) {
+    auto flush = [&](const Item& it, int place) {
       const float lo = warp_sum(below), hi = warp_sum(above);
       below = above = 0.f;
       if (lane == 0) {
@@ -1001,7 +1002,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         sums[2 * reach] = hi;
       }
       if (!group_sync()) return;
-      float* out = p.partial + (((long long)it.h * p.c.B * p.nq + (long long)it.b * p.nq + it.t) * 2 + g) * entries;
+      float* out = p.partial + (((long long)it.h * p.c.B * p.nq + (long long)it.b * p.nq + it.t) * 2 + place) * entries;
       for (int i = in_group; i < entries; i += 128) {
         float v = 0.f;
 #pragma unroll
@@ -1021,7 +1022,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       if (w.tiles == 0) {
         store(w, w.kind != 0, 0u, true);
         if (BOTH) store(w, true, 0u, true);
-        if (BOTH || w.kind) flush(w);
+        if (BOTH || w.kind) flush(w, g);
         continue;
       }
       const int r = w.t * 128 + rt;                    // query or key of this thread
@@ -1050,11 +1051,13 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       else lim0 = r < w.keys ? (p.c.causal ? rel0 : -(1 << 30)) : 1 << 30;
       const int lo0 = __shfl_sync(0xffffffffu, rel0, w.kind ? 31 : 0) - (w.kind ? 0 : 63);
       const int tight0 = w.kind ? __reduce_min_sync(0xffffffffu, lim0) : __reduce_max_sync(0xffffffffu, lim0);
+      int place = 0;
       for (int done = 0; done < w.tiles && ok; done += w.each) {
         const float* bias = bias_s + (run & 1u) * p.c.pitch;
         ok = __all_sync(0xffffffffu, mbar_wait(b_full + 8 * (run & 1u), (run >> 1) & 1u, 60));
         // this group's tiles of the run: every second one
         const int skip = (n & 1u) == (uint32_t)g ? 0 : 1;
+        place = skip;
         n += w.each;
         auto advance = [&](uint32_t by) {
           st += by;
@@ -1155,7 +1158,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         finish(prev, live - 1u);
         if (!ok) break;
       }
-      if (BOTH || w.kind) flush(w);
+      if (BOTH || w.kind) flush(w, place);             // (one run, then)
       prev = w;
       have = true;
       ++live;

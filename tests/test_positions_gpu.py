@@ -464,6 +464,26 @@ def test_few_queries_far_behind_the_last_key(P, behind):
     assert ((lse - want['lse']).abs() <= 1e-5 * (1 + want['lse'].abs())).all()
 
 
+@pytest.mark.parametrize('P,J,causal', [(64, 161, False), (128, 161, True), (64, 65, False), (128, 65, True)])
+def test_gradients_are_the_same_each_time(P, J, causal):
+    """Which CTA takes which item changes from call to call, and items of an odd number of tiles change what it does next."""
+    ops = _ops()
+    gen = torch.Generator(device=DEV).manual_seed(J)
+    B, H = 24, 8
+    q, k, v, dout = (_make((P, H, B, J), 'BJHP', torch.float16, gen) for _ in range(4))
+    table = torch.randn(32, H, generator=gen, device=DEV).half()
+    lengths = torch.arange(J - 2 * B, J, 2, dtype=torch.int32, device=DEV)
+    how = dict(buckets=ops.relative_buckets(32, 64, True), scale=P ** -0.5, causal=causal, lengths=lengths)
+    out, lse = torch.empty_like(q), torch.empty(H, B, J, device=DEV)
+    ops.relative_attention(q, k, v, table, out, lse, **how)
+    want = None
+    for _ in range(60):
+        got = [torch.empty_like(x) for x in (q, k, v, table)]
+        ops.backward_relative_attention(dout, q, k, v, table, out, lse, *got, **how)
+        want = want or got
+        assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
 def test_few_queries_agree_with_many():
     """The last queries of a causal sequence, one call for all or a call for the last ones against the cache."""
     ops = _ops()
