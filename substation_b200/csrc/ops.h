@@ -111,6 +111,9 @@ int launch_qk_norm_bwd(cudaStream_t s, void* scratch, Proj dq_out, Proj dk_out, 
 struct RelBias { const void* table; long long sN, sH; int n, bidirectional; const int32_t* starts; };
 struct RelSpan { float scale; int causal; const int* lengths; const int* first; };
 struct RelRows { float* p; long long sH, sB, sJ; };   // float32 [H,B,J]
+// Whether a row met no key, from its sum of exponentials: the key of its maximum adds at least one.  A sum that is not a number
+// came from a score that was none, or infinite, and stays one in the row's results.
+__host__ __device__ __forceinline__ bool sees_none(float sum) { return sum == 0.f; }
 constexpr int kRelMaxBuckets = 512;                   // of one direction
 constexpr int kRelMaxReach = 832;                     // first distance of the last bucket
 constexpr int kRelMaxHead = 128;

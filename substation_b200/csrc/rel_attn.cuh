@@ -573,7 +573,7 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       }
       if (!ok) break;
       sb_half* out = reinterpret_cast<sb_half*>(p.out.p) + (long long)w.h * p.out.sH + (long long)w.b * p.out.sB + (long long)j * p.out.sR;
-      const float inv = state.l > 0.f ? 1.f / state.l : 0.f;
+      const float inv = sees_none(state.l) ? 0.f : 1.f / state.l;
       if (w.tiles > 0) {
         if (lane == 0) mbar_arrive(b_empty + 8 * bb);
         ok = __all_sync(0xffffffffu, mbar_wait(p_free + 8 * ((n - 1u) & 1u), ((n - 1u) >> 1) & 1u, 47));
@@ -594,7 +594,7 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       }
       if (row && p.lse.p)
         p.lse.p[(long long)w.h * p.lse.sH + (long long)w.b * p.lse.sB + (long long)j * p.lse.sJ] =
-            state.l > 0.f ? (state.m + log2f(state.l)) * 0.6931471805599453f : -INFINITY;
+            sees_none(state.l) ? -INFINITY : (state.m + log2f(state.l)) * 0.6931471805599453f;
       if (w.tiles > 0) {
         tc_fence_before();
         __syncwarp();

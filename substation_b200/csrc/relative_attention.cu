@@ -409,13 +409,12 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
 #pragma unroll
     for (int w = 1; w < 4; ++w) mm = fmaxf(mm, sm[w * 16 + r]);
     float sum = 0.f, v = 0.f;
-    if (mm > -INFINITY) {
+    const float ref = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float e = ex2_unit(sm[w * 16 + r] - mm);
-        sum = fmaf(sl[w * 16 + r], e, sum);
-        v = fmaf(so[(w * 16 + r) * P + f], e, v);
-      }
+    for (int w = 0; w < 4; ++w) {
+      const float e = ex2_unit(sm[w * 16 + r] - ref);
+      sum = fmaf(sl[w * 16 + r], e, sum);
+      v = fmaf(so[(w * 16 + r) * P + f], e, v);
     }
     const int h = hk * rep + row / a.J, j = row % a.J;
     if (p.partial) {
@@ -426,8 +425,8 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
         d[P + 1] = sum;
       }
     } else {
-      if (f < a.P) const_cast<sb_half*>(row_of(a.o, h, b, j))[f * a.o.sP] = sb_f2h(sum > 0.f ? v / sum : 0.f);
-      if (f == 0 && a.lse.p) a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] = sum > 0.f ? (mm + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+      if (f < a.P) const_cast<sb_half*>(row_of(a.o, h, b, j))[f * a.o.sP] = sb_f2h(sees_none(sum) ? 0.f : v / sum);
+      if (f == 0 && a.lse.p) a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] = sees_none(sum) ? -INFINITY : (mm + log2f(sum)) * 0.6931471805599453f;
     }
   }
 }
@@ -449,22 +448,22 @@ join_splits_kernel(const __grid_constant__ FewParams p) {
   for (int s = lane; s < p.splits; s += 32) mm = fmaxf(mm, src[s * (P + 2) + P]);
   mm = group_max<32>(mm);
   float sum = 0.f, v[P / 32];
+  const float ref = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
   for (int c = 0; c < P / 32; ++c) v[c] = 0.f;
-  if (mm > -INFINITY)
 #pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
-      const float* d = src + s * (P + 2);
-      const float e = ex2_unit(d[P] - mm);
-      sum = fmaf(d[P + 1], e, sum);
+  for (int s = 0; s < p.splits; ++s) {
+    const float* d = src + s * (P + 2);
+    const float e = ex2_unit(d[P] - ref);
+    sum = fmaf(d[P + 1], e, sum);
 #pragma unroll
-      for (int c = 0; c < P / 32; ++c) v[c] = fmaf(d[c * 32 + lane], e, v[c]);
-    }
+    for (int c = 0; c < P / 32; ++c) v[c] = fmaf(d[c * 32 + lane], e, v[c]);
+  }
   sb_half* out = const_cast<sb_half*>(row_of(a.o, h, b, j));
 #pragma unroll
   for (int c = 0; c < P / 32; ++c)
-    if (c * 32 + lane < a.P) out[(c * 32 + lane) * a.o.sP] = sb_f2h(sum > 0.f ? v[c] / sum : 0.f);
-  if (lane == 0 && a.lse.p) a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] = sum > 0.f ? (mm + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    if (c * 32 + lane < a.P) out[(c * 32 + lane) * a.o.sP] = sb_f2h(sees_none(sum) ? 0.f : v[c] / sum);
+  if (lane == 0 && a.lse.p) a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] = sees_none(sum) ? -INFINITY : (mm + log2f(sum)) * 0.6931471805599453f;
 }
 
 // What the backward pass knows of 64 query rows (RelBackward in ops.h), four threads a row, and in the blocks before those the rows
