@@ -258,6 +258,21 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return d;
 }
 
+// Largest magnitudes of pairs of 16-bit numbers; a NaN is passed over.
+__device__ __forceinline__ sb_half2 half2_of(uint32_t u) { return *reinterpret_cast<const sb_half2*>(&u); }
+__device__ __forceinline__ sb_half2 larger(sb_half2 m, const uint4& u) {
+  const sb_half2 a = __hmax2(__habs2(half2_of(u.x)), __habs2(half2_of(u.y))), b = __hmax2(__habs2(half2_of(u.z)), __habs2(half2_of(u.w)));
+  return __hmax2(m, __hmax2(a, b));
+}
+__device__ __forceinline__ float larger_half(sb_half2 m) {
+  const float2 f = sb_h22f2(m);
+  return fmaxf(f.x, f.y);
+}
+__device__ __forceinline__ float finite_size(sb_half2 m) {   // 0 beside an infinity
+  const float f = larger_half(m);
+  return f < INFINITY ? f : 0.f;
+}
+
 // ---- 8-element accessors -------------------------------------------------
 __device__ __forceinline__ void unpack8(const uint4& u, float v[8]) {
   const sb_half2* h = reinterpret_cast<const sb_half2*>(&u);

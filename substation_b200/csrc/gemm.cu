@@ -1671,10 +1671,9 @@ int launch_rel_tiles_bwd(cudaStream_t s, Proj dout, Proj q, Proj k, Proj v, RelT
   p.first_q = k.H * k.B * p.nk;
   p.items = p.first_q + q.H * q.B * p.nq;
   p.scale = span.scale;
-  p.records = w.records; p.partial = w.partial; p.next = w.next;
+  p.records = w.records; p.sizes = w.sizes; p.partial = w.partial; p.next = w.next;
   p.dq = dq; p.dk = dk; p.dv = dv;
-  // Units of one tile each way give all three gradients in one item; with shared key heads dQ would have to be stored per head.
-  const bool both = q.P <= 64 && p.nq == 1 && p.nk == 1 && q.H == k.H;
+  const bool both = rel_both(q, k);
   if (both) p.items = p.first_q;
   return both ? rel_bwd<64, true>(s, m, p) : q.P <= 64 ? rel_bwd<64, false>(s, m, p) : rel_bwd<128, false>(s, m, p);
 }

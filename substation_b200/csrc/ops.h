@@ -123,10 +123,22 @@ struct RelTables { const float* rows; int pitch, reach; };
 bool rel_direct(const Proj& x);
 // The tcgen05 kernels; q, k, v are rel_direct.  `next`: a zero in device memory.
 int launch_rel_tiles_fwd(cudaStream_t s, Proj q, Proj k, Proj v, RelTables t, int* next, Proj out, RelRows lse, const RelSpan& span);
+// Whether what the backward pass rounds to 16 bits, softmax weights and score gradients, is multiplied by a power of two first.
+// float16 has few exponents: a weight of one in 4096 and an output gradient of 1e-3 make a score gradient among its smallest steps,
+// and output gradients of 1e4 one beyond its largest.
+#ifdef SB_BF16
+constexpr bool kRelScaled = false;
+#else
+constexpr bool kRelScaled = true;
+#endif
 // Backward: `records` [B][H][ceil(J / 64)][192]: of 64 query rows the log-sum-exps in units of log2 (+inf: row without keys, or
-// none), D and the weight (0 or 1) of the row in the table's sums; `partial` [H][B * ceil(J / 128) * 2][2 * reach + 1] sums of
-// score gradients by relative position; `next`: a zero.
-struct RelBackward { const float* records; float* partial; int* next; };
+// none), D and the weight (0 or 1) of the row in the table's sums; `sizes` (kRelScaled): for 64 rows of dout,
+// [B][H][ceil(J / 64)], then, but for rel_both, of v, [B][G][ceil(K / 64)], eight numbers whose largest is the largest
+// magnitude, not counting rows without keys, behind the length or with an infinity, and no NaN; `partial` [H][B * ceil(J / 128) * 2][2 * reach + 1]
+// sums of score gradients by relative position; `next`: a zero.
+struct RelBackward { const float* records; const float* sizes; float* partial; int* next; };
+// Units of one tile each way give all three gradients in one item; with shared key heads dQ would have to be stored per head.
+inline bool rel_both(const Proj& q, const Proj& k) { return q.P <= 64 && q.R <= 128 && k.R <= 128 && q.H == k.H; }
 int launch_rel_tiles_bwd(cudaStream_t s, Proj dout, Proj q, Proj k, Proj v, RelTables t, RelBackward w, Proj dq, Proj dk, Proj dv,
                          const RelSpan& span);
 size_t rel_attn_scratch_bytes(const Proj& q, const Proj& k, const Proj& v, const RelBias& bias);

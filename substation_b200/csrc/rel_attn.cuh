@@ -613,7 +613,8 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------
-constexpr int kBwdThreads = 352;                     // producer warp, two MMA warps, two groups of four element warps
+// producer warp, two MMA warps, two groups of four element warps, and in float16 a warp that puts the items' shifts into their biases
+constexpr int kBwdThreads = kRelScaled ? 384 : 352;
 constexpr int kRecord = 192;                         // floats of 64 query rows: log2-sum-exps, D, weights of the table's sums
 
 struct BwdParams {
@@ -625,6 +626,7 @@ struct BwdParams {
   int sets;                                          // rows of sums per warp (1 or 2)
   float scale;
   const float* records;                              // [B][H][ceil(J / 64)][kRecord]
+  const float* sizes;                                // [B][H][ceil(J / 64)][8], but for BOTH [B][G][ceil(K / 64)][8]
   float* partial;                                    // [H][B * nq * 2][2 * reach + 1]
   int* next;                                         // work queue
   Proj dq, dk, dv;
@@ -659,6 +661,30 @@ __device__ __forceinline__ Item bwd_item(const BwdParams& p, int i) {
   return it;
 }
 
+// float16: an item's score gradients are rounded to 16 bits times 2^shift, its softmax weights times 2^max(shift, 0), which results lose
+// again.  A weight w is at most one, so that a shift of at most 15 keeps it.  A score gradient is w (dP - D), a difference of values of
+// dP, which are at most N = P max|dout| max|v| in size, times w (1 - w): at most N / 2.  Times 2^16 over the next power of two from N on
+// that is at most 2^15.  The maxima are of all rows that the item meets (dK and dV sum over them, so they share a factor).
+
+// The largest of n magnitudes, as the lane finds it.
+__device__ __forceinline__ float largest_of(const float* at, int n, int lane) {
+  float m = 0.f;
+#pragma unroll 1
+  for (int i = lane; i < n; i += 128) {
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = i + 32 * k < n ? at[i + 32 * k] : 0.f;
+    m = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), m);
+  }
+  return m;
+}
+__device__ __forceinline__ int item_shift(float g, float v, int P) {
+  const uint32_t mg = __reduce_max_sync(0xffffffffu, __float_as_uint(g)), mv = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+  const float n = __uint_as_float(mg) * __uint_as_float(mv) * (float)P;   // (of float16's numbers: 0, or from 2^-48 to 2^39)
+  return n > 0.f ? min(15, 142 - (int)(__float_as_uint(n) >> 23)) : 15;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
 // BOTH: units of one tile of queries and one of keys, each key head with one query head: an item gives all three gradients and
 // everything is computed once.  dQ needs score gradients with the keys as the summed index, so they go to shared memory as
 // well ([128 keys x 128 queries], 32 KB).
@@ -672,7 +698,7 @@ struct BwdCfg {
   static constexpr int kBuf = P == 64 && !BOTH ? 3 : 2;
   static constexpr uint32_t kAcc = P == 64 ? 384 : 256, kAccQ = 256;
   static constexpr int smem(int stages, int held, int sets, int pitch, int reach) {
-    return held * kHeld + stages * kStage + kStaged + (BOTH ? 8 * kStoreBytes : 0) + 2 * pitch * 4 + sets * 8 * ((2 * reach + 4) & ~3) * 4 + 1024 + 400 + 48 * kSlots;
+    return held * kHeld + stages * kStage + kStaged + (BOTH ? 8 * kStoreBytes : 0) + 2 * pitch * 4 + sets * 8 * ((2 * reach + 4) & ~3) * 4 + 1024 + 400 + 48 * kSlots + 32;
   }
 };
 
@@ -681,9 +707,10 @@ struct BwdCfg {
 // What differs between the two kinds of items: in key tiles (KEYS) a thread is a key, log-sum-exps and D change along columns
 // (L, D in shared memory), visible columns are c >= lim; in query tiles a thread is a query and visible columns are c < lim.
 // `emit` gets every score gradient, `block` is told after each 32 columns; `staged`: where the row goes in shared memory too.
+// In masked tiles of keys score gradients are times `gf`, which their weights are not.
 template <bool KEYS, bool NEAR, bool MASK, class Emit, class Block>
 __device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float flat, const float* L, const float* D, float lse, float dsum,
-                                          int lim, float c2, Emit&& emit, Block&& block, uint8_t* staged = nullptr, int row7 = 0) {
+                                          int lim, float c2, Emit&& emit, Block&& block, uint8_t* staged = nullptr, int row7 = 0, float gf = 1.f) {
   const float2 c22 = make_float2(c2, c2), minus = make_float2(-1.f, -1.f);
 #pragma unroll 1
   for (int c = 0; c < 2; ++c) {
@@ -709,6 +736,7 @@ __device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float fl
         pr.x = attn::ex2_approx(pr.x);
         pr.y = attn::ex2_approx(pr.y);
         float2 ds = mul2(pr, fma2(d, minus, pair(g, i)));
+        if (kRelScaled && KEYS && MASK) ds = mul2(ds, make_float2(gf, gf));
         if (MASK) {
           const bool seen0 = KEYS ? col >= lim : col < lim, seen1 = KEYS ? col + 1 >= lim : col + 1 < lim;
           pr = make_float2(seen0 ? pr.x : 0.f, seen1 ? pr.y : 0.f);
@@ -728,6 +756,61 @@ __device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float fl
         *reinterpret_cast<uint4*>(staged + (((c * 4 + v) ^ row7) << 4)) = make_uint4(dm[4 * v], dm[4 * v + 1], dm[4 * v + 2], dm[4 * v + 3]);
     }
     block(c);
+  }
+}
+
+// float16: the warp that finds the items' shifts.  Added to the biases of a key item they make its exponentials 2^shift times as large.
+// A CTA's first item waits for that (and for every line of this code to be fetched, which is why it is short), later ones do not.  All
+// that float16 has for its range, this warp and the sizes that row_records_kernel finds, takes 5.5 us of a forward and backward call at
+// B=8, L=512 (108.9 -> 114.4), as many at B=96, L=128 (115.4 -> 120.9) and 3 at B=2, L=4096 (884 -> 887).
+struct ShiftWarp {
+  const uint8_t *slots, *held;
+  float4* biases;                                    // two rows
+  int* shifts;                                       // of the last four items with tiles
+  uint32_t item_full, item_empty, h_full, b_full, b_ready;
+};
+template <int P, bool BOTH>
+__device__ __forceinline__ void shift_warp(const BwdParams& p, const ShiftWarp& s) {
+  const int lane = threadIdx.x & 31, rep = p.c.H / p.c.G, blocks = (p.c.J + 63) >> 6, blocks_v = (p.c.K + 63) >> 6;
+  uint32_t taken = 0, live = 0, run = 0;
+  bool ok = true;
+  Item w;
+  while (ok && take_item(s.slots, s.item_full, s.item_empty, &taken, lane, &w, &ok)) {
+    if (w.tiles == 0) continue;
+    const float mg = largest_of(p.sizes + 8 * (((long long)w.b * p.c.H + (w.kind ? w.h : w.h * rep)) * blocks + (w.kind ? 2 * w.t : 0)),
+                                8 * (w.kind ? min(2, blocks - 2 * w.t) : rep * blocks), lane);
+    float mv = 0.f;
+    if (BOTH) {                                      // the held values, 16 bytes at a time
+      const uint32_t hb = p.held == 2 ? live & 1u : 0u, hp = p.held == 2 ? live >> 1 : live;
+      ok = __all_sync(0xffffffffu, mbar_wait(s.h_full + 8 * hb, hp & 1u, 63));
+      if (!ok) return;
+      const uint4* tile = reinterpret_cast<const uint4*>(s.held + hb * BwdCfg<P, BOTH>::kHeld + 256 * P);
+#pragma unroll 2
+      for (int i = lane; i < w.keys * 8; i += 32) mv = fmaxf(mv, finite_size(larger(half2_of(0u), tile[i])));
+    } else {
+      mv = largest_of(p.sizes + 8 * ((long long)p.c.B * p.c.H * blocks + ((long long)w.b * p.c.G + (w.kind ? w.h / rep : w.h)) * blocks_v),
+                      8 * ((w.keys + 63) >> 6), lane);
+    }
+    const int shift = item_shift(mg, mv, p.c.P);
+    for (int done = 0; done < w.tiles; done += w.each, ++run) {
+      ok = __all_sync(0xffffffffu, mbar_wait(s.b_full + 8 * (run & 1u), (run >> 1) & 1u, 63));
+      if (!ok) return;
+      // (four items before, whose place this is: its results were stored before the run but one before this began)
+      if (lane == 0 && done == 0) s.shifts[live & 3u] = shift;
+      if (!w.kind) {                                 // (query items have the log-sum-exps in registers)
+        float4* row = s.biases + (run & 1u) * (p.c.pitch / 4);
+        const float add = (float)max(shift, 0);
+#pragma unroll 1
+        for (int i = lane; i < p.c.pitch / 4; i += 32) {
+          const float4 v = row[i];
+          row[i] = make_float4(v.x + add, v.y + add, v.z + add, v.w + add);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s.b_ready + 8 * (run & 1u));
+    }
+    ++live;
   }
 }
 
@@ -761,14 +844,15 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
   uint8_t* gen = smem_raw + (sheld - raw);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (bars + 320 - sheld));
   uint8_t* slots = gen + (bars + 400 - sheld);
-  const uint32_t g_sync = bars + 352, buf_free = bars + 368, q_free = bars + 392;
+  const uint32_t g_sync = bars + 352, buf_free = bars + 368, q_free = bars + 392, b_ready = kRelScaled ? bars + 400 + 48 * kSlots : b_full;
+  int* shifts = reinterpret_cast<int*>(slots + 48 * kSlots + 16);   // of the last four items with tiles
   const float* bias_s = reinterpret_cast<const float*>(gen + (sbias - sheld));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(item_full + 8 * i, 1);
-      mbar_init(item_empty + 8 * i, 10);
+      mbar_init(item_empty + 8 * i, kBwdThreads / 32 - 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(h_full + 8 * i, 1);
@@ -776,6 +860,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       mbar_init(b_full + 8 * i, 1);
       mbar_init(b_empty + 8 * i, 8);
       mbar_init(g_sync + 8 * i, 4);
+      if (kRelScaled) mbar_init(b_ready + 8 * i, 1);
     }
     for (int i = 0; i < Cfg::kBuf; ++i) {
       mbar_init(s_full + 8 * i, 1);
@@ -930,6 +1015,8 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       }
       ++live;
     }
+  } else if (kRelScaled && warp == 11) {
+    shift_warp<P, BOTH>(p, ShiftWarp{slots, gen, reinterpret_cast<float4*>(gen + (sbias - sheld)), shifts, item_full, item_empty, h_full, b_full, b_ready});
   } else {
     // ---------------- element warps ----------------
     const int q = warp & 3, g = (warp - 3) >> 2, rt = q * 32 + lane;
@@ -943,12 +1030,15 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     bool ok = true, have = false;
     Item prev;
     float below = 0.f, above = 0.f;                    // sums outside the varying part of the bias
-    // An item's results: dK (group 0) and dV (group 1) of a key, or dQ of a query, 32 features in turn.
-    auto store = [&](const Item& it, bool queries, uint32_t acc, bool zero) {
+    // What undoes the shift of the `n`-th item's score gradients, and of its weights.
+    auto unshift = [&](uint32_t n) { return kRelScaled ? power_of_two(-shifts[n & 3u]) : 1.f; };
+    auto unshift_weights = [&](uint32_t n) { return kRelScaled ? power_of_two(-max(shifts[n & 3u], 0)) : 1.f; };
+    // The `n`-th item's results: dK (group 0) and dV (group 1) of a key, or dQ of a query, 32 features in turn.
+    auto store = [&](const Item& it, bool queries, uint32_t acc, bool zero, uint32_t n) {
       const int r = it.t * 128 + rt;
       const Proj& o = queries ? p.dq : g ? p.dv : p.dk;
       sb_half* out = reinterpret_cast<sb_half*>(o.p) + (long long)it.h * o.sH + (long long)it.b * o.sB + (long long)r * o.sR;
-      const float f = queries || !g ? p.scale : 1.f;
+      const float f = zero ? 0.f : queries || !g ? p.scale * unshift(n) : unshift_weights(n);
 #pragma unroll 1
       for (int c = queries ? g : 0; c < P / 32; c += queries ? 2 : 1) {
         uint32_t v[32];
@@ -970,8 +1060,8 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       ok = __all_sync(0xffffffffu, mbar_wait(acc_full, s & 1u, 59));
       if (!ok) return;
       tc_fence_after();
-      store(it, it.kind != 0, tmem + Cfg::kAcc, false);
-      if (BOTH) store(it, true, tmem + Cfg::kAccQ, false);
+      store(it, it.kind != 0, tmem + Cfg::kAcc, false, s);
+      if (BOTH) store(it, true, tmem + Cfg::kAccQ, false, s);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(acc_empty);
@@ -994,7 +1084,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     // The group's sums of a query tile to memory, to row `place`: 0 for the item's even tiles, 1 for its odd ones, whichever group had
     // them (that depends on the items before).  The rows are left at zero for the next but one such item; with one set it
     // is the next one, and everybody has to be done with them.
-    auto flush = [&](const Item& it, int place) {
+    auto flush = [&](const Item& it, int place, float factor) {
       const float lo = warp_sum(below), hi = warp_sum(above);
       below = above = 0.f;
       if (lane == 0) {
@@ -1010,7 +1100,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
           v += group_sums[w * width + i];
           group_sums[w * width + i] = 0.f;
         }
-        out[i] = v;
+        out[i] = v * factor;
       }
       group_sums += other_set;
       sums += other_set;
@@ -1020,9 +1110,9 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
     Item w;
     while (ok && take(&w, &ok)) {
       if (w.tiles == 0) {
-        store(w, w.kind != 0, 0u, true);
-        if (BOTH) store(w, true, 0u, true);
-        if (BOTH || w.kind) flush(w, g);
+        store(w, w.kind != 0, 0u, true, 0u);
+        if (BOTH) store(w, true, 0u, true, 0u);
+        if (BOTH || w.kind) flush(w, g, 1.f);
         continue;
       }
       const int r = w.t * 128 + rt;                    // query or key of this thread
@@ -1054,7 +1144,8 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       int place = 0;
       for (int done = 0; done < w.tiles && ok; done += w.each) {
         const float* bias = bias_s + (run & 1u) * p.c.pitch;
-        ok = __all_sync(0xffffffffu, mbar_wait(b_full + 8 * (run & 1u), (run >> 1) & 1u, 60));
+        ok = __all_sync(0xffffffffu, mbar_wait(b_ready + 8 * (run & 1u), (run >> 1) & 1u, 60));
+        if (kRelScaled && w.kind) lse -= (float)shifts[live & 3u];   // (one run)
         // this group's tiles of the run: every second one
         const int skip = (n & 1u) == (uint32_t)g ? 0 : 1;
         place = skip;
@@ -1067,6 +1158,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         };
         if (skip) advance(1);
         int rel = rel0 + skip * step, lo = lo0 + skip * step, lim = lim0 - skip * moves, tight = tight0 - skip * moves, i = skip;
+        if (kRelScaled && !w.kind && shifts[live & 3u] < 0) tight = 1 << 29;   // (score gradients with a factor of their own: masked tiles)
         for (; i < w.each && ok; i += 2) {
           const bool near = lo + 94 > -reach && lo < reach;
           // outside the varying part, a place in the row where the 64 entries in use have the end's value
@@ -1100,6 +1192,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
             }
           } else {
             const float* L = reinterpret_cast<const float*>(gen + (ring - sheld) + st * Cfg::kStage + Cfg::kStream);
+            auto smaller = [&] { return kRelScaled ? power_of_two(min(shifts[live & 3u], 0)) : 1.f; };
             if (BOTH) {
               // the diagonals of a block run the other way: lane l gets those of key - query = l and l - 32
               float up = 0.f, down = 0.f;
@@ -1123,13 +1216,13 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
                 if (!ok) break;
               }
               uint8_t* row = gen + (staged - sheld) + i * 16384 + rt * 128;
-              if (tight > 0 || some) turn_tile<true, true, true>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, weigh, next, row, rt & 7);
+              if (tight > 0 || some) turn_tile<true, true, true>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, weigh, next, row, rt & 7, smaller());
               else turn_tile<true, true, false>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, sum, block, row, rt & 7);
               asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             } else {
               auto none = [](int, float) {};
               auto after = [](int) {};
-              if (tight > 0) turn_tile<true, true, true>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
+              if (tight > 0) turn_tile<true, true, true>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after, nullptr, 0, smaller());
               else if (near) turn_tile<true, true, false>(ts, bp, 0.f, L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
               else turn_tile<true, false, false>(ts, bp, bp[0], L, L + 64, 0.f, 0.f, lim, p.c.c2, none, after);
             }
@@ -1158,7 +1251,7 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
         finish(prev, live - 1u);
         if (!ok) break;
       }
-      if (BOTH || w.kind) flush(w, place);             // (one run, then)
+      if (BOTH || w.kind) flush(w, place, unshift(live));   // (one run, then)
       prev = w;
       have = true;
       ++live;

@@ -467,14 +467,29 @@ join_splits_kernel(const __grid_constant__ FewParams p) {
 }
 
 // What the backward pass knows of 64 query rows (RelBackward in ops.h), four threads a row, and in the blocks before those the rows
-// of biases.  `vec`: both tensors have unit-stride features in 16-byte pieces; else lanes run along rows.  Bound by reading dout and out
-// once (B=96, L=128, 16 heads of 64, 50 MB: 11 us, 70 % of the copy bandwidth), so everything is asked for before anything is
-// waited for: one trip to memory a block (18 us with a barrier before the sums and another trip behind it).
+// of biases.  `vec`, `vec_v`: dout and out, and v, have unit-stride features in 16-byte pieces; else lanes run along rows.  Bound by
+// reading dout and out once (B=96, L=128, 16 heads of 64, 50 MB: 11 us, 70 % of the copy bandwidth), so everything is asked for before
+// anything is waited for: one trip to memory a block (18 us with a barrier before the sums and another trip behind it).  The sizes of
+// v, float16 only, are shared out to the same blocks, so that they are under way beside the rest; maxima go out per warp, without a barrier
+// (2 us less at B=96).
+__device__ __forceinline__ float sum_of_four(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+__device__ __forceinline__ float largest_of_four(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+// The largest of a warp's values, none negative, to the warp's place; what is not finite does not count.
+__device__ __forceinline__ void store_largest(float value, float* to) {
+  const uint32_t most = __reduce_max_sync(0xffffffffu, value < INFINITY ? __float_as_uint(value) : 0u);
+  if ((threadIdx.x & 31) == 0) to[threadIdx.x >> 5] = __uint_as_float(most);
+}
 template <int P>
 __global__ void __launch_bounds__(256)
-row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const __grid_constant__ Expand x, float* records, int vec,
-                   int expanding) {
-  __shared__ float part[4][64];
+row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const __grid_constant__ Expand x, float* records, float* sizes,
+                   int vec, int vec_v, int expanding, int values) {
+  __shared__ float part[4][64], large[4][64];
   grid_dependency_sync();
   const int it = (int)blockIdx.x - expanding;
   if (it < 0) {
@@ -488,7 +503,7 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
   const bool live = j < a.J;
   const sb_half* g = row_of(a.g, h, b, live ? j : 0);
   const sb_half* o = row_of(a.o, h, b, live ? j : 0);
-  uint4 gv[P / 32], ov[P / 32];
+  uint4 gv[P / 32], ov[P / 32], vv[P / 32];
   if (vec)
 #pragma unroll
     for (int c = 0; c < P / 32; ++c) {
@@ -499,6 +514,27 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
         ov[c] = *reinterpret_cast<const uint4*>(o + p);
       }
     }
+  // the n-th 64 rows of v: this thread's part of its row, zeros behind the length
+  const int vrow = vec_v ? threadIdx.x >> 2 : threadIdx.x & 63, vi = vec_v ? threadIdx.x & 3 : threadIdx.x >> 6, blocks_v = (a.K + 63) / 64;
+  struct Rows { const sb_half* at; float* to; };             // at: null behind the length
+  auto rows_of_v = [&](int n) {
+    const int hk = n % a.G, bv = n / a.G / blocks_v, k = n / a.G % blocks_v * 64 + vrow;
+    return Rows{k < keys_of(a, bv) ? row_of(a.v, hk, bv, k) : nullptr,
+                sizes + ((long long)a.B * a.H * blocks + ((long long)bv * a.G + hk) * blocks_v + n / a.G % blocks_v) * 8};
+  };
+  auto load_v = [&](const sb_half* at) {
+#pragma unroll
+    for (int c = 0; c < P / 32; ++c) {
+      const int p = vi * 8 + c * 32;
+      vv[c] = make_uint4(0u, 0u, 0u, 0u);
+      if (at && p < a.P) vv[c] = *reinterpret_cast<const uint4*>(at + p);
+    }
+  };
+  Rows rv = {nullptr, nullptr};
+  if (kRelScaled && it < values) {
+    rv = rows_of_v(it);
+    if (vec_v) load_v(rv.at);
+  }
   float lse = 0.f;
   int n = 0, pos = 0;
   if (i == 0) {
@@ -506,7 +542,7 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
     n = keys_of(a, b);
     pos = first_of(a, b) + j;
   }
-  float sum = 0.f;
+  float sum = 0.f, size = 0.f;
   if (vec) {
 #pragma unroll
     for (int c = 0; c < P / 32; ++c) {
@@ -516,14 +552,27 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = fmaf(u[e], v[e], sum);
     }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    sum = sum_of_four(sum);
+    if (kRelScaled) {
+      sb_half2 m = half2_of(0u);
+#pragma unroll
+      for (int c = 0; c < P / 32; ++c) m = larger(m, gv[c]);
+      size = largest_of_four(larger_half(m));
+    }
   } else {
 #pragma unroll 4
-    for (int p = i; p < a.P; p += 4) sum = fmaf(sb_h2f(g[p * a.g.sP]), sb_h2f(o[p * a.o.sP]), sum);
+    for (int p = i; p < a.P; p += 4) {
+      const float u = sb_h2f(g[p * a.g.sP]);
+      sum = fmaf(u, sb_h2f(o[p * a.o.sP]), sum);
+      if (kRelScaled) size = fmaxf(size, fabsf(u));
+    }
     part[i][row] = sum;
+    if (kRelScaled) large[i][row] = size;
     __syncthreads();
-    if (i == 0) sum = (part[0][row] + part[1][row]) + (part[2][row] + part[3][row]);
+    if (i == 0) {
+      sum = (part[0][row] + part[1][row]) + (part[2][row] + part[3][row]);
+      if (kRelScaled) size = fmaxf(fmaxf(large[0][row], large[1][row]), fmaxf(large[2][row], large[3][row]));
+    }
   }
   if (i == 0) {
     if (a.causal) n = max(0, min(n, pos + 1));
@@ -537,6 +586,31 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
     r[0] = live && lse != -INFINITY ? lse * 1.4426950408889634f : INFINITY;
     r[64] = live ? sum : 0.f;
     r[128] = live && alike ? 0.f : 1.f;
+  }
+  if (kRelScaled) {
+    store_largest(i == 0 && live && lse != -INFINITY ? size : 0.f, sizes + (((long long)b * a.H + h) * blocks + block) * 8);
+    for (int m = it; m < values; m += (int)gridDim.x - expanding) {
+      if (m != it) {
+        rv = rows_of_v(m);
+        if (vec_v) load_v(rv.at);
+      }
+      float s = 0.f;
+      if (vec_v) {
+        sb_half2 m2 = half2_of(0u);
+#pragma unroll
+        for (int c = 0; c < P / 32; ++c) m2 = larger(m2, vv[c]);
+        s = largest_of_four(larger_half(m2));
+      } else {
+        if (rv.at)
+#pragma unroll 4
+          for (int p = vi; p < a.P; p += 4) s = fmaxf(s, fabsf(sb_h2f(rv.at[p * a.v.sP])));
+        __syncthreads();                                     // (`large` may still be read)
+        large[vi][vrow] = s;
+        __syncthreads();
+        s = vi == 0 ? fmaxf(fmaxf(large[0][vrow], large[1][vrow]), fmaxf(large[2][vrow], large[3][vrow])) : 0.f;
+      }
+      store_largest(s, rv.to);
+    }
   }
 }
 
@@ -726,13 +800,15 @@ int launch_rel_attn_fwd(cudaStream_t s, void* scratch, Proj q, Proj k, Proj v, c
 
 namespace {
 // and for the backward pass records and sums
-struct BwdPlan { Plan p; size_t records, partial, bytes; int rows; };
+struct BwdPlan { Plan p; size_t records, sizes, partial, bytes; int rows; };
 BwdPlan bwd_plan(const Proj& dout, const Proj& q, const Proj& k, const Proj& v, const RelBias& bias) {
   BwdPlan b;
   b.p = plan_of({&dout, &q, &k, &v}, q.H, bias);
   b.rows = q.B * ((q.R + 127) / 128) * 2;
   b.records = b.p.bytes;
-  b.partial = b.records + align256(sizeof(float) * 192 * (size_t)q.H * q.B * ((q.R + 63) / 64));
+  const size_t blocks = (size_t)q.H * q.B * ((q.R + 63) / 64), blocks_v = (size_t)v.H * v.B * ((v.R + 63) / 64);
+  b.sizes = b.records + align256(sizeof(float) * 192 * blocks);
+  b.partial = b.sizes + (kRelScaled ? align256(sizeof(float) * 8 * (blocks + blocks_v)) : 0);
   b.bytes = b.partial + align256(sizeof(float) * (size_t)q.H * b.rows * (2 * b.p.reach + 1));
   return b;
 }
@@ -754,12 +830,13 @@ int launch_rel_attn_bwd(cudaStream_t s, void* scratch, Proj dout, Proj q, Proj k
     return x.sP == 1 && x.P % 8 == 0 && !((x.sH | x.sB | x.sR) & 7) && !(reinterpret_cast<uintptr_t>(x.p) & 15u);
   };
   float* records = reinterpret_cast<float*>(base + pl.records);
-  const int expanding = a.H * expand_blocks(x.pitch);
+  float* sizes = reinterpret_cast<float*>(base + pl.sizes);
+  const int expanding = a.H * expand_blocks(x.pitch), values = kRelScaled && !rel_both(q, k) ? a.G * a.B * ((a.K + 63) / 64) : 0;
   SB_LAUNCH_OK(launch_k(q.P <= 64 ? row_records_kernel<64> : row_records_kernel<128>, (unsigned)(expanding + a.H * a.B * ((a.J + 63) / 64)), 256, 0, s, a, st, x, records,
-                        pieces(dout) && pieces(out) ? 1 : 0, expanding));
+                        sizes, pieces(dout) && pieces(out) ? 1 : 0, pieces(v) ? 1 : 0, expanding, values));
   SB_TRY(pack_indirect(s, scratch, pl.p.at, {&dout, &q, &k, &v}));
   float* partial = reinterpret_cast<float*>(base + pl.partial);
-  SB_TRY(launch_rel_tiles_bwd(s, dout, q, k, v, tables_of(x), RelBackward{records, partial, x.next}, dq, dk, dv, span));
+  SB_TRY(launch_rel_tiles_bwd(s, dout, q, k, v, tables_of(x), RelBackward{records, sizes, partial, x.next}, dq, dk, dv, span));
   SB_LAUNCH_OK(launch_k(table_finish_kernel, dim3(a.buckets, a.H), 512, 0, s, a, st, partial, pl.rows, pl.p.reach,
                         reinterpret_cast<sb_half*>(dtable), dt_sN, dt_sH));
   return SB_OK;

@@ -1,5 +1,5 @@
 """Position operators on the GPU at the ends of their ranges, against float64 and against themselves: NaN and infinity inside a
-sequence."""
+sequence, gradients of any size."""
 
 import pytest
 import torch
@@ -72,3 +72,127 @@ def test_gradients_of_a_query_that_is_nan(dtype):
         hit[:, 1, 1, J - 1] = True
         assert torch.equal(got[0].isnan(), hit), case
         assert got[1][:, 1 // (H // G), 1].isnan().all() and not got[1][:, :, 0].isnan().any(), case
+
+
+# ---- gradients of any size ---------------------------------------------------------------------------------------------
+F32 = 1e-5                # as in position_reference
+
+
+def _gradients(q, k, v, table, buckets, scale, causal, dout, used, h):
+    """float64 gradients, and for dq, dk and dv the variance that roundings give each element: a rounding to 16 bits is uniform
+    within half a step, at most h |x| (or 2^-25, half of float16's smallest step), of variance (h x)^2 / 3, and roundings are
+    independent of one another.  Exponentials and score gradients are rounded once, results once; 32-bit sums count with F32 of
+    their terms' sizes.  What the rounded output adds through D is returned by itself: it is known."""
+    P, H, B, J = q.shape
+    G, K = k.shape[1], k.shape[3]
+    rep = H // G
+    q, k, v, g = q.double(), k.double(), v.double(), dout.double()
+    kk, vv = k.repeat_interleave(rep, 1), v.repeat_interleave(rep, 1)
+    rel = torch.arange(K, device=DEV) - torch.arange(J, device=DEV)[:, None]
+    lookup = torch.tensor([buckets.bucket(r) for r in range(1 - J, K)], device=DEV)
+    s = scale * torch.einsum('phbj,phbk->hbjk', q, kk) + table.double()[lookup[rel + J - 1]].permute(2, 0, 1)[:, None]
+    if causal:
+        s = s.masked_fill(rel > 0, -float('inf'))
+    p = s.softmax(-1)
+    out = torch.einsum('hbjk,phbk->phbj', p, vv)
+    dp = torch.einsum('phbj,phbk->hbjk', g, vv)
+    ds = p * (dp - (g * out).sum(0)[..., None])
+    size = (g.abs() * out.abs()).sum(0)[..., None] + torch.einsum('phbj,phbk->hbjk', g.abs(), vv.abs())
+    var = (h * ds) ** 2 / 3 + (F32 * p * size) ** 2
+    via_d = -p * (g * (used.double() - out)).sum(0)[..., None]
+    fold = lambda x: x.unflatten(1, (G, rep)).sum(2)
+    end = lambda x: (h * x.abs()).clamp(min=2.0 ** -25) ** 2 / 3
+    want, noise, known = {}, {}, {}
+    to_q = lambda w, x: torch.einsum('hbjk,phbk->phbj', w, x)
+    to_k = lambda w, x: fold(torch.einsum('hbjk,phbj->phbk', w, x))
+    want['dq'], known['dq'] = scale * to_q(ds, kk), scale * to_q(via_d, kk)
+    noise['dq'] = scale ** 2 * to_q(var, kk ** 2) + end(want['dq'])
+    want['dk'], known['dk'] = scale * to_k(ds, q), scale * to_k(via_d, q)
+    noise['dk'] = scale ** 2 * to_k(var, q ** 2) + end(want['dk'])
+    want['dv'], known['dv'] = to_k(p, g), torch.zeros_like(v)
+    noise['dv'] = to_k(((h * p) ** 2 / 3 + (F32 * p) ** 2), g ** 2) + end(want['dv'])
+    return want, noise, known
+
+
+def _check_gradients(P, H, G, B, J, K, causal, dtype, make_dout, vs=1.0, ks=1.0, mirror=False):
+    ops = _ops()
+    gen = torch.Generator(device=DEV).manual_seed(P + J + K)
+    q, k, v = (_make((P, n, B, m), 'BJHP', dtype, gen, x) for n, m, x in ((H, J, 1.0), (G, K, ks), (G, K, vs)))
+    if mirror:
+        for x in (q, k, v):
+            x[:, :, 1] = x[:, :, 0]
+    table = (0.5 * torch.randn(32, H, generator=gen, device=DEV)).to(dtype)
+    buckets = ops.relative_buckets(32, 128, not causal)
+    out, lse = torch.empty_like(q), torch.empty(H, B, J, device=DEV)
+    how = dict(buckets=buckets, scale=P ** -0.5, causal=causal)
+    ops.relative_attention(q, k, v, table, out, lse, **how)
+    dout = make_dout(torch.randn(B, J, H, P, generator=gen, device=DEV)).to(dtype).permute(3, 2, 0, 1)
+    got = {'dq': _nan(q.shape, 'BJHP', dtype), 'dk': _nan(k.shape, 'BJHP', dtype), 'dv': _nan(v.shape, 'BJHP', dtype),
+           'dtable': torch.full_like(table, float('nan'))}
+    ops.backward_relative_attention(dout, q, k, v, table, out, lse, *got.values(), **how)
+    h = torch.finfo(dtype).eps / 2
+    want, noise, known = _gradients(q, k, v, table, dout=dout, used=out, h=h, **how)
+    for name in want:
+        held = want[name].abs() < torch.finfo(dtype).max               # (what is larger is infinite)
+        assert got[name][held].isfinite().all(), name
+        norm = lambda x: (x.square() * held).sum((0, 1, 3)).sqrt()     # of each sample
+        off, may = norm((got[name].double() - want[name]).where(held, 0.0)), (noise[name] * held).sum((0, 1, 3)).sqrt()
+        # hundreds of independent roundings at least: their norm is the expected one to a few percent, and the variances are upper ends
+        assert (off <= 1.1 * may + norm(known[name])).all(), (name, off, may, norm(known[name]))
+    full, bound = ref.attention(q, k, v, table, half=h, dout=dout, out_used=out, **how)
+    assert ((got['dtable'].double() - full['dtable']).abs() <= bound['dtable']).all(), 'dtable'
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+@pytest.mark.parametrize('size', [1.0, 1e-3, 1e-4, 1e-5, 300.0])
+@pytest.mark.parametrize('P,H,G,B,J,K,causal', [(64, 2, 2, 1, 2048, 2048, False), (128, 2, 1, 2, 700, 1500, False), (64, 4, 2, 1, 1000, 1000, True),
+                                                (64, 8, 8, 4, 128, 128, False), (48, 4, 4, 2, 100, 77, False)])
+def test_gradients_of_any_size_keep_their_digits(P, H, G, B, J, K, causal, size, dtype):
+    """Score gradients are products of a probability and an output's gradient, and far smaller than the results.  With 16-bit numbers
+    of few exponent bits they must not fall among the smallest steps while results are far from those."""
+    _check_gradients(P, H, G, B, J, K, causal, dtype, lambda g: g * size)
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+def test_gradients_of_many_keys_keep_their_digits(dtype):
+    """Probabilities of one in 65536 on their way into dv."""
+    _check_gradients(64, 1, 1, 1, 128, 65536, False, dtype, lambda g: g)
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+def test_gradients_of_samples_of_very_different_sizes(dtype):
+    """One sample's gradients are ten thousand times those of the next one's."""
+    _check_gradients(64, 2, 2, 4, 500, 500, False, dtype, lambda g: g * torch.tensor([30.0, 3e-3, 1.0, 1e-4], device=DEV)[:, None, None, None])
+
+
+def test_score_gradients_beyond_what_16_bits_hold():
+    """Output gradients as a large loss scale gives them: score gradients exceed 65504, their products with small keys do not.  The
+    second sample has the opposite gradients, so that the table's stay representable."""
+    sign = torch.tensor([1.0, -1.0], device=DEV)[:, None, None, None]
+    for P, J, K in ((64, 6, 8), (64, 150, 8), (128, 6, 8)):
+        _check_gradients(P, 2, 2, 2, J, K, False, torch.float16, lambda g: (g[:1] * 1.2e4).clamp(-5e4, 5e4) * sign * (1 if J < 100 else 0.3),
+                         vs=8.0, ks=0.02, mirror=True)
+
+
+def test_a_gradient_without_a_number_leaves_other_queries_theirs():
+    """A row of dout that is infinite does not decide how the others are rounded."""
+    ops = _ops()
+    for P, J in ((64, 100), (64, 300), (128, 200)):
+        gen = torch.Generator(device=DEV).manual_seed(J)
+        q, k, v, dout = (_make((P, 2, 1, J), 'BJHP', torch.float16, gen) for _ in range(4))
+        dout *= 1e-3
+        table = torch.randn(32, 2, generator=gen, device=DEV).half()
+        how = dict(buckets=ops.relative_buckets(), scale=P ** -0.5)
+        out, lse = torch.empty_like(q), torch.empty(2, 1, J, device=DEV)
+        ops.relative_attention(q, k, v, table, out, lse, **how)
+        got = []
+        for bad in (False, True):
+            if bad:
+                dout[:, 0, 0, 7] = float('inf')
+            got.append([torch.empty_like(x) for x in (q, k, v, table)])
+            ops.backward_relative_attention(dout, q, k, v, table, out, lse, *got[-1], **how)
+        hit = torch.zeros(2, 1, J, dtype=torch.bool, device=DEV)
+        hit[0, 0, 7] = True
+        assert not got[1][0][:, hit].isfinite().any()
+        a, b = (g[0][:, ~hit].double() for g in got)
+        assert (a - b).norm() <= 2e-3 * a.norm()
