@@ -375,10 +375,10 @@ typedef struct sb_attention_span {
  * q, out: [P,H,B,J]; k, v: [P,G,B,K], H a multiple of G (head h reads h / (H/G)); P at most 128; lse: float32 [H,B,J] or
  * NULL.  A query that sees no key gives out = 0 and lse = -inf; one that meets a NaN score or one of +inf gives NaN for both.  NaN or
  * infinity at a key within the length, in v, in k behind a bias of -inf, or in the backward pass in any operand, may reach queries of
- * the sample that do not see that key.  Scores are not stored anywhere; exponentials are rounded to 16 bits where they meet v, sums
- * are fp32.  Few queries against many keys are split along the keys and joined by a second kernel.
- * out overlaps none of the inputs.  scratch: sb_relative_attention_scratch_bytes() for the same operands (may be 0), 16-byte
- * aligned, as above. */
+ * the sample that do not see that key.  Scores are not stored anywhere; exponentials are rounded to 16 bits where they meet v (float16
+ * holds them in steps of 2^-31 of the row's largest or finer), sums are fp32.  Few queries against many keys are split along the
+ * keys and joined by a second kernel.  out overlaps none of the inputs.  scratch: sb_relative_attention_scratch_bytes() for the
+ * same operands (may be 0), 16-byte aligned, as above. */
 int sb_relative_attention(void* stream, void* scratch, size_t scratch_bytes, const sb_tensor* q, const sb_tensor* k,
                           const sb_tensor* v, const sb_relative_bias* bias, const sb_tensor* out, const sb_tensor* lse,
                           const sb_attention_span* span);

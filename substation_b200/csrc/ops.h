@@ -123,9 +123,9 @@ struct RelTables { const float* rows; int pitch, reach; };
 bool rel_direct(const Proj& x);
 // The tcgen05 kernels; q, k, v are rel_direct.  `next`: a zero in device memory.
 int launch_rel_tiles_fwd(cudaStream_t s, Proj q, Proj k, Proj v, RelTables t, int* next, Proj out, RelRows lse, const RelSpan& span);
-// Whether what the backward pass rounds to 16 bits, softmax weights and score gradients, is multiplied by a power of two first.
-// float16 has few exponents: a weight of one in 4096 and an output gradient of 1e-3 make a score gradient among its smallest steps,
-// and output gradients of 1e4 one beyond its largest.
+// Whether exponentials, softmax weights and score gradients are multiplied by a power of two before they are rounded to 16 bits.  float16
+// has few exponents: a weight of one in 4096 and an output gradient of 1e-3 make a score gradient among its smallest steps, output
+// gradients of 1e4 one beyond its largest, and keys of a weight below 2^-25 of the row's largest were lost however many there are.
 #ifdef SB_BF16
 constexpr bool kRelScaled = false;
 #else

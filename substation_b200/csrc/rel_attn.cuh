@@ -15,6 +15,9 @@ namespace rel {
 
 constexpr int kPad = 96;                             // 64 columns and the 32 rows of a warp
 constexpr float kLazy = 8.f;                         // log2 units a row's reference may lag behind its maximum
+// The forward pass' exponentials are times 2^kRaise, as far up as float16 goes beside that, so that many small ones do not vanish in it:
+// steps are 2^-31 of the reference's exponential instead of 2^-24.
+constexpr float kRaise = kRelScaled ? 15.f - kLazy : 0.f;
 
 struct Common {
   int J, K, H, G, B, P;
@@ -356,7 +359,7 @@ __device__ __forceinline__ void row_tile(uint32_t s, uint32_t to, bool started, 
       }
     }
     const float ref = row.m == -INFINITY ? 0.f : row.m;
-    const float2 off = make_float2((NEAR ? 0.f : flat) - ref, (NEAR ? 0.f : flat) - ref);
+    const float2 off = make_float2((NEAR ? kRaise : flat + kRaise) - ref, (NEAR ? kRaise : flat + kRaise) - ref);
     uint32_t w[16];
 #pragma unroll
     for (int e = 0; e < 32; e += 2) {
@@ -594,7 +597,7 @@ rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       }
       if (row && p.lse.p)
         p.lse.p[(long long)w.h * p.lse.sH + (long long)w.b * p.lse.sB + (long long)j * p.lse.sJ] =
-            sees_none(state.l) ? -INFINITY : (state.m + log2f(state.l)) * 0.6931471805599453f;
+            sees_none(state.l) ? -INFINITY : (state.m + (log2f(state.l) - kRaise)) * 0.6931471805599453f;
       if (w.tiles > 0) {
         tc_fence_before();
         __syncwarp();

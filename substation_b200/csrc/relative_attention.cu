@@ -145,6 +145,7 @@ pack_rows_kernel(const __grid_constant__ PackJobs jobs) {
 // copy bandwidth); tcgen05's smallest tile would be 64 or 128 rows for the one to 16 there are, and the matrix work here
 // is a few percent of the time.
 constexpr int kFewThreads = 128;
+constexpr float kFewRaise = kRelScaled ? 15.f : 0.f;   // exponentials, at most one here, are times 2^kFewRaise (see kRaise of the tile kernels)
 template <int P>
 struct FewCfg {
   static constexpr int kKeys = P == 64 ? 32 : 16;    // of a piece
@@ -359,7 +360,7 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
         }
       }
     }
-    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+    const float ref[2] = {(m[0] == -INFINITY ? 0.f : m[0]) - kFewRaise, (m[1] == -INFINITY ? 0.f : m[1]) - kFewRaise};
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
@@ -426,7 +427,7 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
       }
     } else {
       if (f < a.P) const_cast<sb_half*>(row_of(a.o, h, b, j))[f * a.o.sP] = sb_f2h(sees_none(sum) ? 0.f : v / sum);
-      if (f == 0 && a.lse.p) a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] = sees_none(sum) ? -INFINITY : (mm + log2f(sum)) * 0.6931471805599453f;
+      if (f == 0 && a.lse.p) a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] = sees_none(sum) ? -INFINITY : (mm + (log2f(sum) - kFewRaise)) * 0.6931471805599453f;
     }
   }
 }
@@ -463,7 +464,7 @@ join_splits_kernel(const __grid_constant__ FewParams p) {
 #pragma unroll
   for (int c = 0; c < P / 32; ++c)
     if (c * 32 + lane < a.P) out[(c * 32 + lane) * a.o.sP] = sb_f2h(sees_none(sum) ? 0.f : v[c] / sum);
-  if (lane == 0 && a.lse.p) a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] = sees_none(sum) ? -INFINITY : (mm + log2f(sum)) * 0.6931471805599453f;
+  if (lane == 0 && a.lse.p) a.lse.p[h * a.lse.sH + b * a.lse.sB + j * a.lse.sJ] = sees_none(sum) ? -INFINITY : (mm + (log2f(sum) - kFewRaise)) * 0.6931471805599453f;
 }
 
 // What the backward pass knows of 64 query rows (RelBackward in ops.h), four threads a row, and in the blocks before those the rows

@@ -1,5 +1,5 @@
 """Position operators on the GPU at the ends of their ranges, against float64 and against themselves: NaN and infinity inside a
-sequence, gradients of any size."""
+sequence, gradients of any size, caches of many small weights."""
 
 import pytest
 import torch
@@ -196,3 +196,30 @@ def test_a_gradient_without_a_number_leaves_other_queries_theirs():
         assert not got[1][0][:, hit].isfinite().any()
         a, b = (g[0][:, ~hit].double() for g in got)
         assert (a - b).norm() <= 2e-3 * a.norm()
+
+
+# ---- long caches -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', BOTH)
+@pytest.mark.parametrize('H,J', [(150, 1), (20, 130)])
+def test_many_small_weights_count(dtype, H, J):
+    """Four keys outweigh each of 131068 others by 2^26, together those have a weight of 2^-11, and all of the values.  One share of the
+    keys, and the tile kernel."""
+    ops = _ops()
+    K, P = 1 << 17, 64
+    q = torch.zeros(1, J, H, P, dtype=dtype, device=DEV).permute(3, 2, 0, 1)
+    q[0] = 4.0
+    k = torch.zeros(1, K, 1, P, dtype=dtype, device=DEV)
+    k[0, 0:128:32, 0, 0] = 4.5
+    v = torch.ones(1, K, 1, P, dtype=dtype, device=DEV)
+    v[0, 0:128:32] = 0
+    k, v = (x.permute(3, 2, 0, 1).expand(P, H, 1, K) for x in (k, v))
+    table = torch.zeros(1, H, dtype=dtype, device=DEV)
+    out, lse = torch.empty_like(q), torch.empty(H, 1, J, device=DEV)
+    ops.relative_attention(q, k, v, table, out, lse, buckets=ops.RelativeBuckets([0], False), scale=1.0)
+    few = (K - 4) * torch.tensor(-18.0, dtype=torch.float64).exp()
+    want, h = (few / (4 + few)).item(), torch.finfo(dtype).eps / 2
+    # exponentials are rounded once (all alike), the result once; float16 holds them in steps of 2^-31 of the largest in the tile
+    # kernel, of 2^-39 elsewhere
+    step = 0.0 if dtype is torch.bfloat16 else 2.0 ** -32 * K / 4 if J > 1 else 2.0 ** -40 * K / 4
+    assert ((out.double() - want).abs() <= 2.02 * h * want + F32 * want + step).all(), (out.flatten()[0].item(), want)
+    assert ((lse.double() - (18 + (4 + few).log())).abs() <= 1e-5 * 20).all()
