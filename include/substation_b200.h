@@ -354,7 +354,7 @@ int sb_backward_query_key_norm_rotation(void* stream, void* scratch, size_t scra
  * buckets that start together only the last is met).  With `bidirectional`, keys before the query and at its place use
  * buckets 0 .. n-1 and keys behind it n .. 2n-1; without, keys behind it count as distance 0.  table: [2n or n, H].  At most
  * 512 buckets a direction, and the last one starts at a distance of at most 832.  An entry of -inf, or one at or below
- * -2^126 (which only bfloat16 has), hides the keys of its bucket. */
+ * -2^126 (which only bfloat16 has), hides the keys of its bucket; one above 2^127, +inf among them, counts as 2^127. */
 typedef struct sb_relative_bias {
   const sb_tensor* table;
   int32_t n;

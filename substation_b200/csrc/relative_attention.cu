@@ -13,6 +13,13 @@ namespace {
 constexpr int kMaxP = kRelMaxHead;
 constexpr int kRelPad = 96;                         // as the tile kernels' kPad
 constexpr float kHidden = -8.507059173023462e37f;   // -2^126: entries at or below hide their keys
+constexpr float kLargest = 1.7014118346046923e38f;   // 2^127: entries above count as this, so that log2(e) of them is finite and leaves room
+
+// A table's entry in units of log2.
+__device__ __forceinline__ float bias_of_entry(sb_half entry) {
+  const float b = sb_h2f(entry);
+  return b <= kHidden ? -INFINITY : (b > kLargest ? kLargest : b) * 1.4426950408889634f;
+}
 
 struct Starts { int s[kRelMaxBuckets]; };
 struct AttnArgs {
@@ -48,7 +55,7 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
 }
 
 // rows[h][i] = log2(e) * bias of head h at relative position i - kRelPad - reach, which stays at its end values beyond the reach.
-// Biases of up to 2^127 in size stay finite, so that a row of nothing but float16's lowest still has a maximum.
+// Biases stay finite, so that a row of nothing but float16's lowest still has a maximum.
 // Block `part` of expand_blocks() for the head.  A launch and a search among the starts: 1.9 us alone, whatever the size.
 struct Expand { float* rows; int pitch, reach; int* next; };   // next: the work queue of the kernel that follows
 __host__ __device__ constexpr int expand_blocks(int pitch) { return (pitch + 255) / 256; }
@@ -57,8 +64,7 @@ __device__ __forceinline__ void expand_part(const AttnArgs& a, const int* starts
   const int i = part * 256 + threadIdx.x;
   if (i >= x.pitch) return;
   const int rel = max(-x.reach, min(x.reach, i - kRelPad - x.reach));
-  const float b = sb_h2f(a.table[bucket_of(a, starts, rel) * a.t_sN + h * a.t_sH]);
-  x.rows[(long long)h * x.pitch + i] = b <= kHidden ? -INFINITY : b * 1.4426950408889634f;
+  x.rows[(long long)h * x.pitch + i] = bias_of_entry(a.table[bucket_of(a, starts, rel) * a.t_sN + h * a.t_sH]);
 }
 __global__ void __launch_bounds__(256)
 expand_bias_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const __grid_constant__ Expand x) {
@@ -265,10 +271,7 @@ few_queries_kernel(const __grid_constant__ FewParams p, const __grid_constant__ 
         qf[s][y * 2 + x] = pack_pair(u, v);
       }
   }
-  auto bias_of = [&](int bucket, int h) {
-    const float v = sb_h2f(a.table[bucket * a.t_sN + h * a.t_sH]);
-    return v <= kHidden ? -INFINITY : v * 1.4426950408889634f;
-  };
+  auto bias_of = [&](int bucket, int h) { return bias_of_entry(a.table[bucket * a.t_sN + h * a.t_sH]); };
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     lo[x] = bias_of(p.before, head[x]);

@@ -1,5 +1,6 @@
 """Position operators on the GPU at the ends of their ranges, against float64 and against themselves: NaN and infinity inside a
-sequence, gradients of any size, caches of many small weights."""
+sequence, gradients of any size, caches of many small weights,
+biases of any size."""
 
 import pytest
 import torch
@@ -223,3 +224,43 @@ def test_many_small_weights_count(dtype, H, J):
     step = 0.0 if dtype is torch.bfloat16 else 2.0 ** -32 * K / 4 if J > 1 else 2.0 ** -40 * K / 4
     assert ((out.double() - want).abs() <= 2.02 * h * want + F32 * want + step).all(), (out.flatten()[0].item(), want)
     assert ((lse.double() - (18 + (4 + few).log())).abs() <= 1e-5 * 20).all()
+
+
+# ---- biases of any size ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', BOTH)
+@pytest.mark.parametrize('J', [1, 150])
+def test_biases_up_to_the_largest(dtype, J):
+    """The largest number of the type in one bucket: its keys share the row, and nothing is NaN.  What is above 2^127 counts as 2^127."""
+    ops = _ops()
+    gen = torch.Generator(device=DEV).manual_seed(J)
+    P, H, K = 64, 3, 400
+    q, k, v = (_make((P, H, 2, n), 'BJHP', dtype, gen) for n in (J, K, K))
+    table = torch.randn(8, H, generator=gen, device=DEV).to(dtype)
+    table[1, 0] = table[5, 1] = table[0, 2] = torch.finfo(dtype).max
+    table[3, 2] = 0.75 * torch.finfo(dtype).max
+    how = dict(buckets=ops.relative_buckets(8, 20, True), scale=0.125, first=torch.tensor([0, 200], dtype=torch.int32, device=DEV))
+    out, lse = _forward(q, k, v, table, how)
+    full = dict(how, table=table.double().clamp(max=2.0 ** 127))
+    h = torch.finfo(dtype).eps / 2
+    want, bound = ref.attention(q, k, v, half=h, **full)
+    assert ((lse - want['lse']).abs() <= 1e-5 * (1 + want['lse'].abs())).all()
+    # A score beside a bias of 2^104 or more is below half a step of their 32-bit sum, and whether it is rounded away depends on the
+    # order of the sums: of such rows only that the keys with the largest bias share them, so that each feature lies between those
+    # keys' least and largest value.  (65504 in 32 bits moves an exponent by half a step of that, 2^-9.)
+    rel = torch.arange(K, device=DEV) - torch.arange(J, device=DEV)[:, None] - how['first'][:, None, None]            # [B,J,K]
+    lookup = torch.tensor([how['buckets'].bucket(r) for r in range(-K - J, K + J)], device=DEV)
+    bias = full['table'][lookup[rel + K + J]].permute(3, 0, 1, 2)                                                    # [H,B,J,K]
+    top = bias.amax(-1, keepdim=True)
+    huge = (top > 2.0 ** 100).squeeze(-1)
+    shares = bias == top
+    off = 2.02 * h * v.abs().max().double() + ref.SMALL
+    for p in range(P):
+        x = v[p].double()[:, :, None].expand(H, 2, J, K)
+        least, most = x.masked_fill(~shares, torch.inf).amin(-1), x.masked_fill(~shares, -torch.inf).amax(-1)
+        assert ((out[p] >= least - off) & (out[p] <= most + off))[huge].all()
+    loose = 2.0 ** -8 * want['out'].abs().max() if dtype is torch.float16 else 0.0
+    assert ((out.double() - want['out']).abs() <= bound['out'] + loose)[:, ~huge].all()
+    dout = _make(q.shape, 'BJHP', dtype, gen)
+    got = [torch.empty_like(x) for x in (q, k, v, table)]
+    ops.backward_relative_attention(dout, q, k, v, table, out, lse, *got, **how)
+    assert all(x.isfinite().all() for x in got)
