@@ -326,7 +326,8 @@ int sb_set_sm_budget(int n_sms);
  * their digits); one rounding at the end.  q, q_out: [P,H,B,J]; k, k_out: [P,G,B,J] with any number of heads, or k, k_gain
  * and k_out all NULL; gains: [P], contiguous; positions: int32 [B,J], any strides (0 to share them), any sign.  P is at most
  * 256, rotary even and at most P (0: no rotation).  An output may be its input (same pointer and strides).  No counterpart
- * in the reference. */
+ * in the reference.  Other outputs and inputs do not overlap (those that start together are refused).  All of these operators
+ * refuse operands that are not aligned to their elements. */
 typedef enum sb_pairing { SB_PAIR_HALVES = 0, SB_PAIR_ADJACENT = 1 } sb_pairing;
 typedef struct sb_rotation {
   double base;
@@ -341,7 +342,7 @@ int sb_query_key_norm_rotation(void* stream, const sb_tensor* q, const sb_tensor
  *   g = dout turned back,   dgain[p] = sum_{h,b,j} g n,   dx = rsqrt(..) * (g gain - n mean_p(g gain n)).
  * scratch: sb_query_key_norm_scratch_bytes() of 16-byte aligned device memory, contents of no interest before or after, not
  * shared by calls that may run at the same time.  Sums run in a fixed order.  dq may be dq_out or q, dk may be dk_out or k
- * (same pointer and strides). */
+ * (same pointer and strides); nothing else of dq, dk, dq_gain and dk_gain overlaps. */
 size_t sb_query_key_norm_scratch_bytes(void);
 int sb_backward_query_key_norm_rotation(void* stream, void* scratch, size_t scratch_bytes, const sb_tensor* dq_out,
                                         const sb_tensor* dk_out, const sb_tensor* q, const sb_tensor* k,
@@ -377,7 +378,7 @@ typedef struct sb_attention_span {
  * infinity at a key within the length, in v, in k behind a bias of -inf, or in the backward pass in any operand, may reach queries of
  * the sample that do not see that key.  Scores are not stored anywhere; exponentials are rounded to 16 bits where they meet v (float16
  * holds them in steps of 2^-31 of the row's largest or finer), sums are fp32.  Few queries against many keys are split along the
- * keys and joined by a second kernel.  out overlaps none of the inputs.  scratch: sb_relative_attention_scratch_bytes() for the
+ * keys and joined by a second kernel.  out and lse overlap neither each other nor any input.  scratch: sb_relative_attention_scratch_bytes() for the
  * same operands (may be 0), 16-byte aligned, as above. */
 int sb_relative_attention(void* stream, void* scratch, size_t scratch_bytes, const sb_tensor* q, const sb_tensor* k,
                           const sb_tensor* v, const sb_relative_bias* bias, const sb_tensor* out, const sb_tensor* lse,
@@ -391,7 +392,7 @@ int sb_relative_attention_scratch_bytes(const sb_tensor* q, const sb_tensor* k, 
  * multiplication by powers of two that follow from the largest |dout| and |v| of the rows concerned, so that neither underflows
  * or overflows before the results do; D is taken from the rounded out; sums are fp32.
  * dk and dv of shared heads are sums over the query heads, and 0 behind a sample's length; every element of the five outputs
- * is written, and they overlap none of the inputs.  Sums run in a fixed order: the same call gives the same bits.  No
+ * is written, and they overlap neither each other nor any input.  Sums run in a fixed order: the same call gives the same bits.  No
  * counterpart in the reference, which has neither positions nor padding. */
 int sb_backward_relative_attention(void* stream, void* scratch, size_t scratch_bytes, const sb_tensor* dout,
                                    const sb_tensor* q, const sb_tensor* k, const sb_tensor* v,

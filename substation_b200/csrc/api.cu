@@ -200,9 +200,13 @@ extern "C" int sb_softmax_dropout(void* stream, const sb_tensor* beta, const sb_
 // ---------------------------------------------------------------------------
 namespace {
 
+int on_grid(const void* p, unsigned bytes, const char* what) {
+  return aligned(p, bytes) ? SB_OK : fail(SB_ERR_ALIGNMENT, std::string(what) + ": not aligned to its elements");
+}
 int to_projection(const sb_tensor* t, const char* what, Proj* o) {
   SB_TRY(check_tensor(t, 4, what));
   SB_TRY(fits_int(t, what));
+  SB_TRY(on_grid(t->ptr, 2, what));
   o->p = t->ptr; o->sP = t->stride[0]; o->sH = t->stride[1]; o->sB = t->stride[2]; o->sR = t->stride[3];
   o->P = (int)t->size[0]; o->H = (int)t->size[1]; o->B = (int)t->size[2]; o->R = (int)t->size[3];
   return SB_OK;
@@ -218,7 +222,22 @@ int to_projection_out(const sb_tensor* t, const sb_tensor* like, const char* wha
   SB_TRY(same_shape(like, t, what));
   return distinct(t, what);
 }
-int to_gain(const sb_tensor* t, const sb_tensor* x, const char* what, void** p) { return to_param(t, x->size[0], what, p); }
+int to_gain(const sb_tensor* t, const sb_tensor* x, const char* what, void** p) {
+  SB_TRY(to_param(t, x->size[0], what, p));
+  return on_grid(*p, 2, what);
+}
+// Outputs start apart from one another and from these inputs (null: none).
+int apart(const char* what, std::initializer_list<const void*> outputs, std::initializer_list<const void*> inputs) {
+  const void* const* out = outputs.begin();
+  for (size_t i = 0; i < outputs.size(); ++i) {
+    if (!out[i]) continue;
+    for (const void* in : inputs)
+      if (out[i] == in) return fail(SB_ERR_ARG, std::string(what) + ": an output lies in an input's place");
+    for (size_t j = 0; j < i; ++j)
+      if (out[i] == out[j]) return fail(SB_ERR_ARG, std::string(what) + ": two outputs in one place");
+  }
+  return SB_OK;
+}
 
 // What forward and backward of the norms share.  Leaves k->H = 0 when there are no keys.
 int norm_operands(const sb_tensor* q, const sb_tensor* k, const sb_tensor* q_gain, const sb_tensor* k_gain, const sb_tensor* positions,
@@ -240,6 +259,7 @@ int norm_operands(const sb_tensor* q, const sb_tensor* k, const sb_tensor* q_gai
   if ((long long)pq->B * pq->R > 1LL << 30) return fail(SB_ERR_UNSUPPORTED, "norm: more than 2^30 tokens");
   if ((long long)pq->H + pk->H > 65535) return fail(SB_ERR_UNSUPPORTED, "norm: more than 65535 heads");
   SB_TRY(check_tensor(positions, 2, "norm.positions"));
+  SB_TRY(on_grid(positions->ptr, 4, "norm.positions"));
   if (positions->size[0] != pq->B || positions->size[1] != pq->R)
     return fail(SB_ERR_ARG, "norm.positions: extent mismatch between operands");
   pos->p = positions->ptr; pos->sB = positions->stride[0]; pos->sJ = positions->stride[1];
@@ -274,6 +294,11 @@ extern "C" int sb_query_key_norm_rotation(void* stream, const sb_tensor* q, cons
   if (k) SB_TRY(to_projection_out(k_out, k, "norm.k_out", &ok));
   if (other_place(pq, oq) || (k && other_place(pk, ok)))
     return fail(SB_ERR_ARG, "norm: an output in its input's place needs its strides");
+  if (pq.B > 0 && pq.R > 0) {   // (blocks of queries and of keys run side by side)
+    SB_TRY(apart("norm", {oq.p}, {pk.p, gq, gk, pos.p}));
+    SB_TRY(apart("norm", {ok.p}, {pq.p, gq, gk, pos.p}));
+    SB_TRY(apart("norm", {oq.p, ok.p}, {}));
+  }
   return launch_qk_norm_fwd((cudaStream_t)stream, pq, pk, gq, gk, pos, oq, ok, rot);
 }
 
@@ -305,6 +330,11 @@ extern "C" int sb_backward_query_key_norm_rotation(void* stream, void* scratch, 
   }
   if (other_place(gq_out, oq) || other_place(pq, oq) || (k && (other_place(gk_out, ok) || other_place(pk, ok))))
     return fail(SB_ERR_ARG, "norm: an output in its input's place needs its strides");
+  if (pq.B > 0 && pq.R > 0) {
+    SB_TRY(apart("norm", {oq.p}, {pk.p, gk_out.p, gq, gk, pos.p}));
+    SB_TRY(apart("norm", {ok.p}, {pq.p, gq_out.p, gq, gk, pos.p}));
+    SB_TRY(apart("norm", {oq.p, ok.p, dgq, dgk}, {}));
+  }
   if (!scratch || scratch_bytes < qk_norm_scratch_bytes()) return fail(SB_ERR_ARG, "norm: scratch is missing or too small");
   if (!aligned(scratch, 16)) return fail(SB_ERR_ALIGNMENT, "norm: scratch is not 16-byte aligned");
   return launch_qk_norm_bwd((cudaStream_t)stream, scratch, gq_out, gk_out, pq, pk, gq, gk, pos, oq, ok, dgq, dgk, rot);
@@ -335,6 +365,7 @@ int relative_operands(const sb_tensor* q, const sb_tensor* k, const sb_tensor* v
   if (n > kRelMaxBuckets)
     return fail(SB_ERR_UNSUPPORTED, "relative attention: " + std::to_string(n) + " buckets a direction, at most " + std::to_string(kRelMaxBuckets));
   SB_TRY(check_tensor(bias->table, 2, "relative attention.table"));
+  SB_TRY(on_grid(bias->table->ptr, 2, "relative attention.table"));
   if (bias->table->size[0] != (bias->bidirectional ? 2 * n : n) || bias->table->size[1] != pq->H)
     return fail(SB_ERR_ARG, "relative attention.table: extents are not [buckets, heads]");
   if (bias->starts[0] != 0) return fail(SB_ERR_ARG, "relative attention: the first bucket starts at distance 0");
@@ -360,17 +391,10 @@ int to_lse(const sb_tensor* t, const sb_tensor* q, RelRows* o) {
   memset(o, 0, sizeof(*o));
   if (!t) return SB_OK;
   SB_TRY(check_tensor(t, 3, "relative attention.lse"));
+  SB_TRY(on_grid(t->ptr, 4, "relative attention.lse"));
   for (int i = 0; i < 3; ++i)
     if (t->size[i] != q->size[i + 1]) return fail(SB_ERR_ARG, "relative attention.lse: extent mismatch between operands");
   o->p = reinterpret_cast<float*>(t->ptr); o->sH = t->stride[0]; o->sB = t->stride[1]; o->sJ = t->stride[2];
-  return SB_OK;
-}
-
-// Outputs are written while other tiles of the inputs are still to be read.
-int apart(std::initializer_list<const void*> outputs, std::initializer_list<const void*> inputs) {
-  for (const void* o : outputs)
-    for (const void* i : inputs)
-      if (o == i) return fail(SB_ERR_ARG, "relative attention: an output lies in an input's place");
   return SB_OK;
 }
 
@@ -402,11 +426,12 @@ extern "C" int sb_relative_attention(void* stream, void* scratch, size_t scratch
   RelRows rows;
   SB_TRY(relative_operands(q, k, v, bias, &pq, &pk, &pv, &rb));
   SB_TRY(to_projection_out(out, q, "relative attention.out", &po));
-  SB_TRY(apart({po.p}, {pq.p, pk.p, pv.p, rb.table}));
+  SB_TRY(apart("relative attention", {po.p}, {pq.p, pk.p, pv.p, rb.table}));
   SB_TRY(to_lse(lse, q, &rows));
   if (lse) SB_TRY(distinct(lse, "relative attention.lse"));
   SB_TRY(to_span(span, &sp));
   SB_TRY(check_scratch(scratch, scratch_bytes, rel_attn_scratch_bytes(pq, pk, pv, rb)));
+  SB_TRY(apart("relative attention", {po.p, rows.p}, {pq.p, pk.p, pv.p, rb.table, sp.lengths, sp.first}));
   return launch_rel_attn_fwd((cudaStream_t)stream, scratch, pq, pk, pv, rb, po, rows, sp);
 }
 
@@ -441,11 +466,13 @@ extern "C" int sb_backward_relative_attention(void* stream, void* scratch, size_
   SB_TRY(to_projection_out(dk, k, "relative attention.dk", &ok));
   SB_TRY(to_projection_out(dv, v, "relative attention.dv", &ov));
   SB_TRY(check_tensor(dtable, 2, "relative attention.dtable"));
-  SB_TRY(apart({oq.p, ok.p, ov.p, dtable->ptr}, {pg.p, pq.p, pk.p, pv.p, po.p, rb.table, rows.p}));
+  SB_TRY(on_grid(dtable->ptr, 2, "relative attention.dtable"));
+  SB_TRY(apart("relative attention", {oq.p, ok.p, ov.p, dtable->ptr}, {pg.p, pq.p, pk.p, pv.p, po.p, rb.table, rows.p}));
   SB_TRY(same_shape(bias->table, dtable, "relative attention.dtable"));
   SB_TRY(distinct(dtable, "relative attention.dtable"));
   SB_TRY(to_span(span, &sp));
   SB_TRY(check_scratch(scratch, scratch_bytes, rel_attn_bwd_scratch_bytes(pg, pq, pk, pv, rb)));
+  SB_TRY(apart("relative attention", {oq.p, ok.p, ov.p, dtable->ptr}, {sp.lengths, sp.first}));
   return launch_rel_attn_bwd((cudaStream_t)stream, scratch, pg, pq, pk, pv, rb, po, rows, oq, ok, ov, dtable->ptr, dtable->stride[0],
                              dtable->stride[1], sp);
 }
