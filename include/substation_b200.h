@@ -310,8 +310,10 @@ int sb_mma_peak_probe(void* stream, int k_blocks, int bf16, double* flops);
  * fixed number per SM) walks the work.  When another kernel must run next to them (the NCCL
  * gradient allreduce of the data-parallel path), tell the library to size every such grid
  * for n_sms SMs only, so that no CTA waits behind the other kernel and then runs its share
- * as a second round (0 = use every SM, the default).  Process-wide.  No counterpart in the
- * reference, which has no multi-GPU path. */
+ * as a second round (0 = use every SM, the default).  Outputs do not depend on it (parameter
+ * gradients that are column sums may by rounding); grids that would change an order of
+ * summation, as that of sb_relative_attention with few queries, therefore stay as they are.
+ * Process-wide.  No counterpart in the reference, which has no multi-GPU path. */
 int sb_set_sm_budget(int n_sms);
 
 /* ------------------------------------------------------------------------- */

@@ -733,13 +733,16 @@ bool piecewise(const Proj& x) {
 // when there are not more CTAs than items: every key is read as often (64 x 16 heads, one query, 512 keys: 38 against 41 us), with
 // heads that share keys less often (64 x 16 heads on 8, 4096 keys: 84 against 225); with more than four queries the tensor cores
 // of the tile kernel outweigh that (16 queries, 512 keys: 52 against 41).
+// The device's SMs count here and not the budget of sb_set_sm_budget: the number of shares is an order of summation, and results do not
+// depend on the budget.  (Its CTAs are many short ones, which make room for another kernel's as they end.)
 int few_splits(const Proj& q, const Proj& k) {
+  const long long sms = device_facts().sms;
   const long long blocks = ((long long)(q.H / k.H) * q.R + 15) / 16, ctas = blocks * k.B * k.H, items = (long long)q.B * q.H * ((q.R + 127) / 128);
-  const bool idle = ctas <= 148 && (blocks == 1 || k.R >= 1024);
+  const bool idle = ctas <= sms && (blocks == 1 || k.R >= 1024);
   if (!idle && ctas * (q.R > 4 ? 2 : 1) > items) return 0;
-  // two CTAs for each of 148 SMs and no more, which would wait for those (B=16, 16 heads on 8, 8192 keys of 128 features, 128 CTAs: two
+  // two CTAs for each SM and no more, which would wait for those (B=16, 16 heads on 8, 8192 keys of 128 features, 128 CTAs: two
   // shares 87 us, four 97, five 114), at least 256 keys a share
-  return (int)std::max<long long>(1, std::min<long long>({296 / ctas, (k.R + 255) / 256, 64}));
+  return (int)std::max<long long>(1, std::min<long long>({2 * sms / ctas, (k.R + 255) / 256, 64}));
 }
 struct FewPlan { int splits; size_t k, v, bytes; };
 FewPlan few_plan(const Proj& q, const Proj& k, const Proj& v) {

@@ -1,6 +1,6 @@
 """Position operators on the GPU at the ends of their ranges, against float64 and against themselves: NaN and infinity inside a
 sequence, gradients of any size, caches of many small weights,
-biases of any size."""
+biases of any size, budgets of SMs."""
 
 import pytest
 import torch
@@ -264,3 +264,36 @@ def test_biases_up_to_the_largest(dtype, J):
     got = [torch.empty_like(x) for x in (q, k, v, table)]
     ops.backward_relative_attention(dout, q, k, v, table, out, lse, *got, **how)
     assert all(x.isfinite().all() for x in got)
+
+
+# ---- a budget of SMs ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('P,H,G,B,J,K', [(64, 16, 16, 2, 1, 3000), (128, 16, 4, 8, 2, 900), (64, 8, 8, 2, 300, 300), (64, 6, 6, 30, 128, 128),
+                                         (128, 8, 2, 2, 200, 257)])
+def test_results_do_not_depend_on_the_sm_budget(P, H, G, B, J, K):
+    """Outputs and gradients keep their bits; the gains' gradients, sums over a different number of rows, stay within rounding."""
+    ops = _ops()
+    gen = torch.Generator(device=DEV).manual_seed(K)
+    q, k, v, dout = (_make((P, h, B, n), 'BJHP', torch.float16, gen) for h, n in ((H, J), (G, K), (G, K), (H, J)))
+    table, gain = torch.randn(32, H, generator=gen, device=DEV).half(), (1 + 0.1 * torch.randn(P, generator=gen, device=DEV)).half()
+    how = dict(buckets=ops.relative_buckets(), scale=P ** -0.5)
+    pos = torch.arange(J, dtype=torch.int32, device=DEV).expand(B, J)
+
+    def run():
+        out, lse = _forward(q, k, v, table, how)
+        got = [torch.empty_like(x) for x in (q, k, v, table)]
+        ops.backward_relative_attention(dout, q, k, v, table, out, lse, *got, **how)
+        y, dx, dg = torch.empty_like(q), torch.empty_like(q), torch.empty_like(gain)
+        ops.query_key_norm_rotation(q, None, gain, None, pos, y, None)
+        ops.backward_query_key_norm_rotation(dout, None, q, None, gain, None, pos, dx, None, dg, None)
+        return [out, lse, y, dx] + got, dg
+    try:
+        seen = []
+        for budget in (0, 136, 100, 3):
+            ops.set_sm_budget(budget)
+            seen.append(run())
+    finally:
+        ops.set_sm_budget(0)
+    for got, dg in seen[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got, seen[0][0]))
+        assert (dg.float() - seen[0][1].float()).norm() <= 2e-3 * seen[0][1].float().norm()
+    assert ops.device_error() == 0
