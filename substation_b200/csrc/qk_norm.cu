@@ -531,23 +531,30 @@ gain_finish_kernel(const float* q_partial, const float* k_partial, int q_rows, i
   if ((threadIdx.x & 31) == 0 && blockIdx.x * 32 + i < P) (blockIdx.y ? k : q)[blockIdx.x * 32 + i] = sb_f2h(s);
 }
 
-// The frequencies of one rotation, remembered per thread: a program uses one or two.
+// The frequencies of a rotation.  Each takes about 0.3 us of host time to work out, so a thread keeps those of the last eight rotations: a
+// model's layers may alternate between a few.
 const Turns& turns_of(const Rotation& r) {
-  static thread_local Turns t;
-  static thread_local double base = 0.0;
-  static thread_local int rotary = -1;
-  if (base != r.base || rotary != r.rotary) {
-    for (int i = 0; i < kMaxPairs; ++i) {
-      t.t[i] = 0;
-      if (2 * i >= r.rotary) continue;
-      const long double turns = std::pow((long double)r.base, -2.0L * i / r.rotary) / 6.283185307179586476925286766559L;
-      const long double scaled = std::ldexp(turns - std::floor(turns), 64);
-      t.t[i] = scaled < 18446744073709551615.0L ? (unsigned long long)scaled : ~0ull;
-    }
-    base = r.base;
-    rotary = r.rotary;
+  struct Known {
+    Turns turns;
+    double base = 0.0;
+    int rotary = -1;
+  };
+  static thread_local Known known[8];
+  static thread_local int next = 0;
+  for (const Known& k : known)
+    if (k.base == r.base && k.rotary == r.rotary) return k.turns;
+  Known& k = known[next];
+  next = (next + 1) % 8;
+  for (int i = 0; i < kMaxPairs; ++i) {
+    k.turns.t[i] = 0;
+    if (2 * i >= r.rotary) continue;
+    const long double turns = std::pow((long double)r.base, -2.0L * i / r.rotary) / 6.283185307179586476925286766559L;
+    const long double scaled = std::ldexp(turns - std::floor(turns), 64);
+    k.turns.t[i] = scaled < 18446744073709551615.0L ? (unsigned long long)scaled : ~0ull;
   }
-  return t;
+  k.base = r.base;
+  k.rotary = r.rotary;
+  return k.turns;
 }
 
 NormArgs norm_args(const Proj& q, const Proj& k, const void* q_gain, const void* k_gain, const View2& pos, const Rotation& rot) {

@@ -1,6 +1,6 @@
 """Position operators on the GPU at the ends of their ranges, against float64 and against themselves: NaN and infinity inside a
 sequence, gradients of any size, caches of many small weights,
-biases of any size, budgets of SMs."""
+biases of any size, budgets of SMs, several rotations."""
 
 import pytest
 import torch
@@ -297,3 +297,53 @@ def test_results_do_not_depend_on_the_sm_budget(P, H, G, B, J, K):
         assert all(torch.equal(a, b) for a, b in zip(got, seen[0][0]))
         assert (dg.float() - seen[0][1].float()).norm() <= 2e-3 * seen[0][1].float().norm()
     assert ops.device_error() == 0
+
+
+# ---- two rotations in turn ---------------------------------------------------------------------------------------------
+def test_alternating_rotations_cost_no_more_than_one():
+    """Layers of local and of global attention have bases of their own.  Host time of a call, the least of many: frequencies are not
+    worked out again (11 us a call for 64 features, 22 for 128)."""
+    import time
+    ops = _ops()
+    q = torch.randn(1, 1, 1, 128, device=DEV).half().permute(3, 2, 0, 1)
+    gain, pos, out = torch.ones(128, device=DEV).half(), torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.empty_like(q)
+
+    def least(bases):
+        best = 1e9
+        for _ in range(400):
+            torch.cuda.synchronize()
+            t = time.perf_counter()
+            for b in bases:
+                ops.query_key_norm_rotation(q, None, gain, None, pos, out, None, base=b)
+            best = min(best, time.perf_counter() - t)
+        return best / len(bases)
+    one, four = least([1e4] * 4), least([1e4, 1e6, 5e5, 500.0])
+    assert four <= one + 4e-6, (one, four)
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+def test_many_rotations_in_turn(dtype):
+    """More rotations than are remembered, twice each, in one thread and in another beside it."""
+    import threading
+    ops = _ops()
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    q = _make((64, 2, 2, 9), 'BJHP', dtype, gen)
+    gain = torch.ones(64, device=DEV).to(dtype)
+    pos = torch.randint(-5000, 1 << 21, (2, 9), generator=gen, device=DEV, dtype=torch.int32)
+    rotations = [(b, r) for b in (100.0, 1e4, 1e6) for r in (0, 2, 32, 64)]
+    wrong = []
+
+    def turns():
+        for base, rotary in 2 * rotations + rotations[::-1]:
+            out = torch.empty_like(q)
+            ops.query_key_norm_rotation(q, None, gain, None, pos, out, None, base=base, rotary=rotary)
+            want = ref.norm_forward(q, gain, pos, base, rotary, 'halves', 1e-6)
+            bound = torch.finfo(dtype).eps / 2 * 1.01 * want.abs() + 2e-6 * want.abs().amax(0, keepdim=True) + ref.SMALL
+            if ((out.double() - want).abs() > bound).any():
+                wrong.append((base, rotary))
+    threads = [threading.Thread(target=turns) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
