@@ -92,3 +92,52 @@ def test_misaligned_operands_of_attention(backward, kw):
 def test_outputs_of_attention_in_the_wrong_place(backward, kw):
     st, text = _attention_call(backward, **{**_APART, **kw})
     assert st == 1 and 'place' in text, (st, text)
+
+
+def test_packed_descriptors_are_the_structures():
+    """What ``ops`` packs as bytes reads back field by field through the structures that follow the header."""
+    import torch
+    from substation_b200 import ops
+    x = torch.empty(3, 5, 7, 11)
+    for t in (x.permute(2, 0, 3, 1), x[0, 0], x[:, 0, 0, 0], x[0], x[..., None].expand(-1, -1, -1, -1, 2)):
+        raw = ops._packed(t)
+        d = _lib.SbTensor.from_buffer_copy(raw)
+        assert len(raw) == ctypes.sizeof(_lib.SbTensor) and d.ptr == t.data_ptr() and d.ndim == t.dim()
+        assert tuple(d.size)[:t.dim()] == t.shape and tuple(d.stride)[:t.dim()] == t.stride()
+    raw = ops._rotation(x, 5e5, 2, 'adjacent', 0.25)
+    r = _lib.SbRotation.from_buffer_copy(raw)
+    assert len(raw) == ctypes.sizeof(_lib.SbRotation) and (r.base, r.rotary, r.pairing, r.eps) == (5e5, 2, _lib.SB_PAIR_ADJACENT, 0.25)
+    buckets = ops.RelativeBuckets([0, 1, 4], bidirectional=True)
+    raw = ops._relative_bias(x[0, 0], buckets)
+    b = _lib.SbRelativeBias.from_buffer_copy(raw)
+    assert len(raw) == ctypes.sizeof(_lib.SbRelativeBias) and (b.n, b.bidirectional) == (3, 1)
+    assert b.starts[:3] == [0, 1, 4] and b.table.contents.ptr == x.data_ptr() and b.table.contents.size[:2] == [7, 11]
+    lengths, first = torch.zeros(7, dtype=torch.int32), torch.ones(7, dtype=torch.int32)
+    raw = ops._span(x, 0.5, True, lengths, first)
+    s = _lib.SbAttentionSpan.from_buffer_copy(raw)
+    assert len(raw) == ctypes.sizeof(_lib.SbAttentionSpan)
+    assert (s.scale, s.causal, s.lengths, s.first) == (0.5, 1, lengths.data_ptr(), first.data_ptr())
+    s = _lib.SbAttentionSpan.from_buffer_copy(ops._span(x, 2.0, False, None, None))
+    assert (s.scale, s.causal, s.lengths, s.first) == (2.0, 0, None, None)
+
+
+def test_structures_are_the_headers(tmp_path):
+    """Sizes and offsets of the ctypes structures against what a C compiler makes of the header."""
+    import os
+    import shutil
+    import subprocess
+    cc = shutil.which('gcc') or shutil.which('cc')
+    if cc is None:
+        pytest.skip('no C compiler')
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'include')
+    classes = {'sb_tensor': _lib.SbTensor, 'sb_rotation': _lib.SbRotation, 'sb_relative_bias': _lib.SbRelativeBias,
+               'sb_attention_span': _lib.SbAttentionSpan}
+    lines = ['#include <stddef.h>', '#include "substation_b200.h"']
+    for name, cls in classes.items():
+        lines.append(f'_Static_assert(sizeof({name}) == {ctypes.sizeof(cls)}, "{name}");')
+        for field, *_ in cls._fields_:
+            lines.append(f'_Static_assert(offsetof({name}, {field}) == {getattr(cls, field).offset}, "{name}.{field}");')
+    source = tmp_path / 'layout.c'
+    source.write_text('\n'.join(lines) + '\n')
+    r = subprocess.run([cc, '-std=c11', '-fsyntax-only', '-I', include, str(source)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
