@@ -489,7 +489,7 @@ __device__ __forceinline__ void store_largest(float value, float* to) {
   const uint32_t most = __reduce_max_sync(0xffffffffu, value < INFINITY ? __float_as_uint(value) : 0u);
   if ((threadIdx.x & 31) == 0) to[threadIdx.x >> 5] = __uint_as_float(most);
 }
-template <int P>
+template <int P, bool VALUES>
 __global__ void __launch_bounds__(256)
 row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const __grid_constant__ Expand x, float* records, float* sizes,
                    int vec, int vec_v, int expanding, int values) {
@@ -535,7 +535,7 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
     }
   };
   Rows rv = {nullptr, nullptr};
-  if (kRelScaled && it < values) {
+  if (VALUES && it < values) {
     rv = rows_of_v(it);
     if (vec_v) load_v(rv.at);
   }
@@ -593,7 +593,7 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
   }
   if (kRelScaled) {
     store_largest(i == 0 && live && lse != -INFINITY ? size : 0.f, sizes + (((long long)b * a.H + h) * blocks + block) * 8);
-    for (int m = it; m < values; m += (int)gridDim.x - expanding) {
+    for (int m = it; VALUES && m < values; m += (int)gridDim.x - expanding) {
       if (m != it) {
         rv = rows_of_v(m);
         if (vec_v) load_v(rv.at);
@@ -839,7 +839,9 @@ int launch_rel_attn_bwd(cudaStream_t s, void* scratch, Proj dout, Proj q, Proj k
   float* records = reinterpret_cast<float*>(base + pl.records);
   float* sizes = reinterpret_cast<float*>(base + pl.sizes);
   const int expanding = a.H * expand_blocks(x.pitch), values = kRelScaled && !rel_both(q, k) ? a.G * a.B * ((a.K + 63) / 64) : 0;
-  SB_LAUNCH_OK(launch_k(q.P <= 64 ? row_records_kernel<64> : row_records_kernel<128>, (unsigned)(expanding + a.H * a.B * ((a.J + 63) / 64)), 256, 0, s, a, st, x, records,
+  auto kernel = values ? (q.P <= 64 ? row_records_kernel<64, kRelScaled> : row_records_kernel<128, kRelScaled>)
+                       : (q.P <= 64 ? row_records_kernel<64, false> : row_records_kernel<128, false>);
+  SB_LAUNCH_OK(launch_k(kernel, (unsigned)(expanding + a.H * a.B * ((a.J + 63) / 64)), 256, 0, s, a, st, x, records,
                         sizes, pieces(dout) && pieces(out) ? 1 : 0, pieces(v) ? 1 : 0, expanding, values));
   SB_TRY(pack_indirect(s, scratch, pl.p.at, {&dout, &q, &k, &v}));
   float* partial = reinterpret_cast<float*>(base + pl.partial);
