@@ -372,8 +372,8 @@ __device__ __forceinline__ void row_tile(uint32_t s, uint32_t to, bool started, 
 // multiplied a tile ahead of the softmax, by a warp of their own: with one warp for both products and one buffer, issuing and
 // handing over took most of the time.  Exponentials go back into tensor memory as 16-bit pairs (rounded once, as an operand of the
 // second product has to be), where that product takes them from.  Softmax warps: thread = row.
-// B=2, L=4096, 16 heads of 64 (137 GFLOP): 244 us, 34 % of the measured matrix rate; B=8, L=512: 27 us; B=2, L=2000 causal, 16 heads
-// of 128 on 4: 55 us.  Bound by the softmax warps, of which a scheduler has two: exponentials keep their unit busy for 53 % of the
+// Calls, with the rows of biases, replayed from a graph: B=2, L=4096, 16 heads of 64 (137 GFLOP) 242 us, 35 % of the measured matrix rate;
+// B=8, L=512: 26 us; B=2, L=2000 causal, 16 heads of 128 on 4: 53 us.  Bound by the softmax warps, of which a scheduler has two: exponentials keep their unit busy for 53 % of the
 // time (without any 20 % less), half of it per tile of 64 columns is waiting for one's own results; without softmax 140 us.
 template <int P>
 __global__ void __launch_bounds__(kFwdThreads, 2)
@@ -752,7 +752,8 @@ __device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float fl
 // float16: the warp that finds the items' shifts.  Added to the biases of a key item they make its exponentials 2^shift times as large.
 // A CTA's first item waits for that (and for every line of this code to be fetched, which is why it is short), later ones do not.  All
 // that float16 has for its range, this warp and the sizes that row_records_kernel finds, takes 5.5 us of a forward and backward call at
-// B=8, L=512 (108.9 -> 114.4), as many at B=96, L=128 (115.4 -> 120.9) and 3 at B=2, L=4096 (884 -> 887).
+// B=8, L=512 (109.2 -> 114.7), 5 at B=96, L=128 (116.1 -> 121.0) and 5 at B=2, L=4096 (884 -> 889).  One more multiplication for every
+// score gradient of a key item, instead of shifted biases, took 2 us more at B=8 and 10 at L=4096.
 struct ShiftWarp {
   const uint8_t *slots, *held;
   float4* biases;                                    // two rows
@@ -809,10 +810,11 @@ __device__ __forceinline__ void shift_warp(const BwdParams& p, const ShiftWarp& 
 // pairs, rounded once as operands have to be, where the second products take them from.  Everything is
 // computed twice, once per kind of item (but for BOTH); the alternative, dQ summed over key tiles in memory, needs atomics whose order
 // changes the result, or a partial dQ for every key tile.
-// B=2, L=4096, 16 heads of 64 (344 GFLOP, of which 481 are multiplied): 658 us, 32 % of the measured matrix rate; B=2, L=2000 causal, 16
-// heads of 128 on 4: 203 us; B=8, L=512: 77 us; BOTH at B=96, L=128: 74 us, bound by its items' beginnings and ends.  Without element
-// work 410 us, without products 599: the element warps' instructions, two warps per scheduler.  A third group (128 registers a
-// thread) took 694 us, scores from tensor memory 630 at best.
+// Calls, with records and the table's last sums, replayed from a graph: B=2, L=4096, 16 heads of 64 (344 GFLOP needed, 481 multiplied, as
+// scores and dP are computed twice) 666 us, 32 % of the measured matrix rate on what is needed (forward and backward together 904 in that
+// run); B=2, L=2000 causal, 16 heads of 128 on 4: 218 us; B=8, L=512: 83 us; BOTH at B=96, L=128: 88 us, bound by its items' beginnings
+// and ends.  This kernel alone, where it took 658 us: without element work 410, without products 599: the element warps' instructions,
+// two warps per scheduler.  A third group (128 registers a thread) took 694 us, scores from tensor memory 630 at best.
 // The table's gradient: a score gradient belongs to its relative position, a diagonal of the tile.  A warp moves each column of
 // its 32 x 32 blocks so that lane l holds diagonals l and l - 32 (one shuffle a column), adds the sums of a block to its own row
 // of sums over relative positions, and a group of warps adds up its four rows per item.  Tiles outside the varying part of the
