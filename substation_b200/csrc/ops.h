@@ -133,7 +133,7 @@ constexpr bool kRelScaled = true;
 #endif
 // Backward: `records` [B][H][ceil(J / 64)][192]: of 64 query rows the log-sum-exps in units of log2 (+inf: row without keys, or
 // none), D and the weight (0 or 1) of the row in the table's sums; `sizes` (kRelScaled): for 64 rows of dout,
-// [B][H][ceil(J / 64)], then, but for rel_both, of v, [B][G][ceil(K / 64)], eight numbers whose largest is the largest
+// [B][H][ceil(J / 64)], then, but for rel_both, of out and of v, [B][G][ceil(K / 64)], eight numbers whose largest is the largest
 // magnitude, not counting rows without keys, behind the length or with an infinity, and no NaN; `partial` [H][B * ceil(J / 128) * 2][2 * reach + 1]
 // sums of score gradients by relative position; `next`: a zero.
 struct RelBackward { const float* records; const float* sizes; float* partial; int* next; };

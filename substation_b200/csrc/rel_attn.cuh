@@ -616,7 +616,7 @@ struct BwdParams {
   int sets;                                          // rows of sums per warp (1 or 2)
   float scale;
   const float* records;                              // [B][H][ceil(J / 64)][kRecord]
-  const float* sizes;                                // [B][H][ceil(J / 64)][8], but for BOTH [B][G][ceil(K / 64)][8]
+  const float* sizes;                                // [B][H][ceil(J / 64)][8], but for BOTH the same again, [B][G][ceil(K / 64)][8]
   float* partial;                                    // [H][B * nq * 2][2 * reach + 1]
   int* next;                                         // work queue
   Proj dq, dk, dv;
@@ -652,27 +652,32 @@ __device__ __forceinline__ Item bwd_item(const BwdParams& p, int i) {
 }
 
 // float16: an item's score gradients are rounded to 16 bits times 2^shift, its softmax weights times 2^max(shift, 0), which results lose
-// again.  A weight w is at most one, so that a shift of at most 15 keeps it.  A score gradient is w (dP - D), a difference of values of
-// dP, which are at most N = P max|dout| max|v| in size, times w (1 - w): at most N / 2.  Times 2^16 over the next power of two from N on
-// that is at most 2^15.  The maxima are of all rows that the item meets (dK and dV sum over them, so they share a factor).
+// again.  A weight w is at most one, so that a shift of at most 15 keeps it.  A score gradient is w (dP - D) = w dout (v - out), at most
+// N = P max|dout| (max|v| + max|out|): times 2^15 over the next power of two from N on it is held.  The maxima are of the rows that the
+// item meets (dK and dV sum over them, so they share a factor).  An item of queries has the v of all its keys, which bound its out; then
+// the difference is one of two values of dP, at most P max|dout| max|v| each, times w (1 - w), which is half that at most.  So what is looked
+// at for an item grows as its own work does.
 
-// The largest of n magnitudes, as the lane finds it.
-__device__ __forceinline__ float largest_of(const float* at, int n, int lane) {
-  float m = 0.f;
+// The largest magnitudes of three lists, n[.] blocks of eight each, as the lane finds them; all three are on their way together.
+__device__ __forceinline__ void largest_of(const float* const (&at)[3], const int (&n)[3], int lane, float (&m)[3]) {
+  m[0] = m[1] = m[2] = 0.f;
 #pragma unroll 1
-  for (int i = lane; i < n; i += 128) {
-    float v[4];
+  for (int i = lane; i < 2 * max(n[0], max(n[1], n[2])); i += 64) {
+    float4 v[3][2];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = i + 32 * k < n ? at[i + 32 * k] : 0.f;
-    m = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), m);
+    for (int x = 0; x < 3; ++x)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        v[x][k] = i + 32 * k < 2 * n[x] ? reinterpret_cast<const float4*>(at[x])[i + 32 * k] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < 3; ++x)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) m[x] = fmaxf(m[x], fmaxf(fmaxf(v[x][k].x, v[x][k].y), fmaxf(v[x][k].z, v[x][k].w)));
   }
-  return m;
 }
-__device__ __forceinline__ int item_shift(float g, float v, int P) {
-  const uint32_t mg = __reduce_max_sync(0xffffffffu, __float_as_uint(g)), mv = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
-  const float n = __uint_as_float(mg) * __uint_as_float(mv) * (float)P;   // (of float16's numbers: 0, or from 2^-48 to 2^39)
-  return n > 0.f ? min(15, 142 - (int)(__float_as_uint(n) >> 23)) : 15;
-}
+__device__ __forceinline__ float largest_in_warp(float v) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))); }
+// 2^top over the next power of two from n on, 2^15 at most.  (n: of float16's numbers 0, or from 2^-48 to 2^40)
+__device__ __forceinline__ int item_shift(float n, int top) { return n > 0.f ? min(15, top + 126 - (int)(__float_as_uint(n) >> 23)) : 15; }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // BOTH: units of one tile of queries and one of keys, each key head with one query head: an item gives all three gradients and
@@ -751,9 +756,10 @@ __device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float fl
 
 // float16: the warp that finds the items' shifts.  Added to the biases of a key item they make its exponentials 2^shift times as large.
 // A CTA's first item waits for that (and for every line of this code to be fetched, which is why it is short), later ones do not.  All
-// that float16 has for its range, this warp and the sizes that row_records_kernel finds, takes 5.5 us of a forward and backward call at
-// B=8, L=512 (109.2 -> 114.7), 5 at B=96, L=128 (116.1 -> 121.0) and 5 at B=2, L=4096 (884 -> 889).  One more multiplication for every
-// score gradient of a key item, instead of shifted biases, took 2 us more at B=8 and 10 at L=4096.
+// that float16 has for its range, this warp and the sizes that row_records_kernel finds, takes 5 us of a forward and backward call at B=8,
+// L=512 (108.5 -> 113.3), as many at B=96, L=128 (114.9 -> 120.5) and at B=2, L=2000 causal, 128 features (269 -> 273.5), and nothing to
+// be seen at B=2, L=4096.  One more multiplication for every score gradient of a key item, instead of shifted biases, took 2 us more
+// at B=8 and 10 at L=4096; this warp's code behind the others' 1 to 4 us.
 struct ShiftWarp {
   const uint8_t *slots, *held;
   float4* biases;                                    // two rows
@@ -768,21 +774,21 @@ __device__ __forceinline__ void shift_warp(const BwdParams& p, const ShiftWarp& 
   Item w;
   while (ok && take_item(s.slots, s.item_full, s.item_empty, &taken, lane, &w, &ok)) {
     if (w.tiles == 0) continue;
-    const float mg = largest_of(p.sizes + 8 * (((long long)w.b * p.c.H + (w.kind ? w.h : w.h * rep)) * blocks + (w.kind ? 2 * w.t : 0)),
-                                8 * (w.kind ? min(2, blocks - 2 * w.t) : rep * blocks), lane);
-    float mv = 0.f;
+    const long long of_out = 8ll * p.c.B * p.c.H * blocks;
+    const float* rows = p.sizes + 8 * (((long long)w.b * p.c.H + (w.kind ? w.h : w.h * rep)) * blocks + (w.kind ? 2 * w.t : 0));
+    const float* values = p.sizes + 2 * of_out + 8 * (((long long)w.b * p.c.G + (w.kind ? w.h / rep : w.h)) * blocks_v + (w.kind ? 0 : 2 * w.t));
+    const int n = w.kind ? min(2, blocks - 2 * w.t) : rep * blocks;
+    float m[3];                                      // of dout, out, v
+    largest_of({rows, rows + of_out, values}, {n, BOTH || w.kind ? 0 : n, BOTH ? 0 : w.kind ? (w.keys + 63) >> 6 : min(2, blocks_v - 2 * w.t)}, lane, m);
     if (BOTH) {                                      // the held values, 16 bytes at a time
       const uint32_t hb = p.held == 2 ? live & 1u : 0u, hp = p.held == 2 ? live >> 1 : live;
       ok = __all_sync(0xffffffffu, mbar_wait(s.h_full + 8 * hb, hp & 1u, 63));
       if (!ok) return;
       const uint4* tile = reinterpret_cast<const uint4*>(s.held + hb * BwdCfg<P, BOTH>::kHeld + 256 * P);
 #pragma unroll 2
-      for (int i = lane; i < w.keys * 8; i += 32) mv = fmaxf(mv, finite_size(larger(half2_of(0u), tile[i])));
-    } else {
-      mv = largest_of(p.sizes + 8 * ((long long)p.c.B * p.c.H * blocks + ((long long)w.b * p.c.G + (w.kind ? w.h / rep : w.h)) * blocks_v),
-                      8 * ((w.keys + 63) >> 6), lane);
+      for (int i = lane; i < w.keys * 8; i += 32) m[2] = fmaxf(m[2], finite_size(larger(half2_of(0u), tile[i])));
     }
-    const int shift = item_shift(mg, mv, p.c.P);
+    const int shift = item_shift(largest_in_warp(m[0]) * (largest_in_warp(m[1]) + largest_in_warp(m[2])) * (float)p.c.P, BOTH || w.kind ? 16 : 15);
     for (int done = 0; done < w.tiles; done += w.each, ++run) {
       ok = __all_sync(0xffffffffu, mbar_wait(s.b_full + 8 * (run & 1u), (run >> 1) & 1u, 63));
       if (!ok) return;
@@ -886,7 +892,9 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
   uint32_t taken = 0;
   auto take = [&](Item* w, bool* ok) { return take_item(slots, item_full, item_empty, &taken, lane, w, ok); };
 
-  if (warp == 0) {
+  if (kRelScaled && warp == 11) {
+    shift_warp<P, BOTH>(p, ShiftWarp{slots, gen, reinterpret_cast<float4*>(gen + (sbias - sheld)), shifts, item_full, item_empty, h_full, b_full, b_ready});
+  } else if (warp == 0) {
     // ---------------- producer ----------------
     // live: items with tiles; run: tiles of one head in an item, which share a row of biases
     uint32_t put = 0, live = 0, run = 0, st = 0, st_phase = 1;
@@ -1007,8 +1015,6 @@ rel_bwd_kernel(const __grid_constant__ CUtensorMap tmQh, const __grid_constant__
       }
       ++live;
     }
-  } else if (kRelScaled && warp == 11) {
-    shift_warp<P, BOTH>(p, ShiftWarp{slots, gen, reinterpret_cast<float4*>(gen + (sbias - sheld)), shifts, item_full, item_empty, h_full, b_full, b_ready});
   } else {
     // ---------------- element warps ----------------
     const int q = warp & 3, g = (warp - 3) >> 2, rt = q * 32 + lane;

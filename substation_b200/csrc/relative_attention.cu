@@ -473,9 +473,9 @@ join_splits_kernel(const __grid_constant__ FewParams p) {
 // What the backward pass knows of 64 query rows (RelBackward in ops.h), four threads a row, and in the blocks before those the rows
 // of biases.  `vec`, `vec_v`: dout and out, and v, have unit-stride features in 16-byte pieces; else lanes run along rows.  Bound by
 // reading dout and out once (B=96, L=128, 16 heads of 64, 50 MB: 11 us, 70 % of the copy bandwidth), so everything is asked for before
-// anything is waited for: one trip to memory a block (18 us with a barrier before the sums and another trip behind it).  The sizes of
-// v, float16 only, are shared out to the same blocks, so that they are under way beside the rest; maxima go out per warp, without a barrier
-// (2 us less at B=96).
+// anything is waited for: one trip to memory a block (18 us with a barrier before the sums and another trip behind it).  VALUES, float16
+// only: block n also looks at the n-th 64 rows of v, so that they are under way beside the rest; there are as many blocks as the longer of
+// the two needs.  Maxima go out per warp, without a barrier (2 us less at B=96).
 __device__ __forceinline__ float sum_of_four(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 1);
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
@@ -484,16 +484,23 @@ __device__ __forceinline__ float largest_of_four(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
+template <int N>
+__device__ __forceinline__ float largest_of_row(const uint4 (&u)[N]) {
+  sb_half2 m = half2_of(0u);
+#pragma unroll
+  for (int c = 0; c < N; ++c) m = larger(m, u[c]);
+  return largest_of_four(larger_half(m));
+}
 // The largest of a warp's values, none negative, to the warp's place; what is not finite does not count.
 __device__ __forceinline__ void store_largest(float value, float* to) {
   const uint32_t most = __reduce_max_sync(0xffffffffu, value < INFINITY ? __float_as_uint(value) : 0u);
   if ((threadIdx.x & 31) == 0) to[threadIdx.x >> 5] = __uint_as_float(most);
 }
 template <int P, bool VALUES>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, VALUES ? (P == 64 ? 4 : 3) : 1)
 row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const __grid_constant__ Expand x, float* records, float* sizes,
-                   int vec, int vec_v, int expanding, int values) {
-  __shared__ float part[4][64], large[4][64];
+                   int vec, int vec_v, int expanding, int rows, int values) {
+  __shared__ float part[4][64], large[2][4][64];
   grid_dependency_sync();
   const int it = (int)blockIdx.x - expanding;
   if (it < 0) {
@@ -502,119 +509,110 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
     return;
   }
   // blocks that run together share tokens, whose heads usually lie side by side
-  const int blocks = (a.J + 63) / 64, h = it % a.H, block = it / a.H % blocks, b = it / a.H / blocks;
-  const int row = vec ? threadIdx.x >> 2 : threadIdx.x & 63, i = vec ? threadIdx.x & 3 : threadIdx.x >> 6, j = block * 64 + row;
-  const bool live = j < a.J;
-  const sb_half* g = row_of(a.g, h, b, live ? j : 0);
-  const sb_half* o = row_of(a.o, h, b, live ? j : 0);
-  uint4 gv[P / 32], ov[P / 32], vv[P / 32];
-  if (vec)
-#pragma unroll
-    for (int c = 0; c < P / 32; ++c) {
-      const int p = i * 8 + c * 32;
-      gv[c] = ov[c] = make_uint4(0u, 0u, 0u, 0u);
-      if (p < a.P) {
-        gv[c] = *reinterpret_cast<const uint4*>(g + p);
-        ov[c] = *reinterpret_cast<const uint4*>(o + p);
-      }
-    }
-  // the n-th 64 rows of v: this thread's part of its row, zeros behind the length
-  const int vrow = vec_v ? threadIdx.x >> 2 : threadIdx.x & 63, vi = vec_v ? threadIdx.x & 3 : threadIdx.x >> 6, blocks_v = (a.K + 63) / 64;
-  struct Rows { const sb_half* at; float* to; };             // at: null behind the length
-  auto rows_of_v = [&](int n) {
-    const int hk = n % a.G, bv = n / a.G / blocks_v, k = n / a.G % blocks_v * 64 + vrow;
-    return Rows{k < keys_of(a, bv) ? row_of(a.v, hk, bv, k) : nullptr,
-                sizes + ((long long)a.B * a.H * blocks + ((long long)bv * a.G + hk) * blocks_v + n / a.G % blocks_v) * 8};
-  };
-  auto load_v = [&](const sb_half* at) {
+  const int blocks = (a.J + 63) / 64, blocks_v = (a.K + 63) / 64;
+  const long long sizes_of_out = 8ll * a.B * a.H * blocks;
+  const int vrow = vec_v ? threadIdx.x >> 2 : threadIdx.x & 63, vi = vec_v ? threadIdx.x & 3 : threadIdx.x >> 6;
+  const int hk = it % a.G, bv = it / a.G / blocks_v, block_v = it / a.G % blocks_v, k = block_v * 64 + vrow;
+  uint4 vv[P / 32];
+  const sb_half* v = nullptr;                                // null behind the length
+  if (VALUES && it < values && k < keys_of(a, bv)) v = row_of(a.v, hk, bv, k);
+  if (VALUES && vec_v)
 #pragma unroll
     for (int c = 0; c < P / 32; ++c) {
       const int p = vi * 8 + c * 32;
       vv[c] = make_uint4(0u, 0u, 0u, 0u);
-      if (at && p < a.P) vv[c] = *reinterpret_cast<const uint4*>(at + p);
+      if (v && p < a.P) vv[c] = *reinterpret_cast<const uint4*>(v + p);
     }
-  };
-  Rows rv = {nullptr, nullptr};
-  if (VALUES && it < values) {
-    rv = rows_of_v(it);
-    if (vec_v) load_v(rv.at);
-  }
-  float lse = 0.f;
-  int n = 0, pos = 0;
-  if (i == 0) {
-    lse = a.lse.p[h * a.lse.sH + b * a.lse.sB + (live ? j : 0) * a.lse.sJ];
-    n = keys_of(a, b);
-    pos = first_of(a, b) + j;
-  }
-  float sum = 0.f, size = 0.f;
-  if (vec) {
+  if (!VALUES || it < rows) {
+    const int h = it % a.H, block = it / a.H % blocks, b = it / a.H / blocks;
+    const int row = vec ? threadIdx.x >> 2 : threadIdx.x & 63, i = vec ? threadIdx.x & 3 : threadIdx.x >> 6, j = block * 64 + row;
+    const bool live = j < a.J;
+    const sb_half* g = row_of(a.g, h, b, live ? j : 0);
+    const sb_half* o = row_of(a.o, h, b, live ? j : 0);
+    uint4 gv[P / 32], ov[P / 32];
+    if (vec)
 #pragma unroll
-    for (int c = 0; c < P / 32; ++c) {
-      float u[8], v[8];
-      unpack8(gv[c], u);
-      unpack8(ov[c], v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf(u[e], v[e], sum);
-    }
-    sum = sum_of_four(sum);
-    if (kRelScaled) {
-      sb_half2 m = half2_of(0u);
-#pragma unroll
-      for (int c = 0; c < P / 32; ++c) m = larger(m, gv[c]);
-      size = largest_of_four(larger_half(m));
-    }
-  } else {
-#pragma unroll 4
-    for (int p = i; p < a.P; p += 4) {
-      const float u = sb_h2f(g[p * a.g.sP]);
-      sum = fmaf(u, sb_h2f(o[p * a.o.sP]), sum);
-      if (kRelScaled) size = fmaxf(size, fabsf(u));
-    }
-    part[i][row] = sum;
-    if (kRelScaled) large[i][row] = size;
-    __syncthreads();
+      for (int c = 0; c < P / 32; ++c) {
+        const int p = i * 8 + c * 32;
+        gv[c] = ov[c] = make_uint4(0u, 0u, 0u, 0u);
+        if (p < a.P) {
+          gv[c] = *reinterpret_cast<const uint4*>(g + p);
+          ov[c] = *reinterpret_cast<const uint4*>(o + p);
+        }
+      }
+    float lse = 0.f;
+    int n = 0, pos = 0;
     if (i == 0) {
-      sum = (part[0][row] + part[1][row]) + (part[2][row] + part[3][row]);
-      if (kRelScaled) size = fmaxf(fmaxf(large[0][row], large[1][row]), fmaxf(large[2][row], large[3][row]));
+      lse = a.lse.p[h * a.lse.sH + b * a.lse.sB + (live ? j : 0) * a.lse.sJ];
+      n = keys_of(a, b);
+      pos = first_of(a, b) + j;
     }
-  }
-  if (i == 0) {
-    if (a.causal) n = max(0, min(n, pos + 1));
-    // a row's score gradients sum to zero, so a row whose keys all share a bucket adds nothing to the table: its sum would
-    // only be what D, from the rounded output, is off by
-    // (seldom; most rows have keys on both sides or, of the far ones, before and within the reach, and need no search)
-    const int lo = -pos, hi = n - 1 - pos, last = st.s[a.n - 1];
-    const bool sides = (a.bidirectional && lo <= 0 && hi > 0) || (last > 0 && lo <= -last && hi > -last);
-    const bool alike = n <= 0 || (!sides && bucket_of(a, st.s, lo) == bucket_of(a, st.s, hi));
-    float* r = records + (((long long)b * a.H + h) * blocks + block) * 192 + row;
-    r[0] = live && lse != -INFINITY ? lse * 1.4426950408889634f : INFINITY;
-    r[64] = live ? sum : 0.f;
-    r[128] = live && alike ? 0.f : 1.f;
-  }
-  if (kRelScaled) {
-    store_largest(i == 0 && live && lse != -INFINITY ? size : 0.f, sizes + (((long long)b * a.H + h) * blocks + block) * 8);
-    for (int m = it; VALUES && m < values; m += (int)gridDim.x - expanding) {
-      if (m != it) {
-        rv = rows_of_v(m);
-        if (vec_v) load_v(rv.at);
-      }
-      float s = 0.f;
-      if (vec_v) {
-        sb_half2 m2 = half2_of(0u);
+    float sum = 0.f, size_g = 0.f, size_o = 0.f;
+    if (vec) {
 #pragma unroll
-        for (int c = 0; c < P / 32; ++c) m2 = larger(m2, vv[c]);
-        s = largest_of_four(larger_half(m2));
-      } else {
-        if (rv.at)
-#pragma unroll 4
-          for (int p = vi; p < a.P; p += 4) s = fmaxf(s, fabsf(sb_h2f(rv.at[p * a.v.sP])));
-        __syncthreads();                                     // (`large` may still be read)
-        large[vi][vrow] = s;
-        __syncthreads();
-        s = vi == 0 ? fmaxf(fmaxf(large[0][vrow], large[1][vrow]), fmaxf(large[2][vrow], large[3][vrow])) : 0.f;
+      for (int c = 0; c < P / 32; ++c) {
+        float u[8], w[8];
+        unpack8(gv[c], u);
+        unpack8(ov[c], w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(u[e], w[e], sum);
       }
-      store_largest(s, rv.to);
+      sum = sum_of_four(sum);
+      if (kRelScaled) size_g = largest_of_row(gv);
+      if (VALUES) size_o = largest_of_row(ov);
+    } else {
+#pragma unroll 4
+      for (int p = i; p < a.P; p += 4) {
+        const float u = sb_h2f(g[p * a.g.sP]), w = sb_h2f(o[p * a.o.sP]);
+        sum = fmaf(u, w, sum);
+        if (kRelScaled) size_g = fmaxf(size_g, fabsf(u));
+        if (VALUES) size_o = fmaxf(size_o, fabsf(w));
+      }
+      part[i][row] = sum;
+      if (kRelScaled) large[0][i][row] = size_g;
+      if (VALUES) large[1][i][row] = size_o;
+      __syncthreads();
+      if (i == 0) {
+        auto most = [&](const float (&l)[4][64]) { return fmaxf(fmaxf(l[0][row], l[1][row]), fmaxf(l[2][row], l[3][row])); };
+        sum = (part[0][row] + part[1][row]) + (part[2][row] + part[3][row]);
+        if (kRelScaled) size_g = most(large[0]);
+        if (VALUES) size_o = most(large[1]);
+      }
     }
+    if (i == 0) {
+      if (a.causal) n = max(0, min(n, pos + 1));
+      // a row's score gradients sum to zero, so a row whose keys all share a bucket adds nothing to the table: its sum would
+      // only be what D, from the rounded output, is off by
+      // (seldom; most rows have keys on both sides or, of the far ones, before and within the reach, and need no search)
+      const int lo = -pos, hi = n - 1 - pos, last = st.s[a.n - 1];
+      const bool sides = (a.bidirectional && lo <= 0 && hi > 0) || (last > 0 && lo <= -last && hi > -last);
+      const bool alike = n <= 0 || (!sides && bucket_of(a, st.s, lo) == bucket_of(a, st.s, hi));
+      float* r = records + (((long long)b * a.H + h) * blocks + block) * 192 + row;
+      r[0] = live && lse != -INFINITY ? lse * 1.4426950408889634f : INFINITY;
+      r[64] = live ? sum : 0.f;
+      r[128] = live && alike ? 0.f : 1.f;
+    }
+    if (kRelScaled) {
+      const bool counts = i == 0 && live && lse != -INFINITY;
+      float* to = sizes + (((long long)b * a.H + h) * blocks + block) * 8;
+      store_largest(counts ? size_g : 0.f, to);
+      if (VALUES) store_largest(counts ? size_o : 0.f, to + sizes_of_out);
+    }
+  }
+  if (VALUES && it < values) {
+    float s = 0.f;
+    if (vec_v) {
+      s = largest_of_row(vv);
+    } else {
+      if (v)
+#pragma unroll 4
+        for (int p = vi; p < a.P; p += 4) s = fmaxf(s, fabsf(sb_h2f(v[p * a.v.sP])));
+      __syncthreads();                                       // (`large` may still be read)
+      large[0][vi][vrow] = s;
+      __syncthreads();
+      s = vi == 0 ? fmaxf(fmaxf(large[0][0][vrow], large[0][1][vrow]), fmaxf(large[0][2][vrow], large[0][3][vrow])) : 0.f;
+    }
+    store_largest(s, sizes + 2 * sizes_of_out + (((long long)bv * a.G + hk) * blocks_v + block_v) * 8);
   }
 }
 
@@ -815,7 +813,7 @@ BwdPlan bwd_plan(const Proj& dout, const Proj& q, const Proj& k, const Proj& v, 
   b.records = b.p.bytes;
   const size_t blocks = (size_t)q.H * q.B * ((q.R + 63) / 64), blocks_v = (size_t)v.H * v.B * ((v.R + 63) / 64);
   b.sizes = b.records + align256(sizeof(float) * 192 * blocks);
-  b.partial = b.sizes + (kRelScaled ? align256(sizeof(float) * 8 * (blocks + blocks_v)) : 0);
+  b.partial = b.sizes + (kRelScaled ? align256(sizeof(float) * 8 * (2 * blocks + blocks_v)) : 0);
   b.bytes = b.partial + align256(sizeof(float) * (size_t)q.H * b.rows * (2 * b.p.reach + 1));
   return b;
 }
@@ -841,8 +839,9 @@ int launch_rel_attn_bwd(cudaStream_t s, void* scratch, Proj dout, Proj q, Proj k
   const int expanding = a.H * expand_blocks(x.pitch), values = kRelScaled && !rel_both(q, k) ? a.G * a.B * ((a.K + 63) / 64) : 0;
   auto kernel = values ? (q.P <= 64 ? row_records_kernel<64, kRelScaled> : row_records_kernel<128, kRelScaled>)
                        : (q.P <= 64 ? row_records_kernel<64, false> : row_records_kernel<128, false>);
-  SB_LAUNCH_OK(launch_k(kernel, (unsigned)(expanding + a.H * a.B * ((a.J + 63) / 64)), 256, 0, s, a, st, x, records,
-                        sizes, pieces(dout) && pieces(out) ? 1 : 0, pieces(v) ? 1 : 0, expanding, values));
+  const int rows = a.H * a.B * ((a.J + 63) / 64);
+  SB_LAUNCH_OK(launch_k(kernel, (unsigned)(expanding + std::max(rows, values)), 256, 0, s, a, st, x, records, sizes,
+                        pieces(dout) && pieces(out) ? 1 : 0, pieces(v) ? 1 : 0, expanding, rows, values));
   SB_TRY(pack_indirect(s, scratch, pl.p.at, {&dout, &q, &k, &v}));
   float* partial = reinterpret_cast<float*>(base + pl.partial);
   SB_TRY(launch_rel_tiles_bwd(s, dout, q, k, v, tables_of(x), RelBackward{records, sizes, partial, x.next}, dq, dk, dv, span));
