@@ -380,8 +380,8 @@ typedef struct sb_attention_span {
  * infinity at a key within the length, in v, in k behind a bias of -inf, or in the backward pass in any operand, may reach queries of
  * the sample that do not see that key.  Scores are not stored anywhere; exponentials are rounded to 16 bits where they meet v (float16
  * holds them in steps of 2^-31 of the row's largest or finer), sums are fp32.  Few queries against many keys are split along the
- * keys and joined by a second kernel.  out and lse overlap neither each other nor any input.  scratch: sb_relative_attention_scratch_bytes() for the
- * same operands (may be 0), 16-byte aligned, as above. */
+ * keys and joined by a second kernel.  out and lse overlap neither each other nor any input.  scratch:
+ * sb_relative_attention_scratch_bytes() for the same operands (may be 0), 16-byte aligned, as above. */
 int sb_relative_attention(void* stream, void* scratch, size_t scratch_bytes, const sb_tensor* q, const sb_tensor* k,
                           const sb_tensor* v, const sb_relative_bias* bias, const sb_tensor* out, const sb_tensor* lse,
                           const sb_attention_span* span);
@@ -391,8 +391,8 @@ int sb_relative_attention_scratch_bytes(const sb_tensor* q, const sb_tensor* k, 
  *   D = sum_p dout out,  ds = softmax * (sum_p dout v - D),  dv = sum_{j} softmax dout,  dk = scale sum_j ds q,
  *   dq = scale sum_k ds k,  dtable[n,h] = sum of ds over the batch's pairs in bucket n.
  * Softmax and ds are rounded to 16 bits where they meet dout, q and k (not on their way into dtable), in float16 after a
- * multiplication by powers of two that follow from the largest |dout| and |v| of the rows concerned, so that neither underflows
- * or overflows before the results do; D is taken from the rounded out; sums are fp32.
+ * multiplication by powers of two that follow from the largest |dout|, |v| and |out| of the rows concerned, so that neither
+ * underflows or overflows before the results do; D is taken from the rounded out; sums are fp32.
  * dk and dv of shared heads are sums over the query heads, and 0 behind a sample's length; every element of the five outputs
  * is written, and they overlap neither each other nor any input.  Sums run in a fixed order: the same call gives the same bits.  No
  * counterpart in the reference, which has neither positions nor padding. */

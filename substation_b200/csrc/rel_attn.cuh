@@ -373,8 +373,9 @@ __device__ __forceinline__ void row_tile(uint32_t s, uint32_t to, bool started, 
 // handing over took most of the time.  Exponentials go back into tensor memory as 16-bit pairs (rounded once, as an operand of the
 // second product has to be), where that product takes them from.  Softmax warps: thread = row.
 // Calls, with the rows of biases, replayed from a graph: B=2, L=4096, 16 heads of 64 (137 GFLOP) 242 us, 35 % of the measured matrix rate;
-// B=8, L=512: 26 us; B=2, L=2000 causal, 16 heads of 128 on 4: 53 us.  Bound by the softmax warps, of which a scheduler has two: exponentials keep their unit busy for 53 % of the
-// time (without any 20 % less), half of it per tile of 64 columns is waiting for one's own results; without softmax 140 us.
+// B=8, L=512: 26 us; B=2, L=2000 causal, 16 heads of 128 on 4: 53 us.  Bound by the softmax warps, of which a scheduler has two:
+// exponentials keep their unit busy for 53 % of the time (without any 20 % less), half of it per tile of 64 columns is waiting for one's
+// own results; without softmax 140 us.
 template <int P>
 __global__ void __launch_bounds__(kFwdThreads, 2)
 rel_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -616,7 +617,7 @@ struct BwdParams {
   int sets;                                          // rows of sums per warp (1 or 2)
   float scale;
   const float* records;                              // [B][H][ceil(J / 64)][kRecord]
-  const float* sizes;                                // [B][H][ceil(J / 64)][8], but for BOTH the same again, [B][G][ceil(K / 64)][8]
+  const float* sizes;                                // float16: [B][H][ceil(J / 64)][8], but for BOTH the same again and [B][G][ceil(K / 64)][8]
   float* partial;                                    // [H][B * nq * 2][2 * reach + 1]
   int* next;                                         // work queue
   Proj dq, dk, dv;
