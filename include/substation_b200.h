@@ -391,8 +391,8 @@ int sb_relative_attention_scratch_bytes(const sb_tensor* q, const sb_tensor* k, 
  *   D = sum_p dout out,  ds = softmax * (sum_p dout v - D),  dv = sum_{j} softmax dout,  dk = scale sum_j ds q,
  *   dq = scale sum_k ds k,  dtable[n,h] = sum of ds over the batch's pairs in bucket n.
  * Softmax and ds are rounded to 16 bits where they meet dout, q and k (not on their way into dtable), in float16 after a
- * multiplication by powers of two that follow from the largest |dout|, |v| and |out| of the rows concerned, so that neither
- * underflows or overflows before the results do; D is taken from the rounded out; sums are fp32.
+ * multiplication by powers of two that follow from the longest rows of dout, v and out concerned, so that neither underflows
+ * or overflows before the results do; D is taken from the rounded out; sums are fp32.
  * dk and dv of shared heads are sums over the query heads, and 0 behind a sample's length; every element of the five outputs
  * is written, and they overlap neither each other nor any input.  Sums run in a fixed order: the same call gives the same bits.  No
  * counterpart in the reference, which has neither positions nor padding. */

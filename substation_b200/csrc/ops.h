@@ -133,8 +133,8 @@ constexpr bool kRelScaled = true;
 #endif
 // Backward: `records` [B][H][ceil(J / 64)][192]: of 64 query rows the log-sum-exps in units of log2 (+inf: row without keys, or
 // none), D and the weight (0 or 1) of the row in the table's sums; `sizes` (kRelScaled): for 64 rows of dout,
-// [B][H][ceil(J / 64)], then, but for rel_both, of out and of v, [B][G][ceil(K / 64)], eight numbers whose largest is the largest
-// magnitude, not counting rows without keys, behind the length or with an infinity, and no NaN; `partial`
+// [B][H][ceil(J / 64)], then, but for rel_both, of out and of v, [B][G][ceil(K / 64)], eight numbers whose largest is the largest sum
+// of squares of a row, not counting rows without keys or behind the length and sums that are not finite; `partial`
 // [H][B * ceil(J / 128) * 2][2 * reach + 1] sums of score gradients by relative position; `next`: a zero.
 struct RelBackward { const float* records; const float* sizes; float* partial; int* next; };
 // Units of one tile each way give all three gradients in one item; with shared key heads dQ would have to be stored per head.

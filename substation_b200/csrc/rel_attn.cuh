@@ -654,12 +654,13 @@ __device__ __forceinline__ Item bwd_item(const BwdParams& p, int i) {
 
 // float16: an item's score gradients are rounded to 16 bits times 2^shift, its softmax weights times 2^max(shift, 0), which results lose
 // again.  A weight w is at most one, so that a shift of at most 15 keeps it.  A score gradient is w (dP - D) = w dout (v - out), at most
-// N = P max|dout| (max|v| + max|out|): times 2^15 over the next power of two from N on it is held.  The maxima are of the rows that the
-// item meets (dK and dV sum over them, so they share a factor).  An item of queries has the v of all its keys, which bound its out; then
-// the difference is one of two values of dP, at most P max|dout| max|v| each, times w (1 - w), which is half that at most.  So what is looked
-// at for an item grows as its own work does.
+// N = |dout| (|v| + |out|) with the longest rows that the item meets (dK and dV sum over them, so they share a factor): times 2^15 over
+// the next power of two from N on it is held.  An item of queries has the v of all its keys, which bound its out; then the difference is one
+// of two values of dP, at most |dout| |v| each, times w (1 - w), which is half that at most.  So what is looked at for an item grows as
+// its own work does.  (A tight bound counts: largest magnitudes instead of norms gave shifts smaller by 4 to 5, with which keys of
+// a weight below 1e-6 beside output gradients of 30 lost digits that their own dk could hold, for 2 us less.)
 
-// The largest magnitudes of three lists, n[.] blocks of eight each, as the lane finds them; all three are on their way together.
+// The largest numbers of three lists, n[.] blocks of eight each, as the lane finds them; all three are on their way together.
 __device__ __forceinline__ void largest_of(const float* const (&at)[3], const int (&n)[3], int lane, float (&m)[3]) {
   m[0] = m[1] = m[2] = 0.f;
 #pragma unroll 1
@@ -677,8 +678,8 @@ __device__ __forceinline__ void largest_of(const float* const (&at)[3], const in
   }
 }
 __device__ __forceinline__ float largest_in_warp(float v) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))); }
-// 2^top over the next power of two from n on, 2^15 at most.  (n: of float16's numbers 0, or from 2^-48 to 2^40)
-__device__ __forceinline__ int item_shift(float n, int top) { return n > 0.f ? min(15, top + 126 - (int)(__float_as_uint(n) >> 23)) : 15; }
+// 2^top over the next power of two from the root of n2 on, 2^15 at most.  (n2: of float16's numbers 0, or from 2^-96 to 2^81)
+__device__ __forceinline__ int item_shift(float n2, int top) { return n2 > 0.f ? min(15, top - (((int)(__float_as_uint(n2) >> 23) - 125) >> 1)) : 15; }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // BOTH: units of one tile of queries and one of keys, each key head with one query head: an item gives all three gradients and
@@ -757,9 +758,9 @@ __device__ __forceinline__ void turn_tile(uint32_t ts, const float* bp, float fl
 
 // float16: the warp that finds the items' shifts.  Added to the biases of a key item they make its exponentials 2^shift times as large.
 // A CTA's first item waits for that (and for every line of this code to be fetched, which is why it is short), later ones do not.  All
-// that float16 has for its range, this warp and the sizes that row_records_kernel finds, takes 5 us of a forward and backward call at B=8,
-// L=512 (108.5 -> 113.3), as many at B=96, L=128 (114.9 -> 120.5) and at B=2, L=2000 causal, 128 features (269 -> 273.5), and nothing to
-// be seen at B=2, L=4096.  One more multiplication for every score gradient of a key item, instead of shifted biases, took 2 us more
+// that float16 has for its range, this warp and the sizes that row_records_kernel finds, takes 6.5 us of a forward and backward call at B=8,
+// L=512 (109.2 -> 115.7), 5.5 at B=96, L=128 (116.1 -> 121.6), 4 at B=2, L=2000 causal with 128 features (270 -> 274), and nothing to be
+// seen at B=2, L=4096.  One more multiplication for every score gradient of a key item, instead of shifted biases, took 2 us more
 // at B=8 and 10 at L=4096; this warp's code behind the others' 1 to 4 us.
 struct ShiftWarp {
   const uint8_t *slots, *held;
@@ -779,17 +780,19 @@ __device__ __forceinline__ void shift_warp(const BwdParams& p, const ShiftWarp& 
     const float* rows = p.sizes + 8 * (((long long)w.b * p.c.H + (w.kind ? w.h : w.h * rep)) * blocks + (w.kind ? 2 * w.t : 0));
     const float* values = p.sizes + 2 * of_out + 8 * (((long long)w.b * p.c.G + (w.kind ? w.h / rep : w.h)) * blocks_v + (w.kind ? 0 : 2 * w.t));
     const int n = w.kind ? min(2, blocks - 2 * w.t) : rep * blocks;
-    float m[3];                                      // of dout, out, v
+    float m[3];                                      // of dout, out, v: sums of squares
     largest_of({rows, rows + of_out, values}, {n, BOTH || w.kind ? 0 : n, BOTH ? 0 : w.kind ? (w.keys + 63) >> 6 : min(2, blocks_v - 2 * w.t)}, lane, m);
-    if (BOTH) {                                      // the held values, 16 bytes at a time
+    if (BOTH) {                                      // the held values, 16 bytes at a time: their largest magnitude
       const uint32_t hb = p.held == 2 ? live & 1u : 0u, hp = p.held == 2 ? live >> 1 : live;
       ok = __all_sync(0xffffffffu, mbar_wait(s.h_full + 8 * hb, hp & 1u, 63));
       if (!ok) return;
       const uint4* tile = reinterpret_cast<const uint4*>(s.held + hb * BwdCfg<P, BOTH>::kHeld + 256 * P);
 #pragma unroll 2
       for (int i = lane; i < w.keys * 8; i += 32) m[2] = fmaxf(m[2], finite_size(larger(half2_of(0u), tile[i])));
+      m[2] *= m[2] * (float)p.c.P;
     }
-    const int shift = item_shift(largest_in_warp(m[0]) * (largest_in_warp(m[1]) + largest_in_warp(m[2])) * (float)p.c.P, BOTH || w.kind ? 16 : 15);
+    const float n2 = largest_in_warp(m[0]) * (largest_in_warp(m[1]) + largest_in_warp(m[2]));
+    const int shift = BOTH || w.kind ? item_shift(n2, 16) : item_shift(2.f * n2, 15);   // ((|v| + |out|)^2 is at most 2 |v|^2 + 2 |out|^2)
     for (int done = 0; done < w.tiles; done += w.each, ++run) {
       ok = __all_sync(0xffffffffu, mbar_wait(s.b_full + 8 * (run & 1u), (run >> 1) & 1u, 63));
       if (!ok) return;

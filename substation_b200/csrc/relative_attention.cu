@@ -480,16 +480,13 @@ __device__ __forceinline__ float sum_of_four(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 1);
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
-__device__ __forceinline__ float largest_of_four(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-}
-template <int N>
-__device__ __forceinline__ float largest_of_row(const uint4 (&u)[N]) {
-  sb_half2 m = half2_of(0u);
+__device__ __forceinline__ float2 add_squares(const float (&v)[8], float2 sum) {
 #pragma unroll
-  for (int c = 0; c < N; ++c) m = larger(m, u[c]);
-  return largest_of_four(larger_half(m));
+  for (int e = 0; e < 8; e += 2) {
+    const float2 x = make_float2(v[e], v[e + 1]);
+    sum = fma2(x, x, sum);
+  }
+  return sum;
 }
 // The largest of a warp's values, none negative, to the warp's place; what is not finite does not count.
 __device__ __forceinline__ void store_largest(float value, float* to) {
@@ -497,10 +494,10 @@ __device__ __forceinline__ void store_largest(float value, float* to) {
   if ((threadIdx.x & 31) == 0) to[threadIdx.x >> 5] = __uint_as_float(most);
 }
 template <int P, bool VALUES>
-__global__ void __launch_bounds__(256, VALUES ? (P == 64 ? 4 : 3) : 1)
+__global__ void __launch_bounds__(256, VALUES ? (P == 64 ? 4 : 2) : 1)
 row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Starts st, const __grid_constant__ Expand x, float* records, float* sizes,
                    int vec, int vec_v, int expanding, int rows, int values) {
-  __shared__ float part[4][64], large[2][4][64];
+  __shared__ float part[3][4][64];
   grid_dependency_sync();
   const int it = (int)blockIdx.x - expanding;
   if (it < 0) {
@@ -547,8 +544,9 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
       n = keys_of(a, b);
       pos = first_of(a, b) + j;
     }
-    float sum = 0.f, size_g = 0.f, size_o = 0.f;
+    float sum = 0.f, square_g = 0.f, square_o = 0.f;
     if (vec) {
+      float2 of_g = make_float2(0.f, 0.f), of_o = of_g;
 #pragma unroll
       for (int c = 0; c < P / 32; ++c) {
         float u[8], w[8];
@@ -556,27 +554,29 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
         unpack8(ov[c], w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(u[e], w[e], sum);
+        if (kRelScaled) of_g = add_squares(u, of_g);
+        if (VALUES) of_o = add_squares(w, of_o);
       }
       sum = sum_of_four(sum);
-      if (kRelScaled) size_g = largest_of_row(gv);
-      if (VALUES) size_o = largest_of_row(ov);
+      if (kRelScaled) square_g = sum_of_four(of_g.x + of_g.y);
+      if (VALUES) square_o = sum_of_four(of_o.x + of_o.y);
     } else {
 #pragma unroll 4
       for (int p = i; p < a.P; p += 4) {
         const float u = sb_h2f(g[p * a.g.sP]), w = sb_h2f(o[p * a.o.sP]);
         sum = fmaf(u, w, sum);
-        if (kRelScaled) size_g = fmaxf(size_g, fabsf(u));
-        if (VALUES) size_o = fmaxf(size_o, fabsf(w));
+        if (kRelScaled) square_g = fmaf(u, u, square_g);
+        if (VALUES) square_o = fmaf(w, w, square_o);
       }
-      part[i][row] = sum;
-      if (kRelScaled) large[0][i][row] = size_g;
-      if (VALUES) large[1][i][row] = size_o;
+      part[0][i][row] = sum;
+      if (kRelScaled) part[1][i][row] = square_g;
+      if (VALUES) part[2][i][row] = square_o;
       __syncthreads();
       if (i == 0) {
-        auto most = [&](const float (&l)[4][64]) { return fmaxf(fmaxf(l[0][row], l[1][row]), fmaxf(l[2][row], l[3][row])); };
-        sum = (part[0][row] + part[1][row]) + (part[2][row] + part[3][row]);
-        if (kRelScaled) size_g = most(large[0]);
-        if (VALUES) size_o = most(large[1]);
+        auto all = [&](const float (&l)[4][64]) { return (l[0][row] + l[1][row]) + (l[2][row] + l[3][row]); };
+        sum = all(part[0]);
+        if (kRelScaled) square_g = all(part[1]);
+        if (VALUES) square_o = all(part[2]);
       }
     }
     if (i == 0) {
@@ -595,22 +595,32 @@ row_records_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ S
     if (kRelScaled) {
       const bool counts = i == 0 && live && lse != -INFINITY;
       float* to = sizes + (((long long)b * a.H + h) * blocks + block) * 8;
-      store_largest(counts ? size_g : 0.f, to);
-      if (VALUES) store_largest(counts ? size_o : 0.f, to + sizes_of_out);
+      store_largest(counts ? square_g : 0.f, to);
+      if (VALUES) store_largest(counts ? square_o : 0.f, to + sizes_of_out);
     }
   }
   if (VALUES && it < values) {
     float s = 0.f;
     if (vec_v) {
-      s = largest_of_row(vv);
+      float2 of_v = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < P / 32; ++c) {
+        float u[8];
+        unpack8(vv[c], u);
+        of_v = add_squares(u, of_v);
+      }
+      s = sum_of_four(of_v.x + of_v.y);
     } else {
       if (v)
 #pragma unroll 4
-        for (int p = vi; p < a.P; p += 4) s = fmaxf(s, fabsf(sb_h2f(v[p * a.v.sP])));
-      __syncthreads();                                       // (`large` may still be read)
-      large[0][vi][vrow] = s;
+        for (int p = vi; p < a.P; p += 4) {
+          const float u = sb_h2f(v[p * a.v.sP]);
+          s = fmaf(u, u, s);
+        }
+      __syncthreads();                                       // (`part` may still be read)
+      part[0][vi][vrow] = s;
       __syncthreads();
-      s = vi == 0 ? fmaxf(fmaxf(large[0][0][vrow], large[0][1][vrow]), fmaxf(large[0][2][vrow], large[0][3][vrow])) : 0.f;
+      s = vi == 0 ? (part[0][0][vrow] + part[0][1][vrow]) + (part[0][2][vrow] + part[0][3][vrow]) : 0.f;
     }
     store_largest(s, sizes + 2 * sizes_of_out + (((long long)bv * a.G + hk) * blocks_v + block_v) * 8);
   }

@@ -349,6 +349,32 @@ def test_many_rotations_in_turn(dtype):
     assert not wrong
 
 
+@pytest.mark.parametrize('dtype', BOTH)
+@pytest.mark.parametrize('size,values', [(30.0, 1.0), (30.0, 8.0), (1000.0, 0.05)])
+@pytest.mark.parametrize('P,H,G,B,J,K', [(64, 1, 1, 5, 3, 289), (80, 3, 3, 8, 2, 465), (128, 6, 2, 2, 1, 692), (64, 4, 4, 4, 5, 100)])
+def test_gradients_of_keys_that_hardly_count(P, H, G, B, J, K, size, values, dtype):
+    """Large output gradients, few queries and sharp softmaxes: keys of a weight of 1e-6 and less have gradients that are small beside the
+    others' of their item, but not beside what the type holds."""
+    ops = _ops()
+    gen = torch.Generator(device=DEV).manual_seed(K)
+    q, k, v, dout = (_make((P, h, B, n), 'BJHP', dtype, gen, x) for h, n, x in ((H, J, 2.0), (G, K, 2.0), (G, K, values), (H, J, size)))
+    table = torch.randn(32, H, generator=gen, device=DEV).to(dtype)
+    how = dict(buckets=ops.relative_buckets(), scale=P ** -0.5)
+    out, lse = _forward(q, k, v, table, how)
+    got = {n: torch.empty_like(x) for n, x in (('dq', q), ('dk', k), ('dv', v), ('dtable', table))}
+    ops.backward_relative_attention(dout, q, k, v, table, out, lse, *got.values(), **how)
+    want, bound = ref.attention(q, k, v, table, half=torch.finfo(dtype).eps / 2, dout=dout, out_used=out, **how)
+    # float16's numbers spread over 2^40, from 2^-24 on: an item whose score gradients may be as large as N = |dout| (|v| + |out|) rounds
+    # them in steps of 2^-24 times 2^-shift, and 2^-shift is below sqrt(2) 2 N / 2^15; the reference counts 2^-24
+    N = (dout.double().norm(dim=0).max() * (v.double().norm(dim=0).max() + out.double().norm(dim=0).max())).item()
+    coarse = 2.0 ** -25 * max(0.0, 2 ** 1.5 * N / 2 ** 15 - 1) if dtype is torch.float16 else 0.0
+    bound['dq'] = bound['dq'] + coarse * how['scale'] * k.double().abs().sum(3, keepdim=True).repeat_interleave(H // G, 1)
+    bound['dk'] = bound['dk'] + coarse * how['scale'] * q.double().abs().sum(3, keepdim=True).unflatten(1, (G, H // G)).sum(2)
+    for name in got:
+        held = want[name].abs() + bound[name] < torch.finfo(dtype).max
+        assert ((got[name].double() - want[name]).abs() <= bound[name])[held].all(), name
+
+
 # ---- what float16's range costs ----------------------------------------------------------------------------------------
 @pytest.mark.parametrize('J,K', [(64, 65536), (16384, 128)])
 def test_the_range_of_float16_costs_little_whatever_the_shape(J, K):
