@@ -305,7 +305,9 @@ __device__ __noinline__ void rescale(uint32_t to, uint32_t tp, bool started, int
 
 // A thread's row of 64 scores, 32 columns at a time while the next 32 are on their way: exponentials against the row's
 // reference as 16-bit pairs, which overwrite scores already read.  `settled` waits for the output.  The reference lags behind the
-// maximum by at most 2^kLazy; a chunk that exceeds it makes it rise before its own exponentials are taken.
+// maximum by at most 2^kLazy; a chunk that exceeds it makes it rise before its own exponentials are taken.  Exponentials of the tile's
+// first chunk, if there are any, are then rounded a second time.  (References that rise by whole powers of two would avoid that, but then
+// the row's largest exponential is rounded too, which is 1 otherwise: rows that one key rules lose more.)
 // NEAR: the bias varies, bp[c] is column c's; else it is `flat`.  MASK: columns from lim on are hidden.
 template <int P, bool NEAR, bool MASK, class Settled>
 __device__ __forceinline__ void row_tile(uint32_t s, uint32_t to, bool started, const float* bp, float flat, int lim, float c2, Row& row,
